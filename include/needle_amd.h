@@ -279,6 +279,141 @@ int nd_attend_step_i8_exact(nd_ctx *ctx, const nd_kv_geom *g, const void *kv,
                             const int32_t *hi, const float *q, float scale,
                             int quant_query, float *out);
 
+/* ---- rotary positions ------------------------------------------------------ */
+
+/* How a head vector of `dim` elements is turned by its position: the first
+ * rot_dim elements in pairs, pair j by the angle pos * f_j, the others left
+ * as they are.
+ *   pairs   ND_ROPE_HALVES: elements j and j + rot_dim / 2 (the Needle-3
+ *           forward's layout, with rot_dim == dim); ND_ROPE_PAIRS: 2j, 2j + 1
+ *   f_j     theta^(-2j / rot_dim), then for longer contexts than the trained
+ *           one: ND_ROPE_PLAIN as it is; ND_ROPE_LINEAR f_j / factor;
+ *           ND_ROPE_PARTS f_j (g + (1 - g) / factor), where g rises from 0 to
+ *           1 as the turns f_j makes over `trained` positions, trained f_j /
+ *           (2 pi), go from turns_lo to turns_hi
+ *   gain    multiplies the turned elements
+ * The angle is the fp64 product of the position and the fp64 f_j; sine,
+ * cosine and the turn are fp64 and rounded to fp32 once, so positions in the
+ * millions lose nothing.  rot_dim is even, 2 .. 256; theta, factor, trained
+ * positive; 0 <= turns_lo < turns_hi (the last three only looked at where
+ * the scaling uses them); gain finite. */
+enum { ND_ROPE_HALVES = 0, ND_ROPE_PAIRS = 1 };
+enum { ND_ROPE_PLAIN = 0, ND_ROPE_LINEAR = 1, ND_ROPE_PARTS = 2 };
+typedef struct nd_rope {
+    int32_t layout, scaling, rot_dim;
+    double theta, factor, trained, turns_lo, turns_hi, gain;
+} nd_rope;
+
+/* The rot_dim / 2 frequencies f_j (host).  Host only. */
+int nd_rope_freqs(const nd_rope *r, double *freq);
+
+/* y[i] = x[i] turned by pos[i], for `rows` rows of `heads` head vectors of
+ * `dim` (<= 256) elements: row i at x + i*x_stride and y + i*y_stride
+ * (elements), its heads one after another.  pos: device int32[rows]; a row
+ * of negative position is not written.  y may be x (with its stride), or
+ * must not overlap it.  The forward's norm_and_rope (v3/model.rs:388-413)
+ * without its norm, for any layout. */
+int nd_rope_rows(nd_ctx *ctx, const nd_rope *r, size_t rows, const int32_t *pos, size_t heads,
+                 size_t dim, const float *x, size_t x_stride, float *y, size_t y_stride);
+
+/* nd_rope_rows on the keys (and, where q is given, the queries) and
+ * nd_kv_write, in one launch.  Row i < count belongs to the block at kv +
+ * (i / per_block)*kv_stride bytes (per_block 1: a row a block; a drafted
+ * tree or a chunk: its rows a block) and is stored at slot pos[i] % cap,
+ * its key turned by rot_pos[i] (NULL: pos[i]); a row of negative pos is left
+ * out altogether.  q[i] ([num_heads][qk]) turned goes to q_out[i]; q and
+ * q_out may both be NULL, and may be the same.  Row strides in elements, so
+ * that one projection's rows can hold q, k and v side by side.  The codes
+ * and scales are those that nd_kv_write stores for the turned key.  Two rows
+ * for one block must not map to one slot. */
+int nd_kv_write_rope(nd_ctx *ctx, const nd_kv_geom *g, const nd_rope *r, void *kv,
+                     size_t kv_stride, size_t count, size_t per_block, const int32_t *pos,
+                     const int32_t *rot_pos, const float *q, size_t q_stride, float *q_out,
+                     size_t q_out_stride, const float *k, size_t k_stride, const float *v,
+                     size_t v_stride);
+
+/* The cache read back: k[i] ([num_kv_heads][qk]) and v[i] as the block at kv
+ * + (i / per_block)*kv_stride bytes holds them at slot pos[i] % cap, codes
+ * times scale in fp32 (dequantised as attend_step reads them,
+ * attention.rs:191-216).  A negative pos gives rows of zeros, as
+ * nd_cq_dequantize_rows does.  k or v may be NULL. */
+int nd_kv_read(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride, size_t count,
+               size_t per_block, const int32_t *pos, float *k, float *v);
+
+/* ---- attention of drafted trees over the int8 cache ------------------------ */
+
+/*
+ * For every session i < count, a tree of `nodes` (1 .. 256) drafted tokens
+ * whose keys and values lie in the session's block (kv + i*kv_stride bytes)
+ * behind its committed positions: node j at position base[i] + j.  Node n
+ * attends to the committed positions lo[i][n] .. base[i] - 1 (lo >= base:
+ * none) and to the nodes j whose bit is set in its mask (bit j % 32 of word
+ * mask[i][n][j / 32], ceil(nodes / 32) words a node; usually its ancestors
+ * and itself):
+ *   out[i][n] ([num_heads][v]) = softmax(scale q[i][n] . k) v,
+ * heads as in nd_attend_step_i8, quant_query too.  Only the first length[i]
+ * nodes of session i are there (NULL: all): bits of the others are ignored,
+ * and their rows of out are not written.  A node that attends to nothing
+ * gets zeros.  NaN where a session's numbers cannot be: length[i] outside 0
+ * .. nodes (every row of the session), base[i] or lo[i][n] negative, or more
+ * than cap positions between the first and the tree's end.
+ * qk 48 or 64, v 64.  `work`: device memory for partial sums, of
+ * nd_attend_tree_i8_work(..) bytes or more, 16-byte aligned, that no other
+ * call uses at the same time; NULL: the context's own (not while its stream
+ * is being captured into a graph, which would keep an address that a later
+ * call may free).  No reference counterpart: the reference decodes one token
+ * a step.
+ */
+size_t nd_attend_tree_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes);
+int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride,
+                      size_t count, size_t nodes, const int32_t *base, const int32_t *length,
+                      const int32_t *lo, const uint32_t *mask, const float *q, float scale,
+                      int quant_query, float *out, void *work, size_t work_bytes);
+
+/* ---- logits under rules ---------------------------------------------------- */
+
+/* What changes row i of the logits before its token is picked; every pointer
+ * is a device pointer and may be NULL, which leaves its rule out.
+ *   hist[i]      (rows hist_stride apart) the hist_len[i] tokens of the
+ *                sequence so far (hist_len NULL: hist_stride of them), the
+ *                generated ones from out_from[i] on (NULL: all of them); a
+ *                token outside 0 .. n-1 is skipped
+ *   repeat[i]    every token of the history: l > 0 ? l / repeat : l * repeat
+ *   frequency[i] a token generated c times: l - c * frequency
+ *   presence[i]  a token generated at least once: l - presence
+ *   bias[i]      (rows bias_stride apart) added to the logits of the
+ *                bias_len[i] tokens bias_id[i] (bias_len NULL: bias_stride);
+ *                biases of a token listed twice are first added up, in order
+ *   mask         rows of ceil(n / 32) words, mask_stride words apart: row
+ *                mask_row[i] of mask_rows (NULL: row i) holds the tokens
+ *                allowed, bit t % 32 of word t / 32; the others get -inf.  A
+ *                mask_row outside 0 .. mask_rows - 1 allows every token.
+ * The rules apply in this order, each step rounded to fp32. */
+typedef struct nd_logits_rules {
+    const int32_t *hist;
+    size_t hist_stride;
+    const int32_t *hist_len, *out_from;
+    const float *repeat, *frequency, *presence;
+    const int32_t *bias_id;
+    const float *bias;
+    size_t bias_stride;
+    const int32_t *bias_len;
+    const uint32_t *mask;
+    size_t mask_stride, mask_rows;
+    const int32_t *mask_row;
+} nd_logits_rules;
+
+/* y[i] = row i of x ([count] rows of n logits, x_stride elements apart) under
+ * the rules (y_stride elements apart; y may be x, or must not overlap it),
+ * and next[i] the first maximum of y[i]: as nd_argmax_rows, but -1 where
+ * nothing is above -inf (a mask that leaves no token).  y or next may be
+ * NULL.  n <= 2^24.  `work` as for nd_attend_tree_i8, of
+ * nd_logits_adjust_work(..) bytes; 0 bytes where next is NULL. */
+size_t nd_logits_adjust_work(nd_ctx *ctx, size_t count, size_t n);
+int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, size_t n,
+                     const nd_logits_rules *rules, float *y, size_t y_stride, int32_t *next,
+                     void *work, size_t work_bytes);
+
 /* ---- libm on the device (crates/needle-core/src/math.rs:3-46) ------------- */
 
 /* y[i] = f(x[i]) for i < n (device buffers), f the device copy of the

@@ -77,6 +77,20 @@ int workspace(nd_ctx *ctx, size_t bytes, void **out)
     return ND_OK;
 }
 
+int call_workspace(nd_ctx *ctx, size_t bytes, void *work, size_t work_bytes, void **out)
+{
+    if (work) {
+        ND_REQUIRE(work_bytes >= bytes, "work holds %zu bytes, %zu needed", work_bytes, bytes);
+        ND_REQUIRE((reinterpret_cast<uintptr_t>(work) & 15) == 0, "work must be 16-byte aligned");
+        *out = work;
+        return ND_OK;
+    }
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    ND_HIP(hipStreamIsCapturing(ctx->stream, &s));
+    ND_REQUIRE(s == hipStreamCaptureStatusNone, "a captured call needs its own work buffer (%zu bytes)", bytes);
+    return workspace(ctx, bytes, out);
+}
+
 int check_launch(const char *kernel)
 {
     hipError_t e = hipGetLastError();

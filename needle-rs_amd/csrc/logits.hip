@@ -1,0 +1,207 @@
+// Logits under a request's rules -- penalties for repeated tokens, biases,
+// grammar masks -- and the greedy pick.
+//
+// A block takes a slice of kSlice tokens of one row: it counts the history's
+// tokens that fall into the slice in LDS (whole numbers: the order of the
+// atomics changes nothing), then passes over the logits once.  Bound by
+// memory: 4 bytes in and 4 out a logit, the history a second time for every
+// slice after the first (from L2).
+//
+// Every step is one fp32 rounding (the file is compiled without contraction),
+// so results do not depend on slice, lane or the presence of other rules.
+#include "nd_internal.h"
+#include "nd_lanes.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSlice = 4096;
+constexpr uint32_t kEver = 1u << 30, kBias = 1u << 31;  // beside the count of a token
+
+struct Pick {
+    float v;
+    int i;
+};
+
+// The first of equal maxima; a NaN never wins.
+__device__ inline void take(Pick &a, float v, int i)
+{
+    if (v > a.v || (v == a.v && i < a.i)) a = Pick{v, i};
+}
+
+__device__ inline int clamp_len(const int32_t *len, size_t row, size_t most)
+{
+    const int m = int(most);
+    return len ? min(max(len[row], 0), m) : m;
+}
+
+template <int H>
+__device__ inline void meet(Pick &a)
+{
+    const float v = ndl::wave_xor<H>(a.v);
+    take(a, v, ndl::wave_xor_int<H>(a.i));
+}
+
+__device__ inline void meet_wave(Pick &a)
+{
+    meet<32>(a), meet<16>(a), meet<8>(a), meet<4>(a), meet<2>(a), meet<1>(a);
+}
+
+constexpr int kNone = 0x7fffffff;
+
+__global__ __launch_bounds__(kThreads) void adjust_kernel(const float *x, size_t x_stride, int n, int slices,
+                                                          nd_logits_rules r, float *y, size_t y_stride,
+                                                          int32_t *next, Pick *part)
+{
+    __shared__ uint32_t st[kSlice];
+    __shared__ float bias[kSlice];
+    __shared__ int twice;
+    __shared__ Pick best[kThreads / 64];
+    const size_t row = blockIdx.x / unsigned(slices);
+    const int slice = int(blockIdx.x % unsigned(slices)), t0 = slice * kSlice, t = threadIdx.x;
+    const int cnt = min(kSlice, n - t0);
+    for (int i = t; i < kSlice; i += kThreads) st[i] = 0;
+    if (t == 0) twice = 0;
+    __syncthreads();
+    if (r.hist) {
+        const int32_t *h = r.hist + row * r.hist_stride;
+        const int len = clamp_len(r.hist_len, row, r.hist_stride);
+        const int from = r.out_from ? r.out_from[row] : 0;
+        for (int i = t; i < len; i += kThreads) {
+            const uint32_t k = uint32_t(h[i]) - uint32_t(t0);
+            if (k < uint32_t(cnt)) {
+                atomicOr(&st[k], kEver);
+                if (i >= from) atomicAdd(&st[k], 1u);
+            }
+        }
+    }
+    const int nb = r.bias ? clamp_len(r.bias_len, row, r.bias_stride) : 0;
+    const int32_t *bi = r.bias_id + row * r.bias_stride;
+    const float *bv = r.bias + row * r.bias_stride;
+    for (int i = t; i < nb; i += kThreads) {
+        const uint32_t k = uint32_t(bi[i]) - uint32_t(t0);
+        if (k < uint32_t(cnt)) {
+            if (atomicOr(&st[k], kBias) & kBias) twice = 1;
+            bias[k] = bv[i];
+        }
+    }
+    __syncthreads();
+    if (twice) {  // the first entry of a token adds up all of its entries, in order
+        for (int i = t; i < nb; i += kThreads) {
+            const int id = bi[i];
+            const uint32_t k = uint32_t(id) - uint32_t(t0);
+            if (k >= uint32_t(cnt)) continue;
+            bool first = true;
+            for (int j = 0; j < i && first; ++j) first = bi[j] != id;
+            if (!first) continue;
+            float s = bv[i];
+            for (int j = i + 1; j < nb; ++j)
+                if (bi[j] == id) s += bv[j];
+            bias[k] = s;
+        }
+        __syncthreads();
+    }
+    const float rep = r.repeat ? r.repeat[row] : 1.0f;
+    const float fr = r.frequency ? r.frequency[row] : 0.0f, pr = r.presence ? r.presence[row] : 0.0f;
+    const uint32_t *mask = nullptr;
+    if (r.mask) {
+        const int m = r.mask_row ? r.mask_row[row] : int(row);
+        if (m >= 0 && size_t(m) < r.mask_rows) mask = r.mask + size_t(m) * r.mask_stride;
+    }
+    Pick b{-INFINITY, kNone};
+    for (int k = t; k < cnt; k += kThreads) {
+        float l = x[row * x_stride + t0 + k];
+        const uint32_t s = st[k];
+        if (s) {
+            const uint32_t c = s & (kEver - 1);
+            if ((s & kEver) && r.repeat) l = l > 0.0f ? l / rep : l * rep;
+            if (c && r.frequency) l -= float(c) * fr;
+            if (c && r.presence) l -= pr;
+            if (s & kBias) l += bias[k];
+        }
+        const int tok = t0 + k;
+        if (mask && !(mask[tok >> 5] >> (tok & 31) & 1)) l = -INFINITY;
+        if (y) y[row * y_stride + tok] = l;
+        if (l > b.v) b = Pick{l, tok};
+    }
+    if (!next) return;
+    meet_wave(b);
+    if ((t & 63) == 0) best[t >> 6] = b;
+    __syncthreads();
+    if (t == 0) {
+        for (int w = 1; w < kThreads / 64; ++w) take(b, best[w].v, best[w].i);
+        if (slices == 1)
+            next[row] = b.i == kNone ? -1 : b.i;
+        else
+            part[row * slices + slice] = b;
+    }
+}
+
+// A wave a row: the best of its slices.
+__global__ __launch_bounds__(64) void join_kernel(const Pick *__restrict__ part, int slices,
+                                                  int32_t *__restrict__ next)
+{
+    Pick b{-INFINITY, kNone};
+    for (int s = threadIdx.x; s < slices; s += 64) {
+        const Pick p = part[size_t(blockIdx.x) * slices + s];
+        take(b, p.v, p.i);
+    }
+    meet_wave(b);
+    if (threadIdx.x == 0) next[blockIdx.x] = b.i == kNone ? -1 : b.i;
+}
+
+size_t slices_of(size_t n) { return (n + kSlice - 1) / kSlice; }
+
+}  // namespace
+
+extern "C" {
+
+size_t nd_logits_adjust_work(nd_ctx *, size_t count, size_t n)
+{
+    const size_t s = slices_of(n);
+    return s > 1 ? count * s * sizeof(Pick) : 0;
+}
+
+int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, size_t n,
+                     const nd_logits_rules *rules, float *y, size_t y_stride, int32_t *next,
+                     void *work, size_t work_bytes)
+{
+    ND_ENTER(ctx);
+    ND_REQUIRE(rules, "null rules");
+    ND_REQUIRE(n > 0 && n <= (size_t(1) << 24), "n %zu must be in 1..2^24", n);
+    if (count == 0 || (!y && !next)) return ND_OK;
+    ND_REQUIRE(x, "null buffer");
+    ND_REQUIRE(count == 1 || (x_stride >= n && (!y || y_stride >= n)), "row strides below n %zu", n);
+    const size_t slices = slices_of(n);
+    ND_REQUIRE(count <= 0x7fffffff && count * slices <= (size_t(1) << 23), "%zu rows of %zu logits are too many",
+               count, n);
+    const nd_logits_rules &r = *rules;
+    ND_REQUIRE(!r.hist || r.hist_stride < (size_t(1) << 30), "hist_stride too large");
+    ND_REQUIRE(!r.bias == !r.bias_id, "bias and bias_id are given together or not at all");
+    ND_REQUIRE(!r.bias || r.bias_stride < (size_t(1) << 30), "bias_stride too large");
+    ND_REQUIRE(!r.mask || r.mask_stride >= (n + 31) / 32, "mask_stride %zu below %zu words", r.mask_stride,
+               (n + 31) / 32);
+    ND_REQUIRE(!r.mask || r.mask_row || r.mask_rows >= count, "%zu mask rows for %zu rows", r.mask_rows, count);
+    if (y && y != x) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+        ND_REQUIRE(a + ((count - 1) * x_stride + n) * 4 <= b || b + ((count - 1) * y_stride + n) * 4 <= a,
+                   "y overlaps x");
+    }
+    ND_REQUIRE(y != x || count == 1 || x_stride == y_stride, "y is x with another stride");
+    Pick *part = nullptr;
+    if (next && slices > 1) {
+        void *p = nullptr;
+        if (int rc = nd::call_workspace(ctx, count * slices * sizeof(Pick), work, work_bytes, &p)) return rc;
+        part = static_cast<Pick *>(p);
+    }
+    hipLaunchKernelGGL(adjust_kernel, dim3(unsigned(count * slices)), dim3(kThreads), 0, ctx->stream, x, x_stride,
+                       int(n), int(slices), r, y, y_stride, next, part);
+    if (int rc = nd::check_launch("logits_adjust")) return rc;
+    if (part) {
+        hipLaunchKernelGGL(join_kernel, dim3(unsigned(count)), dim3(64), 0, ctx->stream, part, int(slices), next);
+        return nd::check_launch("logits_join");
+    }
+    return ND_OK;
+}
+
+}  // extern "C"

@@ -75,6 +75,12 @@ public:
 // Ensures the context workspace holds at least `bytes`.
 int workspace(nd_ctx *ctx, size_t bytes, void **out);
 
+// Device memory for one call's partials: the caller's `work` once it is large
+// enough and 16-byte aligned, or the context's workspace where it is null --
+// refused while the stream is captured, since the graph would keep an address
+// that a later, larger call frees.
+int call_workspace(nd_ctx *ctx, size_t bytes, void *work, size_t work_bytes, void **out);
+
 // Looks up, once per device and with that device current, the device
 // address of the no-allocation entry point's scratch array.
 int noalloc_setup(int device);

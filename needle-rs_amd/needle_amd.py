@@ -39,6 +39,20 @@ class KvGeom(C.Structure):
                 ("qk_head_dim", C.c_int32), ("v_head_dim", C.c_int32), ("cap", C.c_int32)]
 
 
+class Rope(C.Structure):
+    _fields_ = [("layout", C.c_int32), ("scaling", C.c_int32), ("rot_dim", C.c_int32),
+                ("theta", C.c_double), ("factor", C.c_double), ("trained", C.c_double),
+                ("turns_lo", C.c_double), ("turns_hi", C.c_double), ("gain", C.c_double)]
+
+
+class LogitsRules(C.Structure):
+    _fields_ = [("hist", C.c_void_p), ("hist_stride", C.c_size_t), ("hist_len", C.c_void_p),
+                ("out_from", C.c_void_p), ("repeat", C.c_void_p), ("frequency", C.c_void_p),
+                ("presence", C.c_void_p), ("bias_id", C.c_void_p), ("bias", C.c_void_p),
+                ("bias_stride", C.c_size_t), ("bias_len", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_stride", C.c_size_t), ("mask_rows", C.c_size_t), ("mask_row", C.c_void_p)]
+
+
 _lib = None
 _vp, _sz = C.c_void_p, C.c_size_t
 
@@ -107,6 +121,17 @@ _SIGS = [
                                            C.c_float, _vp]),
     ("nd_v3_batch_create_ex", C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, C.c_int, C.POINTER(_vp)]),
     ("nd_libm_map", C.c_int, [_vp, C.c_int, _vp, _sz, _vp]),
+    ("nd_rope_freqs", C.c_int, [C.POINTER(Rope), C.POINTER(C.c_double)]),
+    ("nd_rope_rows", C.c_int, [_vp, C.POINTER(Rope), _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz]),
+    ("nd_kv_write_rope", C.c_int, [_vp, C.POINTER(KvGeom), C.POINTER(Rope), _vp, _sz, _sz, _sz, _vp,
+                                   _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz]),
+    ("nd_kv_read", C.c_int, [_vp, C.POINTER(KvGeom), _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
+    ("nd_attend_tree_i8_work", _sz, [_vp, C.POINTER(KvGeom), _sz, _sz]),
+    ("nd_attend_tree_i8", C.c_int, [_vp, C.POINTER(KvGeom), _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp,
+                                    C.c_float, C.c_int, _vp, _vp, _sz]),
+    ("nd_logits_adjust_work", _sz, [_vp, _sz, _sz]),
+    ("nd_logits_adjust", C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(LogitsRules), _vp, _sz, _vp, _vp,
+                                   _sz]),
 ]
 
 
@@ -581,6 +606,253 @@ def attend_i8_prefill(ctx, num_heads, num_kv_heads, qk, vd, q, k, v, window=0, q
     kv_write(ctx, g, blk, 0, hi, k.contiguous(), v.contiguous())
     scale = float(np.float32(1.0) / np.float32(math.sqrt(qk)))
     return attend_step_i8(ctx, g, blk, 0, lo, hi, q.contiguous(), scale, quant_query)
+
+
+# ---- rotary positions --------------------------------------------------------
+
+_LAYOUTS = {"halves": 0, "pairs": 1}
+_SCALINGS = {"plain": 0, "linear": 1, "parts": 2}
+
+
+def rope(rot_dim, theta=10000.0, layout="halves", scaling="plain", factor=1.0, trained=0,
+         turns=(1.0, 32.0), gain=1.0):
+    """How positions turn a head vector (nd_rope, include/needle_amd.h): its
+    first rot_dim elements in pairs (j, j + rot_dim / 2) or (2j, 2j + 1), by
+    theta^(-2j / rot_dim) a position; scaling "linear" divides the frequencies
+    by factor, "parts" those that make fewer than turns[0] turns over `trained`
+    positions, none of those above turns[1], and in between in part; gain
+    multiplies the turned elements."""
+    if layout not in _LAYOUTS or scaling not in _SCALINGS:
+        raise ValueError(f"layout {layout!r}: halves or pairs; scaling {scaling!r}: plain, linear or parts")
+    return Rope(_LAYOUTS[layout], _SCALINGS[scaling], rot_dim, theta, factor, trained, turns[0], turns[1], gain)
+
+
+def rope_freqs(r):
+    """The rot_dim / 2 angles a position (fp64).  Host only."""
+    out = np.zeros(max(r.rot_dim // 2, 1), np.float64)
+    _check(lib().nd_rope_freqs(C.byref(r), out.ctypes.data_as(C.POINTER(C.c_double))))
+    return out
+
+
+def _near(ctx, t, name):
+    """`t` is on the context's device."""
+    if t.device.index != ctx.device:
+        raise ValueError(f"{name}: on {t.device}, the context is on device {ctx.device}")
+
+
+def _rows_arg(ctx, t, rows, width, name):
+    """(address, row stride) of fp32 rows whose elements lie one after another."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(rows, width)}")
+    if t.dtype != _torch().float32 or not t.is_cuda:
+        raise ValueError(f"{name}: a device tensor of float32 is required, not {t.dtype} on {t.device}")
+    _near(ctx, t, name)
+    if rows and ((t.stride(1) != 1 and width > 1) or (rows > 1 and t.stride(0) < width)):
+        raise ValueError(f"{name}: strides {t.stride()}: rows must be contiguous and apart")
+    return t.data_ptr(), t.stride(0)
+
+
+def _dev_arg(ctx, t, dtype, name, numel=0):
+    if t is None:
+        return None
+    p = _arg(t, dtype, name, numel)
+    _near(ctx, t, name)
+    return p
+
+
+def _empty(ctx, shape, dtype):
+    """An output of a call: allocated for the context's stream, and kept until
+    torch's current stream is done with it too where that is another one."""
+    torch = _torch()
+    now = torch.cuda.current_stream(ctx.device)
+    if now.cuda_stream == ctx.stream.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
+    with torch.cuda.stream(ctx.stream):
+        t = torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
+    t.record_stream(now)
+    return t
+
+
+def rope_rows(ctx, r, x, pos, heads, out=None):
+    """Rows of `heads` head vectors ([rows][heads * dim] fp32, rows may be
+    apart) turned by their positions (int32; a row of negative position is not
+    written).  out may be x."""
+    torch = _torch()
+    rows, width = x.shape
+    if heads < 1 or width % heads:
+        raise ValueError(f"x: {width} elements a row are not {heads} heads")
+    xp, xs = _rows_arg(ctx, x, rows, width, "x")
+    if out is None:
+        out = _empty(ctx, (rows, width), torch.float32)
+    yp, ys = _rows_arg(ctx, out, rows, width, "out")
+    _check(lib().nd_rope_rows(ctx.h, C.byref(r), rows, _dev_arg(ctx, pos, torch.int32, "pos", rows), heads,
+                              width // heads, xp, xs, yp, ys))
+    return out
+
+
+def kv_write_rope(ctx, g, r, kv, kv_stride, pos, k, v, q=None, q_out=None, rot_pos=None, per_block=1):
+    """kv_write of keys turned by rot_pos (pos by default), per_block rows a
+    block, and the queries turned in the same launch (returned; q_out may be
+    q).  q, k and v are [count][heads * dim] fp32 whose rows may be apart, e.g.
+    parts of one projection."""
+    torch = _torch()
+    n, i32 = pos.numel(), torch.int32
+    if per_block < 1:
+        raise ValueError(f"per_block {per_block} must be positive")
+    blocks = kv_block_bytes(g) + (n - 1) // per_block * kv_stride if n else 0
+    kp, ks = _rows_arg(ctx, k, n, g.num_kv_heads * g.qk_head_dim, "k")
+    vp, vs = _rows_arg(ctx, v, n, g.num_kv_heads * g.v_head_dim, "v")
+    qp = op = None
+    qs = os_ = 0
+    if q is not None:
+        width = g.num_heads * g.qk_head_dim
+        qp, qs = _rows_arg(ctx, q, n, width, "q")
+        if q_out is None:
+            q_out = _empty(ctx, (n, width), torch.float32)
+        op, os_ = _rows_arg(ctx, q_out, n, width, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _check(lib().nd_kv_write_rope(
+        ctx.h, C.byref(g), C.byref(r), _dev_arg(ctx, kv, torch.uint8, "kv", blocks), kv_stride, n, per_block,
+        _dev_arg(ctx, pos, i32, "pos"), _dev_arg(ctx, rot_pos, i32, "rot_pos", n), qp, qs, op, os_, kp, ks, vp, vs))
+    return q_out
+
+
+def kv_read(ctx, g, kv, kv_stride, pos, per_block=1, k=None, v=None):
+    """The cache's rows at `pos` as fp32, codes times scale: (k [count][kvh *
+    qk], v [count][kvh * vd]); zeros where pos is negative."""
+    torch = _torch()
+    n, f32 = pos.numel(), torch.float32
+    if per_block < 1:
+        raise ValueError(f"per_block {per_block} must be positive")
+    blocks = kv_block_bytes(g) + (n - 1) // per_block * kv_stride if n else 0
+    wk, wv = g.num_kv_heads * g.qk_head_dim, g.num_kv_heads * g.v_head_dim
+    if k is None:
+        k = _empty(ctx, (n, wk), f32)
+    if v is None:
+        v = _empty(ctx, (n, wv), f32)
+    _check(lib().nd_kv_read(ctx.h, C.byref(g), _dev_arg(ctx, kv, torch.uint8, "kv", blocks), kv_stride, n, per_block,
+                            _dev_arg(ctx, pos, torch.int32, "pos"), _dev_arg(ctx, k, f32, "k", n * wk),
+                            _dev_arg(ctx, v, f32, "v", n * wv)))
+    return k, v
+
+
+# ---- drafted trees -------------------------------------------------------------
+
+def tree_mask(parents):
+    """The masks of trees of drafted tokens (int32 words, [..][nodes][ceil(nodes
+    / 32)], a numpy array for the device): parents [..][nodes] holds each node's
+    parent, an earlier node, or a negative number for a root; a node attends to
+    its ancestors and itself."""
+    up = np.asarray(parents)
+    n = up.shape[-1]
+    if n < 1 or (up >= np.arange(n)).any():
+        raise ValueError("parents: every node's parent must come before it")
+    flat = up.reshape(-1, n)
+    see = np.zeros((flat.shape[0], n, (n + 31) // 32), np.uint32)
+    rows = np.arange(flat.shape[0])
+    for j in range(n):
+        see[:, j] = np.where((flat[:, j] >= 0)[:, None], see[rows, np.maximum(flat[:, j], 0)], 0)
+        see[:, j, j // 32] |= np.uint32(1 << (j % 32))
+    return see.view(np.int32).reshape(up.shape + (-1,))
+
+
+def _work_arg(ctx, work):
+    if work is None:
+        return None, 0
+    p = _dev_arg(ctx, work, _torch().uint8, "work")
+    return p, work.numel()
+
+
+def attend_tree_i8(ctx, g, kv, kv_stride, base, lo, mask, q, length=None, scale=None, quant_query=False,
+                   out=None, work=None):
+    """Attention of every session's drafted tree (nd_attend_tree_i8): base [S]
+    committed positions, lo [S][N] the first one each node attends to, mask
+    [S][N][ceil(N / 32)] int32 words of the nodes it attends to, length [S]
+    nodes there are; q [S][N][heads * qk] fp32, out [S][N][heads * v] (rows
+    past a tree's length are left as they are, zeros in a new `out`).  work: a
+    uint8 device tensor of attend_tree_i8_work() bytes, needed while a graph is
+    captured."""
+    torch = _torch()
+    i32, f32 = torch.int32, torch.float32
+    if q.dim() != 3:
+        raise ValueError(f"q: shape {tuple(q.shape)}, expected [sessions][nodes][heads * qk]")
+    s, n = q.shape[0], q.shape[1]
+    wo = g.num_heads * g.v_head_dim
+    if scale is None:
+        scale = float(np.float32(1.0) / np.sqrt(np.float32(g.qk_head_dim)))
+    if out is None:
+        out = _empty(ctx, (s, n, wo), f32)
+        if length is not None:
+            with torch.cuda.stream(ctx.stream):
+                out.zero_()
+    blocks = kv_block_bytes(g) + (s - 1) * kv_stride if s else 0
+    wp, wb = _work_arg(ctx, work)
+    _check(lib().nd_attend_tree_i8(
+        ctx.h, C.byref(g), _dev_arg(ctx, kv, torch.uint8, "kv", blocks), kv_stride, s, n,
+        _dev_arg(ctx, base, i32, "base", s), _dev_arg(ctx, length, i32, "length", s),
+        _dev_arg(ctx, lo, i32, "lo", s * n), _dev_arg(ctx, mask, i32, "mask", s * n * ((n + 31) // 32)),
+        _dev_arg(ctx, q, f32, "q", s * n * g.num_heads * g.qk_head_dim), scale, int(bool(quant_query)),
+        _dev_arg(ctx, out, f32, "out", s * n * wo), wp, wb))
+    return out
+
+
+def attend_tree_i8_work(ctx, g, sessions, nodes):
+    """Bytes of `work` that attend_tree_i8 needs."""
+    return lib().nd_attend_tree_i8_work(ctx.h, C.byref(g), sessions, nodes)
+
+
+# ---- logits under rules --------------------------------------------------------
+
+def logits_adjust(ctx, x, hist=None, hist_len=None, out_from=None, repeat=None, presence=None, frequency=None,
+                  bias_id=None, bias=None, bias_len=None, mask=None, mask_row=None, out=None, pick=False,
+                  write=True, work=None):
+    """Rows of logits ([count][n] fp32, rows may be apart) under penalties for
+    repeated tokens, biases and grammar masks (nd_logits_adjust): hist [count][
+    m] int32 tokens (-1: none) with hist_len and out_from [count], repeat,
+    presence and frequency [count] fp32, bias_id and bias [count][b] with
+    bias_len [count], mask [rows][ceil(n / 32)] int32 words with mask_row
+    [count].  Returns the new logits (`out`, which may be x); with pick=True
+    (logits, next), next[i] the first maximum of row i, -1 where no token is
+    left; with write=False next alone."""
+    torch = _torch()
+    i32, f32 = torch.int32, torch.float32
+    count, n = x.shape
+    xp, xs = _rows_arg(ctx, x, count, n, "x")
+    rules = LogitsRules()
+    if hist is not None:
+        if hist.dim() != 2 or hist.shape[0] != count:
+            raise ValueError(f"hist: shape {tuple(hist.shape)}, expected {count} rows")
+        rules.hist, rules.hist_stride = _dev_arg(ctx, hist, i32, "hist"), hist.shape[1]
+    if bias is not None and bias_id is not None:
+        if bias.dim() != 2 or bias.shape[0] != count or bias.shape != bias_id.shape:
+            raise ValueError(f"bias: shape {tuple(bias.shape)}, bias_id {tuple(bias_id.shape)}: [count][b] both")
+        rules.bias_stride = bias.shape[1]
+    rules.bias, rules.bias_id = _dev_arg(ctx, bias, f32, "bias"), _dev_arg(ctx, bias_id, i32, "bias_id")
+    for name, t, dtype in (("hist_len", hist_len, i32), ("out_from", out_from, i32), ("repeat", repeat, f32),
+                           ("presence", presence, f32), ("frequency", frequency, f32), ("bias_len", bias_len, i32),
+                           ("mask_row", mask_row, i32)):
+        if t is not None:
+            setattr(rules, name, _dev_arg(ctx, t, dtype, name, count))
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[1] < (n + 31) // 32:
+            raise ValueError(f"mask: shape {tuple(mask.shape)}, expected rows of {(n + 31) // 32} words")
+        rules.mask, rules.mask_rows, rules.mask_stride = _dev_arg(ctx, mask, i32, "mask"), mask.shape[0], mask.shape[1]
+    yp = ys = None
+    if write:
+        if out is None:
+            out = _empty(ctx, (count, n), f32)
+        yp, ys = _rows_arg(ctx, out, count, n, "out")
+    nxt = _empty(ctx, (count,), i32) if pick or not write else None
+    wp, wb = _work_arg(ctx, work)
+    _check(lib().nd_logits_adjust(ctx.h, xp, xs, count, n, C.byref(rules), yp, ys or 0,
+                                  nxt.data_ptr() if nxt is not None else None, wp, wb))
+    return (out, nxt) if write and pick else out if write else nxt
+
+
+def logits_adjust_work(ctx, count, n):
+    """Bytes of `work` that logits_adjust needs."""
+    return lib().nd_logits_adjust_work(ctx.h, count, n)
 
 
 # ---- Needle-3 forward on the device ----------------------------------------

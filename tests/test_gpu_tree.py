@@ -1,0 +1,373 @@
+"""Attention of drafted trees over the int8 cache against a plain 64-bit form.
+
+Tolerance.  A score is a dot of at most 64 products summed in fp32 and three
+products: off by at most 67 * 2^-24 of the sum of the products' magnitudes,
+which for these N(0, 1) draws stays below 64 * 0.8 = 51 before and 7.4 after
+the scale, so below 3.0e-5, and by a root's share of that (4e-6) in any draw.
+A weight is off by as much, by a few steps of its exponential (4 * 2^-24) and
+by the 22 bits or more it is held in; an output, a mean of |v| < 5.5 under
+such weights in numerator and sum, by 2 * (4e-6 + 5e-7) * 5.5 / 2 = 2.5e-5 at
+the very most and in draws of many positions far less: 2e-5 is the bar, as
+for the other int8 attention.  Larger or smaller values scale it.
+"""
+import numpy as np
+import pytest
+import torch
+
+import needle_amd as nd
+import tree_ref as R
+from conftest import dev, host
+
+pytestmark = pytest.mark.gpu
+TOL = 2e-5
+
+
+def _block(ctx, rng, H, KVH, QK, cap, upto, count, k_size=1.0, v_size=1.0):
+    """Blocks that hold positions upto - cap .. upto - 1; the rest is garbage."""
+    g = nd.kv_geom(H, KVH, QK, 64, cap)
+    blk, nb = nd.kv_alloc(g, count)
+    blk.fill_(0xff)
+    for i in range(count):
+        p0 = max(0, upto - cap)
+        n = upto - p0
+        k = (rng.normal(size=(n, KVH * QK)) * k_size).astype(np.float32)
+        v = (rng.normal(size=(n, KVH * 64)) * v_size).astype(np.float32)
+        nd.kv_write(ctx, g, blk[i * nb:(i + 1) * nb], 0, torch.arange(p0, upto, dtype=torch.int32, device="cuda"),
+                    dev(k), dev(v))
+    return g, blk, nb
+
+
+def _parents(rng, count, nodes, branch=3):
+    up = np.zeros((count, nodes), np.int64)
+    for j in range(nodes):
+        up[:, j] = -1 if j == 0 else np.maximum(j - 1 - rng.integers(0, branch + 1, count), -1)
+    return up
+
+
+def _want(g, blk, nb, base, length, lo, see, q, quant, scale=None):
+    """[S][N][H * 64], NaN where a row is not to be compared."""
+    S, N = lo.shape
+    H, QK = g.num_heads, g.qk_head_dim
+    scale = 1.0 / np.sqrt(QK) if scale is None else scale
+    out = np.full((S, N, H * 64), np.nan)
+    for i in range(S):
+        k, ks, v, vs = nd.kv_unpack(g, blk[i * nb:(i + 1) * nb])
+        m = N if length is None else int(length[i])
+        for n in range(m):
+            first = min(int(lo[i, n]), int(base[i]))
+            pos = np.arange(first, base[i] + m)
+            slot = pos % g.cap
+            sees = np.concatenate([np.ones(int(base[i]) - first, bool), see[i, n, :m] != 0])
+            used = np.where(sees, slot, 0)
+            kk = k[used] * np.where(sees[:, None], ks[used], 1).astype(np.float64)[..., None]
+            vv = v[used] * np.where(sees[:, None], vs[used], 1).astype(np.float64)[..., None]
+            qq = q[i, n].reshape(H, QK)
+            if quant:
+                c, s = R.stand_for(qq)
+                qq = c * s.astype(np.float64)[:, None]
+            out[i, n] = R.attend(qq, kk, vv, sees, scale).reshape(-1)
+    return out
+
+
+def _check(ctx, g, blk, nb, base, lo, see, q, length=None, quant=False, scale=None, tol=TOL, rows=None):
+    base, lo = np.asarray(base, np.int32), np.asarray(lo, np.int32)
+    S, N = lo.shape
+    out = torch.full((S, N, g.num_heads * 64), 7.0, device="cuda")
+    args = (ctx, g, blk, nb, dev(base), dev(lo), dev(R.words_of(see)), dev(q.reshape(S, N, -1)))
+    kw = dict(length=None if length is None else dev(np.asarray(length, np.int32)), quant_query=quant, scale=scale)
+    got = host(nd.attend_tree_i8(*args, out=out, **kw))
+    # the same call with its own workspace, bit for bit
+    need = nd.attend_tree_i8_work(ctx, g, S, N)
+    own = torch.full((need + 256,), 0xa5, dtype=torch.uint8, device="cuda")
+    twice = torch.full_like(out, 7.0)
+    nd.attend_tree_i8(*args, out=twice, work=own[:max(need, 16)], **kw)
+    assert np.array_equal(host(twice), got, equal_nan=True) and (host(own)[max(need, 16):] == 0xa5).all()
+    b = host(blk)
+    pick = range(S) if rows is None else rows
+    for i in pick:
+        one = slice(i, i + 1)
+        want = _want(g, b[i * nb:(i + 1) * nb] if nb else b, nb or len(b), base[one],
+                     None if length is None else length[one], lo[one], see[one], q[one], quant, scale)[0]
+        there = ~np.isnan(want)
+        assert not np.isnan(got[i][there]).any(), i
+        assert np.max(np.abs(got[i][there] - want[there]), initial=0) <= tol, (i, np.abs(got[i][there] - want[there]).max())
+        assert (got[i][~there] == 7.0).all(), i  # rows behind the tree's end
+    return got
+
+
+SHAPES = [(12, 2, 48), (12, 12, 64), (16, 2, 64), (5, 1, 48), (7, 1, 64), (6, 2, 64), (4, 2, 48)]
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("H,KVH,QK", SHAPES)
+@pytest.mark.parametrize("nodes,base,cap", [(1, 0, 1), (1, 5, 6), (2, 31, 33), (8, 32, 40), (16, 70, 129), (33, 0, 64),
+                                            (31, 200, 700), (64, 1, 65), (13, 500, 513)])
+def test_trees(ctx, H, KVH, QK, nodes, base, cap, quant):
+    """Ragged trees and bases, rings below a tile and just large enough."""
+    rng = np.random.default_rng(nodes * 100 + cap + H)
+    S = 3
+    g, blk, nb = _block(ctx, rng, H, KVH, QK, cap, base + nodes, S)
+    bases = base - np.minimum(np.arange(S) * 7, base)
+    length = np.maximum(nodes - np.arange(S) * 3, 0)
+    see = R.bits_of(nd.tree_mask(_parents(rng, S, nodes)), nodes)
+    # a ring holds its last `cap` positions: what a shorter base would read before them is not there
+    lo = np.maximum(bases + length - cap, max(0, base + nodes - cap))[:, None] + np.zeros((1, nodes), int)
+    q = rng.normal(size=(S, nodes, H * QK)).astype(np.float32)
+    _check(ctx, g, blk, nb, bases, np.minimum(lo, bases[:, None] + 1), see, q, length, quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("H,KVH,QK", [(12, 2, 48), (12, 12, 64), (8, 1, 64)])
+@pytest.mark.parametrize("nodes,base,cap,window", [(40, 5000, 1061, 1000), (21, 999, 300, 256), (7, 4097, 64, 50),
+                                                   (100, 3001, 3200, 0), (256, 700, 1000, 0), (3, 9000, 9003, 0)])
+def test_windows_and_wrapped_rings(ctx, H, KVH, QK, nodes, base, cap, window, quant):
+    rng = np.random.default_rng(cap + nodes)
+    g, blk, nb = _block(ctx, rng, H, KVH, QK, cap, base + nodes, 1)
+    up = _parents(rng, 1, nodes)
+    depth = np.zeros((1, nodes), int)
+    for j in range(nodes):
+        depth[0, j] = depth[0, up[0, j]] + 1 if up[0, j] >= 0 else 0
+    lo = np.maximum(base + depth + 1 - window, 0) if window else np.zeros_like(depth)
+    lo = np.maximum(lo, base + nodes - cap)
+    see = R.bits_of(nd.tree_mask(up), nodes)
+    q = rng.normal(size=(1, nodes, H * QK)).astype(np.float32)
+    _check(ctx, g, blk, nb, [base], lo, see, q, quant=quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("sessions,nodes,base", [(65, 16, 300), (130, 5, 90), (300, 2, 40), (9, 30, 2000)])
+def test_many_sessions(ctx, sessions, nodes, base, quant):
+    """Every launch shape: few sessions with long spans, many with short ones."""
+    rng = np.random.default_rng(sessions)
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, base + nodes, base + nodes, sessions)
+    bases = base - np.arange(sessions) % 17
+    see = R.bits_of(nd.tree_mask(_parents(rng, sessions, nodes)), nodes)
+    length = nodes - np.arange(sessions) % 3 % nodes
+    lo = np.zeros((sessions, nodes), int)
+    q = rng.normal(size=(sessions, nodes, 12 * 48)).astype(np.float32)
+    _check(ctx, g, blk, nb, bases, lo, see, q, length, quant, rows=sorted({0, 1, 7, sessions // 2, sessions - 1}))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("base", [0, 3, 100, 2100])
+def test_any_mask_and_rows_that_see_nothing(ctx, base, quant):
+    """Masks that are no tree, bits behind the tree's end, rows with nothing
+    (zeros), with the committed positions alone, and with one node alone."""
+    rng = np.random.default_rng(base)
+    nodes, S = 37, 3
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, base + nodes, base + nodes, S)
+    see = rng.integers(0, 2, (S, nodes, nodes)).astype(np.uint8)
+    see[:, 4] = 0
+    see[:, 5] = 0
+    see[:, 6] = 0
+    see[:, 6, 30] = 1
+    length = np.array([nodes, 31, 6])
+    lo = rng.integers(0, base + 1, (S, nodes))
+    lo[:, [4, 6]] = base + np.array([0, 5])
+    q = rng.normal(size=(S, nodes, 12 * 48)).astype(np.float32)
+    got = _check(ctx, g, blk, nb, np.full(S, base), lo, see, q, length, quant)
+    assert not got[:, 4].any() and got[0, 6].any() and not got[1, 6, 0] == 0
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_garbage_in_places_no_row_reads(ctx, quant):
+    """NaN and infinite scales before the window, behind the tree and in nodes
+    outside a row's mask reach nobody but the rows that read them."""
+    rng = np.random.default_rng(2)
+    nodes, base, cap = 10, 90, 128
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, cap, base + nodes, 1)
+    off = nd.kv_offsets(g)
+    for part in ("ks", "vs"):
+        s = blk[off[part]:off[part] + 4 * 2 * cap].view(torch.float32).view(2, cap)
+        s[:, :20] = float("nan")
+        s[:, 20:30] = float("inf")
+        s[:, base + 7] = float("nan")  # node 7
+        s[:, base + 8] = float("inf")  # node 8
+        s[:, base + nodes:] = float("nan")
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes).copy()
+    see[:, :, 7:9] = 0
+    see[0, 7, 7] = see[0, 8, 8] = 1
+    q = rng.normal(size=(1, nodes, 12 * 48)).astype(np.float32)
+    lo = np.full((1, nodes), 30)
+    lo[0, 2] = 57
+    clean = np.array([0, 1, 2, 3, 4, 5, 6, 9])
+    args = (ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(lo.astype(np.int32)), dev(R.words_of(see)), dev(q))
+    got = host(nd.attend_tree_i8(*args, quant_query=quant))
+    want = _want(g, host(blk), nb, [base], None, lo, see, q, quant)
+    assert np.abs(got[0, clean] - want[0, clean]).max() <= TOL
+    assert np.isnan(got[0, 7]).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("k_size,v_size", [(1e-6, 1e6), (30.0, 1e-12), (1e-30, 1e-30), (3.0, 1e30)])
+def test_sizes_of_values(ctx, k_size, v_size, quant):
+    """Values far from 1, and V rows of very different sizes in one span."""
+    rng = np.random.default_rng(5)
+    nodes, base = 16, 200
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 256, base + nodes, 1, k_size, v_size)
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    q = (rng.normal(size=(1, nodes, 12 * 48)) / max(k_size, 1e-30)).astype(np.float32)
+    _check(ctx, g, blk, nb, [base], np.zeros((1, nodes), int), see, q, quant=quant, tol=TOL * v_size)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("spread", [1e3, 1e6, 1e12])
+def test_small_values_beside_large_ones(ctx, spread, quant):
+    """Rows whose window holds small values only, beside rows that read large
+    ones: each row's error is measured against its own values."""
+    rng = np.random.default_rng(7)
+    nodes, base = 24, 320
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 400, base + nodes, 1)
+    off = nd.kv_offsets(g)
+    s = blk[off["vs"]:off["vs"] + 4 * 2 * 400].view(torch.float32).view(2, 400)
+    s[:, :100] *= spread
+    s[:, 150:200:3] /= spread
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    lo = np.where(np.arange(nodes) % 2, 100, 0)[None]
+    q = rng.normal(size=(1, nodes, 12 * 48)).astype(np.float32)
+    args = (ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(lo.astype(np.int32)), dev(R.words_of(see)), dev(q))
+    got = host(nd.attend_tree_i8(*args, quant_query=quant))
+    want = _want(g, host(blk), nb, [base], None, lo, see, q, quant)
+    assert np.abs(got[0, 1::2] - want[0, 1::2]).max() <= TOL
+    assert np.abs(got[0, ::2] - want[0, ::2]).max() <= TOL * spread
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_weight_on_a_row_of_small_values(ctx, quant):
+    """Most of the weight on a position whose values are tiny (a sink): the
+    rest, 2^-20 of the weight, decides the output."""
+    rng = np.random.default_rng(9)
+    nodes, base = 9, 200
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 256, base + nodes, 1)
+    off = nd.kv_offsets(g)
+    q = np.abs(rng.normal(size=(1, nodes, 12 * 48))).astype(np.float32)
+    kv = blk[:2 * 256 * 48].view(torch.int8).view(2, 256, 48)
+    kv[:, 5] = 100
+    blk[off["ks"]:off["ks"] + 4 * 512].view(torch.float32).view(2, 256)[:, 5] = 0.03
+    blk[off["vs"]:off["vs"] + 4 * 512].view(torch.float32).view(2, 256)[:, 5] = 1e-9
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    lo = np.zeros((1, nodes), int)
+    args = (ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(lo.astype(np.int32)), dev(R.words_of(see)), dev(q))
+    got = host(nd.attend_tree_i8(*args, quant_query=quant))
+    want = _want(g, host(blk), nb, [base], None, lo, see, q, quant)
+    # scores here reach 20: their fp32 steps, 20 * 67 * 2^-24 in the worst case, are a relative error of the weights
+    assert np.linalg.norm(got - want) <= 8e-5 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_any_scale(ctx, scale):
+    rng = np.random.default_rng(11)
+    nodes, base = 12, 100
+    g, blk, nb = _block(ctx, rng, 6, 2, 64, 128, base + nodes, 1)
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    q = rng.normal(size=(1, nodes, 6 * 64)).astype(np.float32)
+    for quant in (False, True):
+        # scores grow with the scale, their errors too (the bar is set for 1 / 8)
+        _check(ctx, g, blk, nb, [base], np.zeros((1, nodes), int), see, q, quant=quant, scale=scale,
+               tol=TOL * max(1, 8 * abs(scale)))
+
+
+def test_wrong_numbers_give_nan(ctx):
+    """Rows whose numbers cannot be, and only those."""
+    rng = np.random.default_rng(4)
+    nodes, cap = 4, 50
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, cap, 44, 7)
+    see = np.repeat(np.eye(nodes, dtype=np.uint8)[None], 7, 0)
+    base = np.array([40, -1, 40, 40, 40, 2 ** 31 - 3, 40], np.int32)
+    length = np.array([4, 4, 5, -1, 0, 4, 4], np.int32)
+    lo = np.zeros((7, nodes), np.int32)
+    lo[0, 1], lo[6] = -1, -2 ** 31
+    lo[5] = 2 ** 31 - 5
+    q = rng.normal(size=(7, nodes, 12 * 48)).astype(np.float32)
+    out = torch.full((7, nodes, 12 * 64), 7.0, device="cuda")
+    got = host(nd.attend_tree_i8(ctx, g, blk, nb, dev(base), dev(lo), dev(R.words_of(see)), dev(q), length=dev(length),
+                                 out=out))
+    assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, [0, 2, 3]]).all()
+    for i in (1, 2, 3, 5, 6):
+        assert np.isnan(got[i]).all(), i
+    assert (got[4] == 7.0).all()
+    # a span one longer than the ring (51 positions written: every slot holds one)
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, cap, 51, 1)
+    lo = np.array([[0, 1, 0, 1]], np.int32)
+    got = host(nd.attend_tree_i8(ctx, g, blk[:nb], nb, dev(np.array([47], np.int32)), dev(lo),
+                                 dev(R.words_of(see[:1])), dev(q[:1])))
+    assert np.isnan(got[0, [0, 2]]).all() and np.isfinite(got[0, [1, 3]]).all()
+
+
+def test_sessions_over_one_block(ctx):
+    """kv_stride 0: several trees tried over one session's cache."""
+    rng = np.random.default_rng(6)
+    nodes, base = 6, 77
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 90, base + nodes, 1)
+    see = R.bits_of(nd.tree_mask(_parents(rng, 3, nodes)), nodes)
+    q = rng.normal(size=(3, nodes, 12 * 48)).astype(np.float32)
+    _check(ctx, g, blk, 0, [base] * 3, np.zeros((3, nodes), int), see, q)
+
+
+def test_a_tree_of_one_node_is_a_decode_step(ctx):
+    """One node a session: nd_attend_step_i8's answer for the same span."""
+    rng = np.random.default_rng(8)
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 300, 300, 5)
+    base = np.array([299, 0, 31, 32, 100], np.int32)
+    q = dev(rng.normal(size=(5, 12 * 48)).astype(np.float32))
+    zero = dev(np.zeros(5, np.int32))
+    for quant in (False, True):
+        a = nd.attend_step_i8(ctx, g, blk, nb, zero, dev(base), q, quant_query=quant)
+        b = nd.attend_tree_i8(ctx, g, blk, nb, dev(base), zero.view(5, 1), dev(np.ones((5, 1, 1), np.int32)),
+                              q.view(5, 1, -1), quant_query=quant)
+        assert (a - b.view(5, -1)).abs().max().item() <= TOL
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """A block of 4.4 GB, the window and the tree near its end."""
+    g = nd.kv_geom(4, 2, 64, 64, 1 << 24)
+    blk = torch.empty(nd.kv_block_bytes(g), dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(10)
+    first, nodes = (1 << 24) - 80, 20
+    k, v = (rng.normal(size=(100, 128)).astype(np.float32) for _ in range(2))
+    pos = torch.arange(first, first + 100, dtype=torch.int32, device="cuda")  # wraps after 80
+    nd.kv_write(ctx, g, blk, 0, pos, dev(k), dev(v))
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    q = rng.normal(size=(1, nodes, 256)).astype(np.float32)
+    got = host(nd.attend_tree_i8(ctx, g, blk, 0, dev(np.array([first + 80], np.int32)),
+                                 dev(np.full((1, nodes), first, np.int32)), dev(R.words_of(see)), dev(q)))
+    kc, ks = R.stand_for(k.reshape(100, 2, 64))
+    vc, vs = R.stand_for(v.reshape(100, 2, 64))
+    for n in range(nodes):
+        sees = np.concatenate([np.ones(80, bool), see[0, n] != 0])
+        want = R.attend(q[0, n].reshape(4, 64), kc * ks[..., None].astype(np.float64),
+                        vc * vs[..., None].astype(np.float64), sees, 0.125)
+        assert np.abs(got[0, n] - want.reshape(-1)).max() <= TOL
+
+
+def test_refusals(ctx):
+    g = nd.kv_geom(12, 2, 48, 64, 64)
+    blk, nb = nd.kv_alloc(g, 2)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.zeros(2, 4, 576, device="cuda")
+
+    def refused(what, f):
+        with pytest.raises(nd.NeedleError) as e:
+            f()
+        assert e.value.code == nd.ND_ERR_ARG and what in str(e.value), str(e.value)
+
+    big = torch.zeros(1, 257, 576, device="cuda")
+    refused("nodes", lambda: nd.attend_tree_i8(ctx, g, blk, nb, z(1), z(1, 257), z(1, 257, 9), big))
+    refused("nodes", lambda: nd.attend_tree_i8(ctx, g, blk, nb, z(2), z(2, 1), z(2, 1, 1), q[:, :0]))
+    for bad in (nd.kv_geom(12, 2, 32, 64, 64), nd.kv_geom(12, 2, 64, 128, 64), nd.kv_geom(18, 2, 48, 64, 64)):
+        store, bb = nd.kv_alloc(nd.kv_geom(12, 2, 64, 128, 64), 2)
+        refused("", lambda: nd.attend_tree_i8(ctx, bad, store, bb, z(2), z(2, 4), z(2, 4, 1),
+                                              torch.zeros(2, 4, 18 * 64, device="cuda"),
+                                              out=torch.zeros(2, 4, 18 * 128, device="cuda")))
+    refused("aligned", lambda: nd.attend_tree_i8(ctx, g, blk[64:], nb, z(1), z(1, 4), z(1, 4, 1), q[:1]))
+    ok = (z(2), z(2, 4), z(2, 4, 1), q)
+    assert nd.attend_tree_i8(ctx, g, blk, nb, *ok).shape == (2, 4, 768)
+    for args, kw in (((z(1), *ok[1:]), {}), ((ok[0], z(2, 3), *ok[2:]), {}), ((*ok[:2], z(2, 3, 1), q), {}),
+                     ((*ok[:3], q.view(8, 576)), {}), ((*ok[:3], q.double()), {}), (ok, dict(out=q)),
+                     (ok, dict(length=z(1))), ((*ok[:3], q.cpu()), {}), ((ok[0].long(), *ok[1:]), {}),
+                     (ok, dict(work=z(4)))):
+        with pytest.raises(ValueError):
+            nd.attend_tree_i8(ctx, g, blk, nb, *args, **kw)
+    with pytest.raises(ValueError):
+        nd.attend_tree_i8(ctx, g, blk[:nb], nb, *ok)  # two sessions, one block
+    assert nd.attend_tree_i8(ctx, g, blk, nb, z(0), z(0, 4), z(0, 4, 1), q[:0]).shape == (0, 4, 768)
