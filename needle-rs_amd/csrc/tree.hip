@@ -2,18 +2,48 @@
 // tree attends to a window of the committed positions and to the nodes its
 // mask names, whose keys and values lie in the same ring behind them.
 //
-// A block a (node, query head): each thread walks its own positions with a
-// running maximum and sum (scores in bits: e^s = 2^(s log2 e)), and the
-// threads' sums meet at the end.
+// On the matrix cores.  The columns of a (session, kv head) are its (node,
+// query head) pairs: a wave owns 16 NT of them and walks chunks of 32
+// positions with an online softmax; the waves of a block own the same columns
+// and take the chunks in turn, and meet in LDS at the end.  The committed
+// positions and the tree are chunked apart, so that a chunk of the tree is a
+// word of the mask.
+//   scores  S[pos][col] = K Q^T, v_mfma 16x16, A = 16 positions' int8 rows.
+//           With quant_query both sides are codes and the dot is an exact
+//           integer; else the fp32 query is two f16 pieces, 22 bits and more
+//           of a head scaled by a power of two (error 2^-23 of an element, as
+//           much as fp32's own steps leave a sum of products).
+//   softmax scores stay without the column's factor cf (scale, query scale):
+//           the maximum m is kept before it and e = 2^(fma(t, cf, -m cf)).
+//   values  O^T[v][col] = V^T P^T: a score tile's result layout is the layout
+//           of the weights the product needs.  MFMA c takes V columns 4 n + c,
+//           a dword a position.  The weights e vs are two f16 pieces, of which
+//           the first 22 bits are kept (and none below 2^-38 of the largest V
+//           scale met so far), V's codes are exact in f16.  A chunk with a V
+//           scale 2^-9 or less of that largest takes three bf16 pieces, all 24
+//           bits at any size, instead: the values of one position may be far
+//           smaller than its neighbours' and yet decide the output.
+// Sums and statistics are fp32.
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace {
 
 using namespace ndkv;
 
-constexpr int kThreads = 256;
 constexpr int kMaxNodes = 256;
+constexpr int VD = 64;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
+typedef float floatx4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int intx4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 struct Tree {
     const uint8_t *kv;
@@ -21,95 +51,608 @@ struct Tree {
     const int32_t *base, *length, *lo;
     const uint32_t *mask;
     const float *q;
-    float *out;
-    int nodes, words;
-    float scale2;  // scale log2(e)
+    float *out, *part_o, *part_ml;
+    int nodes, words, units, tiles, splits;
+    float scale2;  // |scale| log2(e)
+    int negative;  // scale < 0
 };
 
-template <int QK, bool QQ>
-__global__ __launch_bounds__(kThreads) void tree_kernel(Geom g, Tree tr)
+__device__ inline float i8_at(uint32_t dw, int b) { return float(int32_t(dw << (24 - 8 * b)) >> 24); }
+
+// High halves of two floats: (bf16 of a, bf16 of b) where both are exact.
+__device__ inline uint32_t pack_hi(float a, float b)
 {
-    constexpr int VD = 64, NW = kThreads / 64;
-    __shared__ float qs[QK];
-    __shared__ float mo[NW][VD], mm[NW], ml[NW];
-    const int head = blockIdx.x % g.H, node = blockIdx.x / g.H;
-    const size_t ses = blockIdx.y;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const int len = tr.length ? tr.length[ses] : tr.nodes;
-    float *out = tr.out + ((ses * tr.nodes + node) * g.H + head) * VD;
-    const size_t row = ses * tr.nodes + node;
-    const int base = tr.base[ses], lo = tr.lo[row];
-    const bool wrong = len < 0 || len > tr.nodes;
-    if (!wrong && node >= len) return;
-    const int first = min(lo, base);
-    if (wrong || base < 0 || lo < 0 || base > 0x7fffffff - kMaxNodes || base - first + len > g.cap) {
-        if (t < VD) out[t] = NAN;
-        return;
-    }
-    const int kvh = head / (g.H / g.KVH);
-    const uint8_t *blk = tr.kv + ses * tr.kv_stride;
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+__device__ inline float trunc_hi(float a) { return __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+
+// fmaxf of three (a NaN loses), without the copies the compiler makes of
+// operands it cannot show to be quiet.
+__device__ inline float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// x0, x1 as three bf16 pairs that sum to them exactly.
+__device__ inline void split3(float x0, float x1, uint32_t &h, uint32_t &m, uint32_t &l)
+{
+    h = pack_hi(x0, x1);
+    const float r0 = x0 - trunc_hi(x0), r1 = x1 - trunc_hi(x1);
+    m = pack_hi(r0, r1);
+    l = pack_hi(r0 - trunc_hi(r0), r1 - trunc_hi(r1));
+}
+
+// x0, x1 (below 2^16) as two f16 pairs.  (Written out, the remainder is a
+// conversion and a subtraction; v_fma_mix_f32 does both.)
+__device__ inline void split2(float x0, float x1, uint32_t &h, uint32_t &l)
+{
+    h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(x1));
+    l = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+}
+
+// The sign bits flipped, code c is c + 128; byte c of two dwords as f16 pairs:
+// u + 128 read as a subnormal, times 2^15, less 128 * 2^-9, is code * 2^-9.
+template <int C>
+__device__ inline uint32_t f16_codes(uint32_t lo, uint32_t hi)
+{
+    const uint32_t u = __builtin_amdgcn_perm(hi, lo, 0x0c000c00u | uint32_t(4 + C) << 16 | uint32_t(C));
+    const f16x2_t m = {_Float16(32768.0f), _Float16(32768.0f)}, a = {_Float16(-0.25f), _Float16(-0.25f)};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, u), m, a));
+}
+
+// Bytes 2 I, 2 I + 1 of a dword (sign bits flipped) as an f16 pair of codes:
+// 1024 + (c + 128) - 1152.
+template <int I>
+__device__ inline uint32_t f16_pair(uint32_t x)
+{
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, x, I ? 0x04030402u : 0x04010400u);
+    const f16x2_t a = {_Float16(-1152.0f), _Float16(-1152.0f)};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u) + a);
+}
+
+template <typename T>
+__device__ inline T vec4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __builtin_bit_cast(T, u32x4_t{a, b, c, d});
+}
+
+template <int QK, bool QQ, int NT, int NW>
+__global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, Tree tr)
+{
+    constexpr int SL = QK / 4, KD = SL / 4;    // a lane's slice of a K row; its dwords (3 or 4)
+    constexpr int COLS = 16 * NT, LD = VD + 4, HN = NW / 2;
+    __shared__ __align__(16) float sc_s[NW][64];
+    __shared__ uint32_t mw[COLS][kMaxNodes / 32 + 1];
+    __shared__ __align__(16) float mo[HN][COLS][LD];
+    __shared__ float mm[HN][COLS], ml[HN][COLS];
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 15, qd = lane >> 4;
+    // blocks 8 apart share an XCD's L2: there a unit's column tiles follow each other
+    const int unit = int(blockIdx.x >> 3) / tr.tiles * 8 + int(blockIdx.x & 7), tile = int(blockIdx.x >> 3) % tr.tiles;
+    if (unit >= tr.units) return;
+    const int split = unit % tr.splits, group = unit / tr.splits;
+    const int kvh = group % g.KVH, ses = group / g.KVH;
+    const int R = g.H / g.KVH;
+    const int base = tr.base[ses], len0 = tr.length ? tr.length[ses] : tr.nodes;
+    const bool there = len0 >= 0 && len0 <= tr.nodes;
+    const bool wrong = !there || base < 0 || base > 0x7fffffff - kMaxNodes;
+    const int len = there ? len0 : tr.nodes;
+    const int ncols = len * R;
+    if (tile * COLS >= ncols) return;
+    const uint8_t *blk = tr.kv + size_t(ses) * tr.kv_stride;
     const int8_t *kb = reinterpret_cast<const int8_t *>(blk) + size_t(kvh) * g.cap * QK;
     const int8_t *vb = reinterpret_cast<const int8_t *>(blk + g.v_off) + size_t(kvh) * g.cap * VD;
     const float *ksb = reinterpret_cast<const float *>(blk + g.ks_off) + size_t(kvh) * g.cap;
     const float *vsb = reinterpret_cast<const float *>(blk + g.vs_off) + size_t(kvh) * g.cap;
-    const float *q = tr.q + (row * g.H + head) * QK;
-    for (int e = t; e < QK; e += kThreads) qs[e] = q[e];
-    __syncthreads();
-    if (QQ) {
-        if (w == 0) {
-            float sc, inv;
-            quant_scale_wave(qs, QK, sc, inv);
-            for (int e = lane; e < QK; e += 64) qs[e] = quant_code(qs[e], inv) * sc;
+    const uint32_t cap = uint32_t(g.cap);
+
+    // f / R of a column f < 2^11: (f + 1/2) / R is 1/16 or more away from an
+    // integer (R <= 8)
+    const float inv_r = 1.0f / float(R);
+    auto node_of = [&](int f) { return int((float(f) + 0.5f) * inv_r); };
+    for (int i = t; i < COLS * tr.words; i += NW * 64) {
+        const int col = i / tr.words, word = i - col * tr.words;
+        const int node = node_of(min(tile * COLS + col, ncols - 1));
+        mw[col][word] = tr.mask[(size_t(ses) * tr.nodes + node) * tr.words + word];
+    }
+
+    // ---- the wave's columns: windows and query operands ----
+    uint32_t lo[NT];                      // first committed position; 0xffffffff: none is read at all
+    float cf[NT];                         // factor of a score, in bits
+    intx4_t qi[NT];                       // QQ: codes
+    uint32_t qp[NT][2][KD == 3 ? 6 : 8];  // else: f16 pieces
+    uint32_t ulo = uint32_t(base);
+    bool bad[NT];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int f = min(tile * COLS + 16 * x + n, ncols - 1);  // past the end: a copy, not written
+        const int node = node_of(f), head = kvh * R + f - node * R;
+        const size_t row = size_t(ses) * tr.nodes + node;
+        const int l0 = tr.lo[row];
+        bad[x] = wrong || l0 < 0 || base - min(l0, base) + len > g.cap;
+        lo[x] = bad[x] ? 0xffffffffu : uint32_t(l0);
+        ulo = min(ulo, lo[x]);
+        const float *qh = tr.q + (row * g.H + head) * QK + qd * SL;
+        float v[SL];
+#pragma unroll
+        for (int e = 0; e < SL; ++e) v[e] = qh[e];
+        if (tr.negative) {
+#pragma unroll
+            for (int e = 0; e < SL; ++e) v[e] = -v[e];
+        }
+        float a = 0.0f;
+#pragma unroll
+        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1]));
+        a = fmaxf(a, ndl::wave_xor<16>(a));
+        a = fmaxf(a, ndl::wave_xor<32>(a));
+        float nan = 0.0f;
+        if constexpr (QQ) {
+            // quant_rows (model.rs:289-293): the codes and the head's scale
+            const float qs = a > 0.0f ? a / 127.0f : 1.0f;
+            const float inv = 1.0f / qs;
+            uint32_t dw[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                // quant_code: half away from zero is truncation after adding
+                // the float below a half, for every |y| < 2^22
+                const float y = v[e] * inv;
+                const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
+                nan = y != y ? y : nan;
+                dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
+            }
+            qi[x] = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
+            cf[x] = qs * tr.scale2;
+        } else {
+            // the head in 2^14 .. 2^15, so that the second pieces are normal numbers
+            const int sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                nan = v[e] - v[e] != 0.0f ? NAN : nan;
+                v[e] = __builtin_amdgcn_ldexpf(v[e], sh);
+            }
+#pragma unroll
+            for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[x][0][e / 2], qp[x][1][e / 2]);
+            cf[x] = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
+        }
+        // NaN where the query has one (an infinity gives one too)
+        nan += ndl::wave_xor<16>(nan);
+        nan += ndl::wave_xor<32>(nan);
+        cf[x] += nan;
+    }
+    ulo = min(ulo, uint32_t(ndl::wave_xor_int<1>(int(ulo))));
+    ulo = min(ulo, uint32_t(ndl::wave_xor_int<2>(int(ulo))));
+    ulo = min(ulo, uint32_t(ndl::wave_xor_int<4>(int(ulo))));
+    ulo = min(ulo, uint32_t(ndl::wave_xor_int<8>(int(ulo))));
+    ulo = __builtin_amdgcn_readfirstlane(ulo);
+    bool live = false;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) live = live || !bad[x];
+    __syncthreads();  // the mask words
+
+    // ---- the walk: chunk i is committed positions ulo + 32 i .., then nodes ----
+    const uint32_t before = uint32_t(base) - ulo;
+    const int np = __any(live) ? int((before + 31u) / 32u) : 0;
+    const int nch = __any(live) ? np + (len + 31) / 32 : 0;
+    const int step = tr.splits * NW;
+    int ch = split * NW + w;
+    const uint32_t slo = ulo % cap;
+    uint32_t s0 = 0;
+    int valid = 0;  // positions of the chunk
+    auto place = [&](int i) {
+        const int c = i - np;
+        const uint32_t off = c < 0 ? 32u * uint32_t(i) : before + 32u * uint32_t(c);
+        valid = i >= nch ? 0 : c < 0 ? int(min(32u, before - off)) : min(32, len - 32 * c);
+        // a walk is no longer than the ring: positions wrap at most once
+        s0 = slo + off;
+        if (s0 >= cap) s0 -= cap;
+        if (i >= nch) s0 = 0;  // past the end: any slot
+    };
+    auto slot_of = [&](uint32_t o) { return (s0 + o) % cap; };
+    uint32_t kr[2][KD], vr[8];
+    float scr = 0.0f;
+    auto load_k = [&]() {
+        if (s0 + 32u <= cap) {
+            const int8_t *p = kb + size_t(s0) * QK;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int d = 0; d < KD; ++d)
+                    kr[a][d] = *reinterpret_cast<const uint32_t *>(p + (n * QK + qd * SL) + (16 * a * QK + 4 * d));
+            scr = *(lane < 32 ? ksb + s0 + lane : vsb + s0 + (lane - 32));
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int8_t *p = kb + size_t(slot_of(16 * a + n)) * QK + qd * SL;
+#pragma unroll
+                for (int d = 0; d < KD; ++d) kr[a][d] = *reinterpret_cast<const uint32_t *>(p + 4 * d);
+            }
+            scr = (lane < 32 ? ksb : vsb)[slot_of(lane & 31)];
+        }
+    };
+    auto load_v = [&]() {
+        if (s0 + 32u <= cap) {
+            const int8_t *p = vb + size_t(s0) * VD;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                vr[j] = *reinterpret_cast<const uint32_t *>(p + (4 * qd * VD + 4 * n) + (16 * (j >> 2) + (j & 3)) * VD);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                vr[j] = *reinterpret_cast<const uint32_t *>(
+                    vb + size_t(slot_of(16 * (j >> 2) + 4 * qd + (j & 3))) * VD + 4 * n);
+        }
+    };
+    // loads are never conditional: past the last chunk they read some slot
+    place(ch);
+    load_k();
+    load_v();
+
+    float m_run[NT], mu[NT], l_run[NT];
+    floatx4_t acc[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        m_run[x] = -INFINITY;
+        mu[x] = 0.0f;
+        l_run[x] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[x][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // K and V scales are taken in units of 2^kexp and 2^(vexp - 14), powers of
+    // two that no finite one so far is above: scores before cf, and weights,
+    // stay in range at any size of the cache's values
+    int kexp = 0, vexp = 0;
+    float top = 0.0f;                   // lanes below 32: 2^kexp, the others: 2^vexp
+    int shift = lane < 32 ? 0 : 14;
+
+    for (; ch < nch; ch += step) {
+        // ---- the chunk's scales, zero behind its end ----
+        float sc = (lane & 31) < valid ? scr : 0.0f;
+        if (__any(sc > top)) {
+            float h = sc < INFINITY ? fmaxf(sc, top) : top;
+            h = fmaxf(h, ndl::wave_xor<16>(h));
+            h = fmaxf(h, ndl::wave_xor<8>(h));
+            h = fmaxf(h, ndl::wave_xor<4>(h));
+            h = fmaxf(h, ndl::wave_xor<2>(h));
+            h = fmaxf(h, ndl::wave_xor<1>(h));
+            const int was = lane < 32 ? kexp : vexp;
+            const int now = h > top ? __builtin_amdgcn_frexp_expf(h) : was;
+            top = h > top ? (now > 127 ? 0x1.fffffep127f : __builtin_amdgcn_ldexpf(1.0f, now)) : top;
+            shift += was - now;
+            const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                m_run[x] = __builtin_amdgcn_ldexpf(m_run[x], kexp - kn);
+                cf[x] = __builtin_amdgcn_ldexpf(cf[x], kn - kexp);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - vn);
+            }
+            kexp = kn;
+            vexp = vn;
+        }
+        sc = __builtin_amdgcn_ldexpf(sc, shift);
+        const bool small = __any(lane >= 32 && (lane & 31) < valid && sc < 32.0f);
+        sc_s[w][lane] = sc;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        floatx4_t ks[2], vs[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ks[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][16 * a + 4 * qd]);
+            vs[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][32 + 16 * a + 4 * qd]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        // ---- the positions each column sees ----
+        uint32_t vis[NT];
+        const uint32_t some = valid < 32 ? (1u << valid) - 1u : 0xffffffffu;
+        bool every = true;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            if (ch < np) {
+                const uint32_t p0 = ulo + 32u * uint32_t(ch);
+                vis[x] = lo[x] <= p0 ? some : lo[x] - p0 < 32u ? some & (0xffffffffu << (lo[x] - p0)) : 0u;
+            } else {
+                vis[x] = bad[x] ? 0u : mw[16 * x + n][ch - np] & some;
+            }
+            every = every && vis[x] == 0xffffffffu;
+        }
+        const bool full = __all(every);
+        // ---- scores ----
+        float s[NT][8];
+        if constexpr (QQ) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const intx4_t kf{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi[x], intx4_t{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[x][4 * a + i] = float(d[i]) * ks[a][i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                uint32_t kp[2 * KD];
+#pragma unroll
+                for (int d = 0; d < KD; ++d) {
+                    const uint32_t u = kr[a][d] ^ 0x80808080u;
+                    kp[2 * d] = f16_pair<0>(u);
+                    kp[2 * d + 1] = f16_pair<1>(u);
+                }
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int pc = 1; pc >= 0; --pc) {  // the small pieces first
+                        const uint32_t *qq = qp[x][pc];
+                        // qk 48: a lane's last four codes, doubled to the 32-wide
+                        // product's eight against four zeros of the query
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            vec4<f16x8_t>(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1]),
+                            KD == 3 ? vec4<f16x8_t>(qq[4], qq[5], 0u, 0u)
+                                    : vec4<f16x8_t>(qq[4], qq[5], qq[2 * KD - 2], qq[2 * KD - 1]),
+                            d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(kp[0], kp[1], kp[2], kp[3]),
+                                                                   vec4<f16x8_t>(qq[0], qq[1], qq[2], qq[3]), d, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[x][4 * a + i] = d[i] * ks[a][i];
+                }
+            }
+        }
+        place(ch + step);
+        load_k();  // lands during the softmax and the values
+        // ---- softmax: each lane its column's eight positions ----
+        if (!full) {
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(vis[x] >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u)) s[x][j] = -INFINITY;
+        }
+        bool grew = false;
+        float m_new[NT];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            const float m8 = max3(max3(s[x][0], s[x][1], s[x][2]), max3(s[x][3], s[x][4], s[x][5]),
+                                  max3(s[x][6], s[x][7], m_run[x]));
+            // over the four lane quarters: each swap returns the pair
+            const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(m8), __float_as_uint(m8), false, false);
+            const float m16 = max3(__uint_as_float(s16[0]), __uint_as_float(s16[1]), m8);
+            const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(m16), __float_as_uint(m16), false, false);
+            m_new[x] = max3(__uint_as_float(s32[0]), __uint_as_float(s32[1]), m16);
+            grew = grew || m_new[x] > m_run[x];
+        }
+        if (__any(grew)) {
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                const float mu_new = m_new[x] == -INFINITY ? 0.0f : m_new[x] * cf[x];
+                // nothing is summed yet where there was no maximum
+                const float al = m_run[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu[x] - mu_new);
+                m_run[x] = m_new[x];
+                mu[x] = mu_new;
+                l_run[x] *= al;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[x][c] *= al;
+            }
+        }
+        float wt[NT][8];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                wt[x][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][j], cf[x], -mu[x]));
+                if (full) {
+                    l_run[x] += wt[x][j];
+                    wt[x][j] *= vs[j >> 2][j & 3];
+                }
+            }
+            if (!full) {
+                // where the column does not look there may be anything, a NaN scale too
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool see = vis[x] >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u;
+                    l_run[x] += see ? wt[x][j] : 0.0f;
+                    wt[x][j] = see ? wt[x][j] * vs[j >> 2][j & 3] : 0.0f;
+                }
+            }
+        }
+        // ---- values ----
+        if (!small) {
+            uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split2(wt[x][2 * j], wt[x][2 * j + 1], ph[x][j], pl[x][j]);
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
+            auto column = [&](auto cc) {
+                constexpr int c = decltype(cc)::value;
+                const f16x8_t vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]),
+                                                 f16_codes<c>(u[4], u[5]), f16_codes<c>(u[6], u[7]));
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        vf, vec4<f16x8_t>(pl[x][0], pl[x][1], pl[x][2], pl[x][3]), acc[x][c], 0, 0, 0);
+                    acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        vf, vec4<f16x8_t>(ph[x][0], ph[x][1], ph[x][2], ph[x][3]), acc[x][c], 0, 0, 0);
+                }
+            };
+            column(std::integral_constant<int, 0>{});
+            column(std::integral_constant<int, 1>{});
+            column(std::integral_constant<int, 2>{});
+            column(std::integral_constant<int, 3>{});
+        } else {
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                uint32_t pp[3][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    split3(wt[x][2 * j] * 0x1p-9f, wt[x][2 * j + 1] * 0x1p-9f, pp[0][j], pp[1][j], pp[2][j]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t vp[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vp[j] = pack_hi(i8_at(vr[2 * j], c), i8_at(vr[2 * j + 1], c));
+#pragma unroll
+                    for (int pc = 2; pc >= 0; --pc)
+                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            vec4<bf16x8_t>(vp[0], vp[1], vp[2], vp[3]),
+                            vec4<bf16x8_t>(pp[pc][0], pp[pc][1], pp[pc][2], pp[pc][3]), acc[x][c], 0, 0, 0);
+                }
+            }
+        }
+        load_v();  // lands during the next scores
+    }
+
+    // ---- the block's waves meet, half of them at a time ----
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        l_run[x] += ndl::wave_xor<16>(l_run[x]);
+        l_run[x] += ndl::wave_xor<32>(l_run[x]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - 5);
+        // from here on the maximum is in bits
+        m_run[x] = m_run[x] == -INFINITY ? -INFINITY : mu[x];
+    }
+#pragma unroll
+    for (int h = HN; h >= 1; h /= 2) {
+        if (w >= h && w < 2 * h) {
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                if (qd == 0) {
+                    mm[w - h][16 * x + n] = m_run[x];
+                    ml[w - h][16 * x + n] = l_run[x];
+                }
+                // lane (n, qd) holds V columns 16 qd + 4 i + c
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<floatx4_t *>(&mo[w - h][16 * x + n][16 * qd + 4 * i]) =
+                        floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]};
+            }
         }
         __syncthreads();
-    }
-    const uint32_t *bits = tr.mask + row * tr.words;
-    float m = -INFINITY, l = 0.0f, acc[VD];
+        if (w < h) {
 #pragma unroll
-    for (int e = 0; e < VD; ++e) acc[e] = 0.0f;
-    const int before = base - first;
-    for (int i = t; i < before + len; i += kThreads) {
-        const int j = i - before;
-        if (j >= 0 && !(bits[j >> 5] >> (j & 31) & 1)) continue;
-        const int slot = int((uint32_t(first) + uint32_t(i)) % uint32_t(g.cap));
-        float s = 0.0f;
-        const int8_t *k = kb + size_t(slot) * QK, *v = vb + size_t(slot) * VD;
-        for (int e = 0; e < QK; ++e) s += qs[e] * float(k[e]);
-        s = s * ksb[slot] * tr.scale2;
-        const float mn = fmaxf(m, s);
-        const float al = m == mn ? 1.0f : exp2f(m - mn), p = exp2f(s - mn), wt = p * vsb[slot];
-        l = l * al + p;
+            for (int x = 0; x < NT; ++x) {
+                const float m2 = mm[w][16 * x + n], M = fmaxf(m_run[x], m2);
+                // -inf: sums are 0, or NaN where a score was
+                const float f1 = m_run[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[x] - M);
+                const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - M);
+                m_run[x] = M;
+                l_run[x] = l_run[x] * f1 + ml[w][16 * x + n] * f2;
 #pragma unroll
-        for (int e = 0; e < VD; ++e) acc[e] = acc[e] * al + wt * float(v[e]);
-        m = mn;
-    }
-    const float M = wave_max(m);
-    const float f = m == -INFINITY ? (l != l ? NAN : 0.0f) : exp2f(m - M);
-    l = wave_sum(l * f);
+                for (int i = 0; i < 4; ++i) {
+                    const floatx4_t o = *reinterpret_cast<const floatx4_t *>(&mo[w][16 * x + n][16 * qd + 4 * i]);
 #pragma unroll
-    for (int e = 0; e < VD; ++e) {
-        const float o = wave_sum(m == -INFINITY ? 0.0f : acc[e] * f);
-        if (lane == 0) mo[w][e] = o;
-    }
-    if (lane == 0) mm[w] = M, ml[w] = l;
-    __syncthreads();
-    if (t < VD) {
-        float MM = -INFINITY, O = 0.0f, L = 0.0f;
-        for (int i = 0; i < NW; ++i) MM = fmaxf(MM, mm[i]);
-        for (int i = 0; i < NW; ++i) {
-            const float fi = mm[i] == -INFINITY ? 0.0f : exp2f(mm[i] - MM);
-            O += mo[i][t] * fi;
-            L += ml[i] * (ml[i] != ml[i] ? 1.0f : fi);
+                    for (int c = 0; c < 4; ++c) acc[x][c][i] = acc[x][c][i] * f1 + o[c] * f2;
+                }
+            }
         }
-        out[t] = L == 0.0f ? 0.0f : O / L;
+        if (h > 1) __syncthreads();
     }
+    if (w) return;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int f = tile * COLS + 16 * x + n;
+        if (f >= ncols) continue;
+        const int node = node_of(f), head = kvh * R + f - node * R;
+        const size_t oh = (size_t(ses) * tr.nodes + node) * g.H + head;
+        if (tr.splits == 1) {
+            const float inv = bad[x] ? NAN : l_run[x] == 0.0f ? 0.0f : 1.0f / l_run[x];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<floatx4_u *>(tr.out + oh * VD + 16 * qd + 4 * i) =
+                    floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]} * inv;
+        } else {
+            const size_t at = oh * tr.splits + split;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<floatx4_t *>(tr.part_o + at * VD + 16 * qd + 4 * i) =
+                    floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]};
+            if (qd == 0) {
+                tr.part_ml[2 * at] = m_run[x];
+                tr.part_ml[2 * at + 1] = bad[x] ? NAN : l_run[x];
+            }
+        }
+    }
+}
+
+// The splits of a (row, head) meet: a wave each, a lane a column.
+__global__ __launch_bounds__(256) void tree_join_kernel(int H, Tree tr, size_t total)
+{
+    const size_t oh = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (oh >= total) return;
+    const int lane = threadIdx.x & 63;
+    const size_t row = oh / H, ses = row / tr.nodes;
+    const int len = tr.length ? tr.length[ses] : tr.nodes;
+    // rows behind the tree's end have no partials and are left as they are
+    if (len >= 0 && len <= tr.nodes && int(row - ses * tr.nodes) >= len) return;
+    float M = -INFINITY, L = 0.0f, O = 0.0f;
+    for (int s = 0; s < tr.splits; ++s) M = fmaxf(M, tr.part_ml[2 * (oh * tr.splits + s)]);
+    for (int s = 0; s < tr.splits; ++s) {
+        const size_t at = oh * tr.splits + s;
+        const float m = tr.part_ml[2 * at], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+        L += tr.part_ml[2 * at + 1] * f;
+        O += tr.part_o[at * VD + lane] * f;
+    }
+    tr.out[oh * VD + lane] = L == 0.0f ? 0.0f : O / L;
+}
+
+struct Plan {
+    int nt, nw;
+    size_t tiles, splits;
+};
+
+Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
+{
+    const size_t cus = size_t(ctx && ctx->num_cus > 0 ? ctx->num_cus : 256);
+    const size_t cols = nodes * size_t(g->num_heads / g->num_kv_heads);
+    const size_t groups = count * size_t(g->num_kv_heads);
+    const size_t chunks = (size_t(g->cap) + 31) / 32 + (nodes + 31) / 32;
+    Plan p;
+    p.nt = cols > 16 && groups * ((cols + 31) / 32) >= cus ? 2 : 1;
+    p.tiles = (cols + 16 * p.nt - 1) / (16 * p.nt);
+    const size_t blocks = groups * p.tiles;
+    p.nw = blocks * 4 >= cus * 16 ? 4 : 8;
+    const size_t fill = (cus * 8 + blocks * p.nw - 1) / (blocks * p.nw), most = (chunks + 2 * p.nw - 1) / (2 * p.nw);
+    p.splits = std::max<size_t>(1, std::min<size_t>(std::min(fill, most), 64));
+    return p;
+}
+
+template <int QK, bool QQ>
+auto kernel_of(const Plan &p)
+{
+    if (p.nt == 2) return p.nw == 4 ? tree_kernel<QK, QQ, 2, 4> : tree_kernel<QK, QQ, 2, 8>;
+    return p.nw == 4 ? tree_kernel<QK, QQ, 1, 4> : tree_kernel<QK, QQ, 1, 8>;
+}
+
+size_t partial_floats(const nd_kv_geom *g, size_t count, size_t nodes, size_t splits)
+{
+    return splits > 1 ? count * nodes * g->num_heads * splits * (VD + 2) : 0;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t nd_attend_tree_i8_work(nd_ctx *, const nd_kv_geom *, size_t, size_t) { return 0; }
+size_t nd_attend_tree_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
+{
+    if (!ctx || !g || g->num_kv_heads <= 0 || g->num_heads <= 0 || g->cap <= 0 || !count || !nodes) return 0;
+    return partial_floats(g, count, nodes, plan_of(ctx, g, count, nodes).splits) * sizeof(float);
+}
 
 int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride,
                       size_t count, size_t nodes, const int32_t *base, const int32_t *length,
@@ -118,7 +661,7 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
 {
     ND_ENTER(ctx);
     if (int rc = check_geom(g)) return rc;
-    ND_REQUIRE((g->qk_head_dim == 48 || g->qk_head_dim == 64) && g->v_head_dim == 64,
+    ND_REQUIRE((g->qk_head_dim == 48 || g->qk_head_dim == 64) && g->v_head_dim == VD,
                "no tree attention for qk %d, v %d", g->qk_head_dim, g->v_head_dim);
     ND_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "nodes %zu must be in 1..%d", nodes, kMaxNodes);
     if (count == 0) return ND_OK;
@@ -127,24 +670,54 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     ND_REQUIRE(g->num_heads <= 4096, "num_heads %d above 4096", g->num_heads);
     ND_REQUIRE((reinterpret_cast<uintptr_t>(kv) & 255) == 0 && kv_stride % 256 == 0,
                "kv blocks must be 256-byte aligned");
+    const Plan p = plan_of(ctx, g, count, nodes);
     Tree t{};
-    t.kv = static_cast<const uint8_t *>(kv);
     t.kv_stride = kv_stride;
-    t.base = base;
-    t.length = length;
-    t.lo = lo;
-    t.mask = mask;
-    t.q = q;
-    t.out = out;
     t.nodes = int(nodes);
     t.words = int((nodes + 31) / 32);
-    t.scale2 = float(double(scale) * 1.4426950408889634);
-    const dim3 grid(unsigned(nodes * g->num_heads), unsigned(count));
+    t.tiles = int(p.tiles);
+    t.splits = int(p.splits);
+    t.scale2 = float(double(scale < 0 ? -scale : scale) * 1.4426950408889634);
+    t.negative = scale < 0;
+    float *part = nullptr;
+    if (p.splits > 1) {
+        void *ws = nullptr;
+        const size_t bytes = partial_floats(g, count, nodes, p.splits) * sizeof(float);
+        if (int rc = nd::call_workspace(ctx, bytes, work, work_bytes, &ws)) return rc;
+        part = static_cast<float *>(ws);
+    }
     const bool q48 = g->qk_head_dim == 48;
-    auto *fn = q48 ? (quant_query ? tree_kernel<48, true> : tree_kernel<48, false>)
-                   : (quant_query ? tree_kernel<64, true> : tree_kernel<64, false>);
-    hipLaunchKernelGGL(fn, grid, dim3(kThreads), 0, ctx->stream, make_geom(g), t);
-    return nd::check_launch("attend_tree_i8");
+    auto *fn = q48 ? (quant_query ? kernel_of<48, true>(p) : kernel_of<48, false>(p))
+                   : (quant_query ? kernel_of<64, true>(p) : kernel_of<64, false>(p));
+    // HIP counts a launch's threads in 32 bits: sessions beyond that go in further launches
+    const size_t per = size_t(g->num_kv_heads) * p.splits * p.tiles, most = std::max<size_t>(1, (size_t(1) << 22) / per);
+    const Geom kg = make_geom(g);
+    for (size_t s = 0; s < count; s += most) {
+        const size_t m = std::min(most, count - s), rows = s * nodes;
+        t.kv = static_cast<const uint8_t *>(kv) + s * kv_stride;
+        t.base = base + s;
+        t.length = length ? length + s : nullptr;
+        t.lo = lo + rows;
+        t.mask = mask + rows * t.words;
+        t.q = q + rows * g->num_heads * g->qk_head_dim;
+        t.out = out + rows * g->num_heads * VD;
+        if (part) {
+            const size_t heads = m * nodes * g->num_heads;
+            t.part_o = part;
+            t.part_ml = part + heads * p.splits * VD;
+            part = t.part_ml + heads * p.splits * 2;
+        }
+        t.units = int(m * g->num_kv_heads * p.splits);
+        hipLaunchKernelGGL(fn, dim3(unsigned((t.units + 7) / 8 * 8 * p.tiles)), dim3(p.nw * 64), 0, ctx->stream, kg, t);
+        if (int rc = nd::check_launch("attend_tree_i8")) return rc;
+        if (t.part_o) {
+            const size_t total = m * nodes * g->num_heads;
+            hipLaunchKernelGGL(tree_join_kernel, dim3(unsigned((total + 3) / 4)), dim3(256), 0, ctx->stream,
+                               g->num_heads, t, total);
+            if (int rc = nd::check_launch("tree_join")) return rc;
+        }
+    }
+    return ND_OK;
 }
 
 }  // extern "C"
