@@ -20,9 +20,9 @@
 //           a dword a position.  The weights e vs are two f16 pieces, of which
 //           the first 22 bits are kept (and none below 2^-38 of the largest V
 //           scale met so far), V's codes are exact in f16.  A chunk with a V
-//           scale 2^-9 or less of that largest takes three bf16 pieces, all 24
-//           bits at any size, instead: the values of one position may be far
-//           smaller than its neighbours' and yet decide the output.
+//           scale 2^-9 or less of that largest takes the fp32 matrix product
+//           instead, all 24 bits at any size: the values of one position may be
+//           far smaller than its neighbours' and yet decide the output.
 // Sums and statistics are fp32.
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
@@ -37,7 +37,6 @@ using namespace ndkv;
 constexpr int kMaxNodes = 256;
 constexpr int VD = 64;
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
@@ -59,14 +58,6 @@ struct Tree {
 
 __device__ inline float i8_at(uint32_t dw, int b) { return float(int32_t(dw << (24 - 8 * b)) >> 24); }
 
-// High halves of two floats: (bf16 of a, bf16 of b) where both are exact.
-__device__ inline uint32_t pack_hi(float a, float b)
-{
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-
-__device__ inline float trunc_hi(float a) { return __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
-
 // fmaxf of three (a NaN loses), without the copies the compiler makes of
 // operands it cannot show to be quiet.
 __device__ inline float max3(float a, float b, float c)
@@ -74,15 +65,6 @@ __device__ inline float max3(float a, float b, float c)
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
-}
-
-// x0, x1 as three bf16 pairs that sum to them exactly.
-__device__ inline void split3(float x0, float x1, uint32_t &h, uint32_t &m, uint32_t &l)
-{
-    h = pack_hi(x0, x1);
-    const float r0 = x0 - trunc_hi(x0), r1 = x1 - trunc_hi(x1);
-    m = pack_hi(r0, r1);
-    l = pack_hi(r0 - trunc_hi(r0), r1 - trunc_hi(r1));
 }
 
 // x0, x1 (below 2^16) as two f16 pairs.  (Written out, the remainder is a
@@ -221,6 +203,8 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[x][0][e / 2], qp[x][1][e / 2]);
             cf[x] = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
         }
+        // (a factor of 0 would make no number of a score of -inf)
+        if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
         // NaN where the query has one (an infinity gives one too)
         nan += ndl::wave_xor<16>(nan);
         nan += ndl::wave_xor<32>(nan);
@@ -254,7 +238,12 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         if (s0 >= cap) s0 -= cap;
         if (i >= nch) s0 = 0;  // past the end: any slot
     };
-    auto slot_of = [&](uint32_t o) { return (s0 + o) % cap; };
+    // a chunk inside the ring: scalar base, lane offsets; across its end (or in
+    // a ring below a chunk): each position's slot, the last one's behind it
+    auto slot_of = [&](uint32_t o) {
+        const uint32_t p = s0 + min(o, uint32_t(max(valid, 1) - 1));
+        return p >= cap ? p - cap : p;
+    };
     uint32_t kr[2][KD], vr[8];
     float scr = 0.0f;
     auto load_k = [&]() {
@@ -269,9 +258,9 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         } else {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const int8_t *p = kb + size_t(slot_of(16 * a + n)) * QK + qd * SL;
+                const uint32_t o = slot_of(16 * a + n) * QK + qd * SL;  // below 2^24 64
 #pragma unroll
-                for (int d = 0; d < KD; ++d) kr[a][d] = *reinterpret_cast<const uint32_t *>(p + 4 * d);
+                for (int d = 0; d < KD; ++d) kr[a][d] = *reinterpret_cast<const uint32_t *>(kb + o + 4 * d);
             }
             scr = (lane < 32 ? ksb : vsb)[slot_of(lane & 31)];
         }
@@ -286,7 +275,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 vr[j] = *reinterpret_cast<const uint32_t *>(
-                    vb + size_t(slot_of(16 * (j >> 2) + 4 * qd + (j & 3))) * VD + 4 * n);
+                    vb + (slot_of(16 * (j >> 2) + 4 * qd + (j & 3)) * VD + 4 * n));
         }
     };
     // loads are never conditional: past the last chunk they read some slot
@@ -330,6 +319,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             for (int x = 0; x < NT; ++x) {
                 m_run[x] = __builtin_amdgcn_ldexpf(m_run[x], kexp - kn);
                 cf[x] = __builtin_amdgcn_ldexpf(cf[x], kn - kexp);
+                if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -339,6 +329,10 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             vexp = vn;
         }
         sc = __builtin_amdgcn_ldexpf(sc, shift);
+        // a V scale that is no number makes no number of the columns that see
+        // it, and only of those: a weight of 0 there would not stay 0
+        const uint64_t wild = __ballot(lane >= 32 && !(__builtin_fabsf(sc) < INFINITY));
+        if (wild) sc = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY) ? 0.0f : sc;
         const bool small = __any(lane >= 32 && (lane & 31) < valid && sc < 32.0f);
         sc_s[w][lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -363,6 +357,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                 vis[x] = bad[x] ? 0u : mw[16 * x + n][ch - np] & some;
             }
             every = every && vis[x] == 0xffffffffu;
+            if (wild && (vis[x] & uint32_t(wild >> 32))) l_run[x] = NAN;
         }
         const bool full = __all(every);
         // ---- scores ----
@@ -445,34 +440,25 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                 for (int c = 0; c < 4; ++c) acc[x][c] *= al;
             }
         }
-        float wt[NT][8];
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
+        // the weights of a tile, e vs, and their sum without vs
+        auto weigh = [&](int x, float (&wt)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                wt[x][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][j], cf[x], -mu[x]));
-                if (full) {
-                    l_run[x] += wt[x][j];
-                    wt[x][j] *= vs[j >> 2][j & 3];
-                }
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][j], cf[x], -mu[x]));
+                l_run[x] += e;
+                wt[j] = e * vs[j >> 2][j & 3];
             }
-            if (!full) {
-                // where the column does not look there may be anything, a NaN scale too
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool see = vis[x] >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u;
-                    l_run[x] += see ? wt[x][j] : 0.0f;
-                    wt[x][j] = see ? wt[x][j] * vs[j >> 2][j & 3] : 0.0f;
-                }
-            }
-        }
+        };
         // ---- values ----
         if (!small) {
             uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+            for (int x = 0; x < NT; ++x) {
+                float wt[8];
+                weigh(x, wt);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split2(wt[x][2 * j], wt[x][2 * j + 1], ph[x][j], pl[x][j]);
+                for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[x][j], pl[x][j]);
+            }
             uint32_t u[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
@@ -493,24 +479,18 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             column(std::integral_constant<int, 2>{});
             column(std::integral_constant<int, 3>{});
         } else {
+            float wt[NT][8];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                uint32_t pp[3][4];
+            for (int x = 0; x < NT; ++x) weigh(x, wt[x]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split3(wt[x][2 * j] * 0x1p-9f, wt[x][2 * j + 1] * 0x1p-9f, pp[0][j], pp[1][j], pp[2][j]);
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t vp[4];
+                    const float vc = i8_at(vr[j], c) * 0x1p-9f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) vp[j] = pack_hi(i8_at(vr[2 * j], c), i8_at(vr[2 * j + 1], c));
-#pragma unroll
-                    for (int pc = 2; pc >= 0; --pc)
-                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            vec4<bf16x8_t>(vp[0], vp[1], vp[2], vp[3]),
-                            vec4<bf16x8_t>(pp[pc][0], pp[pc][1], pp[pc][2], pp[pc][3]), acc[x][c], 0, 0, 0);
+                    for (int x = 0; x < NT; ++x)
+                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vc, wt[x][j], acc[x][c], 0, 0, 0);
                 }
-            }
         }
         load_v();  // lands during the next scores
     }
