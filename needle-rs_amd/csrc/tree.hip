@@ -18,7 +18,7 @@
 //   values  O^T[v][col] = V^T P^T: a score tile's result layout is the layout
 //           of the weights the product needs.  MFMA c takes V columns 4 n + c,
 //           a dword a position.  The weights e vs are two f16 pieces, of which
-//           the first 22 bits are kept (and none below 2^-38 of the largest V
+//           the first 22 bits are kept (and none below 2^-34 of the largest V
 //           scale met so far), V's codes are exact in f16.  A chunk with a V
 //           scale 2^-9 or less of that largest takes the fp32 matrix product
 //           instead, all 24 bits at any size: the values of one position may be
@@ -110,7 +110,6 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     constexpr int SL = QK / 4, KD = SL / 4;    // a lane's slice of a K row; its dwords (3 or 4)
     constexpr int COLS = 16 * NT, LD = VD + 4, HN = NW / 2;
     __shared__ __align__(16) float sc_s[NW][64];
-    __shared__ uint32_t mw[COLS][kMaxNodes / 32 + 1];
     __shared__ __align__(16) float mo[HN][COLS][LD];
     __shared__ float mm[HN][COLS], ml[HN][COLS];
 
@@ -122,12 +121,6 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     const int split = unit % tr.splits, group = unit / tr.splits;
     const int kvh = group % g.KVH, ses = group / g.KVH;
     const int R = g.H / g.KVH;
-    const int base = tr.base[ses], len0 = tr.length ? tr.length[ses] : tr.nodes;
-    const bool there = len0 >= 0 && len0 <= tr.nodes;
-    const bool wrong = !there || base < 0 || base > 0x7fffffff - kMaxNodes;
-    const int len = there ? len0 : tr.nodes;
-    const int ncols = len * R;
-    if (tile * COLS >= ncols) return;
     const uint8_t *blk = tr.kv + size_t(ses) * tr.kv_stride;
     const int8_t *kb = reinterpret_cast<const int8_t *>(blk) + size_t(kvh) * g.cap * QK;
     const int8_t *vb = reinterpret_cast<const int8_t *>(blk + g.v_off) + size_t(kvh) * g.cap * VD;
@@ -139,14 +132,28 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     // integer (R <= 8)
     const float inv_r = 1.0f / float(R);
     auto node_of = [&](int f) { return int((float(f) + 0.5f) * inv_r); };
-    for (int i = t; i < COLS * tr.words; i += NW * 64) {
-        const int col = i / tr.words, word = i - col * tr.words;
-        const int node = node_of(min(tile * COLS + col, ncols - 1));
-        mw[col][word] = tr.mask[(size_t(ses) * tr.nodes + node) * tr.words + word];
-    }
 
-    // ---- the wave's columns: windows and query operands ----
-    uint32_t lo[NT];                      // first committed position; 0xffffffff: none is read at all
+    // ---- the wave's columns: windows and query operands, asked for before the
+    // session's numbers are there (rows behind the tree's end are memory too) ----
+    float v[NT][SL];
+    int first[NT];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int f = min(tile * COLS + 16 * x + n, tr.nodes * R - 1);
+        const int node = node_of(f), head = kvh * R + f - node * R;
+        const size_t row = size_t(ses) * tr.nodes + node;
+        const float *qh = tr.q + (row * g.H + head) * QK + qd * SL;
+#pragma unroll
+        for (int e = 0; e < SL; ++e) v[x][e] = qh[e];
+        first[x] = tr.lo[row];
+    }
+    const int base = tr.base[ses], len0 = tr.length ? tr.length[ses] : tr.nodes;
+    const bool there = len0 >= 0 && len0 <= tr.nodes;
+    const bool wrong = !there || base < 0 || base > 0x7fffffff - kMaxNodes;
+    const int len = there ? len0 : tr.nodes;
+    const int ncols = len * R;
+    if (tile * COLS >= ncols) return;
+    uint32_t lo[NT];                      // first committed position
     float cf[NT];                         // factor of a score, in bits
     intx4_t qi[NT];                       // QQ: codes
     uint32_t qp[NT][2][KD == 3 ? 6 : 8];  // else: f16 pieces
@@ -154,24 +161,19 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     bool bad[NT];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-        const int f = min(tile * COLS + 16 * x + n, ncols - 1);  // past the end: a copy, not written
-        const int node = node_of(f), head = kvh * R + f - node * R;
-        const size_t row = size_t(ses) * tr.nodes + node;
-        const int l0 = tr.lo[row];
+        const int l0 = first[x];
         bad[x] = wrong || l0 < 0 || base - min(l0, base) + len > g.cap;
-        lo[x] = bad[x] ? 0xffffffffu : uint32_t(l0);
-        ulo = min(ulo, lo[x]);
-        const float *qh = tr.q + (row * g.H + head) * QK + qd * SL;
-        float v[SL];
-#pragma unroll
-        for (int e = 0; e < SL; ++e) v[e] = qh[e];
+        // these and columns past the end walk along whatever the others read
+        const bool along = bad[x] || tile * COLS + 16 * x + n >= ncols;
+        lo[x] = along ? 0u : uint32_t(l0);
+        ulo = along ? ulo : min(ulo, lo[x]);
         if (tr.negative) {
 #pragma unroll
-            for (int e = 0; e < SL; ++e) v[e] = -v[e];
+            for (int e = 0; e < SL; ++e) v[x][e] = -v[x][e];
         }
         float a = 0.0f;
 #pragma unroll
-        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1]));
+        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[x][e]), __builtin_fabsf(v[x][e + 1]));
         a = fmaxf(a, ndl::wave_xor<16>(a));
         a = fmaxf(a, ndl::wave_xor<32>(a));
         float nan = 0.0f;
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             for (int e = 0; e < SL; ++e) {
                 // quant_code: half away from zero is truncation after adding
                 // the float below a half, for every |y| < 2^22
-                const float y = v[e] * inv;
+                const float y = v[x][e] * inv;
                 const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
                 nan = y != y ? y : nan;
                 dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
@@ -196,11 +198,11 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             const int sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
 #pragma unroll
             for (int e = 0; e < SL; ++e) {
-                nan = v[e] - v[e] != 0.0f ? NAN : nan;
-                v[e] = __builtin_amdgcn_ldexpf(v[e], sh);
+                nan = v[x][e] - v[x][e] != 0.0f ? NAN : nan;
+                v[x][e] = __builtin_amdgcn_ldexpf(v[x][e], sh);
             }
 #pragma unroll
-            for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[x][0][e / 2], qp[x][1][e / 2]);
+            for (int e = 0; e < SL; e += 2) split2(v[x][e], v[x][e + 1], qp[x][0][e / 2], qp[x][1][e / 2]);
             cf[x] = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
         }
         // (a factor of 0 would make no number of a score of -inf)
@@ -215,10 +217,9 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     ulo = min(ulo, uint32_t(ndl::wave_xor_int<4>(int(ulo))));
     ulo = min(ulo, uint32_t(ndl::wave_xor_int<8>(int(ulo))));
     ulo = __builtin_amdgcn_readfirstlane(ulo);
-    bool live = false;
+    bool live = false;  // (a column past the end may be; its walk is empty)
 #pragma unroll
     for (int x = 0; x < NT; ++x) live = live || !bad[x];
-    __syncthreads();  // the mask words
 
     // ---- the walk: chunk i is committed positions ulo + 32 i .., then nodes ----
     const uint32_t before = uint32_t(base) - ulo;
@@ -244,9 +245,16 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         const uint32_t p = s0 + min(o, uint32_t(max(valid, 1) - 1));
         return p >= cap ? p - cap : p;
     };
-    uint32_t kr[2][KD], vr[8];
+    uint32_t kr[2][KD], vr[8], word[NT];
     float scr = 0.0f;
-    auto load_k = [&]() {
+    auto load_k = [&](int i) {
+        if (i >= np && i < nch) {
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                const int node = node_of(min(tile * COLS + 16 * x + n, ncols - 1));
+                word[x] = tr.mask[(size_t(ses) * tr.nodes + node) * tr.words + (i - np)];
+            }
+        }
         if (s0 + 32u <= cap) {
             const int8_t *p = kb + size_t(s0) * QK;
 #pragma unroll
@@ -279,26 +287,33 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         }
     };
     // loads are never conditional: past the last chunk they read some slot
+#pragma unroll
+    for (int x = 0; x < NT; ++x) word[x] = 0;
     place(ch);
-    load_k();
+    load_k(ch);
     load_v();
 
-    float m_run[NT], mu[NT], l_run[NT];
+    // m_run: a score of the column, no other so far is more than kAhead bits
+    // above it (lim, in the scores' units); mu = m_run cf.  A new maximum is
+    // taken, and the sums scaled, only where one gets ahead of that
+    constexpr float kAhead = 5.0f;
+    float m_run[NT], lim[NT], mu[NT], l_run[NT];
     floatx4_t acc[NT][4];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
         m_run[x] = -INFINITY;
+        lim[x] = -INFINITY;
         mu[x] = 0.0f;
         l_run[x] = 0.0f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[x][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // K and V scales are taken in units of 2^kexp and 2^(vexp - 14), powers of
+    // K and V scales are taken in units of 2^kexp and 2^(vexp - 10), powers of
     // two that no finite one so far is above: scores before cf, and weights,
     // stay in range at any size of the cache's values
     int kexp = 0, vexp = 0;
     float top = 0.0f;                   // lanes below 32: 2^kexp, the others: 2^vexp
-    int shift = lane < 32 ? 0 : 14;
+    int shift = lane < 32 ? 0 : 10;
 
     for (; ch < nch; ch += step) {
         // ---- the chunk's scales, zero behind its end ----
@@ -320,6 +335,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                 m_run[x] = __builtin_amdgcn_ldexpf(m_run[x], kexp - kn);
                 cf[x] = __builtin_amdgcn_ldexpf(cf[x], kn - kexp);
                 if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
+                lim[x] = m_run[x] == -INFINITY ? -INFINITY : m_run[x] + kAhead * __builtin_amdgcn_rcpf(cf[x]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -333,7 +349,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         // it, and only of those: a weight of 0 there would not stay 0
         const uint64_t wild = __ballot(lane >= 32 && !(__builtin_fabsf(sc) < INFINITY));
         if (wild) sc = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY) ? 0.0f : sc;
-        const bool small = __any(lane >= 32 && (lane & 31) < valid && sc < 32.0f);
+        const bool small = __any(lane >= 32 && (lane & 31) < valid && sc < 2.0f);
         sc_s[w][lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -354,7 +370,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                 const uint32_t p0 = ulo + 32u * uint32_t(ch);
                 vis[x] = lo[x] <= p0 ? some : lo[x] - p0 < 32u ? some & (0xffffffffu << (lo[x] - p0)) : 0u;
             } else {
-                vis[x] = bad[x] ? 0u : mw[16 * x + n][ch - np] & some;
+                vis[x] = word[x] & some;
             }
             every = every && vis[x] == 0xffffffffu;
             if (wild && (vis[x] & uint32_t(wild >> 32))) l_run[x] = NAN;
@@ -405,7 +421,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             }
         }
         place(ch + step);
-        load_k();  // lands during the softmax and the values
+        load_k(ch + step);  // lands during the softmax and the values
         // ---- softmax: each lane its column's eight positions ----
         if (!full) {
 #pragma unroll
@@ -414,26 +430,23 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                 for (int j = 0; j < 8; ++j)
                     if (!(vis[x] >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u)) s[x][j] = -INFINITY;
         }
-        bool grew = false;
-        float m_new[NT];
+        bool ahead = false;
+        float m8[NT];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            const float m8 = max3(max3(s[x][0], s[x][1], s[x][2]), max3(s[x][3], s[x][4], s[x][5]),
-                                  max3(s[x][6], s[x][7], m_run[x]));
-            // over the four lane quarters: each swap returns the pair
-            const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(m8), __float_as_uint(m8), false, false);
-            const float m16 = max3(__uint_as_float(s16[0]), __uint_as_float(s16[1]), m8);
-            const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(m16), __float_as_uint(m16), false, false);
-            m_new[x] = max3(__uint_as_float(s32[0]), __uint_as_float(s32[1]), m16);
-            grew = grew || m_new[x] > m_run[x];
+            m8[x] = max3(max3(s[x][0], s[x][1], s[x][2]), max3(s[x][3], s[x][4], s[x][5]), max3(s[x][6], s[x][7], s[x][7]));
+            ahead = ahead || m8[x] > lim[x];
         }
-        if (__any(grew)) {
+        if (__any(ahead)) {
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                const float mu_new = m_new[x] == -INFINITY ? 0.0f : m_new[x] * cf[x];
+                float m = max3(m8[x], m_run[x], ndl::wave_xor<16>(m8[x]));
+                m = fmaxf(m, ndl::wave_xor<32>(m));
+                const float mu_new = m == -INFINITY ? 0.0f : m * cf[x];
                 // nothing is summed yet where there was no maximum
                 const float al = m_run[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu[x] - mu_new);
-                m_run[x] = m_new[x];
+                m_run[x] = m;
+                lim[x] = m == -INFINITY ? -INFINITY : m + kAhead * __builtin_amdgcn_rcpf(cf[x]);
                 mu[x] = mu_new;
                 l_run[x] *= al;
 #pragma unroll
@@ -503,7 +516,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - 5);
+            for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - 1);
         // from here on the maximum is in bits
         m_run[x] = m_run[x] == -INFINITY ? -INFINITY : mu[x];
     }
