@@ -35,7 +35,7 @@ namespace {
 using namespace ndkv;
 
 constexpr int kMaxNodes = 256;
-constexpr int VD = 64;
+constexpr int VD = 64, kCols = 16;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -98,6 +98,24 @@ __device__ inline uint32_t f16_pair(uint32_t x)
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u) + a);
 }
 
+// Loads from a head's rows or scales: past the end (a chunk that is not full,
+// at the ring's end) they give zeros.
+typedef __amdgpu_buffer_rsrc_t rows_t;
+
+__device__ inline rows_t rows_at(const void *p, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, int(bytes), 0x00027000);
+}
+
+// x as it is: what is added to it afterwards goes into the loads' own offsets.
+__device__ inline uint32_t here(uint32_t x)
+{
+    asm("" : "+v"(x));
+    return x;
+}
+
+__device__ inline bool any_of(bool b) { return __builtin_amdgcn_ballot_w64(b) != 0; }
+
 template <typename T>
 __device__ inline T vec4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
@@ -122,10 +140,11 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     const int kvh = group % g.KVH, ses = group / g.KVH;
     const int R = g.H / g.KVH;
     const uint8_t *blk = tr.kv + size_t(ses) * tr.kv_stride;
-    const int8_t *kb = reinterpret_cast<const int8_t *>(blk) + size_t(kvh) * g.cap * QK;
-    const int8_t *vb = reinterpret_cast<const int8_t *>(blk + g.v_off) + size_t(kvh) * g.cap * VD;
-    const float *ksb = reinterpret_cast<const float *>(blk + g.ks_off) + size_t(kvh) * g.cap;
-    const float *vsb = reinterpret_cast<const float *>(blk + g.vs_off) + size_t(kvh) * g.cap;
+    const rows_t kb = rows_at(blk + size_t(kvh) * g.cap * QK, uint32_t(g.cap) * QK);
+    const rows_t vb = rows_at(blk + g.v_off + size_t(kvh) * g.cap * VD, uint32_t(g.cap) * VD);
+    // K scales, and vs_off - ks_off bytes on (below 2^32: KVH cap 4) the V scales
+    const uint32_t to_vs = uint32_t(g.vs_off - g.ks_off);
+    const rows_t sb = rows_at(blk + g.ks_off + size_t(kvh) * g.cap * 4, to_vs + uint32_t(g.cap) * 4);
     const uint32_t cap = uint32_t(g.cap);
 
     // f / R of a column f < 2^11: (f + 1/2) / R is 1/16 or more away from an
@@ -157,7 +176,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     float cf[NT];                         // factor of a score, in bits
     intx4_t qi[NT];                       // QQ: codes
     uint32_t qp[NT][2][KD == 3 ? 6 : 8];  // else: f16 pieces
-    uint32_t ulo = uint32_t(base);
+    uint32_t ulo = uint32_t(base), tlo = 0;
     bool bad[NT];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -167,6 +186,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         const bool along = bad[x] || tile * COLS + 16 * x + n >= ncols;
         lo[x] = along ? 0u : uint32_t(l0);
         ulo = along ? ulo : min(ulo, lo[x]);
+        tlo = max(tlo, lo[x]);
         if (tr.negative) {
 #pragma unroll
             for (int e = 0; e < SL; ++e) v[x][e] = -v[x][e];
@@ -212,85 +232,87 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         nan += ndl::wave_xor<32>(nan);
         cf[x] += nan;
     }
-    ulo = min(ulo, uint32_t(ndl::wave_xor_int<1>(int(ulo))));
-    ulo = min(ulo, uint32_t(ndl::wave_xor_int<2>(int(ulo))));
-    ulo = min(ulo, uint32_t(ndl::wave_xor_int<4>(int(ulo))));
-    ulo = min(ulo, uint32_t(ndl::wave_xor_int<8>(int(ulo))));
+    // the first position that some column reads, and the first that all do
+    auto both = [&](auto step) {
+        constexpr int D = decltype(step)::value;
+        ulo = min(ulo, uint32_t(ndl::wave_xor_int<D>(int(ulo))));
+        tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
+    };
+    both(std::integral_constant<int, 1>{});
+    both(std::integral_constant<int, 2>{});
+    both(std::integral_constant<int, 4>{});
+    both(std::integral_constant<int, 8>{});
     ulo = __builtin_amdgcn_readfirstlane(ulo);
+    tlo = __builtin_amdgcn_readfirstlane(tlo);
     bool live = false;  // (a column past the end may be; its walk is empty)
 #pragma unroll
     for (int x = 0; x < NT; ++x) live = live || !bad[x];
 
-    // ---- the walk: chunk i is committed positions ulo + 32 i .., then nodes ----
-    const uint32_t before = uint32_t(base) - ulo;
-    const int np = __any(live) ? int((before + 31u) / 32u) : 0;
-    const int nch = __any(live) ? np + (len + 31) / 32 : 0;
+    // ---- the walk: committed positions up to the ring's end, from its start,
+    // then the tree's nodes likewise, each in chunks of 32 (the last ones of a
+    // part shorter).  A walk is no longer than the ring, so it wraps once ----
+    const uint32_t before = uint32_t(base) - ulo, slo = ulo % cap;
+    const uint32_t n0 = min(before, cap - slo), n1 = before - n0;
+    const uint32_t s2 = slo + before >= cap ? slo + before - cap : slo + before;
+    const uint32_t n2 = min(uint32_t(len), cap - s2), n3 = uint32_t(len) - n2;
+    const int e0 = int((n0 + 31) / 32), e1 = e0 + int((n1 + 31) / 32), e2 = e1 + int((n2 + 31) / 32);
+    const int nch = any_of(live) ? e2 + int((n3 + 31) / 32) : 0;
     const int step = tr.splits * NW;
     int ch = split * NW + w;
-    const uint32_t slo = ulo % cap;
-    uint32_t s0 = 0;
-    int valid = 0;  // positions of the chunk
-    auto place = [&](int i) {
-        const int c = i - np;
-        const uint32_t off = c < 0 ? 32u * uint32_t(i) : before + 32u * uint32_t(c);
-        valid = i >= nch ? 0 : c < 0 ? int(min(32u, before - off)) : min(32, len - 32 * c);
-        // a walk is no longer than the ring: positions wrap at most once
-        s0 = slo + off;
-        if (s0 >= cap) s0 -= cap;
-        if (i >= nch) s0 = 0;  // past the end: any slot
-    };
-    // a chunk inside the ring: scalar base, lane offsets; across its end (or in
-    // a ring below a chunk): each position's slot, the last one's behind it
-    auto slot_of = [&](uint32_t o) {
-        const uint32_t p = s0 + min(o, uint32_t(max(valid, 1) - 1));
-        return p >= cap ? p - cap : p;
+    uint32_t s0 = 0;   // the chunk's first slot,
+    uint32_t p0 = 0;   // position or node,
+    int valid = 0;     // and length; 0 behind the last chunk
+    bool tail = false;
+    auto place = [=, &s0, &p0, &valid, &tail](int i) {
+        const int c = i >= e2 ? i - e2 : i >= e1 ? i - e1 : i >= e0 ? i - e0 : i;
+        const uint32_t off = 32u * uint32_t(c);
+        const uint32_t cnt = i >= nch ? off : i >= e2 ? n3 : i >= e1 ? n2 : i >= e0 ? n1 : n0;
+        tail = i >= e1;
+        s0 = (i >= e2 ? 0u : i >= e1 ? s2 : i >= e0 ? 0u : slo) + off;
+        p0 = (i >= e2 ? n2 : i >= e1 ? 0u : i >= e0 ? ulo + n0 : ulo) + off;
+        valid = int(min(32u, cnt - off));
     };
     uint32_t kr[2][KD], vr[8], word[NT];
     float scr = 0.0f;
-    auto load_k = [&](int i) {
-        if (i >= np && i < nch) {
+    const uint32_t kl = uint32_t(n * QK + qd * SL), vl = uint32_t(4 * qd * VD + 4 * n);
+    const uint32_t scl = (lane & 31) * 4 + (lane < 32 ? 0u : to_vs);
+    auto load_k = [&]() {
+        if (tail && valid) {
+            // bits p0 .. p0 + 31 of the node's mask
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 const int node = node_of(min(tile * COLS + 16 * x + n, ncols - 1));
-                word[x] = tr.mask[(size_t(ses) * tr.nodes + node) * tr.words + (i - np)];
+                const uint32_t *m = tr.mask + (size_t(ses) * tr.nodes + node) * tr.words + (p0 >> 5);
+                word[x] = m[0] >> (p0 & 31u);
+                if ((p0 & 31u) && int(p0 >> 5) + 1 < tr.words) word[x] |= m[1] << (32u - (p0 & 31u));
             }
         }
-        if (s0 + 32u <= cap) {
-            const int8_t *p = kb + size_t(s0) * QK;
+        const uint32_t o = here(kl + s0 * QK);
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+        for (int a = 0; a < 2; ++a) {
+            if constexpr (KD == 3) {
+                const auto r = __builtin_amdgcn_raw_buffer_load_b96(kb, o + 16 * a * QK, 0, 0);
 #pragma unroll
-                for (int d = 0; d < KD; ++d)
-                    kr[a][d] = *reinterpret_cast<const uint32_t *>(p + (n * QK + qd * SL) + (16 * a * QK + 4 * d));
-            scr = *(lane < 32 ? ksb + s0 + lane : vsb + s0 + (lane - 32));
-        } else {
+                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+            } else {
+                const auto r = __builtin_amdgcn_raw_buffer_load_b128(kb, o + 16 * a * QK, 0, 0);
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const uint32_t o = slot_of(16 * a + n) * QK + qd * SL;  // below 2^24 64
-#pragma unroll
-                for (int d = 0; d < KD; ++d) kr[a][d] = *reinterpret_cast<const uint32_t *>(kb + o + 4 * d);
+                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
             }
-            scr = (lane < 32 ? ksb : vsb)[slot_of(lane & 31)];
         }
+        scr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sb, scl + s0 * 4, 0, 0));
     };
     auto load_v = [&]() {
-        if (s0 + 32u <= cap) {
-            const int8_t *p = vb + size_t(s0) * VD;
+        const uint32_t o = here(vl + s0 * VD);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                vr[j] = *reinterpret_cast<const uint32_t *>(p + (4 * qd * VD + 4 * n) + (16 * (j >> 2) + (j & 3)) * VD);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                vr[j] = *reinterpret_cast<const uint32_t *>(
-                    vb + (slot_of(16 * (j >> 2) + 4 * qd + (j & 3)) * VD + 4 * n));
-        }
+        for (int j = 0; j < 8; ++j)
+            vr[j] = __builtin_amdgcn_raw_buffer_load_b32(vb, o + (16 * (j >> 2) + (j & 3)) * VD, 0, 0);
     };
     // loads are never conditional: past the last chunk they read some slot
 #pragma unroll
     for (int x = 0; x < NT; ++x) word[x] = 0;
     place(ch);
-    load_k(ch);
+    load_k();
     load_v();
 
     // m_run: a score of the column, no other so far is more than kAhead bits
@@ -316,9 +338,27 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     int shift = lane < 32 ? 0 : 10;
 
     for (; ch < nch; ch += step) {
+        // ---- the positions each column sees ----
+        const uint32_t some = valid < 32 ? (1u << valid) - 1u : 0xffffffffu;
+        uint32_t vis[NT];
+        bool full = false;
+        if (!tail && p0 >= tlo) {
+            full = valid == 32;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) vis[x] = some;
+        } else {
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+                vis[x] = some & (tail ? word[x] : lo[x] <= p0 ? 0xffffffffu : lo[x] - p0 < 32u ? 0xffffffffu << (lo[x] - p0) : 0u);
+        }
         // ---- the chunk's scales, zero behind its end ----
         float sc = (lane & 31) < valid ? scr : 0.0f;
-        if (__any(sc > top)) {
+        if (any_of(!(sc <= top))) {
+            // a V scale that is no number makes no number of the columns that see
+            // it, and only of those: a weight of 0 there would not stay 0
+            const bool wild = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY);
+            const uint32_t wilds = uint32_t(__builtin_amdgcn_ballot_w64(wild) >> 32);
+            if (wild) sc = 0.0f;
             float h = sc < INFINITY ? fmaxf(sc, top) : top;
             h = fmaxf(h, ndl::wave_xor<16>(h));
             h = fmaxf(h, ndl::wave_xor<8>(h));
@@ -332,6 +372,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
+                if (vis[x] & wilds) l_run[x] = NAN;
                 m_run[x] = __builtin_amdgcn_ldexpf(m_run[x], kexp - kn);
                 cf[x] = __builtin_amdgcn_ldexpf(cf[x], kn - kexp);
                 if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
@@ -345,11 +386,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             vexp = vn;
         }
         sc = __builtin_amdgcn_ldexpf(sc, shift);
-        // a V scale that is no number makes no number of the columns that see
-        // it, and only of those: a weight of 0 there would not stay 0
-        const uint64_t wild = __ballot(lane >= 32 && !(__builtin_fabsf(sc) < INFINITY));
-        if (wild) sc = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY) ? 0.0f : sc;
-        const bool small = __any(lane >= 32 && (lane & 31) < valid && sc < 2.0f);
+        const bool small = (uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32) & some) != 0;
         sc_s[w][lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -360,22 +397,6 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             vs[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][32 + 16 * a + 4 * qd]);
         }
         __builtin_amdgcn_wave_barrier();
-        // ---- the positions each column sees ----
-        uint32_t vis[NT];
-        const uint32_t some = valid < 32 ? (1u << valid) - 1u : 0xffffffffu;
-        bool every = true;
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            if (ch < np) {
-                const uint32_t p0 = ulo + 32u * uint32_t(ch);
-                vis[x] = lo[x] <= p0 ? some : lo[x] - p0 < 32u ? some & (0xffffffffu << (lo[x] - p0)) : 0u;
-            } else {
-                vis[x] = word[x] & some;
-            }
-            every = every && vis[x] == 0xffffffffu;
-            if (wild && (vis[x] & uint32_t(wild >> 32))) l_run[x] = NAN;
-        }
-        const bool full = __all(every);
         // ---- scores ----
         float s[NT][8];
         if constexpr (QQ) {
@@ -421,7 +442,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             }
         }
         place(ch + step);
-        load_k(ch + step);  // lands during the softmax and the values
+        load_k();  // lands during the softmax and the values
         // ---- softmax: each lane its column's eight positions ----
         if (!full) {
 #pragma unroll
@@ -437,7 +458,7 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             m8[x] = max3(max3(s[x][0], s[x][1], s[x][2]), max3(s[x][3], s[x][4], s[x][5]), max3(s[x][6], s[x][7], s[x][7]));
             ahead = ahead || m8[x] > lim[x];
         }
-        if (__any(ahead)) {
+        if (any_of(ahead)) {
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 float m = max3(m8[x], m_run[x], ndl::wave_xor<16>(m8[x]));
@@ -605,7 +626,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(int H, Tree tr, size_t t
 }
 
 struct Plan {
-    int nt, nw;
+    int nw;
     size_t tiles, splits;
 };
 
@@ -616,11 +637,10 @@ Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
     const size_t groups = count * size_t(g->num_kv_heads);
     const size_t chunks = (size_t(g->cap) + 31) / 32 + (nodes + 31) / 32;
     Plan p;
-    p.nt = cols > 16 && groups * ((cols + 31) / 32) >= cus ? 2 : 1;
-    p.tiles = (cols + 16 * p.nt - 1) / (16 * p.nt);
+    p.tiles = (cols + kCols - 1) / kCols;
     const size_t blocks = groups * p.tiles;
-    p.nw = blocks * 4 >= cus * 16 ? 4 : 8;
-    const size_t fill = (cus * 8 + blocks * p.nw - 1) / (blocks * p.nw), most = (chunks + 2 * p.nw - 1) / (2 * p.nw);
+    p.nw = blocks * 8 < cus * 12 ? 8 : 4;
+    const size_t fill = cus * 8 / (blocks * p.nw), most = chunks / (3 * p.nw);
     p.splits = std::max<size_t>(1, std::min<size_t>(std::min(fill, most), 64));
     return p;
 }
@@ -628,7 +648,6 @@ Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
 template <int QK, bool QQ>
 auto kernel_of(const Plan &p)
 {
-    if (p.nt == 2) return p.nw == 4 ? tree_kernel<QK, QQ, 2, 4> : tree_kernel<QK, QQ, 2, 8>;
     return p.nw == 4 ? tree_kernel<QK, QQ, 1, 4> : tree_kernel<QK, QQ, 1, 8>;
 }
 
