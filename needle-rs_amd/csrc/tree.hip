@@ -3,7 +3,7 @@
 // mask names, whose keys and values lie in the same ring behind them.
 //
 // On the matrix cores.  The columns of a (session, kv head) are its (node,
-// query head) pairs: a wave owns 16 NT of them and walks chunks of 32
+// query head) pairs: a wave owns 16 of them and walks chunks of 32
 // positions with an online softmax; the waves of a block own the same columns
 // and take the chunks in turn, and meet in LDS at the end.  The committed
 // positions and the tree are chunked apart, so that a chunk of the tree is a
@@ -44,6 +44,14 @@ typedef float floatx4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef int intx4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
+// x / d for x, d with x d < 2^32, d > 0: 2^32 / d rounded up is above it by less
+// than one, times x / 2^32 by less than 1 / d.
+struct Divisor {
+    uint32_t up;  // 0 for d = 1
+    __host__ static Divisor of(uint32_t d) { return Divisor{uint32_t(((uint64_t(1) << 32) + d - 1) / d)}; }
+    __device__ uint32_t quotient(uint32_t x) const { return up ? __umulhi(x, up) : x; }
+};
+
 struct Tree {
     const uint8_t *kv;
     size_t kv_stride;
@@ -51,7 +59,9 @@ struct Tree {
     const uint32_t *mask;
     const float *q;
     float *out, *part_o, *part_ml;
-    int nodes, words, units, tiles, splits;
+    int nodes, words, splits, rep;
+    uint32_t units;
+    Divisor by_splits, by_kvh;
     float scale2;  // |scale| log2(e)
     int negative;  // scale < 0
 };
@@ -122,23 +132,46 @@ __device__ inline T vec4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
     return __builtin_bit_cast(T, u32x4_t{a, b, c, d});
 }
 
-template <int QK, bool QQ, int NT, int NW>
-__global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, Tree tr)
+template <int QK, bool QQ, int NW>
+__global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
 {
-    constexpr int SL = QK / 4, KD = SL / 4;    // a lane's slice of a K row; its dwords (3 or 4)
-    constexpr int COLS = 16 * NT, LD = VD + 4, HN = NW / 2;
+    constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
+    constexpr int LD = VD + 4, HN = NW / 2;
     __shared__ __align__(16) float sc_s[NW][64];
-    __shared__ __align__(16) float mo[HN][COLS][LD];
-    __shared__ float mm[HN][COLS], ml[HN][COLS];
+    __shared__ __align__(16) float mo[HN][kCols][LD];
+    __shared__ float mm[HN][kCols], ml[HN][kCols];
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
     // blocks 8 apart share an XCD's L2: there a unit's column tiles follow each other
-    const int unit = int(blockIdx.x >> 3) / tr.tiles * 8 + int(blockIdx.x & 7), tile = int(blockIdx.x >> 3) % tr.tiles;
+    const uint32_t unit = blockIdx.z * 8 + blockIdx.x, tile = blockIdx.y;
     if (unit >= tr.units) return;
-    const int split = unit % tr.splits, group = unit / tr.splits;
-    const int kvh = group % g.KVH, ses = group / g.KVH;
-    const int R = g.H / g.KVH;
+    const uint32_t group = tr.by_splits.quotient(unit), split = unit - group * tr.splits;
+    const uint32_t ses = tr.by_kvh.quotient(group), kvh = group - ses * uint32_t(g.KVH);
+    const int R = tr.rep;
+
+    // ---- the wave's columns: window and query operand, asked for before the
+    // session's numbers are there (rows behind the tree's end are memory too).
+    // f / R of a column f < 2^11: (f + 1/2) / R is 1/16 or more away from an
+    // integer (R <= 8) ----
+    const float inv_r = 1.0f / float(R);
+    auto node_of = [&](int f) { return int((float(f) + 0.5f) * inv_r); };
+    const int f = min(int(tile) * kCols + n, tr.nodes * R - 1);
+    const int node = node_of(f), head = int(kvh) * R + f - node * R;
+    const size_t row = size_t(ses) * tr.nodes + node;
+    float v[SL];
+    {
+        const float *qh = tr.q + (row * g.H + head) * QK + qd * SL;
+#pragma unroll
+        for (int e = 0; e < SL; ++e) v[e] = qh[e];
+    }
+    const int l0 = tr.lo[row];
+    const int base = tr.base[ses], len0 = tr.length ? tr.length[ses] : tr.nodes;
+    const bool there = len0 >= 0 && len0 <= tr.nodes;
+    const bool wrong = !there || base < 0 || base > 0x7fffffff - kMaxNodes;
+    const int len = there ? len0 : tr.nodes;
+    const int ncols = len * R;
+    if (int(tile) * kCols >= ncols) return;
     const uint8_t *blk = tr.kv + size_t(ses) * tr.kv_stride;
     const rows_t kb = rows_at(blk + size_t(kvh) * g.cap * QK, uint32_t(g.cap) * QK);
     const rows_t vb = rows_at(blk + g.v_off + size_t(kvh) * g.cap * VD, uint32_t(g.cap) * VD);
@@ -147,94 +180,14 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     const rows_t sb = rows_at(blk + g.ks_off + size_t(kvh) * g.cap * 4, to_vs + uint32_t(g.cap) * 4);
     const uint32_t cap = uint32_t(g.cap);
 
-    // f / R of a column f < 2^11: (f + 1/2) / R is 1/16 or more away from an
-    // integer (R <= 8)
-    const float inv_r = 1.0f / float(R);
-    auto node_of = [&](int f) { return int((float(f) + 0.5f) * inv_r); };
-
-    // ---- the wave's columns: windows and query operands, asked for before the
-    // session's numbers are there (rows behind the tree's end are memory too) ----
-    float v[NT][SL];
-    int first[NT];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        const int f = min(tile * COLS + 16 * x + n, tr.nodes * R - 1);
-        const int node = node_of(f), head = kvh * R + f - node * R;
-        const size_t row = size_t(ses) * tr.nodes + node;
-        const float *qh = tr.q + (row * g.H + head) * QK + qd * SL;
-#pragma unroll
-        for (int e = 0; e < SL; ++e) v[x][e] = qh[e];
-        first[x] = tr.lo[row];
-    }
-    const int base = tr.base[ses], len0 = tr.length ? tr.length[ses] : tr.nodes;
-    const bool there = len0 >= 0 && len0 <= tr.nodes;
-    const bool wrong = !there || base < 0 || base > 0x7fffffff - kMaxNodes;
-    const int len = there ? len0 : tr.nodes;
-    const int ncols = len * R;
-    if (tile * COLS >= ncols) return;
-    uint32_t lo[NT];                      // first committed position
-    float cf[NT];                         // factor of a score, in bits
-    intx4_t qi[NT];                       // QQ: codes
-    uint32_t qp[NT][2][KD == 3 ? 6 : 8];  // else: f16 pieces
-    uint32_t ulo = uint32_t(base), tlo = 0;
-    bool bad[NT];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        const int l0 = first[x];
-        bad[x] = wrong || l0 < 0 || base - min(l0, base) + len > g.cap;
-        // these and columns past the end walk along whatever the others read
-        const bool along = bad[x] || tile * COLS + 16 * x + n >= ncols;
-        lo[x] = along ? 0u : uint32_t(l0);
-        ulo = along ? ulo : min(ulo, lo[x]);
-        tlo = max(tlo, lo[x]);
-        if (tr.negative) {
-#pragma unroll
-            for (int e = 0; e < SL; ++e) v[x][e] = -v[x][e];
-        }
-        float a = 0.0f;
-#pragma unroll
-        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[x][e]), __builtin_fabsf(v[x][e + 1]));
-        a = fmaxf(a, ndl::wave_xor<16>(a));
-        a = fmaxf(a, ndl::wave_xor<32>(a));
-        float nan = 0.0f;
-        if constexpr (QQ) {
-            // quant_rows (model.rs:289-293): the codes and the head's scale
-            const float qs = a > 0.0f ? a / 127.0f : 1.0f;
-            const float inv = 1.0f / qs;
-            uint32_t dw[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < SL; ++e) {
-                // quant_code: half away from zero is truncation after adding
-                // the float below a half, for every |y| < 2^22
-                const float y = v[x][e] * inv;
-                const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
-                nan = y != y ? y : nan;
-                dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
-            }
-            qi[x] = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
-            cf[x] = qs * tr.scale2;
-        } else {
-            // the head in 2^14 .. 2^15, so that the second pieces are normal numbers
-            const int sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
-#pragma unroll
-            for (int e = 0; e < SL; ++e) {
-                nan = v[x][e] - v[x][e] != 0.0f ? NAN : nan;
-                v[x][e] = __builtin_amdgcn_ldexpf(v[x][e], sh);
-            }
-#pragma unroll
-            for (int e = 0; e < SL; e += 2) split2(v[x][e], v[x][e + 1], qp[x][0][e / 2], qp[x][1][e / 2]);
-            cf[x] = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
-        }
-        // (a factor of 0 would make no number of a score of -inf)
-        if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
-        // NaN where the query has one (an infinity gives one too)
-        nan += ndl::wave_xor<16>(nan);
-        nan += ndl::wave_xor<32>(nan);
-        cf[x] += nan;
-    }
+    const bool bad = wrong || l0 < 0 || base - min(l0, base) + len > g.cap;
+    // these and columns past the end walk along whatever the others read
+    const bool along = bad || int(tile) * kCols + n >= ncols;
+    const uint32_t lo = along ? 0u : uint32_t(l0);  // first committed position
     // the first position that some column reads, and the first that all do
-    auto both = [&](auto step) {
-        constexpr int D = decltype(step)::value;
+    uint32_t ulo = along ? uint32_t(base) : min(uint32_t(base), lo), tlo = lo;
+    auto both = [&](auto distance) {
+        constexpr int D = decltype(distance)::value;
         ulo = min(ulo, uint32_t(ndl::wave_xor_int<D>(int(ulo))));
         tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
     };
@@ -244,9 +197,6 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     both(std::integral_constant<int, 8>{});
     ulo = __builtin_amdgcn_readfirstlane(ulo);
     tlo = __builtin_amdgcn_readfirstlane(tlo);
-    bool live = false;  // (a column past the end may be; its walk is empty)
-#pragma unroll
-    for (int x = 0; x < NT; ++x) live = live || !bad[x];
 
     // ---- the walk: committed positions up to the ring's end, from its start,
     // then the tree's nodes likewise, each in chunks of 32 (the last ones of a
@@ -256,36 +206,36 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
     const uint32_t s2 = slo + before >= cap ? slo + before - cap : slo + before;
     const uint32_t n2 = min(uint32_t(len), cap - s2), n3 = uint32_t(len) - n2;
     const int e0 = int((n0 + 31) / 32), e1 = e0 + int((n1 + 31) / 32), e2 = e1 + int((n2 + 31) / 32);
-    const int nch = any_of(live) ? e2 + int((n3 + 31) / 32) : 0;
+    // (a column past the end may be no bad one where all others are; its walk is empty)
+    const int nch = any_of(!bad) ? e2 + int((n3 + 31) / 32) : 0;
     const int step = tr.splits * NW;
-    int ch = split * NW + w;
+    int ch = int(split) * NW + w;
     uint32_t s0 = 0;   // the chunk's first slot,
     uint32_t p0 = 0;   // position or node,
-    int valid = 0;     // and length; 0 behind the last chunk
+    int left = 0;      // positions from there to the part's end; 0 behind the last chunk
+    int stop = 0;      // the part's last chunk, and one
     bool tail = false;
-    auto place = [=, &s0, &p0, &valid, &tail](int i) {
-        const int c = i >= e2 ? i - e2 : i >= e1 ? i - e1 : i >= e0 ? i - e0 : i;
-        const uint32_t off = 32u * uint32_t(c);
-        const uint32_t cnt = i >= nch ? off : i >= e2 ? n3 : i >= e1 ? n2 : i >= e0 ? n1 : n0;
+    auto place = [=, &s0, &p0, &left, &stop, &tail](int i) {
+        const uint32_t off = 32u * uint32_t(i >= e2 ? i - e2 : i >= e1 ? i - e1 : i >= e0 ? i - e0 : i);
+        const uint32_t cnt = i >= e2 ? n3 : i >= e1 ? n2 : i >= e0 ? n1 : n0;
         tail = i >= e1;
-        s0 = (i >= e2 ? 0u : i >= e1 ? s2 : i >= e0 ? 0u : slo) + off;
+        s0 = i >= nch ? 0u : (i >= e2 ? 0u : i >= e1 ? s2 : i >= e0 ? 0u : slo) + off;
         p0 = (i >= e2 ? n2 : i >= e1 ? 0u : i >= e0 ? ulo + n0 : ulo) + off;
-        valid = int(min(32u, cnt - off));
+        left = i >= nch ? 0 : int(cnt - off);
+        stop = i >= e2 ? nch : i >= e1 ? e2 : i >= e0 ? e1 : e0;
     };
-    uint32_t kr[2][KD], vr[8], word[NT];
+    uint32_t kr[2][KD], vr[8], word = 0;
     float scr = 0.0f;
     const uint32_t kl = uint32_t(n * QK + qd * SL), vl = uint32_t(4 * qd * VD + 4 * n);
     const uint32_t scl = (lane & 31) * 4 + (lane < 32 ? 0u : to_vs);
+    // loads of K and V are never conditional: past the last chunk they read some slot
     auto load_k = [&]() {
-        if (tail && valid) {
+        if (tail && left > 0) {
             // bits p0 .. p0 + 31 of the node's mask
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                const int node = node_of(min(tile * COLS + 16 * x + n, ncols - 1));
-                const uint32_t *m = tr.mask + (size_t(ses) * tr.nodes + node) * tr.words + (p0 >> 5);
-                word[x] = m[0] >> (p0 & 31u);
-                if ((p0 & 31u) && int(p0 >> 5) + 1 < tr.words) word[x] |= m[1] << (32u - (p0 & 31u));
-            }
+            const int at = node_of(min(int(tile) * kCols + n, ncols - 1));
+            const uint32_t *m = tr.mask + (size_t(ses) * tr.nodes + at) * tr.words + (p0 >> 5);
+            word = m[0] >> (p0 & 31u);
+            if ((p0 & 31u) && int(p0 >> 5) + 1 < tr.words) word |= m[1] << (32u - (p0 & 31u));
         }
         const uint32_t o = here(kl + s0 * QK);
 #pragma unroll
@@ -308,28 +258,69 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         for (int j = 0; j < 8; ++j)
             vr[j] = __builtin_amdgcn_raw_buffer_load_b32(vb, o + (16 * (j >> 2) + (j & 3)) * VD, 0, 0);
     };
-    // loads are never conditional: past the last chunk they read some slot
-#pragma unroll
-    for (int x = 0; x < NT; ++x) word[x] = 0;
     place(ch);
     load_k();
     load_v();
+
+    // ---- the query operand, while the first chunk is on its way ----
+    float cf;                         // factor of a score, in bits
+    intx4_t qi;                       // QQ: codes
+    uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
+    {
+        if (tr.negative) {
+#pragma unroll
+            for (int e = 0; e < SL; ++e) v[e] = -v[e];
+        }
+        float a = 0.0f;
+#pragma unroll
+        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1]));
+        a = fmaxf(a, ndl::wave_xor<16>(a));
+        a = fmaxf(a, ndl::wave_xor<32>(a));
+        float nan = 0.0f;
+        if constexpr (QQ) {
+            // quant_rows (model.rs:289-293): the codes and the head's scale
+            const float qs = a > 0.0f ? a / 127.0f : 1.0f;
+            const float inv = 1.0f / qs;
+            uint32_t dw[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                // quant_code: half away from zero is truncation after adding
+                // the float below a half, for every |y| < 2^22
+                const float y = v[e] * inv;
+                const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
+                nan = y != y ? y : nan;
+                dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
+            }
+            qi = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
+            cf = qs * tr.scale2;
+        } else {
+            // the head in 2^14 .. 2^15, so that the second pieces are normal numbers
+            const int sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                nan = v[e] - v[e] != 0.0f ? NAN : nan;
+                v[e] = __builtin_amdgcn_ldexpf(v[e], sh);
+            }
+#pragma unroll
+            for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[0][e / 2], qp[1][e / 2]);
+            cf = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
+        }
+        // (a factor of 0 would make no number of a score of -inf)
+        if (cf == 0.0f) cf = 0x1p-126f;
+        // NaN where the query has one (an infinity gives one too)
+        nan += ndl::wave_xor<16>(nan);
+        nan += ndl::wave_xor<32>(nan);
+        cf += nan;
+    }
 
     // m_run: a score of the column, no other so far is more than kAhead bits
     // above it (lim, in the scores' units); mu = m_run cf.  A new maximum is
     // taken, and the sums scaled, only where one gets ahead of that
     constexpr float kAhead = 5.0f;
-    float m_run[NT], lim[NT], mu[NT], l_run[NT];
-    floatx4_t acc[NT][4];
+    float m_run = -INFINITY, lim = -INFINITY, mu = 0.0f, l_run = 0.0f;
+    floatx4_t acc[4];
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        m_run[x] = -INFINITY;
-        lim[x] = -INFINITY;
-        mu[x] = 0.0f;
-        l_run[x] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[x][c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int c = 0; c < 4; ++c) acc[c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
     // K and V scales are taken in units of 2^kexp and 2^(vexp - 10), powers of
     // two that no finite one so far is above: scores before cf, and weights,
     // stay in range at any size of the cache's values
@@ -339,26 +330,21 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
 
     for (; ch < nch; ch += step) {
         // ---- the positions each column sees ----
-        const uint32_t some = valid < 32 ? (1u << valid) - 1u : 0xffffffffu;
-        uint32_t vis[NT];
-        bool full = false;
-        if (!tail && p0 >= tlo) {
-            full = valid == 32;
-#pragma unroll
-            for (int x = 0; x < NT; ++x) vis[x] = some;
-        } else {
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-                vis[x] = some & (tail ? word[x] : lo[x] <= p0 ? 0xffffffffu : lo[x] - p0 < 32u ? 0xffffffffu << (lo[x] - p0) : 0u);
+        const bool full = !tail && p0 >= tlo && left >= 32;
+        uint32_t vis = 0xffffffffu;
+        if (!full) {
+            vis = left < 32 ? (1u << left) - 1u : 0xffffffffu;
+            vis &= tail ? word : lo <= p0 ? 0xffffffffu : lo - p0 < 32u ? 0xffffffffu << (lo - p0) : 0u;
         }
         // ---- the chunk's scales, zero behind its end ----
-        float sc = (lane & 31) < valid ? scr : 0.0f;
+        float sc = (lane & 31) < left ? scr : 0.0f;
         if (any_of(!(sc <= top))) {
             // a V scale that is no number makes no number of the columns that see
             // it, and only of those: a weight of 0 there would not stay 0
             const bool wild = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY);
             const uint32_t wilds = uint32_t(__builtin_amdgcn_ballot_w64(wild) >> 32);
             if (wild) sc = 0.0f;
+            if (vis & wilds) l_run = NAN;
             float h = sc < INFINITY ? fmaxf(sc, top) : top;
             h = fmaxf(h, ndl::wave_xor<16>(h));
             h = fmaxf(h, ndl::wave_xor<8>(h));
@@ -370,23 +356,20 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
             top = h > top ? (now > 127 ? 0x1.fffffep127f : __builtin_amdgcn_ldexpf(1.0f, now)) : top;
             shift += was - now;
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
+            m_run = __builtin_amdgcn_ldexpf(m_run, kexp - kn);
+            cf = __builtin_amdgcn_ldexpf(cf, kn - kexp);
+            if (cf == 0.0f) cf = 0x1p-126f;
+            lim = m_run == -INFINITY ? -INFINITY : m_run + kAhead * __builtin_amdgcn_rcpf(cf);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                if (vis[x] & wilds) l_run[x] = NAN;
-                m_run[x] = __builtin_amdgcn_ldexpf(m_run[x], kexp - kn);
-                cf[x] = __builtin_amdgcn_ldexpf(cf[x], kn - kexp);
-                if (cf[x] == 0.0f) cf[x] = 0x1p-126f;
-                lim[x] = m_run[x] == -INFINITY ? -INFINITY : m_run[x] + kAhead * __builtin_amdgcn_rcpf(cf[x]);
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - vn);
-            }
+                for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - vn);
             kexp = kn;
             vexp = vn;
         }
         sc = __builtin_amdgcn_ldexpf(sc, shift);
-        const bool small = (uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32) & some) != 0;
+        const uint32_t few = uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32);
+        const bool small = (left < 32 ? few & ((1u << left) - 1u) : few) != 0;
         sc_s[w][lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -398,17 +381,14 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
         }
         __builtin_amdgcn_wave_barrier();
         // ---- scores ----
-        float s[NT][8];
+        float s[8];
         if constexpr (QQ) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const intx4_t kf{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
+                const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi, intx4_t{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi[x], intx4_t{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[x][4 * a + i] = float(d[i]) * ks[a][i];
-                }
+                for (int i = 0; i < 4; ++i) s[4 * a + i] = float(d[i]) * ks[a][i];
             }
         } else {
 #pragma unroll
@@ -420,186 +400,148 @@ __global__ __launch_bounds__(NW * 64, NT == 1 ? 4 : 2) void tree_kernel(Geom g, 
                     kp[2 * d] = f16_pair<0>(u);
                     kp[2 * d + 1] = f16_pair<1>(u);
                 }
+                floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int pc = 1; pc >= 0; --pc) {  // the small pieces first
-                        const uint32_t *qq = qp[x][pc];
-                        // qk 48: a lane's last four codes, doubled to the 32-wide
-                        // product's eight against four zeros of the query
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            vec4<f16x8_t>(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1]),
-                            KD == 3 ? vec4<f16x8_t>(qq[4], qq[5], 0u, 0u)
-                                    : vec4<f16x8_t>(qq[4], qq[5], qq[2 * KD - 2], qq[2 * KD - 1]),
-                            d, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(kp[0], kp[1], kp[2], kp[3]),
-                                                                   vec4<f16x8_t>(qq[0], qq[1], qq[2], qq[3]), d, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[x][4 * a + i] = d[i] * ks[a][i];
+                for (int pc = 1; pc >= 0; --pc) {  // the small pieces first
+                    const uint32_t *qq = qp[pc];
+                    // qk 48: a lane's last four codes, doubled to the 32-wide
+                    // product's eight against four zeros of the query
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        vec4<f16x8_t>(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1]),
+                        KD == 3 ? vec4<f16x8_t>(qq[4], qq[5], 0u, 0u)
+                                : vec4<f16x8_t>(qq[4], qq[5], qq[2 * KD - 2], qq[2 * KD - 1]),
+                        d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(kp[0], kp[1], kp[2], kp[3]),
+                                                               vec4<f16x8_t>(qq[0], qq[1], qq[2], qq[3]), d, 0, 0, 0);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * a + i] = d[i] * ks[a][i];
             }
         }
-        place(ch + step);
-        load_k();  // lands during the softmax and the values
+        // the next chunk: its K lands during the softmax and the values
+        if (ch + step < stop) [[likely]] {
+            s0 += 32u * uint32_t(step);
+            p0 += 32u * uint32_t(step);
+            left -= 32 * step;
+        } else {
+            asm volatile("");  // (a branch, not thirty selects in every chunk)
+            place(ch + step);
+        }
+        load_k();
         // ---- softmax: each lane its column's eight positions ----
         if (!full) {
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!(vis[x] >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u)) s[x][j] = -INFINITY;
+            for (int j = 0; j < 8; ++j)
+                if (!(vis >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u)) s[j] = -INFINITY;
         }
-        bool ahead = false;
-        float m8[NT];
+        const float m8 = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[7]));
+        if (any_of(m8 > lim)) {
+            float m = max3(m8, m_run, ndl::wave_xor<16>(m8));
+            m = fmaxf(m, ndl::wave_xor<32>(m));
+            const float mu_new = m == -INFINITY ? 0.0f : m * cf;
+            // nothing is summed yet where there was no maximum
+            const float al = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu - mu_new);
+            m_run = m;
+            lim = m == -INFINITY ? -INFINITY : m + kAhead * __builtin_amdgcn_rcpf(cf);
+            mu = mu_new;
+            l_run *= al;
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            m8[x] = max3(max3(s[x][0], s[x][1], s[x][2]), max3(s[x][3], s[x][4], s[x][5]), max3(s[x][6], s[x][7], s[x][7]));
-            ahead = ahead || m8[x] > lim[x];
+            for (int c = 0; c < 4; ++c) acc[c] *= al;
         }
-        if (any_of(ahead)) {
+        // the weights e vs, and the sum of e
+        float wt[8];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                float m = max3(m8[x], m_run[x], ndl::wave_xor<16>(m8[x]));
-                m = fmaxf(m, ndl::wave_xor<32>(m));
-                const float mu_new = m == -INFINITY ? 0.0f : m * cf[x];
-                // nothing is summed yet where there was no maximum
-                const float al = m_run[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu[x] - mu_new);
-                m_run[x] = m;
-                lim[x] = m == -INFINITY ? -INFINITY : m + kAhead * __builtin_amdgcn_rcpf(cf[x]);
-                mu[x] = mu_new;
-                l_run[x] *= al;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[x][c] *= al;
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cf, -mu));
+            l_run += e;
+            wt[j] = e * vs[j >> 2][j & 3];
         }
-        // the weights of a tile, e vs, and their sum without vs
-        auto weigh = [&](int x, float (&wt)[8]) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][j], cf[x], -mu[x]));
-                l_run[x] += e;
-                wt[j] = e * vs[j >> 2][j & 3];
-            }
-        };
         // ---- values ----
         if (!small) {
-            uint32_t ph[NT][4], pl[NT][4];
+            uint32_t ph[4], pl[4], u[8];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                float wt[8];
-                weigh(x, wt);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[x][j], pl[x][j]);
-            }
-            uint32_t u[8];
+            for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[j], pl[j]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
             auto column = [&](auto cc) {
                 constexpr int c = decltype(cc)::value;
                 const f16x8_t vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]),
                                                  f16_codes<c>(u[4], u[5]), f16_codes<c>(u[6], u[7]));
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        vf, vec4<f16x8_t>(pl[x][0], pl[x][1], pl[x][2], pl[x][3]), acc[x][c], 0, 0, 0);
-                    acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        vf, vec4<f16x8_t>(ph[x][0], ph[x][1], ph[x][2], ph[x][3]), acc[x][c], 0, 0, 0);
-                }
+                acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(pl[0], pl[1], pl[2], pl[3]), acc[c],
+                                                                0, 0, 0);
+                acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(ph[0], ph[1], ph[2], ph[3]), acc[c],
+                                                                0, 0, 0);
             };
             column(std::integral_constant<int, 0>{});
             column(std::integral_constant<int, 1>{});
             column(std::integral_constant<int, 2>{});
             column(std::integral_constant<int, 3>{});
         } else {
-            float wt[NT][8];
-#pragma unroll
-            for (int x = 0; x < NT; ++x) weigh(x, wt[x]);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float vc = i8_at(vr[j], c) * 0x1p-9f;
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(vc, wt[x][j], acc[x][c], 0, 0, 0);
-                }
+                for (int c = 0; c < 4; ++c)
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(i8_at(vr[j], c) * 0x1p-9f, wt[j], acc[c], 0, 0, 0);
         }
         load_v();  // lands during the next scores
     }
 
     // ---- the block's waves meet, half of them at a time ----
+    l_run += ndl::wave_xor<16>(l_run);
+    l_run += ndl::wave_xor<32>(l_run);
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        l_run[x] += ndl::wave_xor<16>(l_run[x]);
-        l_run[x] += ndl::wave_xor<32>(l_run[x]);
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[x][c][i] = __builtin_amdgcn_ldexpf(acc[x][c][i], vexp - 1);
-        // from here on the maximum is in bits
-        m_run[x] = m_run[x] == -INFINITY ? -INFINITY : mu[x];
-    }
+        for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1);
+    // from here on the maximum is in bits
+    m_run = m_run == -INFINITY ? -INFINITY : mu;
 #pragma unroll
     for (int h = HN; h >= 1; h /= 2) {
         if (w >= h && w < 2 * h) {
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                if (qd == 0) {
-                    mm[w - h][16 * x + n] = m_run[x];
-                    ml[w - h][16 * x + n] = l_run[x];
-                }
-                // lane (n, qd) holds V columns 16 qd + 4 i + c
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<floatx4_t *>(&mo[w - h][16 * x + n][16 * qd + 4 * i]) =
-                        floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]};
+            if (qd == 0) {
+                mm[w - h][n] = m_run;
+                ml[w - h][n] = l_run;
             }
+            // lane (n, qd) holds V columns 16 qd + 4 i + c
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<floatx4_t *>(&mo[w - h][n][16 * qd + 4 * i]) =
+                    floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
         }
         __syncthreads();
         if (w < h) {
+            const float m2 = mm[w][n], M = fmaxf(m_run, m2);
+            // -inf: sums are 0, or NaN where a score was
+            const float f1 = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - M);
+            const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - M);
+            m_run = M;
+            l_run = l_run * f1 + ml[w][n] * f2;
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                const float m2 = mm[w][16 * x + n], M = fmaxf(m_run[x], m2);
-                // -inf: sums are 0, or NaN where a score was
-                const float f1 = m_run[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[x] - M);
-                const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - M);
-                m_run[x] = M;
-                l_run[x] = l_run[x] * f1 + ml[w][16 * x + n] * f2;
+            for (int i = 0; i < 4; ++i) {
+                const floatx4_t o = *reinterpret_cast<const floatx4_t *>(&mo[w][n][16 * qd + 4 * i]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const floatx4_t o = *reinterpret_cast<const floatx4_t *>(&mo[w][16 * x + n][16 * qd + 4 * i]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[x][c][i] = acc[x][c][i] * f1 + o[c] * f2;
-                }
+                for (int c = 0; c < 4; ++c) acc[c][i] = acc[c][i] * f1 + o[c] * f2;
             }
         }
         if (h > 1) __syncthreads();
     }
-    if (w) return;
+    if (w || int(tile) * kCols + n >= ncols) return;
+    const size_t oh = row * g.H + head;
+    if (tr.splits == 1) {
+        const float inv = bad ? NAN : l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        const int f = tile * COLS + 16 * x + n;
-        if (f >= ncols) continue;
-        const int node = node_of(f), head = kvh * R + f - node * R;
-        const size_t oh = (size_t(ses) * tr.nodes + node) * g.H + head;
-        if (tr.splits == 1) {
-            const float inv = bad[x] ? NAN : l_run[x] == 0.0f ? 0.0f : 1.0f / l_run[x];
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<floatx4_u *>(tr.out + oh * VD + 16 * qd + 4 * i) =
+                floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]} * inv;
+    } else {
+        const size_t at = oh * tr.splits + split;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<floatx4_u *>(tr.out + oh * VD + 16 * qd + 4 * i) =
-                    floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]} * inv;
-        } else {
-            const size_t at = oh * tr.splits + split;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<floatx4_t *>(tr.part_o + at * VD + 16 * qd + 4 * i) =
-                    floatx4_t{acc[x][0][i], acc[x][1][i], acc[x][2][i], acc[x][3][i]};
-            if (qd == 0) {
-                tr.part_ml[2 * at] = m_run[x];
-                tr.part_ml[2 * at + 1] = bad[x] ? NAN : l_run[x];
-            }
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<floatx4_t *>(tr.part_o + at * VD + 16 * qd + 4 * i) =
+                floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+        if (qd == 0) {
+            tr.part_ml[2 * at] = m_run;
+            tr.part_ml[2 * at + 1] = bad ? NAN : l_run;
         }
     }
 }
@@ -648,7 +590,7 @@ Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
 template <int QK, bool QQ>
 auto kernel_of(const Plan &p)
 {
-    return p.nw == 4 ? tree_kernel<QK, QQ, 1, 4> : tree_kernel<QK, QQ, 1, 8>;
+    return p.nw == 4 ? tree_kernel<QK, QQ, 4> : tree_kernel<QK, QQ, 8>;
 }
 
 size_t partial_floats(const nd_kv_geom *g, size_t count, size_t nodes, size_t splits)
@@ -687,7 +629,9 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     t.kv_stride = kv_stride;
     t.nodes = int(nodes);
     t.words = int((nodes + 31) / 32);
-    t.tiles = int(p.tiles);
+    t.rep = g->num_heads / g->num_kv_heads;
+    t.by_splits = Divisor::of(uint32_t(p.splits));
+    t.by_kvh = Divisor::of(uint32_t(g->num_kv_heads));
     t.splits = int(p.splits);
     t.scale2 = float(double(scale < 0 ? -scale : scale) * 1.4426950408889634);
     t.negative = scale < 0;
@@ -702,7 +646,7 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     auto *fn = q48 ? (quant_query ? kernel_of<48, true>(p) : kernel_of<48, false>(p))
                    : (quant_query ? kernel_of<64, true>(p) : kernel_of<64, false>(p));
     // HIP counts a launch's threads in 32 bits: sessions beyond that go in further launches
-    const size_t per = size_t(g->num_kv_heads) * p.splits * p.tiles, most = std::max<size_t>(1, (size_t(1) << 22) / per);
+    const size_t per = size_t(g->num_kv_heads) * p.splits * p.tiles, most = std::max<size_t>(1, (size_t(1) << 18) / per);
     const Geom kg = make_geom(g);
     for (size_t s = 0; s < count; s += most) {
         const size_t m = std::min(most, count - s), rows = s * nodes;
@@ -719,8 +663,8 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
             t.part_ml = part + heads * p.splits * VD;
             part = t.part_ml + heads * p.splits * 2;
         }
-        t.units = int(m * g->num_kv_heads * p.splits);
-        hipLaunchKernelGGL(fn, dim3(unsigned((t.units + 7) / 8 * 8 * p.tiles)), dim3(p.nw * 64), 0, ctx->stream, kg, t);
+        t.units = uint32_t(m * g->num_kv_heads * p.splits);
+        hipLaunchKernelGGL(fn, dim3(8, unsigned(p.tiles), unsigned((t.units + 7) / 8)), dim3(p.nw * 64), 0, ctx->stream, kg, t);
         if (int rc = nd::check_launch("attend_tree_i8")) return rc;
         if (t.part_o) {
             const size_t total = m * nodes * g->num_heads;
