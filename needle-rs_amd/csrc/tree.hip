@@ -457,7 +457,18 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             wt[j] = e * vs[j >> 2][j & 3];
         }
         // ---- values ----
-        if (!small) {
+        if (small) [[unlikely]] {
+            // (then the product below adds nothing: two ways that each end in
+            // sums cost copies of all of them)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(i8_at(vr[j], c) * 0x1p-9f, wt[j], acc[c], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wt[j] = 0.0f;
+        }
+        {
             uint32_t ph[4], pl[4], u[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[j], pl[j]);
@@ -476,12 +487,6 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             column(std::integral_constant<int, 1>{});
             column(std::integral_constant<int, 2>{});
             column(std::integral_constant<int, 3>{});
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(i8_at(vr[j], c) * 0x1p-9f, wt[j], acc[c], 0, 0, 0);
         }
         load_v();  // lands during the next scores
     }
