@@ -136,10 +136,10 @@ template <int QK, bool QQ, int NW>
 __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
 {
     constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
-    constexpr int LD = VD + 4, HN = NW / 2;
+    constexpr int LD = VD + 4;
     __shared__ __align__(16) float sc_s[NW][64];
-    __shared__ __align__(16) float mo[HN][kCols][LD];
-    __shared__ float mm[HN][kCols], ml[HN][kCols];
+    __shared__ __align__(16) float mo[NW][kCols][LD];
+    __shared__ float mm[NW][kCols], ml[NW][kCols];
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
@@ -491,62 +491,48 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
         load_v();  // lands during the next scores
     }
 
-    // ---- the block's waves meet, half of them at a time ----
+    // ---- the block's waves meet: each leaves its sums, and sixteen threads a
+    // column, four values each, put them together ----
     l_run += ndl::wave_xor<16>(l_run);
     l_run += ndl::wave_xor<32>(l_run);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1);
-    // from here on the maximum is in bits
-    m_run = m_run == -INFINITY ? -INFINITY : mu;
-#pragma unroll
-    for (int h = HN; h >= 1; h /= 2) {
-        if (w >= h && w < 2 * h) {
-            if (qd == 0) {
-                mm[w - h][n] = m_run;
-                ml[w - h][n] = l_run;
-            }
-            // lane (n, qd) holds V columns 16 qd + 4 i + c
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<floatx4_t *>(&mo[w - h][n][16 * qd + 4 * i]) =
-                    floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-        }
-        __syncthreads();
-        if (w < h) {
-            const float m2 = mm[w][n], M = fmaxf(m_run, m2);
-            // -inf: sums are 0, or NaN where a score was
-            const float f1 = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - M);
-            const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - M);
-            m_run = M;
-            l_run = l_run * f1 + ml[w][n] * f2;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const floatx4_t o = *reinterpret_cast<const floatx4_t *>(&mo[w][n][16 * qd + 4 * i]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c][i] = acc[c][i] * f1 + o[c] * f2;
-            }
-        }
-        if (h > 1) __syncthreads();
+    if (qd == 0) {
+        // from here on the maximum is in bits
+        mm[w][n] = m_run == -INFINITY ? -INFINITY : mu;
+        ml[w][n] = bad ? NAN : l_run;
     }
-    if (w || int(tile) * kCols + n >= ncols) return;
-    const size_t oh = row * g.H + head;
-    if (tr.splits == 1) {
-        const float inv = bad ? NAN : l_run == 0.0f ? 0.0f : 1.0f / l_run;
+    // lane (n, qd) holds V columns 16 qd + 4 i + c
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<floatx4_u *>(tr.out + oh * VD + 16 * qd + 4 * i) =
-                floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]} * inv;
+    for (int i = 0; i < 4; ++i) {
+        floatx4_t o;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1);
+        *reinterpret_cast<floatx4_t *>(&mo[w][n][16 * qd + 4 * i]) = o;
+    }
+    __syncthreads();
+    const int col = t >> 4, fo = int(tile) * kCols + col;
+    if (col >= kCols || fo >= ncols) return;
+    float M = -INFINITY, L = 0.0f;
+    floatx4_t O{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NW; ++i) M = fmaxf(M, mm[i][col]);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        // -inf: sums are 0, or NaN where a score was
+        const float m = mm[i][col], by = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+        L += ml[i][col] * by;
+        O += *reinterpret_cast<const floatx4_t *>(&mo[i][col][4 * (t & 15)]) * by;
+    }
+    const int no = node_of(fo);
+    const size_t oh = (size_t(ses) * tr.nodes + no) * g.H + int(kvh) * R + fo - no * R;
+    if (tr.splits == 1) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        *reinterpret_cast<floatx4_u *>(tr.out + oh * VD + 4 * (t & 15)) = O * inv;
     } else {
         const size_t at = oh * tr.splits + split;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<floatx4_t *>(tr.part_o + at * VD + 16 * qd + 4 * i) =
-                floatx4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-        if (qd == 0) {
-            tr.part_ml[2 * at] = m_run;
-            tr.part_ml[2 * at + 1] = bad ? NAN : l_run;
+        *reinterpret_cast<floatx4_t *>(tr.part_o + at * VD + 4 * (t & 15)) = O;
+        if ((t & 15) == 0) {
+            tr.part_ml[2 * at] = M;
+            tr.part_ml[2 * at + 1] = L;
         }
     }
 }
@@ -586,9 +572,20 @@ Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
     Plan p;
     p.tiles = (cols + kCols - 1) / kCols;
     const size_t blocks = groups * p.tiles;
-    p.nw = blocks * 8 < cus * 12 ? 8 : 4;
-    const size_t fill = cus * 8 / (blocks * p.nw), most = chunks / (3 * p.nw);
-    p.splits = std::max<size_t>(1, std::min<size_t>(std::min(fill, most), 64));
+    // Eight waves a block below one and a half blocks a CU, four above (us, 4 / 8:
+    // 96 blocks 9.5 / 8.8, 576 17.9 / 18.0, 768 23.9 / 23.5, 768 longer ones 35.8 /
+    // 37.5, 1024 20.1 / 23.2)
+    p.nw = blocks * 2 < cus * 3 ? 8 : 4;
+    // A chunk costs a wave 0.55 us, a split about 0.25 at the join, the join's
+    // launch 3: as many splits as balance the first two, no more than give every
+    // SIMD two waves, and none that do not pay for the launch (us, one session x
+    // 8000 in 1 / 4 / 8 / 10 splits 26.4 / 15.0 / 13.3 / 14.4; one of 12 kv heads x
+    // 4000 in 1 / 4 / 6 / 8 18.4 / 12.7 / 12.5 / 12.8; 4 sessions x 4000 in 1 / 2 / 4
+    // 18.5 / 15.8 / 16.7; 16 x 1000 in 1 / 2 8.8 / 11.9)
+    const size_t fill = cus * 8 / (blocks * p.nw);
+    p.splits = 1;
+    while (p.splits < fill && p.splits < 64 && (p.splits + 1) * (p.splits + 1) * p.nw <= 2 * chunks) ++p.splits;
+    if (chunks * (p.splits - 1) < 6 * p.nw * p.splits) p.splits = 1;
     return p;
 }
 

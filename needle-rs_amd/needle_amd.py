@@ -642,20 +642,26 @@ def _near(ctx, t, name):
 
 def _rows_arg(ctx, t, rows, width, name):
     """(address, row stride) of fp32 rows whose elements lie one after another."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+    f32 = _torch().float32
+    if t.shape != (rows, width):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(rows, width)}")
-    if t.dtype != _torch().float32 or not t.is_cuda:
-        raise ValueError(f"{name}: a device tensor of float32 is required, not {t.dtype} on {t.device}")
-    _near(ctx, t, name)
-    if rows and ((t.stride(1) != 1 and width > 1) or (rows > 1 and t.stride(0) < width)):
+    if t.dtype != f32 or t.get_device() != ctx.device:
+        if t.dtype != f32 or not t.is_cuda:
+            raise ValueError(f"{name}: a device tensor of float32 is required, not {t.dtype} on {t.device}")
+        _near(ctx, t, name)
+    apart, step = t.stride()
+    if rows and ((step != 1 and width > 1) or (rows > 1 and apart < width)):
         raise ValueError(f"{name}: strides {t.stride()}: rows must be contiguous and apart")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), apart
 
 
 def _dev_arg(ctx, t, dtype, name, numel=0):
+    """_arg of a tensor on the context's device, None of None."""
     if t is None:
         return None
-    p = _arg(t, dtype, name, numel)
+    if t.dtype == dtype and t.get_device() == ctx.device and t.numel() >= numel and t.is_contiguous():
+        return t.data_ptr()
+    p = _arg(t, dtype, name, numel)  # says what is wrong
     _near(ctx, t, name)
     return p
 
@@ -664,12 +670,11 @@ def _empty(ctx, shape, dtype):
     """An output of a call: allocated for the context's stream, and kept until
     torch's current stream is done with it too where that is another one."""
     torch = _torch()
-    now = torch.cuda.current_stream(ctx.device)
-    if now.cuda_stream == ctx.stream.cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:  # (1 us less than current_stream)
+        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
     with torch.cuda.stream(ctx.stream):
-        t = torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
-    t.record_stream(now)
+        t = torch.empty(shape, dtype=dtype, device=ctx.stream.device)
+    t.record_stream(torch.cuda.current_stream(ctx.device))
     return t
 
 
@@ -819,25 +824,26 @@ def logits_adjust(ctx, x, hist=None, hist_len=None, out_from=None, repeat=None, 
     i32, f32 = torch.int32, torch.float32
     count, n = x.shape
     xp, xs = _rows_arg(ctx, x, count, n, "x")
-    rules = LogitsRules()
+    m = b = rows = words = 0
     if hist is not None:
         if hist.dim() != 2 or hist.shape[0] != count:
             raise ValueError(f"hist: shape {tuple(hist.shape)}, expected {count} rows")
-        rules.hist, rules.hist_stride = _dev_arg(ctx, hist, i32, "hist"), hist.shape[1]
+        m = hist.shape[1]
     if bias is not None and bias_id is not None:
         if bias.dim() != 2 or bias.shape[0] != count or bias.shape != bias_id.shape:
             raise ValueError(f"bias: shape {tuple(bias.shape)}, bias_id {tuple(bias_id.shape)}: [count][b] both")
-        rules.bias_stride = bias.shape[1]
-    rules.bias, rules.bias_id = _dev_arg(ctx, bias, f32, "bias"), _dev_arg(ctx, bias_id, i32, "bias_id")
-    for name, t, dtype in (("hist_len", hist_len, i32), ("out_from", out_from, i32), ("repeat", repeat, f32),
-                           ("presence", presence, f32), ("frequency", frequency, f32), ("bias_len", bias_len, i32),
-                           ("mask_row", mask_row, i32)):
-        if t is not None:
-            setattr(rules, name, _dev_arg(ctx, t, dtype, name, count))
+        b = bias.shape[1]
     if mask is not None:
         if mask.dim() != 2 or mask.shape[1] < (n + 31) // 32:
             raise ValueError(f"mask: shape {tuple(mask.shape)}, expected rows of {(n + 31) // 32} words")
-        rules.mask, rules.mask_rows, rules.mask_stride = _dev_arg(ctx, mask, i32, "mask"), mask.shape[0], mask.shape[1]
+        rows, words = mask.shape
+    rules = LogitsRules(
+        _dev_arg(ctx, hist, i32, "hist"), m, _dev_arg(ctx, hist_len, i32, "hist_len", count),
+        _dev_arg(ctx, out_from, i32, "out_from", count), _dev_arg(ctx, repeat, f32, "repeat", count),
+        _dev_arg(ctx, frequency, f32, "frequency", count), _dev_arg(ctx, presence, f32, "presence", count),
+        _dev_arg(ctx, bias_id, i32, "bias_id"), _dev_arg(ctx, bias, f32, "bias"), b,
+        _dev_arg(ctx, bias_len, i32, "bias_len", count), _dev_arg(ctx, mask, i32, "mask"), words, rows,
+        _dev_arg(ctx, mask_row, i32, "mask_row", count))
     yp = ys = None
     if write:
         if out is None:
