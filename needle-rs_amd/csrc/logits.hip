@@ -1,11 +1,12 @@
 // Logits under a request's rules -- penalties for repeated tokens, biases,
 // grammar masks -- and the greedy pick.
 //
-// A block takes a slice of kSlice tokens of one row: it counts the history's
-// tokens that fall into the slice in LDS (whole numbers: the order of the
-// atomics changes nothing), then passes over the logits once.  Bound by
-// memory: 4 bytes in and 4 out a logit, the history a second time for every
-// slice after the first (from L2).
+// A block takes a slice of kSlice tokens of one row, asks for its logits, counts
+// the history's tokens that fall into the slice in LDS meanwhile (whole numbers:
+// the order of the atomics changes nothing), and passes over the logits once.  A
+// token with a bias is left to the thread that holds its entry of the list.
+// Bound by memory: 4 bytes in and 4 out a logit, the history a second time for
+// every slice after the first (from L2).
 //
 // Every step is one fp32 rounding (the file is compiled without contraction),
 // so results do not depend on slice, lane or the presence of other rules.
@@ -14,8 +15,12 @@
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 4096;
+constexpr int kThreads = 512;
+constexpr int kSlice = 8192;  // 32 KiB of counts: four blocks a CU
+constexpr int kChunk = 4 * kThreads, kChunks = kSlice / kChunk;
+
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start anywhere
+typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr uint32_t kEver = 1u << 30, kBias = 1u << 31;  // beside the count of a token
 
 struct Pick {
@@ -53,76 +58,126 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(const float *x, size_t
                                                           nd_logits_rules r, float *y, size_t y_stride,
                                                           int32_t *next, Pick *part)
 {
-    __shared__ uint32_t st[kSlice];
-    __shared__ float bias[kSlice];
+    __shared__ __align__(16) uint32_t st[kSlice];
     __shared__ int twice;
     __shared__ Pick best[kThreads / 64];
     const size_t row = blockIdx.x / unsigned(slices);
     const int slice = int(blockIdx.x % unsigned(slices)), t0 = slice * kSlice, t = threadIdx.x;
     const int cnt = min(kSlice, n - t0);
-    for (int i = t; i < kSlice; i += kThreads) st[i] = 0;
-    if (t == 0) twice = 0;
-    __syncthreads();
-    if (r.hist) {
+    const float *xr = x + row * x_stride + t0;
+    float *yr = y ? y + row * y_stride + t0 : nullptr;
+
+    // ---- the slice's logits, on their way while the tokens are counted ----
+    float v[kChunks][4];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int k = c * kChunk + 4 * t;
+        if (k + 4 <= cnt) {
+            const float4u l = *reinterpret_cast<const float4u *>(xr + k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[c][e] = l[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[c][e] = k + e < cnt ? xr[k + e] : 0.0f;
+        }
+    }
+    const uint32_t *mask = nullptr;
+    if (r.mask) {
+        const int m = r.mask_row ? r.mask_row[row] : int(row);
+        if (m >= 0 && size_t(m) < r.mask_rows) mask = r.mask + size_t(m) * r.mask_stride + (t0 >> 5);
+    }
+    const int nh = r.hist ? clamp_len(r.hist_len, row, r.hist_stride) : 0;
+    const int nb = r.bias ? clamp_len(r.bias_len, row, r.bias_stride) : 0;
+    const bool marks = nh > 0 || nb > 0;
+    const float rep = r.repeat ? r.repeat[row] : 1.0f;
+    const float fr = r.frequency ? r.frequency[row] : 0.0f, pr = r.presence ? r.presence[row] : 0.0f;
+    const int32_t *bi = r.bias_id + row * r.bias_stride;
+    const float *bv = r.bias + row * r.bias_stride;
+    if (marks) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+            *reinterpret_cast<uint4 *>(&st[c * kChunk + 4 * t]) = make_uint4(0, 0, 0, 0);
+        if (t == 0) twice = 0;
+        __syncthreads();
         const int32_t *h = r.hist + row * r.hist_stride;
-        const int len = clamp_len(r.hist_len, row, r.hist_stride);
         const int from = r.out_from ? r.out_from[row] : 0;
-        for (int i = t; i < len; i += kThreads) {
-            const uint32_t k = uint32_t(h[i]) - uint32_t(t0);
+        auto count = [&](int tok, int i) {
+            const uint32_t k = uint32_t(tok) - uint32_t(t0);
             if (k < uint32_t(cnt)) {
                 atomicOr(&st[k], kEver);
                 if (i >= from) atomicAdd(&st[k], 1u);
             }
+        };
+        for (int i = 4 * t; i < nh; i += kChunk) {
+            if (i + 4 <= nh) {
+                const int4u q = *reinterpret_cast<const int4u *>(h + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) count(q[e], i + e);
+            } else {
+                for (int e = i; e < nh; ++e) count(h[e], e);
+            }
         }
-    }
-    const int nb = r.bias ? clamp_len(r.bias_len, row, r.bias_stride) : 0;
-    const int32_t *bi = r.bias_id + row * r.bias_stride;
-    const float *bv = r.bias + row * r.bias_stride;
-    for (int i = t; i < nb; i += kThreads) {
-        const uint32_t k = uint32_t(bi[i]) - uint32_t(t0);
-        if (k < uint32_t(cnt)) {
-            if (atomicOr(&st[k], kBias) & kBias) twice = 1;
-            bias[k] = bv[i];
-        }
-    }
-    __syncthreads();
-    if (twice) {  // the first entry of a token adds up all of its entries, in order
         for (int i = t; i < nb; i += kThreads) {
-            const int id = bi[i];
-            const uint32_t k = uint32_t(id) - uint32_t(t0);
-            if (k >= uint32_t(cnt)) continue;
-            bool first = true;
-            for (int j = 0; j < i && first; ++j) first = bi[j] != id;
-            if (!first) continue;
-            float s = bv[i];
-            for (int j = i + 1; j < nb; ++j)
-                if (bi[j] == id) s += bv[j];
-            bias[k] = s;
+            const uint32_t k = uint32_t(bi[i]) - uint32_t(t0);
+            if (k < uint32_t(cnt) && (atomicOr(&st[k], kBias) & kBias)) twice = 1;
         }
         __syncthreads();
     }
-    const float rep = r.repeat ? r.repeat[row] : 1.0f;
-    const float fr = r.frequency ? r.frequency[row] : 0.0f, pr = r.presence ? r.presence[row] : 0.0f;
-    const uint32_t *mask = nullptr;
-    if (r.mask) {
-        const int m = r.mask_row ? r.mask_row[row] : int(row);
-        if (m >= 0 && size_t(m) < r.mask_rows) mask = r.mask + size_t(m) * r.mask_stride;
-    }
+    // the penalties of a token's marks
+    auto penal = [&](float l, uint32_t s) {
+        const uint32_t c = s & (kEver - 1);
+        if ((s & kEver) && r.repeat) l = l > 0.0f ? l / rep : l * rep;
+        if (c && r.frequency) l -= float(c) * fr;
+        if (c && r.presence) l -= pr;
+        return l;
+    };
     Pick b{-INFINITY, kNone};
-    for (int k = t; k < cnt; k += kThreads) {
-        float l = x[row * x_stride + t0 + k];
-        const uint32_t s = st[k];
-        if (s) {
-            const uint32_t c = s & (kEver - 1);
-            if ((s & kEver) && r.repeat) l = l > 0.0f ? l / rep : l * rep;
-            if (c && r.frequency) l -= float(c) * fr;
-            if (c && r.presence) l -= pr;
-            if (s & kBias) l += bias[k];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int k = c * kChunk + 4 * t;
+        if (k >= cnt) continue;
+        uint4 s = make_uint4(0, 0, 0, 0);
+        if (marks) s = *reinterpret_cast<const uint4 *>(&st[k]);
+        const uint32_t sv[4] = {s.x, s.y, s.z, s.w};
+        const uint32_t allowed = mask ? mask[k >> 5] >> (k & 31) : 0xfu;
+        const uint32_t any = s.x | s.y | s.z | s.w;
+        if (any & ~kBias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[c][e] = penal(v[c][e], sv[e]);
         }
-        const int tok = t0 + k;
-        if (mask && !(mask[tok >> 5] >> (tok & 31) & 1)) l = -INFINITY;
-        if (y) y[row * y_stride + tok] = l;
-        if (l > b.v) b = Pick{l, tok};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!(allowed >> e & 1)) v[c][e] = -INFINITY;
+            if (k + e < cnt && !(sv[e] & kBias) && v[c][e] > b.v) b = Pick{v[c][e], t0 + k + e};
+        }
+        if (yr) {
+            if (k + 4 <= cnt && !(any & kBias)) {
+                *reinterpret_cast<float4u *>(yr + k) = float4u{v[c][0], v[c][1], v[c][2], v[c][3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + e < cnt && !(sv[e] & kBias)) yr[k + e] = v[c][e];
+            }
+        }
+    }
+    // ---- tokens with a bias: the first entry of a token adds up all of its
+    // entries, in order (one, where no token is listed twice) ----
+    for (int i = t; i < nb; i += kThreads) {
+        const int id = bi[i];
+        const uint32_t k = uint32_t(id) - uint32_t(t0);
+        if (k >= uint32_t(cnt)) continue;
+        float add = bv[i];
+        if (twice) {
+            bool first = true;
+            for (int j = 0; j < i && first; ++j) first = bi[j] != id;
+            if (!first) continue;
+            for (int j = i + 1; j < nb; ++j)
+                if (bi[j] == id) add += bv[j];
+        }
+        float l = penal(xr[k], st[k]) + add;
+        if (mask && !(mask[k >> 5] >> (k & 31) & 1)) l = -INFINITY;
+        if (yr) yr[k] = l;
+        if (l > -INFINITY) take(b, l, id);
     }
     if (!next) return;
     meet_wave(b);
