@@ -31,7 +31,7 @@ struct Turn {
 // What a rope or write launch works on: rows of q heads (nq), k heads (nk)
 // and v heads (nk), any of them absent.
 struct Rows {
-    size_t rows, per_block;
+    size_t rows, first, per_block;  // first: the launch's first row
     const int32_t *pos, *rot_pos;
     const float *q, *k, *v;
     float *q_out;
@@ -40,126 +40,189 @@ struct Rows {
     int nq, dim;
 };
 
+// Sine and cosine of |a| < 2^42: a - n pi / 2 with pi / 2 in two parts (the first
+// fma is exact but for the last bit of what is left, so the remainder is off by
+// 2^-53 of at most pi / 4), then the two Taylor series, whose first terms left out
+// are r^17 / 17! < 5e-17 and r^18 / 18! < 3e-18.
+__device__ inline void sine_cosine(double a, double &sn, double &c)
+{
+    const double n = __builtin_rint(a * 0.63661977236758134);
+    double r = __builtin_fma(-n, 0x1.921fb54442d18p+0, a);
+    r = __builtin_fma(-n, 0x1.1a62633145c07p-54, r);
+    const double x = r * r;
+    double s = -1.0 / 1307674368000.0, t = 1.0 / 20922789888000.0;  // 1 / 15!, 1 / 16!
+    s = __builtin_fma(s, x, 1.0 / 6227020800.0);
+    t = __builtin_fma(t, x, -1.0 / 87178291200.0);
+    s = __builtin_fma(s, x, -1.0 / 39916800.0);
+    t = __builtin_fma(t, x, 1.0 / 479001600.0);
+    s = __builtin_fma(s, x, 1.0 / 362880.0);
+    t = __builtin_fma(t, x, -1.0 / 3628800.0);
+    s = __builtin_fma(s, x, -1.0 / 5040.0);
+    t = __builtin_fma(t, x, 1.0 / 40320.0);
+    s = __builtin_fma(s, x, 1.0 / 120.0);
+    t = __builtin_fma(t, x, -1.0 / 720.0);
+    s = __builtin_fma(s, x, -1.0 / 6.0);
+    t = __builtin_fma(t, x, 1.0 / 24.0);
+    t = __builtin_fma(t, x, -0.5);
+    s = __builtin_fma(s * x, r, r);
+    t = __builtin_fma(t, x, 1.0);
+    const int q = int(int64_t(n) & 3);
+    const double u = q & 1 ? t : s, v = q & 1 ? s : t;
+    sn = q & 2 ? -u : u;
+    c = (q + 1) & 2 ? -v : v;
+}
+
+// Where a row lies in the cache, worked out once a block: its block and slot, and
+// its position (-1: left out).
+struct Place {
+    size_t off;
+    int slot, p;
+};
+constexpr int kMaxRows = 16;
+
+__device__ inline Place place_of(const int32_t *pos, size_t i, size_t per_block, size_t kv_stride, int cap)
+{
+    const int p = pos[i];
+    const size_t b = per_block == 1 ? i : (i | per_block) >> 32 ? i / per_block : uint32_t(i) / uint32_t(per_block);
+    return Place{b * kv_stride, p < 0 ? 0 : p % cap, p};
+}
+
 typedef float float4a __attribute__((ext_vector_type(4)));
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start anywhere
 typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
 
 // G lanes a head vector, four elements a lane: element 4 l + e of the head.  FOUR:
 // every head is a multiple of 4 long, and with halves rot / 2 is too, so that a
-// lane's partners are four neighbours.
+// lane's partners are four neighbours.  A group keeps its heads for all rows of
+// the block: q heads, then k heads, then v heads.
 template <int G, bool FOUR>
 __global__ __launch_bounds__(kThreads) void turn_kernel(Turn tn, Rows r, Geom g, int rpb)
 {
     extern __shared__ double2 cs[];  // [rpb][rot / 2]: gain cos, gain sin
-    constexpr int GROUPS = kThreads / G;
-    const int t = threadIdx.x, l = t % G;
+    __shared__ Place at_row[kMaxRows];
+    const int t = threadIdx.x, l = t % G, e0 = 4 * l, groups = blockDim.x / G;
     const int half = tn.rot / 2;
     const bool pairs = tn.layout == ND_ROPE_PAIRS;
-    const int heads = r.nq + (r.kv ? 2 * g.KVH : 0);
-    auto head = [&](size_t i0, int row, int h) {
-        const size_t i = i0 + row;
-        const int p = r.pos[i];
-        const bool isq = h < r.nq, isv = h >= r.nq + g.KVH;
-        const int hk = h - r.nq - (isv ? g.KVH : 0);
-        const int dim = isq ? r.dim : isv ? g.VD : g.QK;
-        const float *x = isq ? r.q + i * r.q_stride + size_t(h) * dim
-                         : isv ? r.v + i * r.v_stride + size_t(hk) * dim
-                               : r.k + i * r.k_stride + size_t(hk) * dim;
-        const int e0 = 4 * l;
-        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // where pair k of a row lies in LDS: what the lanes of a group read at once,
+    // pairs 4 l + e or 2 l + e / 2, one after another
+    const int q4 = half / 4, q2 = half / 2;
+    auto place_in = [&](int k) { return !FOUR ? k : pairs ? (k & 1) * q2 + k / 2 : (k & 3) * q4 + k / 4; };
+
+    // the lane's elements of a head, as they are
+    auto load = [&](const float *x, int dim, float (&y)[4]) {
         if (FOUR ? e0 < dim : e0 + 4 <= dim) {
             const float4u q = *reinterpret_cast<const float4u *>(x + e0);
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = q[e];
-        } else if (!FOUR) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = e0 + e < dim ? x[e0 + e] : 0.0f;
-        }
-        if (!isv && e0 < tn.rot) {
-            const double2 *a = cs + row * half;
-            if (pairs) {
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    if (e0 + e >= tn.rot) continue;
-                    const double2 z = a[(e0 + e) / 2];
-                    const double u = y[e], w = y[e + 1];
-                    y[e] = float(u * z.x - w * z.y);
-                    y[e + 1] = float(u * z.y + w * z.x);
-                }
-            } else if (FOUR) {
-                const bool second = e0 >= half;
-                const int j = second ? e0 - half : e0;
-                const float4u o = *reinterpret_cast<const float4u *>(x + (second ? j : e0 + half));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const double2 z = a[j + e];
-                    y[e] = float(double(y[e]) * z.x + double(o[e]) * (second ? z.y : -z.y));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (e0 + e >= tn.rot) continue;
-                    const bool second = e0 + e >= half;
-                    const int j = second ? e0 + e - half : e0 + e;
-                    const double2 z = a[j];
-                    y[e] = float(double(y[e]) * z.x + double(x[second ? j : j + half]) * (second ? z.y : -z.y));
-                }
-            }
-        }
-        if (p < 0) return;  // left out; what was read is memory all the same
-        if (isq) {
-            float *out = r.q_out + i * r.q_out_stride + size_t(h) * dim;
-            if (FOUR ? e0 < dim : e0 + 4 <= dim) {
-                *reinterpret_cast<float4u *>(out + e0) = float4u{y[0], y[1], y[2], y[3]};
-            } else if (!FOUR) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e0 + e < dim) out[e0 + e] = y[e];
-            }
         } else {
-            // quant_into (cache.rs:80-104): heads are multiples of 16 long
-            float m = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float av = y[e] < 0.0f ? -y[e] : y[e];
-                if (av > m) m = av;
-            }
-            m = fmaxf(m, ndl::wave_xor<1>(m));
-            m = fmaxf(m, ndl::wave_xor<2>(m));
-            m = fmaxf(m, ndl::wave_xor<4>(m));
-            m = fmaxf(m, ndl::wave_xor<8>(m));
-            if (G >= 32) m = fmaxf(m, ndl::wave_xor<16>(m));
-            if (G >= 64) m = fmaxf(m, ndl::wave_xor<32>(m));
-            const float scale = m > 0.0f ? m / 127.0f : 1.0f;
-            const float inv = 1.0f / scale;
-            uint32_t codes = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                codes |= (uint32_t(int32_t(int8_t(quant_code(y[e], inv)))) & 0xffu) << (8 * e);
-            uint8_t *blk = r.kv + (i / r.per_block) * r.kv_stride;
-            const size_t at = size_t(hk) * g.cap + p % g.cap;
-            if (e0 < dim)
-                *reinterpret_cast<uint32_t *>(blk + (isv ? g.v_off : 0) + at * dim + e0) = codes;
-            if (l == 0) reinterpret_cast<float *>(blk + (isv ? g.vs_off : g.ks_off))[at] = scale;
+            for (int e = 0; e < 4; ++e) y[e] = !FOUR && e0 + e < dim ? x[e0 + e] : 0.0f;
         }
     };
-    for (size_t i0 = size_t(blockIdx.x) * rpb; i0 < r.rows; i0 += size_t(gridDim.x) * rpb) {
-        const int rows = int(min(size_t(rpb), r.rows - i0));
-        if (i0 >= size_t(gridDim.x) * rpb) __syncthreads();
-        for (int j = t; j < rows * half; j += kThreads) {
-            const int row = j / half;
-            const int p = r.rot_pos ? r.rot_pos[i0 + row] : r.pos[i0 + row];
-            double sn, c;
-            sincos(double(p) * tn.f[j - row * half], &sn, &c);
-            cs[j] = double2{tn.gain * c, tn.gain * sn};
+    // and turned
+    auto turn = [&](const float *x, int row, float (&y)[4]) {
+        if (e0 >= tn.rot) return;
+        const double2 *a = cs + row * half;
+        if (pairs) {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                if (!FOUR && e0 + e >= tn.rot) continue;
+                const double2 z = a[FOUR ? (e / 2) * q2 + l : (e0 + e) / 2];
+                const double u = y[e], w = y[e + 1];
+                y[e] = float(u * z.x - w * z.y);
+                y[e + 1] = float(u * z.y + w * z.x);
+            }
+        } else if (FOUR) {
+            const bool second = e0 >= half;
+            const int j = second ? e0 - half : e0;
+            const float4u o = *reinterpret_cast<const float4u *>(x + (second ? j : e0 + half));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double2 z = a[e * q4 + j / 4];
+                y[e] = float(double(y[e]) * z.x + double(second ? o[e] : -o[e]) * z.y);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (e0 + e >= tn.rot) continue;
+                const bool second = e0 + e >= half;
+                const int j = second ? e0 + e - half : e0 + e;
+                const float o = x[second ? j : j + half];
+                y[e] = float(double(y[e]) * a[j].x + double(second ? o : -o) * a[j].y);
+            }
         }
-        __syncthreads();
-        int row = 0, h = t / G;
-        while (h >= heads && row < rows) h -= heads, ++row;
-        while (row < rows) {
-            head(i0, row, h);
-            h += GROUPS;
-            while (h >= heads && row < rows) h -= heads, ++row;
+    };
+    // quant_into (cache.rs:80-104) and the store of k or v head h; heads are
+    // multiples of 16 long
+    auto keep = [&](const Place &place, const float (&y)[4], int h, int dim, size_t part, size_t scales) {
+        float m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float av = y[e] < 0.0f ? -y[e] : y[e];
+            if (av > m) m = av;
+        }
+        m = fmaxf(m, ndl::wave_xor<1>(m));
+        m = fmaxf(m, ndl::wave_xor<2>(m));
+        m = fmaxf(m, ndl::wave_xor<4>(m));
+        m = fmaxf(m, ndl::wave_xor<8>(m));
+        if (G >= 32) m = fmaxf(m, ndl::wave_xor<16>(m));
+        if (G >= 64) m = fmaxf(m, ndl::wave_xor<32>(m));
+        if (place.p < 0) return;
+        const float scale = m > 0.0f ? m / 127.0f : 1.0f;
+        const float inv = 1.0f / scale;
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) codes |= (uint32_t(int32_t(int8_t(quant_code(y[e], inv)))) & 0xffu) << (8 * e);
+        uint8_t *blk = r.kv + place.off;
+        const size_t at = size_t(h) * g.cap + place.slot;
+        if (e0 < dim) *reinterpret_cast<uint32_t *>(blk + part + at * dim + e0) = codes;
+        if (l == 0) reinterpret_cast<float *>(blk + scales)[at] = scale;
+    };
+
+    const size_t i0 = r.first + size_t(blockIdx.x) * rpb;
+    const int rows = int(min(size_t(rpb), r.rows - i0));
+    if (t < rows) at_row[t] = place_of(r.pos, i0 + t, r.per_block, r.kv_stride, r.kv ? g.cap : 1);
+    for (int j = t; j < rows * half; j += blockDim.x) {
+        const int row = j / half, k = j - row * half;
+        const int p = r.rot_pos ? r.rot_pos[i0 + row] : r.pos[i0 + row];
+        double sn, c;
+        sine_cosine(double(p) * tn.f[k], sn, c);
+        cs[row * half + place_in(k)] = double2{tn.gain * c, tn.gain * sn};
+    }
+    __syncthreads();
+    const int heads = r.nq + (r.kv ? 2 * g.KVH : 0);
+    for (int h = t / G; h < heads; h += groups) {
+        float y[4];
+        if (h < r.nq) {
+            const float *x = r.q + i0 * r.q_stride + size_t(h) * r.dim;
+            float *out = r.q_out + i0 * r.q_out_stride + size_t(h) * r.dim;
+            for (int row = 0; row < rows; ++row, x += r.q_stride, out += r.q_out_stride) {
+                load(x, r.dim, y);
+                turn(x, row, y);
+                if (at_row[row].p < 0) continue;  // left out; what was read is memory all the same
+                if (FOUR ? e0 < r.dim : e0 + 4 <= r.dim) {
+                    __builtin_nontemporal_store(float4u{y[0], y[1], y[2], y[3]}, reinterpret_cast<float4u *>(out + e0));
+                } else if (!FOUR) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e0 + e < r.dim) out[e0 + e] = y[e];
+                }
+            }
+        } else if (h < r.nq + g.KVH) {
+            const int hk = h - r.nq;
+            const float *x = r.k + i0 * r.k_stride + size_t(hk) * g.QK;
+            for (int row = 0; row < rows; ++row, x += r.k_stride) {
+                load(x, g.QK, y);
+                turn(x, row, y);
+                keep(at_row[row], y, hk, g.QK, 0, g.ks_off);
+            }
+        } else {
+            const int hk = h - r.nq - g.KVH;
+            const float *x = r.v + i0 * r.v_stride + size_t(hk) * g.VD;
+            for (int row = 0; row < rows; ++row, x += r.v_stride) {
+                load(x, g.VD, y);
+                keep(at_row[row], y, hk, g.VD, g.v_off, g.vs_off);
+            }
         }
     }
 }
@@ -167,50 +230,36 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(Turn tn, Rows r, Geom g,
 // Sixteen bytes of a result a lane: four codes of a head vector and its scale.
 // Item j of a row is dword j of its K heads, then of its V heads.
 __global__ __launch_bounds__(kThreads) void read_kernel(Geom g, const uint8_t *__restrict__ kv,
-                                                        size_t kv_stride, size_t rows, size_t per_block,
-                                                        const int32_t *__restrict__ pos,
-                                                        float *__restrict__ k, float *__restrict__ v, int rpb)
+                                                        size_t kv_stride, size_t rows, size_t first,
+                                                        size_t per_block, const int32_t *__restrict__ pos,
+                                                        float *__restrict__ k, float *__restrict__ v, int rpb,
+                                                        uint32_t by_qk, uint32_t by_vd)
 {
+    __shared__ Place at_row[kMaxRows];
     const int wk = k ? g.KVH * g.QK / 4 : 0, wv = v ? g.KVH * g.VD / 4 : 0, items = wk + wv;
-    for (size_t i0 = size_t(blockIdx.x) * rpb; i0 < rows; i0 += size_t(gridDim.x) * rpb) {
-        const int n = int(min(size_t(rpb), rows - i0));
-        for (int row = 0, j = threadIdx.x;; j += kThreads) {
-            while (j >= items) j -= items, ++row;
-            if (row >= n) break;
-            const size_t i = i0 + row;
-            const bool isv = j >= wk;
-            const int dim = isv ? g.VD : g.QK, e = 4 * (isv ? j - wk : j), h = e / dim;
-            const int p = pos[i];
-            const uint8_t *blk = kv + (i / per_block) * kv_stride;
-            const size_t at = size_t(h) * g.cap + (p < 0 ? 0 : p % g.cap);
-            const uint32_t c = *reinterpret_cast<const uint32_t *>(blk + (isv ? g.v_off : 0) + at * dim + (e - h * dim));
-            const float s = reinterpret_cast<const float *>(blk + (isv ? g.vs_off : g.ks_off))[at];
-            float4a o;
+    const size_t i0 = first + size_t(blockIdx.x) * rpb;
+    const int n = int(min(size_t(rpb), rows - i0));
+    if (int(threadIdx.x) < n) at_row[threadIdx.x] = place_of(pos, i0 + threadIdx.x, per_block, kv_stride, g.cap);
+    __syncthreads();
+    for (int row = 0, j = threadIdx.x;; j += kThreads) {
+        while (j >= items) j -= items, ++row;
+        if (row >= n) break;
+        const size_t i = i0 + row;
+        const bool isv = j >= wk;
+        // dword d of the heads: d / (dim / 4) by 2^32 / (dim / 4) rounded up, d below 2^16 64
+        const int d = isv ? j - wk : j, dim = isv ? g.VD : g.QK, e = 4 * d;
+        const int h = int(__umulhi(uint32_t(d), isv ? by_vd : by_qk));
+        const Place &place = at_row[row];
+        const uint8_t *blk = kv + place.off;
+        const size_t at = size_t(h) * g.cap + place.slot;
+        const uint32_t c = *reinterpret_cast<const uint32_t *>(blk + (isv ? g.v_off : 0) + at * dim + (e - h * dim));
+        const float s = reinterpret_cast<const float *>(blk + (isv ? g.vs_off : g.ks_off))[at];
+        float4a o;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) o[b] = p < 0 ? 0.0f : float(int32_t(c << (24 - 8 * b)) >> 24) * s;
-            float *out = (isv ? v : k) + i * size_t(g.KVH) * dim + e;
-            *reinterpret_cast<float4u *>(out) = o;
-        }
+        for (int b = 0; b < 4; ++b) o[b] = place.p < 0 ? 0.0f : float(int32_t(c << (24 - 8 * b)) >> 24) * s;
+        float *out = (isv ? v : k) + i * size_t(g.KVH) * dim + e;
+        __builtin_nontemporal_store(float4u(o), reinterpret_cast<float4u *>(out));
     }
-}
-
-int check_rope(const nd_rope *r)
-{
-    ND_REQUIRE(r, "null rope");
-    ND_REQUIRE(r->layout == ND_ROPE_HALVES || r->layout == ND_ROPE_PAIRS, "rope layout %d unknown", r->layout);
-    ND_REQUIRE(r->scaling >= ND_ROPE_PLAIN && r->scaling <= ND_ROPE_PARTS, "rope scaling %d unknown", r->scaling);
-    ND_REQUIRE(r->rot_dim >= 2 && r->rot_dim % 2 == 0 && r->rot_dim <= kMaxDim,
-               "rot_dim %d must be even and in 2..%d", r->rot_dim, kMaxDim);
-    ND_REQUIRE(std::isfinite(r->theta) && r->theta > 0, "theta must be positive");
-    ND_REQUIRE(std::isfinite(r->gain), "gain must be finite");
-    if (r->scaling != ND_ROPE_PLAIN)
-        ND_REQUIRE(std::isfinite(r->factor) && r->factor > 0, "factor must be positive");
-    if (r->scaling == ND_ROPE_PARTS) {
-        ND_REQUIRE(std::isfinite(r->trained) && r->trained > 0, "trained must be positive");
-        ND_REQUIRE(r->turns_lo >= 0 && std::isfinite(r->turns_hi) && r->turns_hi > r->turns_lo,
-                   "0 <= turns_lo < turns_hi is required");
-    }
-    return ND_OK;
 }
 
 void freqs(const nd_rope *r, double *f)
@@ -225,6 +274,32 @@ void freqs(const nd_rope *r, double *f)
             f[j] *= g + (1.0 - g) / r->factor;
         }
     }
+}
+
+int check_rope(const nd_rope *r)
+{
+    ND_REQUIRE(r, "null rope");
+    ND_REQUIRE(r->layout == ND_ROPE_HALVES || r->layout == ND_ROPE_PAIRS, "rope layout %d unknown", r->layout);
+    ND_REQUIRE(r->scaling >= ND_ROPE_PLAIN && r->scaling <= ND_ROPE_PARTS, "rope scaling %d unknown", r->scaling);
+    ND_REQUIRE(r->rot_dim >= 2 && r->rot_dim % 2 == 0 && r->rot_dim <= kMaxDim,
+               "rot_dim %d must be even and in 2..%d", r->rot_dim, kMaxDim);
+    ND_REQUIRE(std::isfinite(r->theta) && r->theta > 0, "theta must be positive");
+    ND_REQUIRE(std::isfinite(r->gain), "gain must be finite");
+    // (the angles' reduction: 2^31 positions of 2^10 are below 2^42)
+    const auto top_of = [&] {
+        double f[kMaxPairs];
+        freqs(r, f);
+        return *std::max_element(f, f + r->rot_dim / 2);
+    };
+    if (r->scaling != ND_ROPE_PLAIN)
+        ND_REQUIRE(std::isfinite(r->factor) && r->factor > 0, "factor must be positive");
+    if (r->scaling == ND_ROPE_PARTS) {
+        ND_REQUIRE(std::isfinite(r->trained) && r->trained > 0, "trained must be positive");
+        ND_REQUIRE(r->turns_lo >= 0 && std::isfinite(r->turns_hi) && r->turns_hi > r->turns_lo,
+                   "0 <= turns_lo < turns_hi is required");
+    }
+    ND_REQUIRE(top_of() <= 1024.0, "a frequency is above 1024 a position");
+    return ND_OK;
 }
 
 Turn make_turn(const nd_rope *r)
@@ -253,20 +328,36 @@ bool clash(const float *x, size_t xs, const float *y, size_t ys, size_t wx, size
 // Rows a block, so that there are `want` blocks or more of it, at most `most`.
 size_t rows_a_block(size_t rows, size_t want, size_t most) { return std::min(std::max<size_t>(rows / want, 1), most); }
 
-// Blocks of them: the kernels go round where there are more than a launch holds
-// (HIP counts its threads in 32 bits).
-dim3 row_blocks(size_t rows, size_t rpb) { return dim3(unsigned(std::min<size_t>((rows + rpb - 1) / rpb, size_t(1) << 23))); }
+// Launches of at most 2^23 blocks of rpb rows (HIP counts a launch's threads in 32
+// bits): f(first row, blocks) for each.
+template <typename F>
+void launches(size_t rows, size_t rpb, F f)
+{
+    const size_t most = (size_t(1) << 23) * rpb;
+    for (size_t i = 0; i < rows; i += most) f(i, dim3(unsigned((std::min(most, rows - i) + rpb - 1) / rpb)));
+}
 
-int launch_turn(nd_ctx *ctx, const nd_rope *r, const Rows &a, const Geom &g, const char *what)
+int launch_turn(nd_ctx *ctx, const nd_rope *r, Rows a, const Geom &g, const char *what)
 {
     const int longest = a.kv ? std::max(g.QK, g.VD) : a.dim, half = r->rot_dim / 2;
     const bool four = a.dim % 4 == 0 && (r->layout == ND_ROPE_PAIRS ? r->rot_dim % 4 == 0 : half % 4 == 0);
-    const size_t rpb = rows_a_block(a.rows, 2048, 8);
+    // four rows a block give each lane a few heads and leave blocks for all CUs (us,
+    // 8000 rows of 12 + 24 heads with their read-back: 2 / 4 / 8 rows 43.6 / 41.5 /
+    // 46.9; 6001 rows of 12 heads 9.5 / 8.8 / 8.9)
+    const size_t rpb = rows_a_block(a.rows, 1024, 4);
     const size_t lds = rpb * half * sizeof(double2);
     auto *fn = longest <= 64    ? (four ? turn_kernel<16, true> : turn_kernel<16, false>)
                : longest <= 128 ? (four ? turn_kernel<32, true> : turn_kernel<32, false>)
                                 : (four ? turn_kernel<64, true> : turn_kernel<64, false>);
-    hipLaunchKernelGGL(fn, row_blocks(a.rows, rpb), dim3(kThreads), lds, ctx->stream, make_turn(r), a, g, int(rpb));
+    // as many groups as give each the same number of heads (36 heads: 12 groups)
+    const int lanes = longest <= 64 ? 16 : longest <= 128 ? 32 : 64, most = kThreads / lanes;
+    const int heads = a.nq + (a.kv ? 2 * g.KVH : 0), turns = (heads + most - 1) / most;
+    const int threads = ((heads + turns - 1) / turns * lanes + 63) / 64 * 64;
+    const Turn turn = make_turn(r);
+    launches(a.rows, rpb, [&](size_t first, dim3 grid) {
+        a.first = first;
+        hipLaunchKernelGGL(fn, grid, dim3(threads), lds, ctx->stream, turn, a, g, int(rpb));
+    });
     return nd::check_launch(what);
 }
 
@@ -367,15 +458,20 @@ int nd_kv_read(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_strid
     ND_ENTER(ctx);
     if (int rc = check_geom(g)) return rc;
     ND_REQUIRE(per_block > 0, "per_block must be positive");
+    ND_REQUIRE(g->num_kv_heads <= 65536, "num_kv_heads %d above 65536", g->num_kv_heads);
     if (count == 0 || (!k && !v)) return ND_OK;
     ND_REQUIRE(kv && pos, "null buffer");
     ND_REQUIRE(count <= 0x7fffffff, "count too large");
     ND_REQUIRE((reinterpret_cast<uintptr_t>(kv) & 255) == 0 && kv_stride % 256 == 0,
                "kv blocks must be 256-byte aligned");
-    const size_t rpb = rows_a_block(count, 2048, 16);
-    hipLaunchKernelGGL(read_kernel, row_blocks(count, rpb), dim3(kThreads), 0, ctx->stream,
-                       make_geom(g), static_cast<const uint8_t *>(kv), kv_stride, count, per_block, pos, k, v,
-                       int(rpb));
+    const size_t rpb = rows_a_block(count, 2048, kMaxRows);
+    auto up = [](int d) { return uint32_t(((uint64_t(1) << 32) + d - 1) / d); };
+    const Geom kg = make_geom(g);
+    launches(count, rpb, [&](size_t first, dim3 grid) {
+        hipLaunchKernelGGL(read_kernel, grid, dim3(kThreads), 0, ctx->stream, kg, static_cast<const uint8_t *>(kv),
+                           kv_stride, count, first, per_block, pos, k, v, int(rpb), up(g->qk_head_dim / 4),
+                           up(g->v_head_dim / 4));
+    });
     return nd::check_launch("kv_read");
 }
 
