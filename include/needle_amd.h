@@ -295,8 +295,8 @@ int nd_attend_step_i8_exact(nd_ctx *ctx, const nd_kv_geom *g, const void *kv,
  * The angle is the fp64 product of the position and the fp64 f_j; sine,
  * cosine and the turn are fp64 and rounded to fp32 once, so positions in the
  * millions lose nothing.  rot_dim is even, 2 .. 256; theta, factor, trained
- * positive; 0 <= turns_lo < turns_hi (the last three only looked at where
- * the scaling uses them); gain finite. */
+ * positive; 0 <= turns_lo < turns_hi (the last four only looked at where
+ * the scaling uses them); gain finite; no f_j above 1024. */
 enum { ND_ROPE_HALVES = 0, ND_ROPE_PAIRS = 1 };
 enum { ND_ROPE_PLAIN = 0, ND_ROPE_LINEAR = 1, ND_ROPE_PARTS = 2 };
 typedef struct nd_rope {

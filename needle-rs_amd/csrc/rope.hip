@@ -276,7 +276,8 @@ void freqs(const nd_rope *r, double *f)
     }
 }
 
-int check_rope(const nd_rope *r)
+// Checks a rope and fills the kernels' form of it.
+int make_turn(const nd_rope *r, Turn &t)
 {
     ND_REQUIRE(r, "null rope");
     ND_REQUIRE(r->layout == ND_ROPE_HALVES || r->layout == ND_ROPE_PAIRS, "rope layout %d unknown", r->layout);
@@ -285,12 +286,6 @@ int check_rope(const nd_rope *r)
                "rot_dim %d must be even and in 2..%d", r->rot_dim, kMaxDim);
     ND_REQUIRE(std::isfinite(r->theta) && r->theta > 0, "theta must be positive");
     ND_REQUIRE(std::isfinite(r->gain), "gain must be finite");
-    // (the angles' reduction: 2^31 positions of 2^10 are below 2^42)
-    const auto top_of = [&] {
-        double f[kMaxPairs];
-        freqs(r, f);
-        return *std::max_element(f, f + r->rot_dim / 2);
-    };
     if (r->scaling != ND_ROPE_PLAIN)
         ND_REQUIRE(std::isfinite(r->factor) && r->factor > 0, "factor must be positive");
     if (r->scaling == ND_ROPE_PARTS) {
@@ -298,18 +293,14 @@ int check_rope(const nd_rope *r)
         ND_REQUIRE(r->turns_lo >= 0 && std::isfinite(r->turns_hi) && r->turns_hi > r->turns_lo,
                    "0 <= turns_lo < turns_hi is required");
     }
-    ND_REQUIRE(top_of() <= 1024.0, "a frequency is above 1024 a position");
-    return ND_OK;
-}
-
-Turn make_turn(const nd_rope *r)
-{
-    Turn t{};
     t.layout = r->layout;
     t.rot = r->rot_dim;
     t.gain = r->gain;
     freqs(r, t.f);
-    return t;
+    // (the angles' reduction: 2^31 positions of 2^10 are below 2^42)
+    for (int j = 0; j < t.rot / 2; ++j)
+        ND_REQUIRE(t.f[j] <= 1024.0, "frequency %d, %g a position, is above 1024", j, t.f[j]);
+    return ND_OK;
 }
 
 // Whether writing row i at y + i*ys (w elements) can touch a row of x, other
@@ -337,10 +328,10 @@ void launches(size_t rows, size_t rpb, F f)
     for (size_t i = 0; i < rows; i += most) f(i, dim3(unsigned((std::min(most, rows - i) + rpb - 1) / rpb)));
 }
 
-int launch_turn(nd_ctx *ctx, const nd_rope *r, Rows a, const Geom &g, const char *what)
+int launch_turn(nd_ctx *ctx, const Turn &turn, Rows a, const Geom &g, const char *what)
 {
-    const int longest = a.kv ? std::max(g.QK, g.VD) : a.dim, half = r->rot_dim / 2;
-    const bool four = a.dim % 4 == 0 && (r->layout == ND_ROPE_PAIRS ? r->rot_dim % 4 == 0 : half % 4 == 0);
+    const int longest = a.kv ? std::max(g.QK, g.VD) : a.dim, half = turn.rot / 2;
+    const bool four = a.dim % 4 == 0 && (turn.layout == ND_ROPE_PAIRS ? turn.rot % 4 == 0 : half % 4 == 0);
     // four rows a block give each lane a few heads and leave blocks for all CUs (us,
     // 8000 rows of 12 + 24 heads with their read-back: 2 / 4 / 8 rows 43.6 / 41.5 /
     // 46.9; 6001 rows of 12 heads 9.5 / 8.8 / 8.9)
@@ -353,7 +344,6 @@ int launch_turn(nd_ctx *ctx, const nd_rope *r, Rows a, const Geom &g, const char
     const int lanes = longest <= 64 ? 16 : longest <= 128 ? 32 : 64, most = kThreads / lanes;
     const int heads = a.nq + (a.kv ? 2 * g.KVH : 0), turns = (heads + most - 1) / most;
     const int threads = ((heads + turns - 1) / turns * lanes + 63) / 64 * 64;
-    const Turn turn = make_turn(r);
     launches(a.rows, rpb, [&](size_t first, dim3 grid) {
         a.first = first;
         hipLaunchKernelGGL(fn, grid, dim3(threads), lds, ctx->stream, turn, a, g, int(rpb));
@@ -368,9 +358,10 @@ extern "C" {
 int nd_rope_freqs(const nd_rope *r, double *freq)
 {
     nd::clear_error();
-    if (int rc = check_rope(r)) return rc;
+    Turn t;
+    if (int rc = make_turn(r, t)) return rc;
     ND_REQUIRE(freq, "null buffer");
-    freqs(r, freq);
+    std::copy(t.f, t.f + t.rot / 2, freq);
     return ND_OK;
 }
 
@@ -378,7 +369,8 @@ int nd_rope_rows(nd_ctx *ctx, const nd_rope *r, size_t rows, const int32_t *pos,
                  size_t dim, const float *x, size_t x_stride, float *y, size_t y_stride)
 {
     ND_ENTER(ctx);
-    if (int rc = check_rope(r)) return rc;
+    Turn turn;
+    if (int rc = make_turn(r, turn)) return rc;
     ND_REQUIRE(heads > 0 && heads <= 65536, "heads %zu must be in 1..65536", heads);
     ND_REQUIRE(dim >= size_t(r->rot_dim) && dim <= kMaxDim, "dim %zu must be in rot_dim %d..%d", dim,
                r->rot_dim, kMaxDim);
@@ -400,7 +392,7 @@ int nd_rope_rows(nd_ctx *ctx, const nd_rope *r, size_t rows, const int32_t *pos,
     a.q_out_stride = y_stride;
     a.nq = int(heads);
     a.dim = int(dim);
-    return launch_turn(ctx, r, a, Geom{}, "rope_rows");
+    return launch_turn(ctx, turn, a, Geom{}, "rope_rows");
 }
 
 int nd_kv_write_rope(nd_ctx *ctx, const nd_kv_geom *g, const nd_rope *r, void *kv, size_t kv_stride,
@@ -410,7 +402,8 @@ int nd_kv_write_rope(nd_ctx *ctx, const nd_kv_geom *g, const nd_rope *r, void *k
 {
     ND_ENTER(ctx);
     if (int rc = check_geom(g)) return rc;
-    if (int rc = check_rope(r)) return rc;
+    Turn turn;
+    if (int rc = make_turn(r, turn)) return rc;
     ND_REQUIRE(r->rot_dim <= g->qk_head_dim, "rot_dim %d above qk_head_dim %d", r->rot_dim, g->qk_head_dim);
     ND_REQUIRE(per_block > 0, "per_block must be positive");
     ND_REQUIRE(g->num_heads <= 65536, "num_heads %d above 65536", g->num_heads);
@@ -449,7 +442,7 @@ int nd_kv_write_rope(nd_ctx *ctx, const nd_kv_geom *g, const nd_rope *r, void *k
     a.kv = static_cast<uint8_t *>(kv);
     a.nq = q ? g->num_heads : 0;
     a.dim = g->qk_head_dim;
-    return launch_turn(ctx, r, a, make_geom(g), "kv_write_rope");
+    return launch_turn(ctx, turn, a, make_geom(g), "kv_write_rope");
 }
 
 int nd_kv_read(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride, size_t count,

@@ -27,6 +27,7 @@ def test_frequencies(rot, theta, kw):
                                nd.rope(48, scaling="parts", factor=2.0, trained=0),
                                nd.rope(48, scaling="parts", factor=2.0, trained=8, turns=(3.0, 1.0)),
                                nd.rope(48, scaling="parts", factor=2.0, trained=8, turns=(float("nan"), 1.0)),
+                               nd.rope(48, scaling="linear", factor=1e-4), nd.rope(256, theta=1e-300),
                                nd.Rope(2, 0, 48, 1e4, 1, 0, 0, 1, 1), nd.Rope(0, 3, 48, 1e4, 1, 0, 0, 1, 1)])
 def test_frequencies_refused(r):
     with pytest.raises(nd.NeedleError) as e:
