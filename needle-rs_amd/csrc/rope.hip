@@ -22,11 +22,15 @@ using namespace ndkv;
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = kMaxDim / 2;
 
-struct Turn {
+// A rope as the kernels take it, for heads of 2 P elements or fewer: a launch
+// copies its arguments, and most heads are short.
+template <int P>
+struct TurnOf {
     int layout, rot;
     double gain;
-    double f[kMaxPairs];
+    double f[P];
 };
+using Turn = TurnOf<kMaxPairs>;
 
 // What a rope or write launch works on: rows of q heads (nq), k heads (nk)
 // and v heads (nk), any of them absent.
@@ -96,7 +100,7 @@ typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
 // lane's partners are four neighbours.  A group keeps its heads for all rows of
 // the block: q heads, then k heads, then v heads.
 template <int G, bool FOUR>
-__global__ __launch_bounds__(kThreads) void turn_kernel(Turn tn, Rows r, Geom g, int rpb)
+__global__ __launch_bounds__(kThreads) void turn_kernel(TurnOf<2 * G> tn, Rows r, Geom g, int rpb)
 {
     extern __shared__ double2 cs[];  // [rpb][rot / 2]: gain cos, gain sin
     __shared__ Place at_row[kMaxRows];
@@ -328,26 +332,39 @@ void launches(size_t rows, size_t rpb, F f)
     for (size_t i = 0; i < rows; i += most) f(i, dim3(unsigned((std::min(most, rows - i) + rpb - 1) / rpb)));
 }
 
-int launch_turn(nd_ctx *ctx, const Turn &turn, Rows a, const Geom &g, const char *what)
+template <int G>
+void launch_heads(nd_ctx *ctx, const Turn &turn, Rows a, const Geom &g, bool four)
 {
-    const int longest = a.kv ? std::max(g.QK, g.VD) : a.dim, half = turn.rot / 2;
-    const bool four = a.dim % 4 == 0 && (turn.layout == ND_ROPE_PAIRS ? turn.rot % 4 == 0 : half % 4 == 0);
     // four rows a block give each lane a few heads and leave blocks for all CUs (us,
     // 8000 rows of 12 + 24 heads with their read-back: 2 / 4 / 8 rows 43.6 / 41.5 /
     // 46.9; 6001 rows of 12 heads 9.5 / 8.8 / 8.9)
     const size_t rpb = rows_a_block(a.rows, 1024, 4);
-    const size_t lds = rpb * half * sizeof(double2);
-    auto *fn = longest <= 64    ? (four ? turn_kernel<16, true> : turn_kernel<16, false>)
-               : longest <= 128 ? (four ? turn_kernel<32, true> : turn_kernel<32, false>)
-                                : (four ? turn_kernel<64, true> : turn_kernel<64, false>);
     // as many groups as give each the same number of heads (36 heads: 12 groups)
-    const int lanes = longest <= 64 ? 16 : longest <= 128 ? 32 : 64, most = kThreads / lanes;
-    const int heads = a.nq + (a.kv ? 2 * g.KVH : 0), turns = (heads + most - 1) / most;
-    const int threads = ((heads + turns - 1) / turns * lanes + 63) / 64 * 64;
+    const int most = kThreads / G, heads = a.nq + (a.kv ? 2 * g.KVH : 0), turns = (heads + most - 1) / most;
+    const int threads = ((heads + turns - 1) / turns * G + 63) / 64 * 64;
+    TurnOf<2 * G> t;
+    t.layout = turn.layout;
+    t.rot = turn.rot;
+    t.gain = turn.gain;
+    std::copy(turn.f, turn.f + turn.rot / 2, t.f);
+    auto *fn = four ? turn_kernel<G, true> : turn_kernel<G, false>;
     launches(a.rows, rpb, [&](size_t first, dim3 grid) {
         a.first = first;
-        hipLaunchKernelGGL(fn, grid, dim3(threads), lds, ctx->stream, turn, a, g, int(rpb));
+        hipLaunchKernelGGL(fn, grid, dim3(threads), rpb * (turn.rot / 2) * sizeof(double2), ctx->stream, t, a, g,
+                           int(rpb));
     });
+}
+
+int launch_turn(nd_ctx *ctx, const Turn &turn, const Rows &a, const Geom &g, const char *what)
+{
+    const int longest = a.kv ? std::max(g.QK, g.VD) : a.dim;
+    const bool four = a.dim % 4 == 0 && (turn.layout == ND_ROPE_PAIRS ? turn.rot % 4 == 0 : turn.rot % 8 == 0);
+    if (longest <= 64)
+        launch_heads<16>(ctx, turn, a, g, four);
+    else if (longest <= 128)
+        launch_heads<32>(ctx, turn, a, g, four);
+    else
+        launch_heads<64>(ctx, turn, a, g, four);
     return nd::check_launch(what);
 }
 

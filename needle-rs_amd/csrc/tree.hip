@@ -175,7 +175,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     const uint8_t *blk = tr.kv + size_t(ses) * tr.kv_stride;
     const rows_t kb = rows_at(blk + size_t(kvh) * g.cap * QK, uint32_t(g.cap) * QK);
     const rows_t vb = rows_at(blk + g.v_off + size_t(kvh) * g.cap * VD, uint32_t(g.cap) * VD);
-    // K scales, and vs_off - ks_off bytes on (below 2^32: KVH cap 4) the V scales
+    // K scales, and vs_off - ks_off bytes on (KVH cap 4, below 2^32) the V scales
     const uint32_t to_vs = uint32_t(g.vs_off - g.ks_off);
     const rows_t sb = rows_at(blk + g.ks_off + size_t(kvh) * g.cap * 4, to_vs + uint32_t(g.cap) * 4);
     const uint32_t cap = uint32_t(g.cap);
@@ -624,6 +624,9 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     ND_REQUIRE(kv && base && lo && mask && q && out, "null buffer");
     ND_REQUIRE(count <= 65535, "count %zu above 65535", count);
     ND_REQUIRE(g->num_heads <= 4096, "num_heads %d above 4096", g->num_heads);
+    // a buffer of one head's scales reaches from its K scales to its V scales
+    ND_REQUIRE(size_t(g->num_kv_heads) * g->cap <= size_t(1) << 29, "%d kv heads x cap %d above 2^29",
+               g->num_kv_heads, g->cap);
     ND_REQUIRE((reinterpret_cast<uintptr_t>(kv) & 255) == 0 && kv_stride % 256 == 0,
                "kv blocks must be 256-byte aligned");
     const Plan p = plan_of(ctx, g, count, nodes);

@@ -135,6 +135,27 @@ def test_windows_and_wrapped_rings(ctx, H, KVH, QK, nodes, base, cap, window, qu
 
 
 @pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("H,KVH,QK", [(12, 2, 48), (12, 12, 64), (5, 1, 64)])
+@pytest.mark.parametrize("nodes,base,cap,reach", [(40, 170, 100, 60), (64, 95, 128, 64), (256, 1900, 1000, 744),
+                                                  (33, 40, 64, 31), (5, 62, 64, 59), (32, 32, 48, 16), (100, 50, 101, 1),
+                                                  (97, 1097, 98, 1), (2, 63, 64, 0), (70, 999, 1000, 0)])
+def test_a_tree_across_the_rings_end(ctx, H, KVH, QK, nodes, base, cap, reach, quant):
+    """Trees whose nodes lie on both sides of the ring's end, in front of every
+    part of a word of the mask."""
+    rng = np.random.default_rng(nodes + base)
+    assert base % cap + nodes > cap and reach + nodes <= cap
+    g, blk, nb = _block(ctx, rng, H, KVH, QK, cap, base + nodes, 2)
+    bases = np.array([base, base - 1])
+    length = np.array([nodes, max(nodes - 2, 1)])
+    see = np.concatenate([R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes),
+                          rng.integers(0, 2, (1, nodes, nodes)).astype(np.uint8)])
+    lo = bases[:, None] - rng.integers(0, reach + 1, (2, nodes))
+    lo[1] = np.maximum(lo[1], base + nodes - cap)  # what is there of the shorter one
+    q = rng.normal(size=(2, nodes, H * QK)).astype(np.float32)
+    _check(ctx, g, blk, nb, bases, lo, see, q, length, quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("sessions,nodes,base", [(65, 16, 300), (130, 5, 90), (300, 2, 40), (9, 30, 2000)])
 def test_many_sessions(ctx, sessions, nodes, base, quant):
     """Every launch shape: few sessions with long spans, many with short ones."""
@@ -254,6 +275,26 @@ def test_weight_on_a_row_of_small_values(ctx, quant):
     assert np.linalg.norm(got - want) <= 8e-5 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("quant", [False, True])
+def test_queries_that_are_no_numbers(ctx, quant):
+    """A head with a NaN or an infinity gives NaN, its neighbours do not."""
+    rng = np.random.default_rng(12)
+    nodes, base = 5, 70
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 80, base + nodes, 1)
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    q = rng.normal(size=(1, nodes, 12, 48)).astype(np.float32)
+    q[0, 1, 3, 20], q[0, 2, 0, 0], q[0, 4, 11, 47] = np.nan, np.inf, -np.inf
+    q[0, 3, 5] = 0.0
+    args = (ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(np.zeros((1, nodes), np.int32)), dev(R.words_of(see)))
+    got = host(nd.attend_tree_i8(*args, dev(q.reshape(1, nodes, -1)), quant_query=quant)).reshape(nodes, 12, 64)
+    gone = np.zeros((nodes, 12), bool)
+    gone[1, 3] = gone[2, 0] = gone[4, 11] = True
+    assert np.isnan(got[gone]).all()
+    want = _want(g, host(blk), nb, [base], None, np.zeros((1, nodes), int), see,
+                 np.where(gone[None, :, :, None], 0, q).reshape(1, nodes, -1), quant).reshape(nodes, 12, 64)
+    assert np.abs(got[~gone] - want[~gone]).max() <= TOL
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 def test_any_scale(ctx, scale):
     rng = np.random.default_rng(11)
@@ -360,6 +401,10 @@ def test_refusals(ctx):
                                               torch.zeros(2, 4, 18 * 64, device="cuda"),
                                               out=torch.zeros(2, 4, 18 * 128, device="cuda")))
     refused("aligned", lambda: nd.attend_tree_i8(ctx, g, blk[64:], nb, z(1), z(1, 4), z(1, 4, 1), q[:1]))
+    huge = nd.kv_geom(96, 48, 48, 64, 1 << 24)
+    rc = nd.lib().nd_attend_tree_i8(ctx.h, huge, blk.data_ptr(), 0, 1, 1, blk.data_ptr(), None, blk.data_ptr(),
+                                    blk.data_ptr(), q.data_ptr(), 1.0, 0, q.data_ptr(), None, 0)
+    assert rc == nd.ND_ERR_ARG and "2^29" in nd.last_error()
     ok = (z(2), z(2, 4), z(2, 4, 1), q)
     assert nd.attend_tree_i8(ctx, g, blk, nb, *ok).shape == (2, 4, 768)
     for args, kw in (((z(1), *ok[1:]), {}), ((ok[0], z(2, 3), *ok[2:]), {}), ((*ok[:2], z(2, 3, 1), q), {}),
