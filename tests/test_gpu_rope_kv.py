@@ -177,6 +177,28 @@ def test_write_rope(ctx, H, KVH, QK, VD, rot, blocks, per, cap, layout):
     assert np.array_equal(host(t)[:, H * QK:], buf[:, H * QK:])
 
 
+@pytest.mark.parametrize("H,KVH,QK,VD", [(12, 2, 48, 64), (3, 3, 96, 128), (2, 1, 256, 16)])
+def test_write_of_values_that_are_no_numbers(ctx, H, KVH, QK, VD):
+    """NaN, infinities, zeros and values next to fp32's ends: the codes and scales
+    that kv_write stores for the same turned rows, bit for bit."""
+    rng = np.random.default_rng(QK)
+    n = 9
+    k, v = (rng.normal(size=(n, KVH * d)).astype(np.float32) for d in (QK, VD))
+    for x in (k, v):
+        x[0, 3], x[1, 5], x[2, 0], x[3, :] = np.nan, np.inf, -np.inf, 0.0
+        x[4] *= 1e38
+        x[5] *= 1e-38
+        x[6] *= 1e-44
+        x[7, :4] = [3e38, -3e38, 1e-45, 0.0]
+    r, g = nd.rope(QK - 16 if QK > 48 else 48, layout="pairs"), nd.kv_geom(H, KVH, QK, VD, 16)
+    a, _ = _blocks(g, 1)
+    b, _ = _blocks(g, 1)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    nd.kv_write_rope(ctx, g, r, a, 0, pos, dev(k), dev(v), rot_pos=pos + 70, per_block=n)
+    nd.kv_write(ctx, g, b, 0, pos, nd.rope_rows(ctx, r, dev(k), pos + 70, KVH), dev(v))
+    assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("H,KVH,QK,VD", [(12, 2, 48, 64), (12, 12, 64, 64), (5, 1, 16, 256), (6, 3, 96, 16)])
 @pytest.mark.parametrize("blocks,per,cap", [(1, 1, 1), (3, 5, 17), (2, 301, 400)])
 def test_read_back(ctx, H, KVH, QK, VD, blocks, per, cap):
