@@ -8,7 +8,12 @@
 // works out each (row, pair) once, in LDS, for all heads of the row.  A group of
 // 16, 32 or 64 lanes takes a head vector, four elements a lane, so that a code's
 // scale is a maximum over the group's registers.
-// All three calls are bound by memory: a value is read and written once.
+// (Lane moves stay within a group, whose lanes are all there; other groups of a wave
+// may be elsewhere.)
+// All three calls are bound by memory, a value read and written once, results past
+// the caches: 6001 rows of 12 x 64 8.2 us = 4.5 TB/s; 8000 rows of 12 q, 12 k and 12
+// v heads 26 us = 4.3 TB/s, their read-back 14; 16 windows of 8001 positions of 2
+// kv heads read 24.4 us = 6.0 TB/s.
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
 

@@ -24,6 +24,15 @@
 //           instead, all 24 bits at any size: the values of one position may be
 //           far smaller than its neighbours' and yet decide the output.
 // Sums and statistics are fp32.
+//
+// What bounds it: where the cache streams (one query head a kv head) HBM, 64
+// sessions x 13 nodes x 12 heads x 64 at 2048 positions 38.9 us = 5.0 TB/s; with
+// grouped heads the VALU, about 146 operations a chunk (the exponentials 32, V's
+// conversion 40), 64 x 16 nodes x 12 heads over 2 at 2000 21.1 us; small trees the
+// 7 us from launch to merge.  One column tile a wave at four waves a SIMD: two
+// tiles, which share V's conversion but leave three waves, gain at 100 million
+// scores (128 sessions x 4000 65.9 -> 57.4) and lose below (64 x 2000 23.9 -> 26.7,
+// 12 kv heads 32.1 -> 44.0).
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
 
@@ -263,7 +272,8 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     load_v();
 
     // ---- the query operand, while the first chunk is on its way ----
-    float cf;                         // factor of a score, in bits
+    float cf0;                        // factor of a score, in bits, is cf0 2^(kexp - sh)
+    int sh;
     intx4_t qi;                       // QQ: codes
     uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
     {
@@ -292,10 +302,11 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
                 dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
             }
             qi = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
-            cf = qs * tr.scale2;
+            sh = -__builtin_amdgcn_frexp_expf(qs);
+            cf0 = __builtin_amdgcn_ldexpf(qs, sh) * tr.scale2;
         } else {
             // the head in 2^14 .. 2^15, so that the second pieces are normal numbers
-            const int sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
+            sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
 #pragma unroll
             for (int e = 0; e < SL; ++e) {
                 nan = v[e] - v[e] != 0.0f ? NAN : nan;
@@ -303,15 +314,19 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             }
 #pragma unroll
             for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[0][e / 2], qp[1][e / 2]);
-            cf = __builtin_amdgcn_ldexpf(tr.scale2, -sh);
+            cf0 = tr.scale2;
         }
-        // (a factor of 0 would make no number of a score of -inf)
-        if (cf == 0.0f) cf = 0x1p-126f;
         // NaN where the query has one (an infinity gives one too)
         nan += ndl::wave_xor<16>(nan);
         nan += ndl::wave_xor<32>(nan);
-        cf += nan;
+        cf0 += nan;
     }
+    // (a factor of 0 would make no number of a score of -inf)
+    auto factor = [&](int k) {
+        const float c = __builtin_amdgcn_ldexpf(cf0, k - sh);
+        return c == 0.0f ? 0x1p-126f : c;
+    };
+    float cf = factor(0);
 
     // m_run: a score of the column, no other so far is more than kAhead bits
     // above it (lim, in the scores' units); mu = m_run cf.  A new maximum is
@@ -357,8 +372,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             shift += was - now;
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
             m_run = __builtin_amdgcn_ldexpf(m_run, kexp - kn);
-            cf = __builtin_amdgcn_ldexpf(cf, kn - kexp);
-            if (cf == 0.0f) cf = 0x1p-126f;
+            cf = factor(kn);
             lim = m_run == -INFINITY ? -INFINITY : m_run + kAhead * __builtin_amdgcn_rcpf(cf);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
