@@ -11,9 +11,9 @@
 // (Lane moves stay within a group, whose lanes are all there; other groups of a wave
 // may be elsewhere.)
 // All three calls are bound by memory, a value read and written once, results past
-// the caches: 6001 rows of 12 x 64 8.2 us = 4.5 TB/s; 8000 rows of 12 q, 12 k and 12
-// v heads 26 us = 4.3 TB/s, their read-back 14; 16 windows of 8001 positions of 2
-// kv heads read 24.4 us = 6.0 TB/s.
+// the caches (kernel times): 6001 rows of 12 x 64 7.5 us = 4.9 TB/s; 8000 rows of 12
+// q, 12 k and 12 v heads of 64 25.4 us = 4.4 TB/s, their read-back 12.5 us = 5.0;
+// 16 windows of 8001 positions of 2 kv heads, 48 and 64 long, read in 23.9 us = 6.1.
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
 
@@ -37,8 +37,8 @@ struct TurnOf {
 };
 using Turn = TurnOf<kMaxPairs>;
 
-// What a rope or write launch works on: rows of q heads (nq), k heads (nk)
-// and v heads (nk), any of them absent.
+// What a rope or write launch works on: rows of nq q heads, and of a
+// cache's k and v heads, any of them absent.
 struct Rows {
     size_t rows, first, per_block;  // first: the launch's first row
     const int32_t *pos, *rot_pos;
