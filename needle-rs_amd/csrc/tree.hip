@@ -643,6 +643,9 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
                g->num_kv_heads, g->cap);
     ND_REQUIRE((reinterpret_cast<uintptr_t>(kv) & 255) == 0 && kv_stride % 256 == 0,
                "kv blocks must be 256-byte aligned");
+    const uintptr_t qa = reinterpret_cast<uintptr_t>(q), oa = reinterpret_cast<uintptr_t>(out);
+    const size_t heads = count * nodes * g->num_heads * sizeof(float);
+    ND_REQUIRE(qa + heads * g->qk_head_dim <= oa || oa + heads * VD <= qa, "out overlaps q");
     const Plan p = plan_of(ctx, g, count, nodes);
     Tree t{};
     t.kv_stride = kv_stride;
@@ -677,10 +680,10 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
         t.q = q + rows * g->num_heads * g->qk_head_dim;
         t.out = out + rows * g->num_heads * VD;
         if (part) {
-            const size_t heads = m * nodes * g->num_heads;
+            const size_t outs = m * nodes * g->num_heads * p.splits;
             t.part_o = part;
-            t.part_ml = part + heads * p.splits * VD;
-            part = t.part_ml + heads * p.splits * 2;
+            t.part_ml = part + outs * VD;
+            part = t.part_ml + outs * 2;
         }
         t.units = uint32_t(m * g->num_kv_heads * p.splits);
         hipLaunchKernelGGL(fn, dim3(8, unsigned(p.tiles), unsigned((t.units + 7) / 8)), dim3(p.nw * 64), 0, ctx->stream, kg, t);

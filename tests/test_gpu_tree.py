@@ -419,3 +419,17 @@ def test_refusals(ctx):
     with pytest.raises(ValueError):
         nd.attend_tree_i8(ctx, g, blk[:nb], nb, *ok)  # two sessions, one block
     assert nd.attend_tree_i8(ctx, g, blk, nb, z(0), z(0, 4), z(0, 4, 1), q[:0]).shape == (0, 4, 768)
+
+
+def test_an_output_over_the_queries_is_refused(ctx):
+    g = nd.kv_geom(12, 12, 64, 64, 64)
+    blk, nb = nd.kv_alloc(g, 2)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    both = torch.zeros(4 * 4 * 768, device="cuda")
+    part = lambda at: both[at * 4 * 768:][:2 * 4 * 768].view(2, 4, 768)  # noqa: E731
+    args = ctx, g, blk, nb, z(2), z(2, 4), z(2, 4, 1)
+    for q_at, out_at in ((0, 0), (0, 1), (2, 1)):
+        with pytest.raises(nd.NeedleError, match="overlaps"):
+            nd.attend_tree_i8(*args, part(q_at), out=part(out_at))
+    for q_at, out_at in ((0, 2), (2, 0)):
+        nd.attend_tree_i8(*args, part(q_at), out=part(out_at))
