@@ -71,7 +71,7 @@ struct Tree {
     int nodes, words, splits, rep;
     uint32_t units;
     Divisor by_splits, by_kvh;
-    float scale2;  // |scale| log2(e)
+    float scale2;  // |scale| log2(e); below 0 where scale is no number
     int negative;  // scale < 0
 };
 
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     load_v();
 
     // ---- the query operand, while the first chunk is on its way ----
-    float cf0;                        // factor of a score, in bits, is cf0 2^(kexp - sh)
+    float cf0;                        // factor of a score, in bits, is |cf0| 2^(kexp - sh)
     int sh;
     intx4_t qi;                       // QQ: codes
     uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
@@ -316,14 +316,16 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[0][e / 2], qp[1][e / 2]);
             cf0 = tr.scale2;
         }
-        // NaN where the query has one (an infinity gives one too)
+        // a query that has a NaN (or an infinity, which gives one) makes no number
+        // of what its node sees, and zeros of nothing: cf0's sign says so until the
+        // sum is known
         nan += ndl::wave_xor<16>(nan);
         nan += ndl::wave_xor<32>(nan);
-        cf0 += nan;
+        cf0 = nan != nan ? -__builtin_fabsf(cf0) : cf0;
     }
     // (a factor of 0 would make no number of a score of -inf)
     auto factor = [&](int k) {
-        const float c = __builtin_amdgcn_ldexpf(cf0, k - sh);
+        const float c = __builtin_amdgcn_ldexpf(__builtin_fabsf(cf0), k - sh);
         return c == 0.0f ? 0x1p-126f : c;
     };
     float cf = factor(0);
@@ -509,10 +511,11 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     // column, four values each, put them together ----
     l_run += ndl::wave_xor<16>(l_run);
     l_run += ndl::wave_xor<32>(l_run);
+    if (bad || (__float_as_int(cf0) < 0 && l_run != 0.0f)) l_run = NAN;
     if (qd == 0) {
         // from here on the maximum is in bits
         mm[w][n] = m_run == -INFINITY ? -INFINITY : mu;
-        ml[w][n] = bad ? NAN : l_run;
+        ml[w][n] = l_run;
     }
     // lane (n, qd) holds V columns 16 qd + 4 i + c
 #pragma unroll
@@ -655,7 +658,7 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     t.by_splits = Divisor::of(uint32_t(p.splits));
     t.by_kvh = Divisor::of(uint32_t(g->num_kv_heads));
     t.splits = int(p.splits);
-    t.scale2 = float(double(scale < 0 ? -scale : scale) * 1.4426950408889634);
+    t.scale2 = scale == scale ? float(double(scale < 0 ? -scale : scale) * 1.4426950408889634) : -1.0f;
     t.negative = scale < 0;
     float *part = nullptr;
     if (p.splits > 1) {

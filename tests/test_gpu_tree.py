@@ -433,3 +433,28 @@ def test_an_output_over_the_queries_is_refused(ctx):
             nd.attend_tree_i8(*args, part(q_at), out=part(out_at))
     for q_at, out_at in ((0, 2), (2, 0)):
         nd.attend_tree_i8(*args, part(q_at), out=part(out_at))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("sessions,base", [(1, 0), (3, 70), (1, 3000), (300, 200)])
+def test_nothing_to_see_for_a_query_that_is_no_number(ctx, sessions, base, quant):
+    """A node that attends to nothing gets zeros whatever its query holds and
+    whatever the nodes beside it read, and with a scale that is no number."""
+    rng = np.random.default_rng(base)
+    nodes = 5
+    g, blk, _ = _block(ctx, rng, 12, 2, 48, base + nodes, base + nodes, 1)
+    see = np.repeat(np.tril(np.ones((nodes, nodes), np.uint8))[None], sessions, 0)
+    see[:, [1, 3]] = 0
+    lo = np.zeros((sessions, nodes), np.int32)
+    lo[:, 1], lo[:, 3] = base, base + 9
+    q = rng.normal(size=(sessions, nodes, 12, 48)).astype(np.float32)
+    q[:, 1, :, 7], q[:, 3, ::2, 40], q[:, 3, 1::2, 0] = np.nan, np.inf, -np.inf
+    q[:, 2, 4, 47] = np.nan  # sees what the root sees
+    args = (ctx, g, blk, 0, dev(np.full(sessions, base, np.int32)), dev(lo), dev(R.words_of(see)),
+            dev(q.reshape(sessions, nodes, -1)))
+    got = host(nd.attend_tree_i8(*args, quant_query=quant)).reshape(sessions, nodes, 12, 64)
+    assert not got[:, [1, 3]].any()
+    assert np.isnan(got[:, 2, 4]).all()
+    assert np.isfinite(got[:, [0, 4]]).all() and np.isfinite(np.delete(got[:, 2], 4, 1)).all()
+    got = host(nd.attend_tree_i8(*args, quant_query=quant, scale=float("nan")))
+    assert not got[:, [1, 3]].any() and np.isnan(got[:, [0, 2, 4]]).all()
