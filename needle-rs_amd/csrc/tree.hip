@@ -148,7 +148,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     constexpr int LD = VD + 4;
     __shared__ __align__(16) float sc_s[NW][64];
     __shared__ __align__(16) float mo[NW][kCols][LD];
-    __shared__ float mm[NW][kCols], ml[NW][kCols];
+    __shared__ floatx4_t ms[NW][kCols];  // maximum, more, weight
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
@@ -512,31 +512,38 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     l_run += ndl::wave_xor<16>(l_run);
     l_run += ndl::wave_xor<32>(l_run);
     if (bad || (__float_as_int(cf0) < 0 && l_run != 0.0f)) l_run = NAN;
-    if (qd == 0) {
-        // from here on the maximum is in bits
-        mm[w][n] = m_run == -INFINITY ? -INFINITY : mu;
-        ml[w][n] = l_run;
-    }
+    // the sums are left as 2^more of what has a weight of 1/2 to 1: of values near
+    // fp32's end the sum may be beyond it, the mean is not
+    const int more = __builtin_amdgcn_frexp_expf(l_run);
+    // (from here on the maximum is in bits)
+    if (qd == 0)
+        ms[w][n] = floatx4_t{m_run == -INFINITY ? -INFINITY : mu, float(more), __builtin_amdgcn_ldexpf(l_run, -more), 0.0f};
     // lane (n, qd) holds V columns 16 qd + 4 i + c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         floatx4_t o;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1);
+        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more);
         *reinterpret_cast<floatx4_t *>(&mo[w][n][16 * qd + 4 * i]) = o;
     }
     __syncthreads();
     const int col = t >> 4, fo = int(tile) * kCols + col;
     if (col >= kCols || fo >= ncols) return;
+    // Against a maximum 2^3 above the largest, so that no sum of eight leaves the
+    // values' range.  -inf: sums are 0, or NaN where a score was.  (m + more may be
+    // rounded, M with it; m - M is not.)
     float M = -INFINITY, L = 0.0f;
-    floatx4_t O{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, mm[i][col]);
+    floatx4_t O{0.0f, 0.0f, 0.0f, 0.0f}, z[NW];
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-        // -inf: sums are 0, or NaN where a score was
-        const float m = mm[i][col], by = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
-        L += ml[i][col] * by;
+        z[i] = ms[i][col];
+        M = fmaxf(M, z[i][0] + z[i][1]);
+    }
+    M += 3.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const float by = z[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(z[i][0] - M + z[i][1]);
+        L += z[i][2] * by;
         O += *reinterpret_cast<const floatx4_t *>(&mo[i][col][4 * (t & 15)]) * by;
     }
     const int no = node_of(fo);
@@ -564,16 +571,22 @@ __global__ __launch_bounds__(256) void tree_join_kernel(int H, Tree tr, size_t t
     const int len = tr.length ? tr.length[ses] : tr.nodes;
     // rows behind the tree's end have no partials and are left as they are
     if (len >= 0 && len <= tr.nodes && int(row - ses * tr.nodes) >= len) return;
-    float M = -INFINITY, L = 0.0f, O = 0.0f;
-    for (int s = 0; s < tr.splits; ++s) M = fmaxf(M, tr.part_ml[2 * (oh * tr.splits + s)]);
-    for (int s = 0; s < tr.splits; ++s) {
-        const size_t at = oh * tr.splits + s;
-        const float m = tr.part_ml[2 * at], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
-        L += tr.part_ml[2 * at + 1] * f;
-        O += tr.part_o[at * VD + lane] * f;
+    // a lane a split, then a lane a column
+    float m = -INFINITY, l = 0.0f;
+    if (lane < tr.splits) {
+        const size_t at = oh * tr.splits + lane;
+        m = tr.part_ml[2 * at];
+        l = tr.part_ml[2 * at + 1];
     }
-    tr.out[oh * VD + lane] = L == 0.0f ? 0.0f : O / L;
+    const float M = wave_max(m), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M), L = wave_sum(l * f);
+    const float by = L == 0.0f ? 0.0f : f / L;
+    float O = 0.0f;
+    for (int s = 0; s < tr.splits; ++s)
+        O += tr.part_o[(oh * tr.splits + s) * VD + lane] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(by), s));
+    tr.out[oh * VD + lane] = O;
 }
+
+constexpr int kMaxSplits = 64;  // a lane each in the join
 
 struct Plan {
     int nw;
@@ -601,7 +614,7 @@ Plan plan_of(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
     // 18.5 / 15.8 / 16.7; 16 x 1000 in 1 / 2 8.8 / 11.9)
     const size_t fill = cus * 8 / (blocks * p.nw);
     p.splits = 1;
-    while (p.splits < fill && p.splits < 64 && (p.splits + 1) * (p.splits + 1) * p.nw <= 2 * chunks) ++p.splits;
+    while (p.splits < fill && p.splits < kMaxSplits && (p.splits + 1) * (p.splits + 1) * p.nw <= 2 * chunks) ++p.splits;
     if (chunks * (p.splits - 1) < 6 * p.nw * p.splits) p.splits = 1;
     return p;
 }

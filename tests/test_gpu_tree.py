@@ -458,3 +458,22 @@ def test_nothing_to_see_for_a_query_that_is_no_number(ctx, sessions, base, quant
     assert np.isfinite(got[:, [0, 4]]).all() and np.isfinite(np.delete(got[:, 2], 4, 1)).all()
     got = host(nd.attend_tree_i8(*args, quant_query=quant, scale=float("nan")))
     assert not got[:, [1, 3]].any() and np.isnan(got[:, [0, 2, 4]]).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("sessions", [1, 300])
+def test_sums_of_large_values(ctx, sessions, quant):
+    """Thousands of values near fp32's end: their mean is there, their sum is not."""
+    rng = np.random.default_rng(15)
+    nodes, base = 2, 4000
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, base + nodes, base + nodes, 1, 0.05, 5e37)
+    off = nd.kv_offsets(g)
+    v = blk[off["v"]:off["v"] + 2 * (base + nodes) * 64].view(torch.int8)
+    v.copy_(v.abs())
+    see = np.repeat(np.tril(np.ones((nodes, nodes), np.uint8))[None], sessions, 0)
+    q = rng.normal(size=(sessions, nodes, 12 * 48)).astype(np.float32)
+    lo = np.zeros((sessions, nodes), np.int32)
+    got = host(nd.attend_tree_i8(ctx, g, blk, 0, dev(np.full(sessions, base, np.int32)), dev(lo),
+                                 dev(R.words_of(see)), dev(q), quant_query=quant))
+    want = _want(g, host(blk), nb, [base], None, lo[:1], see[:1], q[:1], quant)
+    assert np.abs(got[0] - want[0]).max() <= TOL * 5e37
