@@ -10,15 +10,15 @@
 // word of the mask.
 //   scores  S[pos][col] = K Q^T, v_mfma 16x16, A = 16 positions' int8 rows.
 //           With quant_query both sides are codes and the dot is an exact
-//           integer; else the fp32 query is two f16 pieces, 22 bits and more
-//           of a head scaled by a power of two (error 2^-23 of an element, as
-//           much as fp32's own steps leave a sum of products).
+//           integer; else the fp32 query is two f16 pieces of a head scaled by
+//           a power of two (error 2^-23 of an element at most, either way, less
+//           than fp32's own steps leave a sum of products).
 //   softmax scores stay without the column's factor cf (scale, query scale):
 //           the maximum m is kept before it and e = 2^(fma(t, cf, -m cf)).
 //   values  O^T[v][col] = V^T P^T: a score tile's result layout is the layout
 //           of the weights the product needs.  MFMA c takes V columns 4 n + c,
 //           a dword a position.  The weights e vs are two f16 pieces, of which
-//           the first 22 bits are kept (and none below 2^-34 of the largest V
+//           the first 23 bits are kept (and none below 2^-35 of the largest V
 //           scale met so far), V's codes are exact in f16.  A chunk with a V
 //           scale 2^-9 or less of that largest takes the fp32 matrix product
 //           instead, all 24 bits at any size: the values of one position may be
@@ -48,6 +48,7 @@ constexpr int VD = 64, kCols = 16;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float floatx2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef int intx4_t __attribute__((ext_vector_type(4)));
@@ -86,15 +87,25 @@ __device__ inline float max3(float a, float b, float c)
     return r;
 }
 
-// x0, x1 (below 2^16) as two f16 pairs.  (Written out, the remainder is a
-// conversion and a subtraction; v_fma_mix_f32 does both.)
+// Two numbers as an f16 pair, each to the nearest.
+__device__ inline uint32_t f16_two(float x0, float x1)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2_t{x0, x1}), f16x2_t));
+}
+
+// x0, x1 (below 2^15) as two f16 pairs.  The first piece is off by 2^-11 of x or
+// less and the remainder is exact, so that the second, to the nearest too, leaves
+// 2^-23 of x at most (of x below 1/4, whose second piece is subnormal, 2^-25) on
+// either side: cut off, the pieces left up to 6 2^-24 and always too little.
+// (Written out, the remainder is a conversion and a subtraction; v_fma_mix_f32
+// does both.)
 __device__ inline void split2(float x0, float x1, uint32_t &h, uint32_t &l)
 {
-    h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    h = f16_two(x0, x1);
     float r0, r1;
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x0));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(x1));
-    l = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    l = f16_two(r0, r1);
 }
 
 // The sign bits flipped, code c is c + 128; byte c of two dwords as f16 pairs:
