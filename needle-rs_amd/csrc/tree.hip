@@ -17,12 +17,14 @@
 //           the maximum m is kept before it and e = 2^(fma(t, cf, -m cf)).
 //   values  O^T[v][col] = V^T P^T: a score tile's result layout is the layout
 //           of the weights the product needs.  MFMA c takes V columns 4 n + c,
-//           a dword a position.  The weights e vs are two f16 pieces, of which
-//           the first 23 bits are kept (and none below 2^-35 of the largest V
-//           scale met so far), V's codes are exact in f16.  A chunk with a V
-//           scale 2^-9 or less of that largest takes the fp32 matrix product
-//           instead, all 24 bits at any size: the values of one position may be
-//           far smaller than its neighbours' and yet decide the output.
+//           a dword a position.  The weights e vs are two f16 pieces, 23 bits of
+//           every weight that is not 2^-24 or less of the column's largest so far
+//           (a maximum on values next to zero is no measure of the rest: the
+//           sums then go on against a lower one); V's codes are exact in f16.  A
+//           chunk with a V scale 2^-9 or less of the largest met takes the fp32
+//           matrix product instead, all 24 bits at any size: the values of one
+//           position may be far smaller than its neighbours' and yet decide the
+//           output.
 // Sums and statistics are fp32.
 //
 // What bounds it: where the cache streams (one query head a kv head) HBM, 64
@@ -145,6 +147,13 @@ __device__ inline uint32_t here(uint32_t x)
 }
 
 __device__ inline bool any_of(bool b) { return __builtin_amdgcn_ballot_w64(b) != 0; }
+
+// The same, not 0 where it is so.
+__device__ inline uint32_t any32(bool b)
+{
+    const uint64_t m = __builtin_amdgcn_ballot_w64(b);
+    return uint32_t(m) | uint32_t(m >> 32);
+}
 
 template <typename T>
 __device__ inline T vec4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
@@ -289,6 +298,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
     {
         if (tr.negative) {
+            asm volatile("");  // (a branch)
 #pragma unroll
             for (int e = 0; e < SL; ++e) v[e] = -v[e];
         }
@@ -341,9 +351,9 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     };
     float cf = factor(0);
 
-    // m_run: a score of the column, no other so far is more than kAhead bits
-    // above it (lim, in the scores' units); mu = m_run cf.  A new maximum is
-    // taken, and the sums scaled, only where one gets ahead of that
+    // m_run: a score of the column that the sums are against (mu = m_run cf, in
+    // bits).  Another is taken, and the sums scaled, where one gets more than kAhead
+    // bits ahead of it (lim, in the scores' units), or all stay far behind
     constexpr float kAhead = 5.0f;
     float m_run = -INFINITY, lim = -INFINITY, mu = 0.0f, l_run = 0.0f;
     floatx4_t acc[4];
@@ -355,6 +365,15 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     int kexp = 0, vexp = 0;
     float top = 0.0f;                   // lanes below 32: 2^kexp, the others: 2^vexp
     int shift = lane < 32 ? 0 : 10;
+    // Weights below 2^-2 lose bits of their second pieces.  Where a column has met a
+    // larger one in a product of pieces, those bits are none of the result's, and it
+    // meets one (an e of 1 and a V scale of 2 units or more) with each new m_run; not
+    // where that lies in a chunk of small values, or where the unit of weights has
+    // grown since, by more than 2^3.  From then on (watch: lim lets every chunk in)
+    // a column goes on against the next chunk's own maximum, which may lie far below:
+    // its sums are multiplied (up to 2^100)
+    uint32_t watch = 0;
+    int vmet = 0;                       // vexp then
 
     for (; ch < nch; ch += step) {
         // ---- the positions each column sees ----
@@ -384,9 +403,13 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             top = h > top ? (now > 127 ? 0x1.fffffep127f : __builtin_amdgcn_ldexpf(1.0f, now)) : top;
             shift += was - now;
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
+            if (vn > vmet + 3 || !any32(l_run > 0.0f)) {
+                watch |= any32(l_run > 0.0f);
+                vmet = vn;
+            }
             m_run = __builtin_amdgcn_ldexpf(m_run, kexp - kn);
             cf = factor(kn);
-            lim = m_run == -INFINITY ? -INFINITY : m_run + kAhead * __builtin_amdgcn_rcpf(cf);
+            lim = watch || m_run == -INFINITY ? -INFINITY : m_run + kAhead * __builtin_amdgcn_rcpf(cf);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -396,7 +419,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
         }
         sc = __builtin_amdgcn_ldexpf(sc, shift);
         const uint32_t few = uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32);
-        const bool small = (left < 32 ? few & ((1u << left) - 1u) : few) != 0;
+        uint32_t small = left < 32 ? few & ((1u << left) - 1u) : few;
         sc_s[w][lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -463,13 +486,25 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
         }
         const float m8 = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[7]));
         if (any_of(m8 > lim)) {
-            float m = max3(m8, m_run, ndl::wave_xor<16>(m8));
-            m = fmaxf(m, ndl::wave_xor<32>(m));
-            const float mu_new = m == -INFINITY ? 0.0f : m * cf;
+            // a row of zeros has a scale of 1, which is no measure of its values
+            small |= uint32_t(__builtin_amdgcn_ballot_w64(sc == __builtin_amdgcn_ldexpf(1.0f, shift)) >> 32);
+            float m_new = max3(m8, m_run, ndl::wave_xor<16>(m8));
+            m_new = fmaxf(m_new, ndl::wave_xor<32>(m_new));
+            if (watch && !small) [[unlikely]] {
+                float m = fmaxf(m8, ndl::wave_xor<16>(m8)), l = fmaxf(l_run, ndl::wave_xor<16>(l_run));
+                m = fmaxf(m, ndl::wave_xor<32>(m));
+                l = fmaxf(l, ndl::wave_xor<32>(l));
+                const float behind = mu - m * cf;
+                const bool down = (m > -INFINITY) & (behind + float(__builtin_amdgcn_frexp_expf(l)) < 100.0f);
+                m_new = down ? m : m_new;
+                watch = any32((m_new > -INFINITY) & !down);
+            }
+            watch |= small;
+            const float mu_new = m_new == -INFINITY ? 0.0f : m_new * cf;
             // nothing is summed yet where there was no maximum
             const float al = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu - mu_new);
-            m_run = m;
-            lim = m == -INFINITY ? -INFINITY : m + kAhead * __builtin_amdgcn_rcpf(cf);
+            m_run = m_new;
+            lim = watch || m_new == -INFINITY ? -INFINITY : m_new + kAhead * __builtin_amdgcn_rcpf(cf);
             mu = mu_new;
             l_run *= al;
 #pragma unroll
@@ -522,7 +557,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     // column, four values each, put them together ----
     l_run += ndl::wave_xor<16>(l_run);
     l_run += ndl::wave_xor<32>(l_run);
-    if (bad || (__float_as_int(cf0) < 0 && l_run != 0.0f)) l_run = NAN;
+    l_run = (bad | ((__float_as_int(cf0) < 0) & (l_run != 0.0f))) ? NAN : l_run;
     // the sums are left as 2^more of what has a weight of 1/2 to 1: of values near
     // fp32's end the sum may be beyond it, the mean is not
     const int more = __builtin_amdgcn_frexp_expf(l_run);

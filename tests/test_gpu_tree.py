@@ -477,3 +477,97 @@ def test_sums_of_large_values(ctx, sessions, quant):
                                  dev(R.words_of(see)), dev(q), quant_query=quant))
     want = _want(g, host(blk), nb, [base], None, lo[:1], see[:1], q[:1], quant)
     assert np.abs(got[0] - want[0]).max() <= TOL * 5e37
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("sink", [1e-9, 1e-20, 0.0])
+@pytest.mark.parametrize("ahead", [5, 15, 20, 25, 30, 60])
+@pytest.mark.parametrize("sessions,H,KVH,QK", [(1, 12, 2, 48), (300, 12, 2, 48), (70, 4, 4, 64)])
+def test_the_rest_behind_rows_of_next_to_no_values(ctx, sessions, H, KVH, QK, ahead, sink, quant):
+    """Positions that take all but 2^-ahead of the weight and hold values next to
+    zero, or zeros (of scale 1), one in each of the first 32 chunks, so that each
+    wave meets one before most of its walk: the rest decides the output.
+
+    Tolerance, of each head by itself.  A head's error is at most delta sum(w |v|)
+    / sum(w), delta the relative error of a weight: a score's fp32 sum, 67 * 2^-24
+    of the sum of the products' magnitudes (these queries are a quarter of N(0, 1),
+    keys N(0, 1): below 67 * 2^-24 * 13 / 6.9 = 7.5e-6); its distance from the
+    maximum, less than ahead + 12 bits, of ln 2 each, off by seven roundings (the
+    scale, its product with log2 e, the query's scale, the key's, the product, the
+    difference, the sums' scaling): 5 * 2^-24 (ahead + 12); the weight itself and
+    its sums, 8 * 2^-24.
+    """
+    rng = np.random.default_rng(ahead)
+    nodes, base, cap = 2, 5000, 5100
+    g, blk, nb = _block(ctx, rng, H, KVH, QK, cap, base + nodes, 1)
+    off = nd.kv_offsets(g)
+    part = lambda at, n: blk[at:at + n]  # noqa: E731
+    kc = part(0, KVH * cap * QK).view(torch.int8).view(KVH, cap, QK)
+    vc = part(off["v"], KVH * cap * 64).view(torch.int8).view(KVH, cap, 64)
+    ks, vs = (part(off[s], 4 * KVH * cap).view(torch.float32).view(KVH, cap) for s in ("ks", "vs"))
+    at = torch.arange(32, device="cuda") * 32 + 5
+    kc[:, :, 0] = 0
+    kc[:, at] = 0
+    kc[:, at, 0] = 127
+    vc[:] = vc.abs()  # all of one sign: the rest does not average out
+    vc[:, at] = 100 if sink else 0
+    vs[:, at] = sink if sink else 1.0
+    q = rng.normal(size=(sessions, nodes, H, QK)).astype(np.float32) / 4
+    q[..., 0] = 4.0
+    bits = 1 / np.sqrt(QK) / np.log(2)
+    # the rest: about 5000 weights of 2^0 on average, 2^12.3 together
+    ks[:, at] = (ahead + 12.3 - 5) / (127 * 4 * bits)
+    see = np.repeat(np.tril(np.ones((nodes, nodes), np.uint8))[None], sessions, 0)
+    lo = np.zeros((sessions, nodes), np.int32)
+    got = host(nd.attend_tree_i8(ctx, g, blk, 0, dev(np.full(sessions, base, np.int32)), dev(lo),
+                                 dev(R.words_of(see)), dev(q.reshape(sessions, nodes, -1)), quant_query=quant))
+    delta = 7.5e-6 + 2.0 ** -24 * (8 + 5 * (ahead + 12))
+    b = host(blk)
+    for i in {0, sessions // 2, sessions - 1}:
+        one = (g, b, nb, [base], None, lo[i:i + 1], see[i:i + 1], q[i:i + 1].reshape(1, nodes, -1), quant)
+        want = _want(*one)[0].reshape(nodes, H, 64)
+        # with values of one sign sum(w |v|) / sum(w) is the output itself
+        err = np.linalg.norm(got[i].reshape(nodes, H, 64) - want, axis=-1) / np.linalg.norm(want, axis=-1)
+        assert err.max() <= delta, err.max()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("seed", range(6))
+def test_rows_far_ahead_of_any_size_anywhere(ctx, seed, quant):
+    """Positions up to 2^60 ahead of the others, at any distance from one another,
+    with values of 10^-12 to 1 of theirs, or zeros, among values of sizes that change
+    along the cache.  The tolerance is the one above: values of one sign, the error
+    of a weight."""
+    rng = np.random.default_rng(seed)
+    S, nodes, base, cap, H, KVH, QK = (1, 1, 130, 400)[seed % 4], 3, 6000, 6200, 12, 2, 48
+    g, blk, nb = _block(ctx, rng, H, KVH, QK, cap, base + nodes, 1)
+    off = nd.kv_offsets(g)
+    part = lambda at, n: blk[at:at + n]  # noqa: E731
+    kc = part(0, KVH * cap * QK).view(torch.int8).view(KVH, cap, QK)
+    vc = part(off["v"], KVH * cap * 64).view(torch.int8).view(KVH, cap, 64)
+    ks, vs = (part(off[s], 4 * KVH * cap).view(torch.float32).view(KVH, cap) for s in ("ks", "vs"))
+    vc[:] = vc.abs()
+    vs *= dev(10.0 ** np.repeat(rng.uniform(-2, 2, cap // 200), 200)).float()
+    at = np.cumsum(rng.integers(1, (20, 90, 300)[seed % 3], base))
+    at = dev(at[at < base])
+    kc[:, :, 0] = 0
+    kc[:, at] = 0
+    kc[:, at, 0] = 127
+    bits = 1 / np.sqrt(QK) / np.log(2)
+    ks[:, at] = dev(rng.uniform(0, 60, len(at)) / (127 * 4 * bits)).float()
+    vs[:, at] *= dev(10.0 ** rng.uniform(-12, 0, len(at))).float()
+    none = at[dev(rng.random(len(at)) < 0.3)]
+    vc[:, none], vs[:, none] = 0, 1.0
+    q = rng.normal(size=(S, nodes, H, QK)).astype(np.float32) / 4
+    q[..., 0] = 4.0
+    see = np.repeat(np.tril(np.ones((nodes, nodes), np.uint8))[None], S, 0)
+    lo = rng.integers(0, 400, (S, nodes)).astype(np.int32)
+    got = host(nd.attend_tree_i8(ctx, g, blk, 0, dev(np.full(S, base, np.int32)), dev(lo),
+                                 dev(R.words_of(see)), dev(q.reshape(S, nodes, -1)), quant_query=quant))
+    delta = 7.5e-6 + 2.0 ** -24 * (8 + 5 * 72)
+    b = host(blk)
+    for i in {0, S // 2, S - 1}:
+        want = _want(g, b, nb, [base], None, lo[i:i + 1], see[i:i + 1], q[i:i + 1].reshape(1, nodes, -1), quant)
+        want = want[0].reshape(nodes, H, 64)
+        err = np.linalg.norm(got[i].reshape(nodes, H, 64) - want, axis=-1) / np.linalg.norm(want, axis=-1)
+        assert err.max() <= delta, err.max()
