@@ -17,14 +17,13 @@
 //           the maximum m is kept before it and e = 2^(fma(t, cf, -m cf)).
 //   values  O^T[v][col] = V^T P^T: a score tile's result layout is the layout
 //           of the weights the product needs.  MFMA c takes V columns 4 n + c,
-//           a dword a position.  The weights e vs are two f16 pieces, 23 bits of
-//           every weight that is not 2^-24 or less of the column's largest so far
-//           (a maximum on values next to zero is no measure of the rest: the
-//           sums then go on against a lower one); V's codes are exact in f16.  A
-//           chunk with a V scale 2^-9 or less of the largest met takes the fp32
-//           matrix product instead, all 24 bits at any size: the values of one
-//           position may be far smaller than its neighbours' and yet decide the
-//           output.
+//           a dword a position.  The weights e vs are two f16 pieces, off by
+//           2^-23 of the weight or of the column's largest so far (a maximum on
+//           values next to zero is no measure of the rest: the sums then go on
+//           against a lower one); V's codes are exact in f16.  A chunk with a V
+//           scale 2^-9 or less of the largest met takes the fp32 matrix product
+//           instead, all 24 bits at any size: the values of one position may be
+//           far smaller than its neighbours' and yet decide the output.
 // Sums and statistics are fp32.
 //
 // What bounds it: where the cache streams (one query head a kv head) HBM, 64
@@ -385,14 +384,25 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
         }
         // ---- the chunk's scales, zero behind its end ----
         float sc = (lane & 31) < left ? scr : 0.0f;
-        if (any_of(!(sc <= top))) {
+        if (any_of(!(__builtin_fabsf(sc) <= top))) {
+            // what no column sees may be anything: it sets no unit, and counts as one
+            bool unseen = false;
+            if (tail || p0 < tlo) {
+                uint32_t seen = along ? 0u : vis;
+                seen |= uint32_t(ndl::wave_xor_int<1>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<2>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<4>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<8>(int(seen)));
+                unseen = !(seen >> (lane & 31) & 1u);
+                sc = unseen ? 0.0f : sc;
+            }
             // a V scale that is no number makes no number of the columns that see
             // it, and only of those: a weight of 0 there would not stay 0
             const bool wild = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY);
             const uint32_t wilds = uint32_t(__builtin_amdgcn_ballot_w64(wild) >> 32);
             if (wild) sc = 0.0f;
             if (vis & wilds) l_run = NAN;
-            float h = sc < INFINITY ? fmaxf(sc, top) : top;
+            float h = __builtin_fabsf(sc) < INFINITY ? fmaxf(__builtin_fabsf(sc), top) : top;
             h = fmaxf(h, ndl::wave_xor<16>(h));
             h = fmaxf(h, ndl::wave_xor<8>(h));
             h = fmaxf(h, ndl::wave_xor<4>(h));
@@ -401,6 +411,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             const int was = lane < 32 ? kexp : vexp;
             const int now = h > top ? __builtin_amdgcn_frexp_expf(h) : was;
             top = h > top ? (now > 127 ? 0x1.fffffep127f : __builtin_amdgcn_ldexpf(1.0f, now)) : top;
+            sc = unseen ? top : sc;
             shift += was - now;
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
             if (vn > vmet + 3 || !any32(l_run > 0.0f)) {

@@ -571,3 +571,25 @@ def test_rows_far_ahead_of_any_size_anywhere(ctx, seed, quant):
         want = want[0].reshape(nodes, H, 64)
         err = np.linalg.norm(got[i].reshape(nodes, H, 64) - want, axis=-1) / np.linalg.norm(want, axis=-1)
         assert err.max() <= delta, err.max()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("garbage", [3e38, -3e38, -np.inf, 1e30, -1e-40])
+def test_scales_of_nodes_no_row_names(ctx, garbage, quant):
+    """A node of the tree that no mask names need not have been written: whatever
+    numbers lie there, the others' outputs are what they were."""
+    rng = np.random.default_rng(14)
+    nodes, base, cap = 40, 900, 1000
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, cap, base + nodes, 1, 1.0, 1e-3)
+    see = np.tril(np.ones((nodes, nodes), np.uint8))[None].copy()
+    see[:, :, [3, 33, 38]] = 0
+    q = rng.normal(size=(1, nodes, 12 * 48)).astype(np.float32)
+    off = nd.kv_offsets(g)
+    for part in ("ks", "vs"):
+        s = blk[off[part]:off[part] + 4 * 2 * cap].view(torch.float32).view(2, cap)
+        s[:, [base + 3, base + 33, base + 38]] = garbage
+    lo = np.zeros((1, nodes), int)
+    got = host(nd.attend_tree_i8(ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(lo.astype(np.int32)),
+                                 dev(R.words_of(see)), dev(q), quant_query=quant))
+    want = _want(g, host(blk), nb, [base], None, lo, see, q, quant)
+    assert np.abs(got - want).max() <= 1e-3 * TOL
