@@ -359,11 +359,11 @@ int nd_kv_read(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_strid
  * than cap positions between the first and the tree's end.
  * qk 48 or 64, v 64, at most 2^29 positions x kv heads a block and 65535
  * sessions; out must not overlap q.  `work`: device memory for partial sums,
- * of nd_attend_tree_i8_work(..) bytes or more, 16-byte aligned, that no other
- * call uses at the same time; NULL: the context's own (not while its stream
- * is being captured into a graph, which would keep an address that a later
- * call may free).  No reference counterpart: the reference decodes one token
- * a step.
+ * of nd_attend_tree_i8_work(..) bytes or more (0 also for sizes that are
+ * refused), 16-byte aligned, that no other call uses at the same time; NULL:
+ * the context's own (not while its stream is being captured into a graph,
+ * which would keep an address that a later call may free).  No reference
+ * counterpart: the reference decodes one token a step.
  */
 size_t nd_attend_tree_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes);
 int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride,

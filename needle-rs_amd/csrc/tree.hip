@@ -682,6 +682,21 @@ auto kernel_of(const Plan &p)
     return p.nw == 4 ? tree_kernel<QK, QQ, 4> : tree_kernel<QK, QQ, 8>;
 }
 
+// What a call and its workspace's size are refused for.
+int check_tree(const nd_kv_geom *g, size_t count, size_t nodes)
+{
+    if (int rc = check_geom(g)) return rc;
+    ND_REQUIRE((g->qk_head_dim == 48 || g->qk_head_dim == 64) && g->v_head_dim == VD,
+               "no tree attention for qk %d, v %d", g->qk_head_dim, g->v_head_dim);
+    ND_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "nodes %zu must be in 1..%d", nodes, kMaxNodes);
+    ND_REQUIRE(count <= 65535, "count %zu above 65535", count);
+    ND_REQUIRE(g->num_heads <= 4096, "num_heads %d above 4096", g->num_heads);
+    // a buffer of one head's scales reaches from its K scales to its V scales
+    ND_REQUIRE(size_t(g->num_kv_heads) * g->cap <= size_t(1) << 29, "%d kv heads x cap %d above 2^29",
+               g->num_kv_heads, g->cap);
+    return ND_OK;
+}
+
 size_t partial_floats(const nd_kv_geom *g, size_t count, size_t nodes, size_t splits)
 {
     return splits > 1 ? count * nodes * g->num_heads * splits * (VD + 2) : 0;
@@ -693,7 +708,8 @@ extern "C" {
 
 size_t nd_attend_tree_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t nodes)
 {
-    if (!ctx || !g || g->num_kv_heads <= 0 || g->num_heads <= 0 || g->cap <= 0 || !count || !nodes) return 0;
+    nd::clear_error();
+    if (!ctx || check_tree(g, count, nodes) != ND_OK || !count) return 0;
     return partial_floats(g, count, nodes, plan_of(ctx, g, count, nodes).splits) * sizeof(float);
 }
 
@@ -703,17 +719,9 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
                       int quant_query, float *out, void *work, size_t work_bytes)
 {
     ND_ENTER(ctx);
-    if (int rc = check_geom(g)) return rc;
-    ND_REQUIRE((g->qk_head_dim == 48 || g->qk_head_dim == 64) && g->v_head_dim == VD,
-               "no tree attention for qk %d, v %d", g->qk_head_dim, g->v_head_dim);
-    ND_REQUIRE(nodes >= 1 && nodes <= kMaxNodes, "nodes %zu must be in 1..%d", nodes, kMaxNodes);
+    if (int rc = check_tree(g, count, nodes)) return rc;
     if (count == 0) return ND_OK;
     ND_REQUIRE(kv && base && lo && mask && q && out, "null buffer");
-    ND_REQUIRE(count <= 65535, "count %zu above 65535", count);
-    ND_REQUIRE(g->num_heads <= 4096, "num_heads %d above 4096", g->num_heads);
-    // a buffer of one head's scales reaches from its K scales to its V scales
-    ND_REQUIRE(size_t(g->num_kv_heads) * g->cap <= size_t(1) << 29, "%d kv heads x cap %d above 2^29",
-               g->num_kv_heads, g->cap);
     ND_REQUIRE((reinterpret_cast<uintptr_t>(kv) & 255) == 0 && kv_stride % 256 == 0,
                "kv blocks must be 256-byte aligned");
     const uintptr_t qa = reinterpret_cast<uintptr_t>(q), oa = reinterpret_cast<uintptr_t>(out);

@@ -593,3 +593,13 @@ def test_scales_of_nodes_no_row_names(ctx, garbage, quant):
                                  dev(R.words_of(see)), dev(q), quant_query=quant))
     want = _want(g, host(blk), nb, [base], None, lo, see, q, quant)
     assert np.abs(got - want).max() <= 1e-3 * TOL
+
+
+def test_work_of_sizes_that_are_refused(ctx):
+    g = nd.kv_geom(12, 2, 48, 64, 4096)
+    assert nd.attend_tree_i8_work(ctx, g, 1, 4) > 0
+    for bad, count, nodes in ((nd.kv_geom(2, 4, 48, 64, 4096), 1, 4), (nd.kv_geom(18, 2, 48, 64, 4096), 1, 4),
+                              (nd.kv_geom(12, 5, 48, 64, 4096), 1, 4), (nd.kv_geom(12, 2, 32, 64, 4096), 1, 4),
+                              (nd.kv_geom(12, 2, 48, 64, (1 << 24) + 1), 1, 4), (g, 65536, 4), (g, 1 << 63, 4),
+                              (g, 1, 0), (g, 0, 4), (g, 1, 257), (g, 1, 1 << 62)):
+        assert nd.attend_tree_i8_work(ctx, bad, count, nodes) == 0
