@@ -738,17 +738,18 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
     t.splits = int(p.splits);
     t.scale2 = scale == scale ? float(double(scale < 0 ? -scale : scale) * 1.4426950408889634) : -1.0f;
     t.negative = scale < 0;
-    float *part = nullptr;
     if (p.splits > 1) {
         void *ws = nullptr;
         const size_t bytes = partial_floats(g, count, nodes, p.splits) * sizeof(float);
         if (int rc = nd::call_workspace(ctx, bytes, work, work_bytes, &ws)) return rc;
-        part = static_cast<float *>(ws);
+        t.part_o = static_cast<float *>(ws);
+        t.part_ml = t.part_o + count * nodes * g->num_heads * p.splits * VD;
     }
     const bool q48 = g->qk_head_dim == 48;
     auto *fn = q48 ? (quant_query ? kernel_of<48, true>(p) : kernel_of<48, false>(p))
                    : (quant_query ? kernel_of<64, true>(p) : kernel_of<64, false>(p));
-    // HIP counts a launch's threads in 32 bits: sessions beyond that go in further launches
+    // HIP counts a launch's threads in 32 bits: sessions beyond that go in further
+    // launches (never those of a split call, whose waves are two a SIMD at most)
     const size_t per = size_t(g->num_kv_heads) * p.splits * p.tiles, most = std::max<size_t>(1, (size_t(1) << 18) / per);
     const Geom kg = make_geom(g);
     for (size_t s = 0; s < count; s += most) {
@@ -760,12 +761,6 @@ int nd_attend_tree_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t k
         t.mask = mask + rows * t.words;
         t.q = q + rows * g->num_heads * g->qk_head_dim;
         t.out = out + rows * g->num_heads * VD;
-        if (part) {
-            const size_t outs = m * nodes * g->num_heads * p.splits;
-            t.part_o = part;
-            t.part_ml = part + outs * VD;
-            part = t.part_ml + outs * 2;
-        }
         t.units = uint32_t(m * g->num_kv_heads * p.splits);
         hipLaunchKernelGGL(fn, dim3(8, unsigned(p.tiles), unsigned((t.units + 7) / 8)), dim3(p.nw * 64), 0, ctx->stream, kg, t);
         if (int rc = nd::check_launch("attend_tree_i8")) return rc;

@@ -603,3 +603,18 @@ def test_work_of_sizes_that_are_refused(ctx):
                               (nd.kv_geom(12, 2, 48, 64, (1 << 24) + 1), 1, 4), (g, 65536, 4), (g, 1 << 63, 4),
                               (g, 1, 0), (g, 0, 4), (g, 1, 257), (g, 1, 1 << 62)):
         assert nd.attend_tree_i8_work(ctx, bad, count, nodes) == 0
+
+
+def test_more_sessions_than_a_launch_holds(ctx):
+    """Sessions on both sides of the border between two launches."""
+    rng = np.random.default_rng(17)
+    S, base, KVH = 50000, 6, 12
+    first = (1 << 18) // KVH  # of the second launch
+    g, blk, nb = _block(ctx, rng, KVH, KVH, 64, base + 1, base + 1, 1)
+    bases = np.arange(S) % (base + 1)
+    length = (np.arange(S) % 11 != 3).astype(np.int32)
+    lo = np.minimum(np.arange(S)[:, None] % 3, bases[:, None])
+    see = (np.arange(S) % 5 != 1).astype(np.uint8).reshape(S, 1, 1)
+    q = rng.normal(size=(S, 1, KVH * 64)).astype(np.float32)
+    rows = sorted({0, 1, 3, S - 1, *(first + np.arange(-12, 12)), *(2 * first + np.arange(-12, 12))})
+    _check(ctx, g, blk, 0, bases, lo, see, q, length, rows=rows)
