@@ -408,7 +408,7 @@ typedef struct nd_logits_rules {
  * the rules (y_stride elements apart; y may be x, or must not overlap it),
  * and next[i] the first maximum of y[i]: as nd_argmax_rows, but -1 where
  * nothing is above -inf (a mask that leaves no token).  y or next may be
- * NULL.  n <= 2^24.  `work` as for nd_attend_tree_i8, of
+ * NULL.  n <= 2^24, count < 2^31.  `work` as for nd_attend_tree_i8, of
  * nd_logits_adjust_work(..) bytes; 0 bytes where next is NULL. */
 size_t nd_logits_adjust_work(nd_ctx *ctx, size_t count, size_t n);
 int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, size_t n,

@@ -17,6 +17,8 @@
 #include "nd_internal.h"
 #include "nd_lanes.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int kThreads = 512;
@@ -58,14 +60,14 @@ __device__ inline void meet_wave(Pick &a)
 
 constexpr int kNone = 0x7fffffff;
 
-__global__ __launch_bounds__(kThreads) void adjust_kernel(const float *x, size_t x_stride, int n, int slices,
+__global__ __launch_bounds__(kThreads) void adjust_kernel(const float *x, size_t x_stride, size_t first, int n, int slices,
                                                           nd_logits_rules r, float *y, size_t y_stride,
                                                           int32_t *next, Pick *part)
 {
     __shared__ __align__(16) uint32_t st[kSlice];
     __shared__ int twice;
     __shared__ Pick best[kThreads / 64];
-    const size_t row = blockIdx.x / unsigned(slices);
+    const size_t row = first + blockIdx.x / unsigned(slices);
     const int slice = int(blockIdx.x % unsigned(slices)), t0 = slice * kSlice, t = threadIdx.x;
     const int cnt = min(kSlice, n - t0);
     const float *xr = x + row * x_stride + t0;
@@ -198,16 +200,17 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(const float *x, size_t
 }
 
 // A wave a row: the best of its slices.
-__global__ __launch_bounds__(64) void join_kernel(const Pick *__restrict__ part, int slices,
+__global__ __launch_bounds__(64) void join_kernel(const Pick *__restrict__ part, size_t first, int slices,
                                                   int32_t *__restrict__ next)
 {
+    const size_t row = first + blockIdx.x;
     Pick b{-INFINITY, kNone};
     for (int s = threadIdx.x; s < slices; s += 64) {
-        const Pick p = part[size_t(blockIdx.x) * slices + s];
+        const Pick p = part[row * slices + s];
         take(b, p.v, p.i);
     }
     meet_wave(b);
-    if (threadIdx.x == 0) next[blockIdx.x] = b.i == kNone ? -1 : b.i;
+    if (threadIdx.x == 0) next[row] = b.i == kNone ? -1 : b.i;
 }
 
 size_t slices_of(size_t n) { return (n + kSlice - 1) / kSlice; }
@@ -233,8 +236,7 @@ int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count,
     ND_REQUIRE(x, "null buffer");
     ND_REQUIRE(count == 1 || (x_stride >= n && (!y || y_stride >= n)), "row strides below n %zu", n);
     const size_t slices = slices_of(n);
-    ND_REQUIRE(count <= 0x7fffffff && count * slices <= (size_t(1) << 23), "%zu rows of %zu logits are too many",
-               count, n);
+    ND_REQUIRE(count <= 0x7fffffff, "count %zu above 2^31 - 1", count);
     const nd_logits_rules &r = *rules;
     ND_REQUIRE(!r.hist || r.hist_stride < (size_t(1) << 30), "hist_stride too large");
     ND_REQUIRE(!r.bias == !r.bias_id, "bias and bias_id are given together or not at all");
@@ -254,12 +256,17 @@ int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count,
         if (int rc = nd::call_workspace(ctx, count * slices * sizeof(Pick), work, work_bytes, &p)) return rc;
         part = static_cast<Pick *>(p);
     }
-    hipLaunchKernelGGL(adjust_kernel, dim3(unsigned(count * slices)), dim3(kThreads), 0, ctx->stream, x, x_stride,
-                       int(n), int(slices), r, y, y_stride, next, part);
-    if (int rc = nd::check_launch("logits_adjust")) return rc;
-    if (part) {
-        hipLaunchKernelGGL(join_kernel, dim3(unsigned(count)), dim3(64), 0, ctx->stream, part, int(slices), next);
-        return nd::check_launch("logits_join");
+    // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
+    const size_t most = size_t(0xffffffff / kThreads) / slices;
+    for (size_t first = 0; first < count; first += most) {
+        const unsigned rows = unsigned(std::min(most, count - first));
+        hipLaunchKernelGGL(adjust_kernel, dim3(rows * unsigned(slices)), dim3(kThreads), 0, ctx->stream, x, x_stride,
+                           first, int(n), int(slices), r, y, y_stride, next, part);
+        if (int rc = nd::check_launch("logits_adjust")) return rc;
+        if (part) {
+            hipLaunchKernelGGL(join_kernel, dim3(rows), dim3(64), 0, ctx->stream, part, first, int(slices), next);
+            if (int rc = nd::check_launch("logits_join")) return rc;
+        }
     }
     return ND_OK;
 }

@@ -235,3 +235,18 @@ def test_no_rows_and_refusals(ctx):
                dict(mask=torch.zeros(2, 157, dtype=torch.int64, device="cuda")), dict(mask_row=ids[0, :1])):
         with pytest.raises(ValueError):
             nd.logits_adjust(ctx, x, **kw)
+
+
+@pytest.mark.parametrize("count,n", [(1 << 23, 1), ((1 << 23) + 5, 3)])
+def test_more_rows_than_a_launch_holds(ctx, count, n):
+    """Rows of every launch, up to the last one."""
+    x = torch.arange(count * n, device="cuda").view(count, n).remainder(1000).float()
+    out, nxt = nd.logits_adjust(ctx, x, repeat=torch.full((count,), 2.0, device="cuda"),
+                                hist=torch.zeros(count, 1, dtype=torch.int32, device="cuda"), pick=True)
+    want = x.clone()
+    want[:, 0] /= 2
+    assert torch.equal(out, want)
+    best = torch.zeros(count, dtype=torch.int32, device="cuda")
+    for j in range(1, n):
+        best = torch.where(want[:, j] > want.gather(1, best[:, None].long())[:, 0], j, best).int()
+    assert torch.equal(nxt, best)
