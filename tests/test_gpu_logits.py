@@ -250,3 +250,27 @@ def test_more_rows_than_a_launch_holds(ctx, count, n):
     for j in range(1, n):
         best = torch.where(want[:, j] > want.gather(1, best[:, None].long())[:, 0], j, best).int()
     assert torch.equal(nxt, best)
+
+
+@pytest.mark.parametrize("n,biases,tokens", [(9000, 20000, 9000), (8192, 30000, 3), (20, 5000, 20), (20001, 4001, 4000)])
+def test_long_lists_of_biases(ctx, n, biases, tokens):
+    """Lists of many entries, a few tokens or all of them listed again and again."""
+    rng = np.random.default_rng(biases)
+    ids = rng.integers(0, tokens, (2, biases)).astype(np.int32)
+    if tokens == 4000:
+        ids[:, :4000] = rng.permutation(4000)  # a single token twice
+    bias = (10.0 ** rng.uniform(-4, 4, (2, biases)) * rng.choice([-1, 1], (2, biases))).astype(np.float32)
+    x = rng.normal(size=(2, n)).astype(np.float32)
+    hist = rng.integers(0, tokens, (2, 50)).astype(np.int32)
+    out, nxt = (host(t) for t in _run(ctx, x, dict(bias_id=ids, bias=bias, hist=hist,
+                                                   presence=np.array([0.5, 1.0], np.float32)), pick=True))
+    want = x.copy()
+    for i in range(2):
+        want[i, np.unique(hist[i])] -= np.float32(0.5 + 0.5 * i)
+        total = {}
+        for t, b in zip(ids[i].tolist(), bias[i]):
+            total[t] = np.float32(total[t] + b) if t in total else b
+        for t, b in total.items():
+            want[i, t] += b
+    assert np.array_equal(out, want)
+    assert nxt.tolist() == want.argmax(1).tolist()
