@@ -618,3 +618,24 @@ def test_more_sessions_than_a_launch_holds(ctx):
     q = rng.normal(size=(S, 1, KVH * 64)).astype(np.float32)
     rows = sorted({0, 1, 3, S - 1, *(first + np.arange(-12, 12)), *(2 * first + np.arange(-12, 12))})
     _check(ctx, g, blk, 0, bases, lo, see, q, length, rows=rows)
+
+
+def test_query_codes_of_a_subnormal_scale(ctx):
+    """A query whose scale's inverse is beyond fp32: codes of 127, -128 and (of
+    0 times infinity) no number, as the quantiser's steps give them."""
+    rng = np.random.default_rng(16)
+    nodes, base = 16, 200
+    g, blk, nb = _block(ctx, rng, 12, 2, 48, 256, base + nodes, 1, 1e37, 1.0)
+    see = R.bits_of(nd.tree_mask(_parents(rng, 1, nodes)), nodes)
+    q = (rng.normal(size=(1, nodes, 12, 48)) * 1e-37).astype(np.float32)
+    q[0, 5, 7, 3] = 0.0
+    args = (ctx, g, blk, nb, dev(np.array([base], np.int32)), dev(np.zeros((1, nodes), np.int32)),
+            dev(R.words_of(see)), dev(q.reshape(1, nodes, -1)))
+    got = host(nd.attend_tree_i8(*args, quant_query=True)).reshape(nodes, 12, 64)
+    assert np.isnan(got[5, 7]).all()
+    q[0, 5, 7, 3] = 1e-37
+    want = _want(g, host(blk), nb, [base], None, np.zeros((1, nodes), int), see, q.reshape(1, nodes, -1), True)
+    there = np.ones((nodes, 12), bool)
+    there[5, 7] = False
+    # every element counts 127 or 128 times qs, 2.5 |q| and more here: scores up to 20, of 48 equal codes
+    assert np.abs(got - want.reshape(nodes, 12, 64))[there].max() <= 8 * TOL
