@@ -254,14 +254,16 @@ _HAND = {}
 
 
 def _needle():
-    """The package and a context on the current stream, as a server holds them."""
-    if not _HAND:
+    """The package and the context of the current stream, as a server holds them."""
+    device = torch.cuda.current_device()
+    key = device, torch._C._cuda_getCurrentRawStream(device)  # (current_stream() takes a microsecond)
+    if key not in _HAND:
         at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "needle-rs_amd")
         if at not in sys.path:
             sys.path.insert(0, at)
         import needle_amd
-        _HAND["nd"], _HAND["ctx"] = needle_amd, needle_amd.Ctx(0)
-    return _HAND["nd"], _HAND["ctx"]
+        _HAND[key] = needle_amd, needle_amd.Ctx(device)
+    return _HAND[key]
 
 
 def _spec(case, nd):
