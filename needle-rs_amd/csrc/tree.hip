@@ -372,7 +372,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
     // a column goes on against the next chunk's own maximum, which may lie far below:
     // its sums are multiplied (up to 2^100)
     uint32_t watch = 0;
-    int vmet = 0;                       // vexp then
+    int vmet = 0x10000;                 // vexp then, and 3
 
     for (; ch < nch; ch += step) {
         // ---- the positions each column sees ----
@@ -414,9 +414,9 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
             sc = unseen ? top : sc;
             shift += was - now;
             const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
-            if (vn > vmet + 3 || !any32(l_run > 0.0f)) {
-                watch |= any32(l_run > 0.0f);
-                vmet = vn;
+            if (vn > vmet) {
+                watch = 1;
+                vmet = vn + 3;
             }
             m_run = __builtin_amdgcn_ldexpf(m_run, kexp - kn);
             cf = factor(kn);
@@ -511,6 +511,7 @@ __global__ __launch_bounds__(NW * 64, 4) void tree_kernel(Geom g, Tree tr)
                 watch = any32((m_new > -INFINITY) & !down);
             }
             watch |= small;
+            vmet = min(vmet, vexp + 3);
             const float mu_new = m_new == -INFINITY ? 0.0f : m_new * cf;
             // nothing is summed yet where there was no maximum
             const float al = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu - mu_new);
