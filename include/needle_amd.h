@@ -353,8 +353,12 @@ int nd_kv_read(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_strid
  *   out[i][n] ([num_heads][v]) = softmax(scale q[i][n] . k) v,
  * heads as in nd_attend_step_i8, quant_query too.  Only the first length[i]
  * nodes of session i are there (NULL: all): bits of the others are ignored,
- * and their rows of out are not written.  A node that attends to nothing
- * gets zeros.  NaN where a session's numbers cannot be: length[i] outside 0
+ * and their rows of out are not written.  What no row attends to need not
+ * have been written.  A node that attends to nothing gets zeros; of what
+ * another sees, a head whose query holds a NaN or an infinity gives NaN.
+ * Statistics and sums are fp32; weights and fp32 queries go into their
+ * products to 2^-23 of themselves, the weights beside the column's largest
+ * (positions more than 2^100 below the largest may be lost).  NaN where a session's numbers cannot be: length[i] outside 0
  * .. nodes (every row of the session), base[i] or lo[i][n] negative, or more
  * than cap positions between the first and the tree's end.
  * qk 48 or 64, v 64, at most 2^29 positions x kv heads a block and 65535

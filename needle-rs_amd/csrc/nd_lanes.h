@@ -9,9 +9,11 @@
 // one ds_swizzle for 4 and DPP quad_perm for 2 and 1.
 //
 // Lanes are numbered threadIdx.x % 64: every caller launches one-dimensional
-// blocks whose width is a multiple of 64, with all lanes of the wave active
-// where it calls (DPP and the lane swaps read the partner's register
-// directly).
+// blocks whose width is a multiple of 64, and every lane that a call reads is
+// active where it is made (DPP and the lane swaps read the partner's register
+// directly): all lanes of the wave for the sums and maxima over it, for a
+// single distance H the lanes of the aligned group of 2 H that hold it (groups of
+// one wave may be in different branches, as the head groups of rope.hip are).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -27,9 +27,9 @@
 // Sums and statistics are fp32.
 //
 // What bounds it: where the cache streams (one query head a kv head) HBM, 64
-// sessions x 13 nodes x 12 heads x 64 at 2048 positions 38.9 us = 5.0 TB/s; with
+// sessions x 13 nodes x 12 heads x 64 at 2048 positions 39.3 us = 5.0 TB/s; with
 // grouped heads the VALU, about 146 operations a chunk (the exponentials 32, V's
-// conversion 40), 64 x 16 nodes x 12 heads over 2 at 2000 21.1 us; small trees the
+// conversion 40), 64 x 16 nodes x 12 heads over 2 at 2000 21.5 us; small trees the
 // 7 us from launch to merge.  One column tile a wave at four waves a SIMD: two
 // tiles, which share V's conversion but leave three waves, gain at 100 million
 // scores (128 sessions x 4000 65.9 -> 57.4) and lose below (64 x 2000 23.9 -> 26.7,
