@@ -217,8 +217,8 @@ def prepare(case, seed):
 def _prepare_sample(case, g):
     rows, n = case["rows"], case["n"]
     x = 2 * _randn(g, rows, n)
-    # a few tokens stand out, as a trained model's do
-    likely = torch.randint(0, n, (rows, 24), generator=g, device="cuda")
+    # a few tokens stand out, as a trained model's do (no token twice: the seed alone decides)
+    likely = (torch.randint(0, n, (rows, 1), generator=g, device="cuda") + torch.arange(24, device="cuda") * (n // 24)) % n
     x.scatter_(1, likely, 7 + 2.5 * _randn(g, rows, 24))
     i = torch.arange(rows, device="cuda")
     # rows under a grammar have lost half of their tokens
