@@ -419,6 +419,110 @@ int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count,
                      const nd_logits_rules *rules, float *y, size_t y_stride, int32_t *next,
                      void *work, size_t work_bytes);
 
+/* ---- a batch that shares its prompts --------------------------------------- */
+
+/*
+ * Sessions that begin with the same text hold its keys and values once: a
+ * prefix is a block of its own (nd_kv_write_rope at the positions 0, 1, ..), a
+ * session's block holds what comes after it, counted from 0 again.  A step has
+ * up to `rows` (1 .. 256; 1: decode) new positions a session.  With
+ *   L = prefix_len[prefix_of[i]] (prefix_of[i] < 0: no prefix, L = 0;
+ *       prefix_of NULL: prefix 0 for all, or none where prefixes is 0),
+ *   u = used[i], the positions that session i's block held before the step,
+ *   m = length[i] (NULL: rows), the rows it has in this one, and
+ *   window, the positions a row attends to, its own the last (0: all),
+ * row n < m of session i attends to its prefix's positions from .. L - 1 and
+ * to its own positions lo .. u + n:
+ *   pos  = u + n        where its key and value go in the session's block
+ *   rot  = L + u + n    the position its query and key are turned by
+ *   from = min(max(0, rot + 1 - window), L)
+ *   lo   = max(0, rot + 1 - window - L)
+ * nd_prefix_plan works these out on the device.  `maps` (may be NULL, as any
+ * of its pointers) receives them as int32 [count][rows], -1 for rows that are
+ * not there; pos and rot are what nd_kv_write_rope takes with per_block =
+ * rows.  order [count * rows] holds the rows (i * rows + n) that have a
+ * prefix, those of a prefix one after another and ascending, -1 behind the
+ * last; prefix p's are first[p] .. first[p + 1] - 1 (first [prefixes + 1]).
+ *
+ * Numbers that cannot be -- prefix_of[i] >= prefixes, L or u negative, m
+ * outside 0 .. rows, rot beyond 2^31 - 1, more positions than a block holds
+ * between the first that a row of the session attends to and the last (of its
+ * prefix: prefix_cap; of its own: the geometry's cap) -- make rows of the
+ * session that are bad: -1 in the maps, in no group, NaN from the attention
+ * (all `rows` of them where m cannot be).
+ *
+ * `plan`: device memory of nd_prefix_plan_bytes(..) bytes (16-byte aligned)
+ * that receives the attention's work list, for any number of
+ * nd_attend_prefix_i8 calls with the same geometry, prefix_cap, count, rows
+ * and prefixes: a step's layers of one window share it.  At most 65535
+ * sessions, 2^20 rows in all and 2048 prefixes.  No reference counterpart: a
+ * V3Engine owns its whole cache.
+ */
+typedef struct nd_prefix_maps {
+    int32_t *pos, *rot, *from, *lo, *order, *first;
+} nd_prefix_maps;
+
+size_t nd_prefix_plan_bytes(const nd_kv_geom *g, size_t count, size_t rows, size_t prefixes);
+int nd_prefix_plan(nd_ctx *ctx, const nd_kv_geom *g, size_t prefix_cap, size_t count, size_t rows,
+                   size_t prefixes, const int32_t *prefix_of, const int32_t *prefix_len,
+                   const int32_t *used, const int32_t *length, int32_t window, void *plan,
+                   size_t plan_bytes, const nd_prefix_maps *maps);
+
+/* out[i][n] ([num_heads][v]) = softmax(scale q[i][n] . k) v over what row n of
+ * session i attends to by the plan: positions of its prefix's block
+ * (prefix_kv + p * prefix_stride bytes, blocks of the geometry with
+ * prefix_cap slots) and of its own (kv + i * kv_stride bytes, the step's keys
+ * and values already written), position p at slot p % the block's slots.
+ * Heads and quant_query as in nd_attend_step_i8.  Rows that are not there are
+ * not written, bad rows are NaN, and so is every row if `plan` was made for
+ * other sizes; a head whose query holds a NaN or an infinity gives NaN.  A
+ * prefix is read for all of its rows at once.  Precision as
+ * nd_attend_tree_i8.  qk 48 or 64, v 64, at most 2^29 positions x kv heads a
+ * block and 4096 heads; out must not overlap q.  `work` as for
+ * nd_attend_tree_i8, of nd_attend_prefix_i8_work(..) bytes. */
+size_t nd_attend_prefix_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t rows,
+                                size_t prefixes);
+int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride,
+                        size_t count, size_t rows, const void *prefix_kv, size_t prefix_stride,
+                        size_t prefix_cap, size_t prefixes, const void *plan, const float *q,
+                        float scale, int quant_query, float *out, void *work, size_t work_bytes);
+
+/* ---- sampling ---------------------------------------------------------------- */
+
+/* How row i's token is drawn; every pointer is a device pointer and may be
+ * NULL, which leaves its rule out.  With l the row's logits, M their maximum,
+ * w_t = exp((l_t - M) / temperature[i]) (NULL: 1), and the tokens in the order
+ * of their logits, the largest first, equal ones by their number:
+ *   min_p[i]   only tokens with w_t >= min_p w_max stay (<= 0: all; the first
+ *              maximum always stays)
+ *   top_k[i]   of those, the first top_k (<= 0: all)
+ *   top_p[i]   of those, the shortest run from the first whose weights come to
+ *              top_p of theirs (>= 1: all; the first always stays)
+ * A temperature that is not above 0 makes row i greedy: its first maximum.
+ * Logits of -inf and NaN are no tokens; where some are +inf, they alone are,
+ * each with the weight 1. */
+typedef struct nd_sampling {
+    const float *temperature, *min_p;
+    const int32_t *top_k;
+    const float *top_p;
+} nd_sampling;
+
+/* next[i] = the token that u[i] (device, in [0, 1)) draws from row i of x
+ * ([count] rows of n logits, x_stride elements apart): the first, in the order
+ * above, at which the weights that stay, added up, exceed u[i] times their
+ * sum; so u = 0 draws the first maximum.  -1 where a row has no token.
+ * prob[i] (may be NULL) = the chance that token had, 1 for a greedy row, 0 for
+ * none.  u is taken as 0 below 0 or as a NaN, as the last token's at 1 and
+ * above.  Weights are fp64 exponentials as whole numbers of a unit of which
+ * the row's sum has 2^60 or more, so sums are exact and a pick is the border's;
+ * tokens of less than half a unit are never drawn.  sampling may be NULL.  n <= 2^24, count < 2^31.  `work` as for nd_attend_tree_i8, of
+ * nd_sample_rows_work(..) bytes.  The reference's generate takes a
+ * temperature alone (needle-c/src/v3.rs:219-250). */
+size_t nd_sample_rows_work(nd_ctx *ctx, size_t count, size_t n);
+int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, size_t n,
+                   const nd_sampling *sampling, const float *u, int32_t *next, float *prob,
+                   void *work, size_t work_bytes);
+
 /* ---- libm on the device (crates/needle-core/src/math.rs:3-46) ------------- */
 
 /* y[i] = f(x[i]) for i < n (device buffers), f the device copy of the

@@ -53,6 +53,15 @@ class LogitsRules(C.Structure):
                 ("mask_stride", C.c_size_t), ("mask_rows", C.c_size_t), ("mask_row", C.c_void_p)]
 
 
+class PrefixMaps(C.Structure):
+    _fields_ = [("pos", C.c_void_p), ("rot", C.c_void_p), ("from_", C.c_void_p), ("lo", C.c_void_p),
+                ("order", C.c_void_p), ("first", C.c_void_p)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("min_p", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p)]
+
+
 _lib = None
 _vp, _sz = C.c_void_p, C.c_size_t
 
@@ -129,6 +138,14 @@ _SIGS = [
     ("nd_attend_tree_i8_work", _sz, [_vp, C.POINTER(KvGeom), _sz, _sz]),
     ("nd_attend_tree_i8", C.c_int, [_vp, C.POINTER(KvGeom), _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp,
                                     C.c_float, C.c_int, _vp, _vp, _sz]),
+    ("nd_prefix_plan_bytes", _sz, [C.POINTER(KvGeom), _sz, _sz, _sz]),
+    ("nd_prefix_plan", C.c_int, [_vp, C.POINTER(KvGeom), _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, C.c_int32, _vp, _sz,
+                                 C.POINTER(PrefixMaps)]),
+    ("nd_attend_prefix_i8_work", _sz, [_vp, C.POINTER(KvGeom), _sz, _sz, _sz]),
+    ("nd_attend_prefix_i8", C.c_int, [_vp, C.POINTER(KvGeom), _vp, _sz, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _vp,
+                                      C.c_float, C.c_int, _vp, _vp, _sz]),
+    ("nd_sample_rows_work", _sz, [_vp, _sz, _sz]),
+    ("nd_sample_rows", C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(Sampling), _vp, _vp, _vp, _vp, _sz]),
     ("nd_logits_adjust_work", _sz, [_vp, _sz, _sz]),
     ("nd_logits_adjust", C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(LogitsRules), _vp, _sz, _vp, _vp,
                                    _sz]),
@@ -859,6 +876,127 @@ def logits_adjust(ctx, x, hist=None, hist_len=None, out_from=None, repeat=None, 
 def logits_adjust_work(ctx, count, n):
     """Bytes of `work` that logits_adjust needs."""
     return lib().nd_logits_adjust_work(ctx.h, count, n)
+
+
+# ---- a batch that shares its prompts -------------------------------------------
+
+class PrefixPlan:
+    """What prefix_plan leaves for attend_prefix_i8: the work list of a step's
+    rows (`data`, a uint8 device tensor) and the sizes it was made for."""
+
+    def __init__(self, data, sizes):
+        self.data, self.sizes = data, sizes
+
+
+def prefix_plan_bytes(g, sessions, rows, prefixes):
+    """Bytes of the plan of a step of `rows` rows a session."""
+    return lib().nd_prefix_plan_bytes(C.byref(g), sessions, rows, prefixes)
+
+
+def prefix_plan(ctx, g, prefix_cap, prefix_len, used, prefix_of=None, length=None, rows=1, window=0, plan=None,
+                maps=None):
+    """A step of `rows` rows a session laid out (nd_prefix_plan): prefix_len [P]
+    positions of each prefix (None: no prefixes), used [S] positions each
+    session's own block holds, prefix_of [S] its prefix (-1: none; None: prefix
+    0), length [S] its rows in this step (None: all), all int32; a row attends to
+    `window` positions (0: all).  Returns (plan, maps): a PrefixPlan for
+    attend_prefix_i8, and the int32 maps (pos, rot, from, lo [S][rows], -1 where
+    a row is not there; order [S * rows], first [P + 1]).  `plan` (a uint8 device
+    tensor of prefix_plan_bytes()) and `maps` (six tensors or Nones, or False for
+    none) are allocated if not given."""
+    torch = _torch()
+    i32 = torch.int32
+    s, p = used.numel(), prefix_len.numel() if prefix_len is not None else 0
+    nb = prefix_plan_bytes(g, s, rows, p)
+    data = plan.data if isinstance(plan, PrefixPlan) else plan
+    if data is None:
+        data = _empty(ctx, (max(nb, 1),), torch.uint8)
+    if maps is None:
+        maps = tuple(_empty(ctx, (s, rows), i32) for _ in range(4)) + (_empty(ctx, (s * rows,), i32),
+                                                                       _empty(ctx, (p + 1,), i32))
+    need = (s * rows,) * 5 + (p + 1,)
+    names = ("pos", "rot", "from", "lo", "order", "first")
+    m = PrefixMaps(*(_dev_arg(ctx, t, i32, f"maps: {n}", k) for t, n, k in zip(maps or (None,) * 6, names, need)))
+    _check(lib().nd_prefix_plan(
+        ctx.h, C.byref(g), prefix_cap, s, rows, p, _dev_arg(ctx, prefix_of, i32, "prefix_of", s),
+        _dev_arg(ctx, prefix_len, i32, "prefix_len", p), _dev_arg(ctx, used, i32, "used"),
+        _dev_arg(ctx, length, i32, "length", s), window, _dev_arg(ctx, data, torch.uint8, "plan"), data.numel(),
+        C.byref(m)))
+    if not isinstance(plan, PrefixPlan):
+        plan = PrefixPlan(data, None)
+    plan.sizes = (s, rows, p, prefix_cap, g.num_heads, g.num_kv_heads, g.cap)
+    return plan, maps
+
+
+def attend_prefix_i8(ctx, g, kv, kv_stride, prefix_kv, prefix_stride, plan, q, scale=None, quant_query=False, out=None,
+                     work=None):
+    """Attention of a step's rows over their shared prefixes and their sessions'
+    own blocks (nd_attend_prefix_i8): q [S][rows][heads * qk] fp32, plan as
+    prefix_plan made it for the same geometry and sizes, prefix_kv the prefixes'
+    blocks, prefix_stride bytes apart.  out [S][rows][heads * v]; rows that are
+    not there are left as they are, zeros in a new `out`.  work: a uint8 device
+    tensor of attend_prefix_i8_work() bytes, needed while a graph is captured."""
+    torch = _torch()
+    f32, u8 = torch.float32, torch.uint8
+    s, n, p, cap = plan.sizes[:4]
+    if q.dim() != 3 or q.shape[:2] != (s, n):
+        raise ValueError(f"q: shape {tuple(q.shape)}, expected [{s}][{n}][heads * qk]")
+    if plan.sizes[4:] != (g.num_heads, g.num_kv_heads, g.cap):
+        raise ValueError("plan: made for another geometry")
+    wo = g.num_heads * g.v_head_dim
+    if scale is None:
+        scale = float(np.float32(1.0) / np.sqrt(np.float32(g.qk_head_dim)))
+    if out is None:
+        out = _empty(ctx, (s, n, wo), f32)
+        with torch.cuda.stream(ctx.stream):
+            out.zero_()
+    blocks = kv_block_bytes(g) + (s - 1) * kv_stride if s else 0
+    many = 0
+    if p:
+        many = kv_block_bytes(KvGeom(g.num_heads, g.num_kv_heads, g.qk_head_dim, g.v_head_dim, cap)) + \
+            (p - 1) * prefix_stride
+        if prefix_kv is None:
+            raise ValueError("prefix_kv: the plan has prefixes")
+    wp, wb = _work_arg(ctx, work)
+    _check(lib().nd_attend_prefix_i8(
+        ctx.h, C.byref(g), _dev_arg(ctx, kv, u8, "kv", blocks), kv_stride, s, n,
+        _dev_arg(ctx, prefix_kv, u8, "prefix_kv", many), prefix_stride, cap, p, _dev_arg(ctx, plan.data, u8, "plan"),
+        _dev_arg(ctx, q, f32, "q", s * n * g.num_heads * g.qk_head_dim), scale, int(bool(quant_query)),
+        _dev_arg(ctx, out, f32, "out", s * n * wo), wp, wb))
+    return out
+
+
+def attend_prefix_i8_work(ctx, g, sessions, rows, prefixes):
+    """Bytes of `work` that attend_prefix_i8 needs."""
+    return lib().nd_attend_prefix_i8_work(ctx.h, C.byref(g), sessions, rows, prefixes)
+
+
+# ---- sampling ------------------------------------------------------------------
+
+def sample_rows(ctx, x, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, prob=None, work=None):
+    """A token drawn from each row of logits ([count][n] fp32, rows may be apart)
+    by the random numbers u ([count] fp32 in [0, 1)) under temperature, min_p,
+    top_p ([count] fp32) and top_k ([count] int32) (nd_sample_rows).  Returns
+    (tokens int32 [count], -1 where a row has none, their chances fp32 [count])."""
+    torch = _torch()
+    i32, f32 = torch.int32, torch.float32
+    count, n = x.shape
+    xp, xs = _rows_arg(ctx, x, count, n, "x")
+    rules = Sampling(_dev_arg(ctx, temperature, f32, "temperature", count), _dev_arg(ctx, min_p, f32, "min_p", count),
+                     _dev_arg(ctx, top_k, i32, "top_k", count), _dev_arg(ctx, top_p, f32, "top_p", count))
+    if out is None:
+        out = _empty(ctx, (count,), i32)
+    if prob is None:
+        prob = _empty(ctx, (count,), f32)
+    wp, wb = _work_arg(ctx, work)
+    _check(lib().nd_sample_rows(ctx.h, xp, xs, count, n, C.byref(rules), _dev_arg(ctx, u, f32, "u", count),
+                                _dev_arg(ctx, out, i32, "out", count), _dev_arg(ctx, prob, f32, "prob", count), wp, wb))
+    return out, prob
+
+
+def sample_rows_work(ctx, count, n):
+    """Bytes of `work` that sample_rows needs."""
+    return lib().nd_sample_rows_work(ctx.h, count, n)
 
 
 # ---- Needle-3 forward on the device ----------------------------------------
