@@ -6,6 +6,7 @@
 #include "nd_kv_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -431,76 +432,518 @@ struct Attend {
     const uint8_t *kv, *pkv;
     size_t kv_stride, pkv_stride;
     const float *q;
-    float *out;
-    float scale;
-    int quant_query;
+    float *out, *part_o, *part_ml;  // sums of (slot, kv head, column), and their maximum and weight
+    Divisor by_rep;
+    float scale2;  // |scale| log2(e); below 0 where scale is no number
+    int negative;  // scale < 0
 };
 
-// A wave a (row, head): 64 positions at a time, a lane each, then a lane a column.
-template <int QK>
-__global__ __launch_bounds__(64) void attend_kernel(Geom g, Geom gp, Attend a)
+__device__ inline bool made_for(const Head &h, const Sizes &z)
 {
-    __shared__ float qs[QK], ws[64];
-    const int lane = threadIdx.x;
-    const uint32_t row = blockIdx.x, head = blockIdx.y, kvh = head / uint32_t(a.z.H / a.z.KVH);
-    const uint32_t i = row / a.z.rows, n = row - i * a.z.rows;
-    const Head hd = *a.plan.head();
-    float *out = a.out + (size_t(row) * a.z.H + head) * VD + lane;
-    const bool fits = hd.magic == kPlanMagic && hd.count == int(a.z.count) && hd.rows == int(a.z.rows) &&
-                      hd.prefixes == int(a.z.prefixes) && hd.heads == a.z.H && hd.kv_heads == a.z.KVH &&
-                      hd.cap == a.z.cap && hd.prefix_cap == a.z.pcap;
-    if (!fits) {
+    return h.magic == kPlanMagic && h.count == int(z.count) && h.rows == int(z.rows) && h.prefixes == int(z.prefixes) &&
+           h.heads == z.H && h.kv_heads == z.KVH && h.cap == z.cap && h.prefix_cap == z.pcap;
+}
+
+template <int QK, bool QQ>
+__global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at)
+{
+    constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
+    constexpr int LD = VD + 4, NW = 4;
+    __shared__ __align__(16) float sc_s[NW][64];
+    __shared__ __align__(16) float mo[NW][kCols][LD];
+    __shared__ floatx4_t ms[NW][kCols];  // maximum, more, weight
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 15, qd = lane >> 4;
+    const Head hd = *at.plan.head();
+    if (!made_for(hd, at.z) || int(blockIdx.x) >= hd.units) return;
+    const Unit un = at.plan.unit()[blockIdx.x];
+    const uint32_t kvh = blockIdx.y, R = uint32_t(gown.H / gown.KVH);
+    const bool own = un.source < 0;
+    const int wide = un.wide, mine = w & (wide - 1), stream = w / wide, step = NW / wide;
+    const uint32_t ncols = uint32_t(un.rows) * R, tile = 4 * uint32_t(un.quad) + uint32_t(mine);
+    if (tile * kCols >= ncols) return;  // (of a quad of three tiles, whose waves do not meet)
+
+    // ---- the wave's columns: what they see, and the query operand.  A column past
+    // the end is a copy of the last ----
+    const uint32_t f = min(tile * kCols + uint32_t(n), ncols - 1), r = at.by_rep.quotient(f);
+    uint32_t row, lo, hi;
+    if (own) {
+        const uint32_t end = uint32_t(un.used) + r;  // the row's own position, below 2^31
+        row = uint32_t(~un.source) * at.z.rows + r;
+        lo = hd.window && end + 1 > uint32_t(hd.window) ? end + 1 - uint32_t(hd.window) : 0;
+        hi = end;
+    } else {
+        const Place pl = at.plan.place()[uint32_t(un.first) + r];
+        row = uint32_t(pl.row);
+        lo = uint32_t(pl.from);
+        hi = 0x7fffffff;
+    }
+    const uint32_t head = kvh * R + f - r * R;
+    float v[SL];
+    {
+        const float *qh = at.q + (size_t(row) * gown.H + head) * QK + qd * SL;
+#pragma unroll
+        for (int e = 0; e < SL; ++e) v[e] = qh[e];
+    }
+    const uint32_t cap = uint32_t(own ? gown.cap : gp.cap);
+    const uint8_t *blk = own ? at.kv + size_t(~un.source) * at.kv_stride : at.pkv + size_t(un.source) * at.pkv_stride;
+    const size_t v_off = own ? gown.v_off : gp.v_off, ks_off = own ? gown.ks_off : gp.ks_off;
+    const rows_t kb = rows_at(blk + size_t(kvh) * cap * QK, cap * QK);
+    const rows_t vb = rows_at(blk + v_off + size_t(kvh) * cap * VD, cap * VD);
+    // K scales, and vs_off - ks_off bytes on (KVH cap 4, below 2^32) the V scales
+    const uint32_t to_vs = uint32_t((own ? gown.vs_off : gp.vs_off) - ks_off);
+    const rows_t sb = rows_at(blk + ks_off + size_t(kvh) * cap * 4, to_vs + cap * 4);
+    // the first position that all columns see, and the last
+    uint32_t tlo = lo, thi = hi;
+    auto both = [&](auto distance) {
+        constexpr int D = decltype(distance)::value;
+        tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
+        thi = min(thi, uint32_t(ndl::wave_xor_int<D>(int(thi))));
+    };
+    both(std::integral_constant<int, 1>{});
+    both(std::integral_constant<int, 2>{});
+    both(std::integral_constant<int, 4>{});
+    both(std::integral_constant<int, 8>{});
+    tlo = __builtin_amdgcn_readfirstlane(tlo);
+    thi = __builtin_amdgcn_readfirstlane(thi);
+
+    // ---- the walk: up to the ring's end, then from its start, in chunks of 32 (the
+    // last of a part shorter).  It is no longer than the ring, so it wraps once ----
+    const uint32_t span = uint32_t(un.span), begin = uint32_t(un.from), slo = begin % cap;
+    const uint32_t n0 = min(span, cap - slo), n1 = span - n0;
+    const int e0 = int((n0 + 31) / 32), nch = un.end;
+    int ch = un.begin + stream;
+    uint32_t s0 = 0;   // the chunk's first slot,
+    uint32_t p0 = 0;   // its position,
+    int left = 0;      // positions from there to the part's end; 0 behind the last chunk
+    int stop = 0;      // the part's last chunk, and one
+    auto place = [=, &s0, &p0, &left, &stop](int i) {
+        const bool second = i >= e0;
+        const uint32_t off = 32u * uint32_t(second ? i - e0 : i);
+        s0 = i >= nch ? 0u : (second ? 0u : slo) + off;
+        p0 = begin + (second ? n0 : 0u) + off;
+        left = i >= nch ? 0 : int((second ? n1 : n0) - off);
+        stop = second ? nch : min(e0, nch);
+    };
+    uint32_t kr[2][KD], vr[8];
+    float scr = 0.0f;
+    const uint32_t kl = uint32_t(n * QK + qd * SL), vl = uint32_t(4 * qd * VD + 4 * n);
+    const uint32_t scl = (lane & 31) * 4 + (lane < 32 ? 0u : to_vs);
+    // loads of K and V are never conditional: past the last chunk they read some slot
+    auto load_k = [&]() {
+        const uint32_t o = here(kl + s0 * QK);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            if constexpr (KD == 3) {
+                const auto r = __builtin_amdgcn_raw_buffer_load_b96(kb, o + 16 * a * QK, 0, 0);
+#pragma unroll
+                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+            } else {
+                const auto r = __builtin_amdgcn_raw_buffer_load_b128(kb, o + 16 * a * QK, 0, 0);
+#pragma unroll
+                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+            }
+        }
+        scr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sb, scl + s0 * 4, 0, 0));
+    };
+    auto load_v = [&]() {
+        const uint32_t o = here(vl + s0 * VD);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            vr[j] = __builtin_amdgcn_raw_buffer_load_b32(vb, o + (16 * (j >> 2) + (j & 3)) * VD, 0, 0);
+    };
+    place(ch);
+    load_k();
+    load_v();
+
+    // ---- the query operand, while the first chunk is on its way ----
+    float cf0;                        // factor of a score, in bits, is |cf0| 2^(kexp - sh)
+    int sh;
+    intx4_t qi;                       // QQ: codes
+    uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
+    {
+        if (at.negative) {
+            asm volatile("");  // (a branch)
+#pragma unroll
+            for (int e = 0; e < SL; ++e) v[e] = -v[e];
+        }
+        float a = 0.0f;
+#pragma unroll
+        for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1]));
+        a = fmaxf(a, ndl::wave_xor<16>(a));
+        a = fmaxf(a, ndl::wave_xor<32>(a));
+        float nan = 0.0f;
+        if constexpr (QQ) {
+            // quant_rows (model.rs:289-293): the codes and the head's scale
+            const float qs = a > 0.0f ? a / 127.0f : 1.0f;
+            const float inv = 1.0f / qs;
+            uint32_t dw[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                // quant_code: half away from zero is truncation after adding
+                // the float below a half, for every |y| < 2^22
+                const float y = v[e] * inv;
+                const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
+                nan = y != y ? y : nan;
+                dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
+            }
+            qi = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
+            sh = -__builtin_amdgcn_frexp_expf(qs);
+            cf0 = __builtin_amdgcn_ldexpf(qs, sh) * at.scale2;
+        } else {
+            // the head in 2^14 .. 2^15, so that the second pieces are normal numbers
+            sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
+#pragma unroll
+            for (int e = 0; e < SL; ++e) {
+                nan = v[e] - v[e] != 0.0f ? NAN : nan;
+                v[e] = __builtin_amdgcn_ldexpf(v[e], sh);
+            }
+#pragma unroll
+            for (int e = 0; e < SL; e += 2) split2(v[e], v[e + 1], qp[0][e / 2], qp[1][e / 2]);
+            cf0 = at.scale2;
+        }
+        // a query that has a NaN (or an infinity, which gives one) makes no number
+        // of what its node sees, and zeros of nothing: cf0's sign says so until the
+        // sum is known
+        nan += ndl::wave_xor<16>(nan);
+        nan += ndl::wave_xor<32>(nan);
+        cf0 = nan != nan ? -__builtin_fabsf(cf0) : cf0;
+    }
+    // (a factor of 0 would make no number of a score of -inf)
+    auto factor = [&](int k) {
+        const float c = __builtin_amdgcn_ldexpf(__builtin_fabsf(cf0), k - sh);
+        return c == 0.0f ? 0x1p-126f : c;
+    };
+    float cf = factor(0);
+
+    // m_run: a score of the column that the sums are against (mu = m_run cf, in
+    // bits).  Another is taken, and the sums scaled, where one gets more than kAhead
+    // bits ahead of it (lim, in the scores' units), or all stay far behind
+    constexpr float kAhead = 5.0f;
+    float m_run = -INFINITY, lim = -INFINITY, mu = 0.0f, l_run = 0.0f;
+    floatx4_t acc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    // K and V scales are taken in units of 2^kexp and 2^(vexp - 10), powers of
+    // two that no finite one so far is above: scores before cf, and weights,
+    // stay in range at any size of the cache's values
+    int kexp = 0, vexp = 0;
+    float top = 0.0f;                   // lanes below 32: 2^kexp, the others: 2^vexp
+    int shift = lane < 32 ? 0 : 10;
+    // Weights below 2^-2 lose bits of their second pieces.  Where a column has met a
+    // larger one in a product of pieces, those bits are none of the result's, and it
+    // meets one (an e of 1 and a V scale of 2 units or more) with each new m_run; not
+    // where that lies in a chunk of small values, or where the unit of weights has
+    // grown since, by more than 2^3.  From then on (watch: lim lets every chunk in)
+    // a column goes on against the next chunk's own maximum, which may lie far below:
+    // its sums are multiplied (up to 2^100)
+    uint32_t watch = 0;
+    int vmet = 0x10000;                 // vexp then, and 3
+
+    for (; ch < nch; ch += step) {
+        // ---- the positions each column sees ----
+        const bool full = p0 >= tlo && p0 + 31 <= thi && left >= 32;
+        uint32_t vis = 0xffffffffu;
+        if (!full) {
+            vis = left < 32 ? (1u << left) - 1u : 0xffffffffu;
+            vis &= lo <= p0 ? 0xffffffffu : lo - p0 < 32u ? 0xffffffffu << (lo - p0) : 0u;
+            vis &= hi < p0 ? 0u : hi - p0 < 31u ? (2u << (hi - p0)) - 1u : 0xffffffffu;
+        }
+        // ---- the chunk's scales, zero behind its end ----
+        float sc = (lane & 31) < left ? scr : 0.0f;
+        if (any_of(!(__builtin_fabsf(sc) <= top))) {
+            // what no column sees may be anything: it sets no unit, and counts as one
+            bool unseen = false;
+            if (!full) {
+                uint32_t seen = vis;
+                seen |= uint32_t(ndl::wave_xor_int<1>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<2>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<4>(int(seen)));
+                seen |= uint32_t(ndl::wave_xor_int<8>(int(seen)));
+                unseen = !(seen >> (lane & 31) & 1u);
+                sc = unseen ? 0.0f : sc;
+            }
+            // a V scale that is no number makes no number of the columns that see
+            // it, and only of those: a weight of 0 there would not stay 0
+            const bool wild = lane >= 32 && !(__builtin_fabsf(sc) < INFINITY);
+            const uint32_t wilds = uint32_t(__builtin_amdgcn_ballot_w64(wild) >> 32);
+            if (wild) sc = 0.0f;
+            if (vis & wilds) l_run = NAN;
+            float h = __builtin_fabsf(sc) < INFINITY ? fmaxf(__builtin_fabsf(sc), top) : top;
+            h = fmaxf(h, ndl::wave_xor<16>(h));
+            h = fmaxf(h, ndl::wave_xor<8>(h));
+            h = fmaxf(h, ndl::wave_xor<4>(h));
+            h = fmaxf(h, ndl::wave_xor<2>(h));
+            h = fmaxf(h, ndl::wave_xor<1>(h));
+            const int was = lane < 32 ? kexp : vexp;
+            const int now = h > top ? __builtin_amdgcn_frexp_expf(h) : was;
+            top = h > top ? (now > 127 ? 0x1.fffffep127f : __builtin_amdgcn_ldexpf(1.0f, now)) : top;
+            sc = unseen ? top : sc;
+            shift += was - now;
+            const int kn = __builtin_amdgcn_readlane(now, 0), vn = __builtin_amdgcn_readlane(now, 32);
+            if (vn > vmet) {
+                watch = 1;
+                vmet = vn + 3;
+            }
+            m_run = __builtin_amdgcn_ldexpf(m_run, kexp - kn);
+            cf = factor(kn);
+            lim = watch || m_run == -INFINITY ? -INFINITY : m_run + kAhead * __builtin_amdgcn_rcpf(cf);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - vn);
+            kexp = kn;
+            vexp = vn;
+        }
+        sc = __builtin_amdgcn_ldexpf(sc, shift);
+        const uint32_t few = uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32);
+        uint32_t small = left < 32 ? few & ((1u << left) - 1u) : few;
+        sc_s[w][lane] = sc;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        floatx4_t ks[2], vs[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ks[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][16 * a + 4 * qd]);
+            vs[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][32 + 16 * a + 4 * qd]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        // ---- scores ----
+        float s[8];
+        if constexpr (QQ) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const intx4_t kf{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
+                const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi, intx4_t{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * a + i] = float(d[i]) * ks[a][i];
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                uint32_t kp[2 * KD];
+#pragma unroll
+                for (int d = 0; d < KD; ++d) {
+                    const uint32_t u = kr[a][d] ^ 0x80808080u;
+                    kp[2 * d] = f16_pair<0>(u);
+                    kp[2 * d + 1] = f16_pair<1>(u);
+                }
+                floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int pc = 1; pc >= 0; --pc) {  // the small pieces first
+                    const uint32_t *qq = qp[pc];
+                    // qk 48: a lane's last four codes, doubled to the 32-wide
+                    // product's eight against four zeros of the query
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        vec4<f16x8_t>(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1]),
+                        KD == 3 ? vec4<f16x8_t>(qq[4], qq[5], 0u, 0u)
+                                : vec4<f16x8_t>(qq[4], qq[5], qq[2 * KD - 2], qq[2 * KD - 1]),
+                        d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(kp[0], kp[1], kp[2], kp[3]),
+                                                               vec4<f16x8_t>(qq[0], qq[1], qq[2], qq[3]), d, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * a + i] = d[i] * ks[a][i];
+            }
+        }
+        // the next chunk: its K lands during the softmax and the values
+        if (ch + step < stop) [[likely]] {
+            s0 += 32u * uint32_t(step);
+            p0 += 32u * uint32_t(step);
+            left -= 32 * step;
+        } else {
+            asm volatile("");  // (a branch, not thirty selects in every chunk)
+            place(ch + step);
+        }
+        load_k();
+        // ---- softmax: each lane its column's eight positions ----
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(vis >> (16 * (j >> 2) + 4 * qd + (j & 3)) & 1u)) s[j] = -INFINITY;
+        }
+        const float m8 = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[7]));
+        if (any_of(m8 > lim)) {
+            // a row of zeros has a scale of 1, which is no measure of its values
+            small |= uint32_t(__builtin_amdgcn_ballot_w64(sc == __builtin_amdgcn_ldexpf(1.0f, shift)) >> 32);
+            float m_new = max3(m8, m_run, ndl::wave_xor<16>(m8));
+            m_new = fmaxf(m_new, ndl::wave_xor<32>(m_new));
+            if (watch && !small) [[unlikely]] {
+                float m = fmaxf(m8, ndl::wave_xor<16>(m8)), l = fmaxf(l_run, ndl::wave_xor<16>(l_run));
+                m = fmaxf(m, ndl::wave_xor<32>(m));
+                l = fmaxf(l, ndl::wave_xor<32>(l));
+                const float behind = mu - m * cf;
+                const bool down = (m > -INFINITY) & (behind + float(__builtin_amdgcn_frexp_expf(l)) < 100.0f);
+                m_new = down ? m : m_new;
+                watch = any32((m_new > -INFINITY) & !down);
+            }
+            watch |= small;
+            vmet = min(vmet, vexp + 3);
+            const float mu_new = m_new == -INFINITY ? 0.0f : m_new * cf;
+            // nothing is summed yet where there was no maximum
+            const float al = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mu - mu_new);
+            m_run = m_new;
+            lim = watch || m_new == -INFINITY ? -INFINITY : m_new + kAhead * __builtin_amdgcn_rcpf(cf);
+            mu = mu_new;
+            l_run *= al;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] *= al;
+        }
+        // the weights e vs, and the sum of e
+        float wt[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], cf, -mu));
+            l_run += e;
+            wt[j] = e * vs[j >> 2][j & 3];
+        }
+        // ---- values ----
+        if (small) [[unlikely]] {
+            // (then the product below adds nothing: two ways that each end in
+            // sums cost copies of all of them)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(i8_at(vr[j], c) * 0x1p-9f, wt[j], acc[c], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wt[j] = 0.0f;
+        }
+        {
+            uint32_t ph[4], pl[4], u[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[j], pl[j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
+            auto column = [&](auto cc) {
+                constexpr int c = decltype(cc)::value;
+                const f16x8_t vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]),
+                                                 f16_codes<c>(u[4], u[5]), f16_codes<c>(u[6], u[7]));
+                acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(pl[0], pl[1], pl[2], pl[3]), acc[c],
+                                                                0, 0, 0);
+                acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(ph[0], ph[1], ph[2], ph[3]), acc[c],
+                                                                0, 0, 0);
+            };
+            column(std::integral_constant<int, 0>{});
+            column(std::integral_constant<int, 1>{});
+            column(std::integral_constant<int, 2>{});
+            column(std::integral_constant<int, 3>{});
+        }
+        load_v();  // lands during the next scores
+    }
+
+    // ---- the sums: a wave's own, or, where waves have shared a tile's chunks, put
+    // together by sixteen threads a column ----
+    l_run += ndl::wave_xor<16>(l_run);
+    l_run += ndl::wave_xor<32>(l_run);
+    l_run = ((__float_as_int(cf0) < 0) & (l_run != 0.0f)) ? NAN : l_run;
+    // the sums are left as 2^more of what has a weight of 1/2 to 1: of values near
+    // fp32's end the sum may be beyond it, the mean is not
+    const int more = __builtin_amdgcn_frexp_expf(l_run);
+    // (from here on the maximum is in bits; -inf: sums are 0, or NaN where a score was)
+    const float mb = m_run == -INFINITY ? -INFINITY : mu, lb = __builtin_amdgcn_ldexpf(l_run, -more);
+    const size_t slot = (size_t(un.slot) + mine) * gown.KVH + kvh;
+    if (step == 1) {
+        // (m + more may be rounded, M with it; m - M is not)
+        const float M = mb + float(more), by = mb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mb - M + float(more));
+        float *po = at.part_o + (slot * kCols + n) * VD + 16 * qd;
+        // lane (n, qd) holds V columns 16 qd + 4 i + c
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            floatx4_t o;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more) * by;
+            *reinterpret_cast<floatx4_t *>(po + 4 * i) = o;
+        }
+        if (qd == 0) *reinterpret_cast<floatx2_t *>(at.part_ml + (slot * kCols + n) * 2) = floatx2_t{M, lb * by};
+        return;
+    }
+    if (qd == 0) ms[w][n] = floatx4_t{mb, float(more), lb, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        floatx4_t o;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more);
+        *reinterpret_cast<floatx4_t *>(&mo[w][n][16 * qd + 4 * i]) = o;
+    }
+    __syncthreads();
+    const int col = t >> 4;
+    for (int j = 0; j < wide; ++j) {
+        // against a maximum 2^3 above the largest, so that no sum of eight leaves the
+        // values' range
+        float M = -INFINITY, L = 0.0f;
+        floatx4_t O{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = j; i < NW; i += wide) M = fmaxf(M, ms[i][col][0] + ms[i][col][1]);
+        M += 3.0f;
+        for (int i = j; i < NW; i += wide) {
+            const floatx4_t z = ms[i][col];
+            const float by = z[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(z[0] - M + z[1]);
+            L += z[2] * by;
+            O += *reinterpret_cast<const floatx4_t *>(&mo[i][col][4 * (t & 15)]) * by;
+        }
+        const size_t to = ((size_t(un.slot) + j) * gown.KVH + kvh) * kCols + col;
+        *reinterpret_cast<floatx4_t *>(at.part_o + to * VD + 4 * (t & 15)) = O;
+        if ((t & 15) == 0) *reinterpret_cast<floatx2_t *>(at.part_ml + to * 2) = floatx2_t{M, L};
+    }
+}
+
+// The sums of a (row, head) meet: a wave each, a lane a run of chunks, then a lane a
+// column.
+__global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t first, uint32_t total)
+{
+    const uint32_t oh = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (oh >= total) return;
+    const int lane = threadIdx.x & 63;
+    const uint32_t H = uint32_t(at.z.H), R = H / uint32_t(at.z.KVH), down = oh / H;
+    const uint32_t row = first + down, head = oh - down * H, kvh = head / R, r = head - kvh * R;
+    const uint32_t i = row / at.z.rows, n = row - i * at.z.rows;
+    float *out = at.out + (size_t(row) * H + head) * VD + lane;
+    if (!made_for(*at.plan.head(), at.z)) {
         *out = NAN;
         return;
     }
-    const Session s = a.plan.session()[i];
+    const Session s = at.plan.session()[i];
     if (int(n) >= s.there) return;
     if (s.bad) {
         *out = NAN;
         return;
     }
-    const float *qh = a.q + (size_t(row) * a.z.H + head) * QK;
-    if (lane < QK) qs[lane] = qh[lane];
-    __syncthreads();
-    if (a.quant_query) {
-        float sc, inv;
-        quant_scale_wave(qs, QK, sc, inv);
-        if (lane < QK) qs[lane] = quant_code(qs[lane], inv) * sc;
-        __syncthreads();
-    }
-    float m = -INFINITY, l = 0.0f;
-    double o = 0.0;  // (of values near fp32's end the sum is beyond it, the mean is not)
-    auto walk = [&](const Geom &gg, const uint8_t *blk, uint32_t lo, int span) {
-        const int8_t *kb = reinterpret_cast<const int8_t *>(blk) + size_t(kvh) * gg.cap * QK;
-        const int8_t *vb = reinterpret_cast<const int8_t *>(blk + gg.v_off) + size_t(kvh) * gg.cap * VD;
-        const float *ks = reinterpret_cast<const float *>(blk + gg.ks_off) + size_t(kvh) * gg.cap;
-        const float *vs = reinterpret_cast<const float *>(blk + gg.vs_off) + size_t(kvh) * gg.cap;
-        for (int done = 0; done < span; done += 64) {
-            const uint32_t p0 = lo + uint32_t(done), cap = uint32_t(gg.cap);
-            const int cnt = min(64, span - done), slot = int((p0 + uint32_t(min(lane, cnt - 1))) % cap);
-            float dot = 0.0f;
-            for (int e = 0; e < QK; ++e) dot += qs[e] * float(kb[size_t(slot) * QK + e]);
-            const float sc = lane < cnt ? dot * ks[slot] * a.scale : -INFINITY;
-            float top = fmaxf(m, wave_max(sc));
-            if (top == -INFINITY) top = 0.0f;
-            const float e = lane < cnt ? expf(sc - top) : 0.0f, al = m == -INFINITY ? 0.0f : expf(m - top);
-            m = top;
-            l = l * al + wave_sum(e);
-            o *= al;
-            ws[lane] = lane < cnt ? e * vs[slot] : 0.0f;
-            __syncthreads();
-            for (int j = 0; j < cnt; ++j) o += double(ws[j]) * double(vb[size_t((p0 + uint32_t(j)) % cap) * VD + lane]);
-            __syncthreads();
+    const uint32_t fp = (uint32_t(s.at) + n) * R + r, fo = n * R + r;
+    Quad qp{}, qo = at.plan.quad()[uint32_t(s.quads) + fo / (4 * kCols)];
+    if (s.prefix >= 0) qp = at.plan.quad()[uint32_t(at.plan.group()[s.prefix].quads) + fp / (4 * kCols)];
+    const int all = qp.runs + qo.runs;
+    float M = -INFINITY, L = 0.0f, O = 0.0f;
+    for (int j0 = 0; j0 < all; j0 += 64) {
+        const int j = j0 + lane, many = min(64, all - j0);
+        const bool old = j < qp.runs;
+        const uint32_t f = old ? fp : fo;
+        size_t to = 0;
+        float m = -INFINITY, l = 0.0f;
+        if (j < all) {
+            const uint32_t slot = (old ? uint32_t(qp.slot + j * qp.wide) : uint32_t(qo.slot + (j - qp.runs) * qo.wide)) +
+                                  f / kCols % 4;
+            to = (size_t(slot) * at.z.KVH + kvh) * kCols + f % kCols;
+            m = at.part_ml[2 * to];
+            l = at.part_ml[2 * to + 1];
         }
-    };
-    if (s.prefix >= 0) {
-        const Group gr = a.plan.group()[s.prefix];
-        const Place at = a.plan.place()[uint32_t(gr.first + s.at) + n];
-        walk(gp, a.pkv + size_t(s.prefix) * a.pkv_stride, uint32_t(at.from), gr.end - at.from);
+        // (a NaN among the weights is one of L; M is a number or -inf)
+        const float top = fmaxf(M, wave_max(m)), by = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        const float was = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        // as means of what is there, so that no sum leaves the values' range
+        const float part = l * by, now = L * was, sum = now + wave_sum(part);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        O *= now * inv;
+        for (int e = 0; e < many; ++e) {
+            const uint32_t a0 = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(to)), e));
+            const uint32_t a1 = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(to >> 32)), e));
+            const float b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(by * inv), e));
+            O += at.part_o[(size_t(a1) << 32 | a0) * VD + lane] * b;
+        }
+        L = sum;
     }
-    const int64_t end = int64_t(s.used) + n + 1, lo = hd.window ? max(end - hd.window, int64_t(0)) : 0;
-    walk(g, a.kv + size_t(i) * a.kv_stride, uint32_t(lo), int(end - lo));
-    *out = float(o / l);
+    *out = L != L ? NAN : O;
 }
 
 // ---- the host's side ------------------------------------------------------------
@@ -528,6 +971,8 @@ Sizes sizes_of(const nd_kv_geom *g, size_t prefix_cap, size_t count, size_t rows
     return Sizes{uint32_t(count), uint32_t(rows), uint32_t(prefixes), g->num_heads, g->num_kv_heads, g->cap,
                  prefixes ? int(prefix_cap) : 1};
 }
+
+size_t partial_floats(const Sizes &z) { return size_t(layout_of(z).slots) * z.KVH * kCols * (VD + 2); }
 
 }  // namespace
 
@@ -566,7 +1011,7 @@ size_t nd_attend_prefix_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, 
 {
     nd::clear_error();
     if (!ctx || check_sizes(g, count, rows, prefixes) != ND_OK || !count) return 0;
-    return 0;
+    return partial_floats(sizes_of(g, 1, count, rows, prefixes)) * sizeof(float);
 }
 
 int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t kv_stride,
@@ -601,14 +1046,28 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     a.pkv_stride = prefix_stride;
     a.q = q;
     a.out = out;
-    a.scale = scale;
-    a.quant_query = quant_query;
+    a.by_rep = Divisor::of(uint32_t(g->num_heads / g->num_kv_heads));
+    a.scale2 = scale == scale ? float(double(scale < 0 ? -scale : scale) * 1.4426950408889634) : -1.0f;
+    a.negative = scale < 0;
+    void *ws = nullptr;
+    if (int rc = nd::call_workspace(ctx, partial_floats(a.z) * sizeof(float), work, work_bytes, &ws)) return rc;
+    a.part_o = static_cast<float *>(ws);
+    a.part_ml = a.part_o + size_t(a.plan.l.slots) * a.z.KVH * kCols * VD;
     nd_kv_geom pg = *g;
     pg.cap = a.z.pcap;
-    auto *fn = g->qk_head_dim == 48 ? attend_kernel<48> : attend_kernel<64>;
-    hipLaunchKernelGGL(fn, dim3(unsigned(count * rows), unsigned(g->num_heads)), dim3(64), 0, ctx->stream, make_geom(g),
+    auto *fn = g->qk_head_dim == 48 ? (quant_query ? prefix_kernel<48, true> : prefix_kernel<48, false>)
+                                    : (quant_query ? prefix_kernel<64, true> : prefix_kernel<64, false>);
+    hipLaunchKernelGGL(fn, dim3(a.plan.l.units, unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
                        make_geom(&pg), a);
-    return nd::check_launch("attend_prefix_i8");
+    if (int rc = nd::check_launch("attend_prefix_i8")) return rc;
+    // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
+    const size_t step = (size_t(1) << 25) / size_t(g->num_heads);
+    for (size_t first = 0; first < count * rows; first += step) {
+        const uint32_t total = uint32_t(std::min(step, count * rows - first) * g->num_heads);
+        hipLaunchKernelGGL(prefix_join_kernel, dim3((total + 3) / 4), dim3(256), 0, ctx->stream, a, uint32_t(first), total);
+        if (int rc = nd::check_launch("prefix_join")) return rc;
+    }
+    return ND_OK;
 }
 
 }  // extern "C"
