@@ -100,6 +100,40 @@ __device__ inline float wave_sum64(float v)
     return v + wave_xor<1>(v);
 }
 
+// The lane C places from this one by a DPP control, 0 where there is none or the
+// row is masked out.
+template <int C, int ROWS>
+__device__ inline uint32_t dpp_or_zero(uint32_t x)
+{
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), C, ROWS, 0xf, true));
+}
+
+template <int C, int ROWS>
+__device__ inline uint64_t dpp_or_zero(uint64_t x)
+{
+    return uint64_t(dpp_or_zero<C, ROWS>(uint32_t(x >> 32))) << 32 | dpp_or_zero<C, ROWS>(uint32_t(x));
+}
+
+// The whole numbers of lanes 0 .. this one added up (T: uint32_t or uint64_t): within
+// rows of 16 by row_shr 1, 2, 4, 8, then each odd row takes the last lane of the row
+// before it (row_bcast:15) and the upper half lane 31 (row_bcast:31).
+template <typename T>
+__device__ inline T wave_scan(T v)
+{
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    return v + dpp_or_zero<0x143, 0xc>(v);
+}
+
+__device__ inline uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
+__device__ inline uint64_t last_lane(uint64_t x)
+{
+    return uint64_t(last_lane(uint32_t(x >> 32))) << 32 | last_lane(uint32_t(x));
+}
+
 // v summed with its partners at lane distances D, 2 D, .., 32, in that
 // order (lanes sharing l mod D end with their group's total).
 template <int D>

@@ -26,31 +26,26 @@ constexpr size_t kMaxSessions = 65535, kMaxRows = 256, kMaxAll = size_t(1) << 20
 // the requests' lengths are, and each leaves its sums in slots, one a tile.
 constexpr int kPlanMagic = 0x6e645031;
 constexpr uint32_t kBlocks = 1024;     // four a CU
-constexpr uint32_t kLeast = 2;         // chunks a wave, at least
+constexpr uint32_t kLeast = 4;         // chunks a wave, at least
 
 struct Head {
     int magic, count, rows, prefixes, heads, kv_heads, cap, prefix_cap;
     int units, slots, window, pad[5];
 };
 
-// there: the rows the session has, bad: no number comes of them; prefix -1: none;
-// at: its first row's place in the prefix's group.
-struct Session {
-    int there, bad, prefix, at;
-    int used, lo, span, quads;  // own positions lo .. lo + span - 1; first quad
-};
-
-struct Group {
-    int first, rows, begin, span;  // places in the order; positions
-    int end, quads, pad0, pad1;    // the prefix's length; first quad
-};
-
 struct Place {
     int row, from;
 };
 
-struct Quad {
-    int slot, runs, wide, pad;  // first slot, runs of chunks; slot + run * wide + tile
+// Where the sums of a row's heads are, in its prefix's slots or its session's: the
+// slot of the quad of its first head's column, the quad's runs (and the next one's,
+// where the other heads' columns may lie, 16 bits on) and wides (4 bits on).
+struct Seat {
+    int slot, runs, wides, column;
+};
+
+struct Seats {
+    Seat prefix, own;  // (own.column: below 0 no row, 1 a bad one)
 };
 
 struct Unit {
@@ -60,9 +55,8 @@ struct Unit {
 };
 
 struct Layout {
-    size_t session, group, quad, place, unit, bytes;  // offsets
-    uint32_t quads_prefix, quads_own;                 // at most: of all prefixes, of a session
-    uint32_t units, slots;                            // at most
+    size_t seat, place, unit, bytes;  // offsets
+    uint32_t units, slots;            // at most
 };
 
 struct Sizes {
@@ -77,19 +71,16 @@ Layout layout_of(const Sizes &z)
     const uint64_t R = uint64_t(z.H / z.KVH), own = ceil_div(z.rows * R, kCols);
     const uint64_t all = ceil_div(uint64_t(z.count) * z.rows * R, kCols);
     Layout l{};
-    l.quads_prefix = z.prefixes ? uint32_t((all + 3) / 4) + z.prefixes : 0;
-    l.quads_own = uint32_t((own + 3) / 4);
     // units: a quad's last run may be short, the full ones come to kBlocks / KVH
     const uint32_t runs = std::max<uint32_t>(1, kBlocks / uint32_t(z.KVH));
-    const uint64_t quads = l.quads_prefix + uint64_t(z.count) * l.quads_own;
+    const uint64_t quads = (z.prefixes ? (all + 3) / 4 + z.prefixes : 0) + uint64_t(z.count) * ((own + 3) / 4);
     l.units = uint32_t(quads + runs);
     // slots: a quad of three tiles has four
     l.slots = uint32_t((z.prefixes ? all + 2 * z.prefixes : 0) + z.count * (own + (own % 4 == 3)) + 4 * runs);
-    l.session = sizeof(Head);
-    l.group = l.session + z.count * sizeof(Session);
-    l.quad = l.group + z.prefixes * sizeof(Group);
-    l.place = l.quad + quads * sizeof(Quad);
-    l.unit = nd::align_up(l.place + size_t(z.count) * z.rows * sizeof(Place), 64);
+    const size_t rows = size_t(z.count) * z.rows;
+    l.seat = sizeof(Head);
+    l.place = l.seat + rows * sizeof(Seats);
+    l.unit = nd::align_up(l.place + rows * sizeof(Place), 64);
     l.bytes = l.unit + l.units * sizeof(Unit);
     return l;
 }
@@ -98,9 +89,7 @@ struct PlanOf {
     uint8_t *p;
     Layout l;
     __host__ __device__ Head *head() const { return reinterpret_cast<Head *>(p); }
-    __host__ __device__ Session *session() const { return reinterpret_cast<Session *>(p + l.session); }
-    __host__ __device__ Group *group() const { return reinterpret_cast<Group *>(p + l.group); }
-    __host__ __device__ Quad *quad() const { return reinterpret_cast<Quad *>(p + l.quad); }
+    __host__ __device__ Seats *seat() const { return reinterpret_cast<Seats *>(p + l.seat); }
     __host__ __device__ Place *place() const { return reinterpret_cast<Place *>(p + l.place); }
     __host__ __device__ Unit *unit() const { return reinterpret_cast<Unit *>(p + l.unit); }
 };
@@ -110,46 +99,52 @@ struct Requests {
     int window;
 };
 
-// One session's numbers.
+// One session's numbers, as they are given and as they are meant.
+struct Given {
+    int prefix, used, length;
+};
+
 struct Want {
     int there, bad, prefix, used, prefix_len, from, lo, span;
     __device__ int rows() const { return bad ? 0 : there; }
 };
 
-__device__ inline Want want_of(const Sizes &z, const Requests &r, uint32_t i)
+__device__ inline Given given_of(const Sizes &z, const Requests &r, uint32_t i)
 {
-    Want w{};
-    const int p = r.prefix_of ? r.prefix_of[i] : z.prefixes ? 0 : -1;
-    const int m = r.length ? r.length[i] : int(z.rows), u = r.used[i];
-    const bool some = p >= 0 && p < int(z.prefixes);
-    const int L = some ? r.prefix_len[p] : 0;
-    const bool fits = m >= 0 && m <= int(z.rows);
-    w.there = fits ? m : int(z.rows);
-    w.prefix = some ? p : -1;
-    w.used = u;
-    w.prefix_len = L;
-    bool bad = !fits || p >= int(z.prefixes) || u < 0 || L < 0 || int64_t(L) + u + m > int64_t(1) << 31;
-    if (!bad) {
-        // the first row's window; the others' begin later
-        w.lo = r.window ? int(max(int64_t(u) + 1 - r.window, int64_t(0))) : 0;
-        w.from = r.window ? int(min(max(int64_t(L) + u + 1 - r.window, int64_t(0)), int64_t(L))) : 0;
-        const int64_t span = int64_t(u) + m - w.lo;
-        w.span = int(min(span, int64_t(z.cap)));
-        bad = m > 0 && (span > z.cap || L - w.from > z.pcap);
-    }
-    w.bad = bad;
+    return Given{r.prefix_of ? r.prefix_of[i] : z.prefixes ? 0 : -1, r.used[i], r.length ? r.length[i] : int(z.rows)};
+}
+
+__device__ inline Want want_of(const Sizes &z, uint32_t window, const Given &g, const uint32_t *prefix_len)
+{
+    Want w;
+    const bool some = uint32_t(g.prefix) < z.prefixes, fits = uint32_t(g.length) <= z.rows;
+    const uint32_t L = some ? prefix_len[g.prefix] : 0, u = uint32_t(g.used), m = fits ? uint32_t(g.length) : z.rows;
+    // the first row's window; the others' begin later
+    const uint32_t end = L + u + 1, open = window && end > window ? end - window : 0;
+    w.there = int(m);
+    w.prefix = some ? g.prefix : -1;
+    w.used = int(u);
+    w.prefix_len = int(L);
+    w.from = int(min(open, L));
+    w.lo = int(open - min(open, L));
+    const uint32_t span = u + m - uint32_t(w.lo);
+    w.span = int(span);
+    // (L and u below 2^31 each: their sum, and m, do not wrap)
+    w.bad = !fits | (g.prefix >= int(z.prefixes)) | (int(u | L) < 0) || L + u > 0x80000000u - m ||
+            (m && (span > uint32_t(z.cap) || L - uint32_t(w.from) > uint32_t(z.pcap)));
     return w;
 }
 
 // Chunks of 32 positions of a walk from `from`: chunks end at the ring's end.
 __host__ __device__ inline uint32_t chunks_of(uint32_t from, uint32_t span, uint32_t cap)
 {
-    const uint32_t n0 = min(span, cap - from % cap), n1 = span - n0;
+    const uint32_t n0 = min(span, cap - (from < cap ? from : from % cap)), n1 = span - n0;
     return (n0 + 31) / 32 + (n1 + 31) / 32;
 }
 
 // What `tiles` tiles over `chunks` chunks come to: waves' chunks (weight), and, a
-// wave having `each`, units and slots.  A last quad of three tiles is one of four.
+// wave having `each` (< 2^21), units and slots.  A last quad of three tiles is one
+// of four.
 struct Shares {
     uint32_t units, slots;
 };
@@ -162,266 +157,257 @@ __device__ inline uint32_t wide_of(uint32_t tiles, uint32_t quad)
 
 __device__ inline uint32_t runs_of(uint32_t wide, uint32_t chunks, uint32_t each)
 {
-    const uint64_t most = uint64_t(each) * (4 / wide);
-    return uint32_t((chunks + most - 1) / most);
+    const uint32_t most = each * (4 / wide);
+    return chunks <= most ? uint32_t(chunks > 0) : (chunks + most - 1) / most;
 }
 
-__device__ inline uint64_t weight_of(uint32_t tiles, uint32_t chunks)
+// (T: 32 bits are enough for a session, of 128 tiles or fewer and 2^19 chunks)
+template <typename T>
+__device__ inline T weight_of(uint32_t tiles, uint32_t chunks)
 {
-    const uint32_t full = tiles / 4, rest = tiles % 4;
-    return uint64_t(full) * chunks + (rest ? runs_of(wide_of(rest, 0), chunks, 1) : 0);
+    const uint32_t rest = tiles % 4, shift = rest == 1 ? 2 : rest == 2 ? 1 : 0;
+    return T(tiles / 4) * chunks + (rest ? (chunks + (1 << shift) - 1) >> shift : 0);
 }
 
 __device__ inline Shares shares_of(uint32_t tiles, uint32_t chunks, uint32_t each)
 {
-    const uint32_t full = tiles / 4, rest = tiles % 4;
-    const uint32_t a = runs_of(4, chunks, each), wide = rest ? wide_of(rest, 0) : 1;
-    const uint32_t b = rest ? runs_of(wide, chunks, each) : 0;
+    const uint32_t full = tiles / 4, rest = tiles % 4, wide = rest ? wide_of(rest, 0) : 1;
+    const uint32_t a = full ? runs_of(4, chunks, each) : 0, b = rest ? runs_of(wide, chunks, each) : 0;
     return Shares{full * a + b, 4 * full * a + wide * b};
 }
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kPlanSessions = 256;
-
-// The sum of v over the block, and over the threads before this one.
-template <typename T>
-__device__ inline T block_scan(T v, T &before, T *room)
+// The seat of column f of a source whose sums begin at `slot`.
+__device__ inline Seat seat_of(uint32_t tiles, uint32_t chunks, uint32_t each, uint32_t slot, uint32_t f)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    T up = v;
-    for (int d = 1; d < 64; d *= 2) {
-        const T o = __shfl_up(up, d);
-        if (lane >= d) up += o;
-    }
-    if (lane == 63) room[w] = up;
-    __syncthreads();
-    T all = 0, mine = 0;
-    for (int i = 0; i < kPlanWaves; ++i) {
-        mine += i < w ? room[i] : 0;
-        all += room[i];
-    }
-    __syncthreads();
-    before = mine + up - v;
-    return all;
+    const uint32_t q = f / (4 * kCols), a = runs_of(4, chunks, each), wide = wide_of(tiles, q);
+    const uint32_t more = 4 * q + 4 < tiles ? wide_of(tiles, q + 1) : 1;
+    const uint32_t runs = wide == 4 ? a : runs_of(wide, chunks, each), next = more == 4 ? a : runs_of(more, chunks, each);
+    return Seat{int(slot + 4 * q * a), int(runs | next << 16), int(wide | more << 4), int(f)};
 }
 
-// A block lays out kPlanSessions sessions, and every blocks-th prefix.  What it has
-// to know of the rest -- the groups, and what the sessions before its own come to --
-// it works out from the requests itself (65535 of them are 64 a thread), so that
+constexpr int kPlanSessions = 64;
+
+// The sums of a and b over the block, and over the threads before this one.
+template <int NT>
+__device__ inline void block_scan(uint64_t a, uint64_t b, uint64_t (&before)[2], uint64_t (&all)[2],
+                                  uint64_t (*room)[NT / 64])
+{
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint64_t ua = ndl::wave_scan(a), ub = ndl::wave_scan(b);
+    if (lane == 63) room[0][w] = ua, room[1][w] = ub;
+    __syncthreads();
+    before[0] = ua - a, before[1] = ub - b, all[0] = all[1] = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        const uint64_t x = room[0][i], y = room[1][i];
+        before[0] += i < w ? x : 0, before[1] += i < w ? y : 0;
+        all[0] += x, all[1] += y;
+    }
+}
+
+// A block lays out kPlanSessions sessions, and its share of the prefixes' units.  What
+// it has to know of the rest -- the groups, and what the sessions before its own come
+// to -- it works out from the requests itself (65535 of them are 64 a thread), so that
 // one launch does without a word between blocks.  Whole numbers: the same plan
 // whatever the order of the atomics.
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(Sizes z, Requests r, PlanOf plan, nd_prefix_maps maps)
+template <int NT>
+__global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf plan, nd_prefix_maps maps)
 {
-    __shared__ uint32_t rows_s[kMaxPrefixes], from_s[kMaxPrefixes], before_s[kMaxPrefixes];
-    __shared__ uint32_t first_s[kMaxPrefixes], units_s[kMaxPrefixes], slots_s[kMaxPrefixes];
-    __shared__ uint64_t room[kPlanWaves], weight_s;
-    __shared__ int which_s[kPlanSessions], mine_s[kPlanSessions], there_s[kPlanSessions], at_s[kPlanSessions];
-    __shared__ int used_s[kPlanSessions], len_s[kPlanSessions];
+    constexpr int kMost = NT < 1024 ? NT : int(kMaxPrefixes);
+    __shared__ uint32_t rows_s[kMost], from_s[kMost], before_s[kMost], end_s[kMost];
+    __shared__ uint32_t first_s[kMost], units_s[kMost], slots_s[kMost];
+    __shared__ uint64_t room[3][2][NT / 64], weight_s;
+    __shared__ __align__(16) uint32_t group_s[kPlanSessions];  // prefix and rows of a session
+    __shared__ int there_s[kPlanSessions], at_s[kPlanSessions], used_s[kPlanSessions], len_s[kPlanSessions];
+    __shared__ uint32_t chunks_s[kPlanSessions], slot_s[kPlanSessions];
     __shared__ uint32_t units_at, slots_at;
     const int t = threadIdx.x, lane = t & 63;
     const uint32_t R = uint32_t(z.H / z.KVH), P = z.prefixes, S = z.count;
-    const uint32_t s0 = blockIdx.x * kPlanSessions, s1 = min(S, s0 + kPlanSessions);
-    for (uint32_t p = t; p < P; p += kPlanThreads) rows_s[p] = before_s[p] = 0, from_s[p] = 0xffffffffu;
+    const uint32_t s0 = blockIdx.x * kPlanSessions, s1 = min(S, s0 + kPlanSessions), i0 = s0 + uint32_t(t);
+    // this block's sessions, and of all the first kHeld a thread
+    constexpr int kHeld = NT < 1024 ? 1 : 4;
+    Given held[kHeld], here{-1, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        held[k] = Given{-1, 0, 0};
+        if (uint32_t(t + k * NT) < S) held[k] = given_of(z, r, uint32_t(t + k * NT));
+    }
+    if (t < kPlanSessions && i0 < s1) here = given_of(z, r, i0);
+    for (uint32_t p = t; p < P; p += NT) {
+        rows_s[p] = before_s[p] = 0, from_s[p] = 0xffffffffu;
+        end_s[p] = uint32_t(r.prefix_len[p]);
+    }
     if (t == 0) weight_s = 0, units_at = slots_at = 0;
     __syncthreads();
+    const Want mine = want_of(z, uint32_t(r.window), here, end_s);
+    // f of every session before `end`
+    auto sessions = [&](uint32_t end, auto f) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (uint32_t(t + k * NT) < end) f(uint32_t(t + k * NT), want_of(z, uint32_t(r.window), held[k], end_s));
+        for (uint32_t i = uint32_t(t + kHeld * NT); i < end; i += NT) f(i, want_of(z, uint32_t(r.window), given_of(z, r, i), end_s));
+    };
+    auto tiles_of = [&](uint32_t rows) { return (rows * R + kCols - 1) / kCols; };
+    auto own_chunks = [&](const Want &w) { return chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)); };
+    auto group_chunks = [&](uint32_t p) { return chunks_of(from_s[p], end_s[p] - from_s[p], uint32_t(z.pcap)); };
+    auto add_weight = [&](uint64_t v) {
+        v = ndl::last_lane(ndl::wave_scan(v));
+        if (lane == 0 && v) atomicAdd(reinterpret_cast<unsigned long long *>(&weight_s), v);
+    };
 
-    // ---- the groups, and all own walks ----
+    // ---- the groups, and all walks ----
     uint64_t weight = 0;
-    for (uint32_t i = t; i < S; i += kPlanThreads) {
-        const Want w = want_of(z, r, i);
+    sessions(S, [&](uint32_t i, const Want &w) {
         const uint32_t m = uint32_t(w.rows());
-        if (!m) continue;
-        weight += weight_of((m * R + kCols - 1) / kCols, chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)));
-        if (w.prefix < 0) continue;
+        if (!m) return;
+        weight += weight_of<uint32_t>(tiles_of(m), own_chunks(w));
+        if (w.prefix < 0) return;
         atomicAdd(&rows_s[w.prefix], m);
         atomicMin(&from_s[w.prefix], uint32_t(w.from));
         if (i < s0) atomicAdd(&before_s[w.prefix], m);
-    }
-    for (int d = 32; d; d /= 2) weight += __shfl_xor(weight, d);
-    if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long *>(&weight_s), weight);
+    });
+    add_weight(weight);
     __syncthreads();
-    auto tiles_of = [&](uint32_t rows) { return (rows * R + kCols - 1) / kCols; };
-    auto group_chunks = [&](uint32_t p) -> uint32_t {  // of a group with rows
-        return chunks_of(from_s[p], uint32_t(r.prefix_len[p]) - from_s[p], uint32_t(z.pcap));
-    };
     weight = 0;
-    for (uint32_t p = t; p < P; p += kPlanThreads)
-        if (rows_s[p]) weight += weight_of(tiles_of(rows_s[p]), group_chunks(p));
-    for (int d = 32; d; d /= 2) weight += __shfl_xor(weight, d);
-    if (lane == 0 && weight) atomicAdd(reinterpret_cast<unsigned long long *>(&weight_s), weight);
+    for (uint32_t p = t; p < P; p += NT)
+        if (rows_s[p]) weight += weight_of<uint64_t>(tiles_of(rows_s[p]), group_chunks(p));
+    add_weight(weight);
     __syncthreads();
-    const uint64_t runs = max(1u, kBlocks / uint32_t(z.KVH));
-    const uint32_t each = uint32_t(min(max(uint64_t(kLeast), (weight_s + runs - 1) / runs), uint64_t(1) << 20));
+    // (a chunk more a wave than runs would need: no more than that many units)
+    const double share = double(weight_s) / double(max(1u, kBlocks / uint32_t(z.KVH)));
+    const uint32_t each = uint32_t(fmin(fmax(share + 1.0, double(kLeast)), 1048576.0));
 
-    // ---- where each group's rows, quads, units and slots begin ----
-    uint32_t rows_all = 0, quads_all = 0, units_all = 0, slots_all = 0;
-    for (uint32_t p0 = 0; p0 < P; p0 += kPlanThreads) {
+    // ---- where each group's rows, units and slots begin ----
+    uint32_t rows_all = 0, units_all = 0, slots_all = 0;
+    for (uint32_t p0 = 0; p0 < P; p0 += NT) {
         const uint32_t p = p0 + t, rows = p < P ? rows_s[p] : 0, tiles = tiles_of(rows);
         const uint32_t chunks = rows ? group_chunks(p) : 0;
         const Shares sh = shares_of(tiles, chunks, each);
-        // (rows and quads below 2^20 each, units and slots below 2^32)
-        uint64_t a, b;
-        const uint64_t all_a = block_scan(uint64_t(rows) << 32 | (tiles + 3) / 4, a, room);
-        const uint64_t all_b = block_scan(uint64_t(sh.units) << 32 | sh.slots, b, room);
+        // (units and slots below 2^32)
+        uint64_t at[2], all[2];
+        if (p0) __syncthreads();
+        block_scan<NT>(rows, uint64_t(sh.units) << 32 | sh.slots, at, all, room[0]);
         if (p < P) {
-            first_s[p] = rows_all + uint32_t(a >> 32);
-            units_s[p] = units_all + uint32_t(b >> 32);
-            slots_s[p] = slots_all + uint32_t(b);
-            if (blockIdx.x == 0) {
-                Group g{};
-                g.first = int(first_s[p]);
-                g.rows = int(rows);
-                g.begin = rows ? int(from_s[p]) : 0;
-                g.end = rows ? r.prefix_len[p] : 0;
-                g.span = g.end - g.begin;
-                g.quads = int(quads_all + uint32_t(a));
-                plan.group()[p] = g;
-                if (maps.first) maps.first[p] = g.first;
-            }
-            // each block its share of the groups
-            if (p % gridDim.x == blockIdx.x) {
-                uint32_t slot = slots_s[p];
-                for (uint32_t q = 0; 4 * q < tiles; ++q) {
-                    const uint32_t wide = wide_of(tiles, q), n = runs_of(wide, chunks, each);
-                    plan.quad()[quads_all + uint32_t(a) + q] = Quad{int(slot), int(n), int(wide), 0};
-                    slot += n * wide;
-                }
-            }
+            first_s[p] = rows_all + uint32_t(at[0]);
+            units_s[p] = units_all + uint32_t(at[1] >> 32);
+            slots_s[p] = slots_all + uint32_t(at[1]);
+            if (blockIdx.x == 0 && maps.first) maps.first[p] = int(first_s[p]);
         }
-        rows_all += uint32_t(all_a >> 32);
-        quads_all += uint32_t(all_a);
-        units_all += uint32_t(all_b >> 32);
-        slots_all += uint32_t(all_b);
+        rows_all += uint32_t(all[0]);
+        units_all += uint32_t(all[1] >> 32);
+        slots_all += uint32_t(all[1]);
     }
-    __syncthreads();
     if (blockIdx.x == 0 && t == 0 && maps.first) maps.first[P] = int(rows_all);
 
-    // ---- the groups' units ----
-    for (uint32_t p = blockIdx.x; p < P; p += gridDim.x) {
-        const uint32_t rows = rows_s[p];
-        if (!rows) continue;
-        const uint32_t tiles = tiles_of(rows), full = tiles / 4, chunks = group_chunks(p);
-        const uint32_t a = runs_of(4, chunks, each);
-        const Shares sh = shares_of(tiles, chunks, each);
-        for (uint32_t i = t; i < sh.units; i += kPlanThreads) {
-            const uint32_t q = i < full * a ? i / a : full, k = i - q * a;
-            const uint32_t wide = wide_of(tiles, q), n = each * (4 / wide);
-            Unit u{};
-            u.source = int(p);
-            u.quad = int(q);
-            u.wide = int(wide);
-            u.slot = int(slots_s[p] + 4 * q * a + k * wide);
-            u.begin = int(k * n);
-            u.end = int(min(chunks, (k + 1) * n));
-            u.rows = int(rows);
-            u.first = int(first_s[p]);
-            u.from = int(from_s[p]);
-            u.span = r.prefix_len[p] - int(from_s[p]);
-            plan.unit()[units_s[p] + i] = u;
-        }
+    // ---- what the sessions before this block's come to, and all ----
+    uint64_t sum = 0;
+    sessions(blockIdx.x ? s0 : S, [&](uint32_t, const Want &w) {
+        const uint32_t m = uint32_t(w.rows());
+        if (!m) return;
+        const Shares sh = shares_of(tiles_of(m), own_chunks(w), each);
+        sum += uint64_t(sh.units) << 32 | sh.slots;
+    });
+    sum = ndl::last_lane(ndl::wave_scan(sum));
+    if (lane == 0) {
+        atomicAdd(&units_at, uint32_t(sum >> 32));
+        atomicAdd(&slots_at, uint32_t(sum));
     }
 
-    // ---- what the sessions before this block's come to, and all ----
-    Shares before{0, 0}, all{0, 0};
-    for (uint32_t i = t; i < S; i += kPlanThreads) {
-        if (blockIdx.x && i >= s1) break;
-        const Want w = want_of(z, r, i);
-        const uint32_t m = uint32_t(w.rows());
-        if (!m) continue;
-        const Shares sh = shares_of(tiles_of(m), chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)), each);
-        all.units += sh.units, all.slots += sh.slots;
-        if (i < s0) before.units += sh.units, before.slots += sh.slots;
-    }
-    for (int d = 32; d; d /= 2) {
-        before.units += __shfl_xor(before.units, d), before.slots += __shfl_xor(before.slots, d);
-        all.units += __shfl_xor(all.units, d), all.slots += __shfl_xor(all.slots, d);
-    }
-    if (lane == 0) {
-        atomicAdd(&units_at, blockIdx.x ? before.units : all.units);
-        atomicAdd(&slots_at, blockIdx.x ? before.slots : all.slots);
-    }
-    __syncthreads();
+    // ---- this block's sessions ----
+    const uint32_t m = uint32_t(mine.rows()), tiles = tiles_of(m), chunks = m ? own_chunks(mine) : 0;
+    const Shares sh = shares_of(tiles, chunks, each);
+    if (t < kPlanSessions) group_s[t] = m && mine.prefix >= 0 ? uint32_t(mine.prefix) << 16 | m : 0xffff0000u;
+    uint64_t at[2], all[2];
+    block_scan<NT>(uint64_t(sh.units) << 32 | sh.slots, 0, at, all, room[1]);  // (a barrier: units_at, group_s)
     const uint32_t units0 = units_all + (blockIdx.x ? units_at : 0), slots0 = slots_all + (blockIdx.x ? slots_at : 0);
     if (blockIdx.x == 0 && t == 0)
         *plan.head() = Head{kPlanMagic, int(z.count), int(z.rows), int(P), z.H, z.KVH, z.cap, z.pcap,
                             int(units_all + units_at), int(slots_all + slots_at), r.window, {}};
-
-    // ---- this block's sessions ----
-    const uint32_t i = s0 + uint32_t(t);
-    const bool mine = t < kPlanSessions && i < s1;
-    Want w{};
-    if (mine) w = want_of(z, r, i);
-    const uint32_t m = mine ? uint32_t(w.rows()) : 0;
-    const uint32_t tiles = tiles_of(m), chunks = m ? chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)) : 0;
-    const Shares sh = shares_of(tiles, chunks, each);
-    if (t < kPlanSessions) which_s[t] = m ? w.prefix : -1, mine_s[t] = int(m);
-    uint64_t at64;
-    block_scan(uint64_t(sh.units) << 32 | sh.slots, at64, room);
-    if (mine) {
-        uint32_t at = w.prefix >= 0 ? before_s[w.prefix] : 0;
-        for (int j = 0; j < t; ++j) at += which_s[j] == w.prefix ? uint32_t(mine_s[j]) : 0u;
-        Session s{};
-        s.there = w.there;
-        s.bad = w.bad;
-        s.prefix = w.bad ? -1 : w.prefix;
-        s.at = int(at);
-        s.used = w.used;
-        s.lo = w.lo;
-        s.span = w.span;
-        s.quads = int(plan.l.quads_prefix + i * plan.l.quads_own);
-        plan.session()[i] = s;
-        uint32_t unit = units0 + uint32_t(at64 >> 32), slot = slots0 + uint32_t(at64);
+    // a session's place among those of its prefix: four threads each
+    if (t < 4 * kPlanSessions) {
+        constexpr int kShare = 4;
+        const int j = t / kShare, part = t % kShare, last = min(j | (64 / kShare - 1), int(s1 - s0) - 1);
+        const uint32_t key = group_s[j] >> 16;
+        uint32_t rank = 0;
+        // (to the wave's last session, alike in all lanes: `last` is)
+        for (int i = 4 * part; i <= last; i += 4 * kShare) {
+            const uint4 g = *reinterpret_cast<const uint4 *>(&group_s[i]);
+            const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rank += i + e < j && gg[e] >> 16 == key ? gg[e] & 0xffffu : 0u;
+        }
+        rank += uint32_t(ndl::wave_xor_int<1>(int(rank)));
+        rank += uint32_t(ndl::wave_xor_int<2>(int(rank)));
+        if (part == 0) at_s[j] = int(rank);
+    }
+    __syncthreads();
+    if (t < kPlanSessions && i0 < s1) {
+        const uint32_t rank = (mine.prefix >= 0 ? before_s[mine.prefix] : 0) + uint32_t(at_s[t]);
+        uint32_t unit = units0 + uint32_t(at[0] >> 32), slot = slots0 + uint32_t(at[0]);
+        chunks_s[t] = chunks;
+        slot_s[t] = slot;
         for (uint32_t q = 0; 4 * q < tiles; ++q) {
-            const uint32_t wide = wide_of(tiles, q), n = each * (4 / wide), k1 = runs_of(wide, chunks, each);
-            plan.quad()[uint32_t(s.quads) + q] = Quad{int(slot), int(k1), int(wide), 0};
-            for (uint32_t k = 0; k < k1; ++k) {
-                Unit u{};
-                u.source = ~int(i);
-                u.quad = int(q);
-                u.wide = int(wide);
-                u.slot = int(slot);
-                u.begin = int(k * n);
-                u.end = int(min(chunks, (k + 1) * n));
-                u.rows = int(m);
-                u.from = w.lo;
-                u.span = w.span;
-                u.used = w.used;
-                plan.unit()[unit++] = u;
+            const uint32_t wide = wide_of(tiles, q), n = each * (4 / wide), runs = runs_of(wide, chunks, each);
+            for (uint32_t k = 0; k < runs; ++k) {
+                plan.unit()[unit++] = Unit{~int(i0), int(q), int(wide), int(slot), int(k * n), int(min(chunks, (k + 1) * n)),
+                                           int(m), 0, mine.lo, mine.span, mine.used, {}};
                 slot += wide;
             }
         }
-        there_s[t] = w.bad ? 0 : w.there;
-        at_s[t] = int(at);
-        used_s[t] = w.used;
-        len_s[t] = w.prefix_len;
+        there_s[t] = mine.bad ? ~mine.there : mine.there;
+        at_s[t] = int(rank);
+        used_s[t] = mine.used;
+        len_s[t] = mine.prefix_len;
     }
     __syncthreads();
 
     // ---- their rows, and what lies behind the last of the order ----
     const uint32_t N = z.rows, total = (s1 > s0 ? s1 - s0 : 0) * N;
-    for (uint32_t k = t; k < total; k += kPlanThreads) {
-        const uint32_t j = k / N, n = k - j * N;
+    for (uint32_t k = t; k < total; k += NT) {
+        const uint32_t j = k / N, n = k - j * N, p = group_s[j] >> 16;
         const int row = int(s0 * N + k);
         int pos = -1, rot = -1, from = -1, lo = -1;
-        if (int(n) < there_s[j]) {
-            const int64_t at = int64_t(len_s[j]) + used_s[j] + n, open = r.window ? max(at + 1 - r.window, int64_t(0)) : 0;
+        Seats seats{};
+        const bool bad = there_s[j] < 0;
+        seats.own.column = bad && int(n) < ~there_s[j] ? 1 : -1;
+        if (!bad && int(n) < there_s[j]) {
+            // (the row's place in the whole is below 2^31)
+            const int end = len_s[j] + used_s[j] + int(n), open = r.window ? max(end - r.window + 1, 0) : 0;
             pos = used_s[j] + int(n);
-            rot = int(at);
-            from = int(min(open, int64_t(len_s[j])));
-            lo = int(max(open - len_s[j], int64_t(0)));
-            if (which_s[j] >= 0) {
-                const uint32_t to = first_s[which_s[j]] + uint32_t(at_s[j]) + n;
+            rot = end;
+            from = min(open, len_s[j]);
+            lo = max(open - len_s[j], 0);
+            if (p < P) {
+                const uint32_t to = first_s[p] + uint32_t(at_s[j]) + n;
                 plan.place()[to] = Place{row, from};
                 if (maps.order) maps.order[to] = row;
+                seats.prefix = seat_of(tiles_of(rows_s[p]), group_chunks(p), each, slots_s[p], (uint32_t(at_s[j]) + n) * R);
             }
+            seats.own = seat_of(tiles_of(uint32_t(there_s[j])), chunks_s[j], each, slot_s[j], n * R);
+            seats.own.column = 0;
         }
+        plan.seat()[row] = seats;
         if (maps.pos) maps.pos[row] = pos;
         if (maps.rot) maps.rot[row] = rot;
         if (maps.from) maps.from[row] = from;
         if (maps.lo) maps.lo[row] = lo;
     }
+    const uint32_t thread = blockIdx.x * NT + t, threads = gridDim.x * NT;
     if (maps.order)
-        for (uint32_t k = rows_all + blockIdx.x * kPlanThreads + t; k < S * N; k += gridDim.x * kPlanThreads)
-            maps.order[k] = -1;
+        for (uint32_t k = rows_all + thread; k < S * N; k += threads) maps.order[k] = -1;
+
+    // ---- the groups' units, over all blocks ----
+    for (uint32_t k = thread; k < units_all; k += threads) {
+        uint32_t p = 0;  // the last group that begins at or before k
+        for (uint32_t d = kMost / 2; d; d /= 2)
+            if (p + d < P && units_s[p + d] <= k) p += d;
+        const uint32_t i = k - units_s[p], rows = rows_s[p], tiles = tiles_of(rows);
+        const uint32_t chunks = group_chunks(p), full = tiles / 4, a = runs_of(4, chunks, each);
+        const uint32_t q = i < full * a ? i / a : full, run = i - q * a, wide = wide_of(tiles, q), n = each * (4 / wide);
+        plan.unit()[k] = Unit{int(p), int(q), int(wide), int(slots_s[p] + 4 * q * a + run * wide), int(run * n),
+                              int(min(chunks, (run + 1) * n)), int(rows), int(first_s[p]), int(from_s[p]),
+                              int(end_s[p] - from_s[p]), 0, {}};
+    }
 }
 
 // ---- attention ----------------------------------------------------------------
@@ -455,9 +441,10 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
+    // (both asked for at once: the list has as many places as the grid blocks)
     const Head hd = *at.plan.head();
-    if (!made_for(hd, at.z) || int(blockIdx.x) >= hd.units) return;
     const Unit un = at.plan.unit()[blockIdx.x];
+    if (!made_for(hd, at.z) || int(blockIdx.x) >= hd.units) return;
     const uint32_t kvh = blockIdx.y, R = uint32_t(gown.H / gown.KVH);
     const bool own = un.source < 0;
     const int wide = un.wide, mine = w & (wide - 1), stream = w / wide, step = NW / wide;
@@ -892,58 +879,70 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
 // column.
 __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t first, uint32_t total)
 {
-    const uint32_t oh = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t oh = blockIdx.x * 4 + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
     if (oh >= total) return;
     const int lane = threadIdx.x & 63;
     const uint32_t H = uint32_t(at.z.H), R = H / uint32_t(at.z.KVH), down = oh / H;
-    const uint32_t row = first + down, head = oh - down * H, kvh = head / R, r = head - kvh * R;
-    const uint32_t i = row / at.z.rows, n = row - i * at.z.rows;
-    float *out = at.out + (size_t(row) * H + head) * VD + lane;
-    if (!made_for(*at.plan.head(), at.z)) {
-        *out = NAN;
+    const uint32_t row = first + down, head = oh - down * H, kvh = at.by_rep.quotient(head), r = head - kvh * R;
+    float *out = at.out + (size_t(row) * H + head) * VD;
+    const Head hd = *at.plan.head();
+    const Seats seats = at.plan.seat()[row];
+    if (!made_for(hd, at.z) || seats.own.column > 0) {
+        out[lane] = NAN;
         return;
     }
-    const Session s = at.plan.session()[i];
-    if (int(n) >= s.there) return;
-    if (s.bad) {
-        *out = NAN;
-        return;
-    }
-    const uint32_t fp = (uint32_t(s.at) + n) * R + r, fo = n * R + r;
-    Quad qp{}, qo = at.plan.quad()[uint32_t(s.quads) + fo / (4 * kCols)];
-    if (s.prefix >= 0) qp = at.plan.quad()[uint32_t(at.plan.group()[s.prefix].quads) + fp / (4 * kCols)];
-    const int all = qp.runs + qo.runs;
+    if (seats.own.column < 0) return;
+    // the first run's sums, their number and how far apart they are (slots)
+    auto find = [&](const Seat &s, uint32_t f, uint32_t &to, int &runs, uint32_t &apart) {
+        const bool next = f / (4 * kCols) != uint32_t(s.column) / (4 * kCols);
+        const uint32_t n0 = uint32_t(s.runs) & 0xffff, w0 = uint32_t(s.wides) & 15;
+        runs = int(next ? uint32_t(s.runs) >> 16 : n0);
+        apart = (next ? uint32_t(s.wides) >> 4 : w0) * uint32_t(at.z.KVH) * kCols;
+        to = ((uint32_t(s.slot) + (next ? n0 * w0 : 0) + f / kCols % 4) * uint32_t(at.z.KVH) + kvh) * kCols + f % kCols;
+    };
+    const uint32_t n = row % at.z.rows;
+    Seat own = seats.own;
+    own.column = int(n * R);
+    uint32_t to[2], apart[2];
+    int runs[2];
+    find(seats.prefix, uint32_t(seats.prefix.column) + r, to[0], runs[0], apart[0]);
+    find(own, n * R + r, to[1], runs[1], apart[1]);
+    const int all = runs[0] + runs[1];
     float M = -INFINITY, L = 0.0f, O = 0.0f;
     for (int j0 = 0; j0 < all; j0 += 64) {
-        const int j = j0 + lane, many = min(64, all - j0);
-        const bool old = j < qp.runs;
-        const uint32_t f = old ? fp : fo;
-        size_t to = 0;
+        const int j = j0 + lane, many = min(64, all - j0), olds = min(max(runs[0] - j0, 0), many);
         float m = -INFINITY, l = 0.0f;
         if (j < all) {
-            const uint32_t slot = (old ? uint32_t(qp.slot + j * qp.wide) : uint32_t(qo.slot + (j - qp.runs) * qo.wide)) +
-                                  f / kCols % 4;
-            to = (size_t(slot) * at.z.KVH + kvh) * kCols + f % kCols;
-            m = at.part_ml[2 * to];
-            l = at.part_ml[2 * to + 1];
+            const size_t p = j < runs[0] ? to[0] + size_t(j) * apart[0] : to[1] + size_t(j - runs[0]) * apart[1];
+            const floatx2_t ml = *reinterpret_cast<const floatx2_t *>(at.part_ml + 2 * p);
+            m = ml[0];
+            l = ml[1];
         }
         // (a NaN among the weights is one of L; M is a number or -inf)
         const float top = fmaxf(M, wave_max(m)), by = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         const float was = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - top);
         M = top;
         // as means of what is there, so that no sum leaves the values' range
-        const float part = l * by, now = L * was, sum = now + wave_sum(part);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float now = L * was, sum = now + wave_sum(l * by);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, share = by * inv;
         O *= now * inv;
-        for (int e = 0; e < many; ++e) {
-            const uint32_t a0 = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(to)), e));
-            const uint32_t a1 = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(to >> 32)), e));
-            const float b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(by * inv), e));
-            O += at.part_o[(size_t(a1) << 32 | a0) * VD + lane] * b;
-        }
+        // lane by lane of this round: the prefix's runs, then the own ones
+        auto add = [&](const float *po, size_t step, int e0, int e1) {
+            int e = e0;
+            for (; e + 4 <= e1; e += 4, po += 4 * step) {
+                const float o[4] = {po[lane], po[step + lane], po[2 * step + lane], po[3 * step + lane]};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    O += o[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), e + k));
+            }
+            for (; e < e1; ++e, po += step)
+                O += po[lane] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), e));
+        };
+        add(at.part_o + (to[0] + size_t(j0) * apart[0]) * VD, size_t(apart[0]) * VD, 0, olds);
+        add(at.part_o + (to[1] + size_t(max(j0 - runs[0], 0)) * apart[1]) * VD, size_t(apart[1]) * VD, olds, many);
         L = sum;
     }
-    *out = L != L ? NAN : O;
+    out[lane] = L != L ? NAN : O;
 }
 
 // ---- the host's side ------------------------------------------------------------
@@ -1000,7 +999,8 @@ int nd_prefix_plan(nd_ctx *ctx, const nd_kv_geom *g, size_t prefix_cap, size_t c
     const Layout l = layout_of(z);
     ND_REQUIRE(plan_bytes >= l.bytes, "plan holds %zu bytes, %zu needed", plan_bytes, l.bytes);
     const unsigned blocks = unsigned(std::max<size_t>(1, (count + kPlanSessions - 1) / kPlanSessions));
-    hipLaunchKernelGGL(plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, ctx->stream, z,
+    const bool small = count <= 256 && prefixes < 256;
+    hipLaunchKernelGGL(small ? plan_kernel<256> : plan_kernel<1024>, dim3(blocks), dim3(small ? 256 : 1024), 0, ctx->stream, z,
                        Requests{prefix_of, prefix_len, used, length, window},
                        PlanOf{static_cast<uint8_t *>(plan), l}, maps ? *maps : nd_prefix_maps{});
     return nd::check_launch("prefix_plan");
