@@ -18,45 +18,46 @@ constexpr size_t kMaxSessions = 65535, kMaxRows = 256, kMaxAll = size_t(1) << 20
 
 // ---- the plan ---------------------------------------------------------------
 //
-// Attention is done in units: a quad of column tiles (16 (row, head) pairs of a kv
-// head each) of one source -- a prefix, for all rows of its group, or a session's
-// own block -- and a run of chunks of 32 positions.  A unit's four waves take its
-// tiles (`wide` of them: 4, 2 or 1) and, where there are fewer than four, the
-// chunks in turn.  The units are as long as leaves about kBlocks blocks, whatever
-// the requests' lengths are, and each leaves its sums in slots, one a tile.
+// Attention is done in units, a wave each: a column tile (16 (row, head) pairs of a kv
+// head) of one source -- a prefix, for all rows of its group, or a session's own block
+// -- and a run of its chunks of 32 positions, as long as leaves about kWaves waves
+// whatever the requests' lengths are.  A unit leaves its sums in a slot of its own
+// number.  A prefix's units are numbered so that a block's four take four tiles over
+// the same chunks: unit base + 4 q runs + k w + j is run k of tile 4 q + j, w the
+// tiles of quad q.
 constexpr int kPlanMagic = 0x6e645031;
-constexpr uint32_t kBlocks = 1024;     // four a CU
-constexpr uint32_t kLeast = 4;         // chunks a wave, at least
+constexpr uint32_t kWaves = 4096;  // four a SIMD
+constexpr uint32_t kLeast = 4;     // chunks a wave, at least
 
 struct Head {
     int magic, count, rows, prefixes, heads, kv_heads, cap, prefix_cap;
-    int units, slots, window, pad[5];
+    int units, window, pad[6];
 };
 
 struct Place {
     int row, from;
 };
 
-// Where the sums of a row's heads are, in its prefix's slots or its session's: the
-// slot of the quad of its first head's column, the quad's runs (and the next one's,
-// where the other heads' columns may lie, 16 bits on) and wides (4 bits on).
+// Where the sums of a row's heads are: their source's first unit, its runs and its
+// tiles, and the column of the row's first head.
 struct Seat {
-    int slot, runs, wides, column;
+    int unit, runs, tiles, column;
 };
 
 struct Seats {
-    Seat prefix, own;  // (own.column: below 0 no row, 1 a bad one)
+    Seat prefix, own;
+    int is, pad[7];  // 0: there, 1: bad, -1: not there
 };
 
 struct Unit {
-    int source, quad, wide, slot;      // prefix, or ~session; of the source; first slot
-    int begin, end, rows, first;       // chunks; rows of the source and the first's place
-    int from, span, used, pad[5];      // positions; own: positions before the step
+    int source, tile, rows, first;  // prefix, or ~session; its rows, the first one's place
+    int begin, end, from, span;     // chunks of the positions from .. from + span - 1
+    int used, pad[7];               // own: positions before the step
 };
 
 struct Layout {
     size_t seat, place, unit, bytes;  // offsets
-    uint32_t units, slots;            // at most
+    uint32_t units;                   // at most
 };
 
 struct Sizes {
@@ -71,12 +72,9 @@ Layout layout_of(const Sizes &z)
     const uint64_t R = uint64_t(z.H / z.KVH), own = ceil_div(z.rows * R, kCols);
     const uint64_t all = ceil_div(uint64_t(z.count) * z.rows * R, kCols);
     Layout l{};
-    // units: a quad's last run may be short, the full ones come to kBlocks / KVH
-    const uint32_t runs = std::max<uint32_t>(1, kBlocks / uint32_t(z.KVH));
-    const uint64_t quads = (z.prefixes ? (all + 3) / 4 + z.prefixes : 0) + uint64_t(z.count) * ((own + 3) / 4);
-    l.units = uint32_t(quads + runs);
-    // slots: a quad of three tiles has four
-    l.slots = uint32_t((z.prefixes ? all + 2 * z.prefixes : 0) + z.count * (own + (own % 4 == 3)) + 4 * runs);
+    // a tile's last run may be short, the full ones come to kWaves / KVH
+    l.units = uint32_t((z.prefixes ? all + 4 * z.prefixes : 0) + z.count * own + std::max<uint32_t>(1, kWaves / uint32_t(z.KVH)));
+    l.units = (l.units + 3) & ~3u;
     const size_t rows = size_t(z.count) * z.rows;
     l.seat = sizeof(Head);
     l.place = l.seat + rows * sizeof(Seats);
@@ -142,66 +140,28 @@ __host__ __device__ inline uint32_t chunks_of(uint32_t from, uint32_t span, uint
     return (n0 + 31) / 32 + (n1 + 31) / 32;
 }
 
-// What `tiles` tiles over `chunks` chunks come to: waves' chunks (weight), and, a
-// wave having `each` (< 2^21), units and slots.  A last quad of three tiles is one
-// of four.
-struct Shares {
-    uint32_t units, slots;
-};
-
-__device__ inline uint32_t wide_of(uint32_t tiles, uint32_t quad)
+// Runs of `each` (< 2^21) chunks.
+__device__ inline uint32_t runs_of(uint32_t chunks, uint32_t each)
 {
-    const uint32_t left = tiles - 4 * quad;
-    return left >= 3 ? 4 : left;
-}
-
-__device__ inline uint32_t runs_of(uint32_t wide, uint32_t chunks, uint32_t each)
-{
-    const uint32_t most = each * (4 / wide);
-    return chunks <= most ? uint32_t(chunks > 0) : (chunks + most - 1) / most;
-}
-
-// (T: 32 bits are enough for a session, of 128 tiles or fewer and 2^19 chunks)
-template <typename T>
-__device__ inline T weight_of(uint32_t tiles, uint32_t chunks)
-{
-    const uint32_t rest = tiles % 4, shift = rest == 1 ? 2 : rest == 2 ? 1 : 0;
-    return T(tiles / 4) * chunks + (rest ? (chunks + (1 << shift) - 1) >> shift : 0);
-}
-
-__device__ inline Shares shares_of(uint32_t tiles, uint32_t chunks, uint32_t each)
-{
-    const uint32_t full = tiles / 4, rest = tiles % 4, wide = rest ? wide_of(rest, 0) : 1;
-    const uint32_t a = full ? runs_of(4, chunks, each) : 0, b = rest ? runs_of(wide, chunks, each) : 0;
-    return Shares{full * a + b, 4 * full * a + wide * b};
-}
-
-// The seat of column f of a source whose sums begin at `slot`.
-__device__ inline Seat seat_of(uint32_t tiles, uint32_t chunks, uint32_t each, uint32_t slot, uint32_t f)
-{
-    const uint32_t q = f / (4 * kCols), a = runs_of(4, chunks, each), wide = wide_of(tiles, q);
-    const uint32_t more = 4 * q + 4 < tiles ? wide_of(tiles, q + 1) : 1;
-    const uint32_t runs = wide == 4 ? a : runs_of(wide, chunks, each), next = more == 4 ? a : runs_of(more, chunks, each);
-    return Seat{int(slot + 4 * q * a), int(runs | next << 16), int(wide | more << 4), int(f)};
+    return chunks <= each ? uint32_t(chunks > 0) : (chunks + each - 1) / each;
 }
 
 constexpr int kPlanSessions = 64;
 
-// The sums of a and b over the block, and over the threads before this one.
+// The sum of v over the block, and over the threads before this one.
 template <int NT>
-__device__ inline void block_scan(uint64_t a, uint64_t b, uint64_t (&before)[2], uint64_t (&all)[2],
-                                  uint64_t (*room)[NT / 64])
+__device__ inline void block_scan(uint64_t v, uint64_t &before, uint64_t &all, uint64_t *room)
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t ua = ndl::wave_scan(a), ub = ndl::wave_scan(b);
-    if (lane == 63) room[0][w] = ua, room[1][w] = ub;
+    const uint64_t up = ndl::wave_scan(v);
+    if (lane == 63) room[w] = up;
     __syncthreads();
-    before[0] = ua - a, before[1] = ub - b, all[0] = all[1] = 0;
+    before = up - v, all = 0;
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) {
-        const uint64_t x = room[0][i], y = room[1][i];
-        before[0] += i < w ? x : 0, before[1] += i < w ? y : 0;
-        all[0] += x, all[1] += y;
+        const uint64_t x = room[i];
+        before += i < w ? x : 0;
+        all += x;
     }
 }
 
@@ -215,12 +175,11 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
 {
     constexpr int kMost = NT < 1024 ? NT : int(kMaxPrefixes);
     __shared__ uint32_t rows_s[kMost], from_s[kMost], before_s[kMost], end_s[kMost];
-    __shared__ uint32_t first_s[kMost], units_s[kMost], slots_s[kMost];
-    __shared__ uint64_t room[3][2][NT / 64], weight_s;
+    __shared__ uint32_t first_s[kMost], units_s[kMost];
+    __shared__ uint64_t room[2][NT / 64], weight_s;
     __shared__ __align__(16) uint32_t group_s[kPlanSessions];  // prefix and rows of a session
     __shared__ int there_s[kPlanSessions], at_s[kPlanSessions], used_s[kPlanSessions], len_s[kPlanSessions];
-    __shared__ uint32_t chunks_s[kPlanSessions], slot_s[kPlanSessions];
-    __shared__ uint32_t units_at, slots_at;
+    __shared__ uint32_t runs_s[kPlanSessions], unit_s[kPlanSessions], units_at;
     const int t = threadIdx.x, lane = t & 63;
     const uint32_t R = uint32_t(z.H / z.KVH), P = z.prefixes, S = z.count;
     const uint32_t s0 = blockIdx.x * kPlanSessions, s1 = min(S, s0 + kPlanSessions), i0 = s0 + uint32_t(t);
@@ -237,7 +196,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
         rows_s[p] = before_s[p] = 0, from_s[p] = 0xffffffffu;
         end_s[p] = uint32_t(r.prefix_len[p]);
     }
-    if (t == 0) weight_s = 0, units_at = slots_at = 0;
+    if (t == 0) weight_s = 0, units_at = 0;
     __syncthreads();
     const Want mine = want_of(z, uint32_t(r.window), here, end_s);
     // f of every session before `end`
@@ -260,7 +219,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     sessions(S, [&](uint32_t i, const Want &w) {
         const uint32_t m = uint32_t(w.rows());
         if (!m) return;
-        weight += weight_of<uint32_t>(tiles_of(m), own_chunks(w));
+        weight += uint64_t(tiles_of(m)) * own_chunks(w);
         if (w.prefix < 0) return;
         atomicAdd(&rows_s[w.prefix], m);
         atomicMin(&from_s[w.prefix], uint32_t(w.from));
@@ -270,59 +229,50 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     __syncthreads();
     weight = 0;
     for (uint32_t p = t; p < P; p += NT)
-        if (rows_s[p]) weight += weight_of<uint64_t>(tiles_of(rows_s[p]), group_chunks(p));
+        if (rows_s[p]) weight += uint64_t(tiles_of(rows_s[p])) * group_chunks(p);
     add_weight(weight);
     __syncthreads();
-    // (a chunk more a wave than runs would need: no more than that many units)
-    const double share = double(weight_s) / double(max(1u, kBlocks / uint32_t(z.KVH)));
+    // (a chunk more than the share: no more units than that many and the tiles)
+    const double share = double(weight_s) / double(max(1u, kWaves / uint32_t(z.KVH)));
     const uint32_t each = uint32_t(fmin(fmax(share + 1.0, double(kLeast)), 1048576.0));
 
-    // ---- where each group's rows, units and slots begin ----
-    uint32_t rows_all = 0, units_all = 0, slots_all = 0;
+    // ---- where each group's rows and units begin ----
+    uint32_t rows_all = 0, units_all = 0;
     for (uint32_t p0 = 0; p0 < P; p0 += NT) {
-        const uint32_t p = p0 + t, rows = p < P ? rows_s[p] : 0, tiles = tiles_of(rows);
-        const uint32_t chunks = rows ? group_chunks(p) : 0;
-        const Shares sh = shares_of(tiles, chunks, each);
-        // (units and slots below 2^32)
-        uint64_t at[2], all[2];
+        const uint32_t p = p0 + t, rows = p < P ? rows_s[p] : 0;
+        const uint32_t units = rows ? (tiles_of(rows) * runs_of(group_chunks(p), each) + 3) & ~3u : 0;
+        uint64_t at, all;
         if (p0) __syncthreads();
-        block_scan<NT>(rows, uint64_t(sh.units) << 32 | sh.slots, at, all, room[0]);
+        block_scan<NT>(uint64_t(rows) << 32 | units, at, all, room[0]);
         if (p < P) {
-            first_s[p] = rows_all + uint32_t(at[0]);
-            units_s[p] = units_all + uint32_t(at[1] >> 32);
-            slots_s[p] = slots_all + uint32_t(at[1]);
+            first_s[p] = rows_all + uint32_t(at >> 32);
+            units_s[p] = units_all + uint32_t(at);
             if (blockIdx.x == 0 && maps.first) maps.first[p] = int(first_s[p]);
         }
-        rows_all += uint32_t(all[0]);
-        units_all += uint32_t(all[1] >> 32);
-        slots_all += uint32_t(all[1]);
+        rows_all += uint32_t(all >> 32);
+        units_all += uint32_t(all);
     }
     if (blockIdx.x == 0 && t == 0 && maps.first) maps.first[P] = int(rows_all);
 
     // ---- what the sessions before this block's come to, and all ----
-    uint64_t sum = 0;
+    uint32_t sum = 0;
     sessions(blockIdx.x ? s0 : S, [&](uint32_t, const Want &w) {
         const uint32_t m = uint32_t(w.rows());
-        if (!m) return;
-        const Shares sh = shares_of(tiles_of(m), own_chunks(w), each);
-        sum += uint64_t(sh.units) << 32 | sh.slots;
+        if (m) sum += tiles_of(m) * runs_of(own_chunks(w), each);
     });
     sum = ndl::last_lane(ndl::wave_scan(sum));
-    if (lane == 0) {
-        atomicAdd(&units_at, uint32_t(sum >> 32));
-        atomicAdd(&slots_at, uint32_t(sum));
-    }
+    if (lane == 0) atomicAdd(&units_at, sum);
 
     // ---- this block's sessions ----
     const uint32_t m = uint32_t(mine.rows()), tiles = tiles_of(m), chunks = m ? own_chunks(mine) : 0;
-    const Shares sh = shares_of(tiles, chunks, each);
+    const uint32_t runs = runs_of(chunks, each);
     if (t < kPlanSessions) group_s[t] = m && mine.prefix >= 0 ? uint32_t(mine.prefix) << 16 | m : 0xffff0000u;
-    uint64_t at[2], all[2];
-    block_scan<NT>(uint64_t(sh.units) << 32 | sh.slots, 0, at, all, room[1]);  // (a barrier: units_at, group_s)
-    const uint32_t units0 = units_all + (blockIdx.x ? units_at : 0), slots0 = slots_all + (blockIdx.x ? slots_at : 0);
+    uint64_t at, all;
+    block_scan<NT>(tiles * runs, at, all, room[1]);  // (a barrier: units_at, group_s)
+    const uint32_t units0 = units_all + (blockIdx.x ? units_at : 0);
     if (blockIdx.x == 0 && t == 0)
         *plan.head() = Head{kPlanMagic, int(z.count), int(z.rows), int(P), z.H, z.KVH, z.cap, z.pcap,
-                            int(units_all + units_at), int(slots_all + slots_at), r.window, {}};
+                            int(units_all + units_at), r.window, {}};
     // a session's place among those of its prefix: four threads each
     if (t < 4 * kPlanSessions) {
         constexpr int kShare = 4;
@@ -343,17 +293,14 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     __syncthreads();
     if (t < kPlanSessions && i0 < s1) {
         const uint32_t rank = (mine.prefix >= 0 ? before_s[mine.prefix] : 0) + uint32_t(at_s[t]);
-        uint32_t unit = units0 + uint32_t(at[0] >> 32), slot = slots0 + uint32_t(at[0]);
-        chunks_s[t] = chunks;
-        slot_s[t] = slot;
-        for (uint32_t q = 0; 4 * q < tiles; ++q) {
-            const uint32_t wide = wide_of(tiles, q), n = each * (4 / wide), runs = runs_of(wide, chunks, each);
-            for (uint32_t k = 0; k < runs; ++k) {
-                plan.unit()[unit++] = Unit{~int(i0), int(q), int(wide), int(slot), int(k * n), int(min(chunks, (k + 1) * n)),
-                                           int(m), 0, mine.lo, mine.span, mine.used, {}};
-                slot += wide;
-            }
-        }
+        uint32_t unit = units0 + uint32_t(at);
+        runs_s[t] = runs;
+        unit_s[t] = unit;
+        for (uint32_t q = 0; 4 * q < tiles; ++q)
+            for (uint32_t k = 0; k < runs; ++k)
+                for (uint32_t j = 4 * q; j < min(tiles, 4 * q + 4); ++j)
+                    plan.unit()[unit++] = Unit{~int(i0), int(j), int(m), 0, int(k * each), int(min(chunks, (k + 1) * each)),
+                                               mine.lo, mine.span, mine.used, {}};
         there_s[t] = mine.bad ? ~mine.there : mine.there;
         at_s[t] = int(rank);
         used_s[t] = mine.used;
@@ -369,7 +316,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
         int pos = -1, rot = -1, from = -1, lo = -1;
         Seats seats{};
         const bool bad = there_s[j] < 0;
-        seats.own.column = bad && int(n) < ~there_s[j] ? 1 : -1;
+        seats.is = bad && int(n) < ~there_s[j] ? 1 : -1;
         if (!bad && int(n) < there_s[j]) {
             // (the row's place in the whole is below 2^31)
             const int end = len_s[j] + used_s[j] + int(n), open = r.window ? max(end - r.window + 1, 0) : 0;
@@ -381,10 +328,11 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
                 const uint32_t to = first_s[p] + uint32_t(at_s[j]) + n;
                 plan.place()[to] = Place{row, from};
                 if (maps.order) maps.order[to] = row;
-                seats.prefix = seat_of(tiles_of(rows_s[p]), group_chunks(p), each, slots_s[p], (uint32_t(at_s[j]) + n) * R);
+                seats.prefix = Seat{int(units_s[p]), int(runs_of(group_chunks(p), each)), int(tiles_of(rows_s[p])),
+                                    int((uint32_t(at_s[j]) + n) * R)};
             }
-            seats.own = seat_of(tiles_of(uint32_t(there_s[j])), chunks_s[j], each, slot_s[j], n * R);
-            seats.own.column = 0;
+            seats.own = Seat{int(unit_s[j]), int(runs_s[j]), int(tiles_of(uint32_t(there_s[j]))), int(n * R)};
+            seats.is = 0;
         }
         plan.seat()[row] = seats;
         if (maps.pos) maps.pos[row] = pos;
@@ -401,12 +349,19 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
         uint32_t p = 0;  // the last group that begins at or before k
         for (uint32_t d = kMost / 2; d; d /= 2)
             if (p + d < P && units_s[p + d] <= k) p += d;
-        const uint32_t i = k - units_s[p], rows = rows_s[p], tiles = tiles_of(rows);
-        const uint32_t chunks = group_chunks(p), full = tiles / 4, a = runs_of(4, chunks, each);
-        const uint32_t q = i < full * a ? i / a : full, run = i - q * a, wide = wide_of(tiles, q), n = each * (4 / wide);
-        plan.unit()[k] = Unit{int(p), int(q), int(wide), int(slots_s[p] + 4 * q * a + run * wide), int(run * n),
-                              int(min(chunks, (run + 1) * n)), int(rows), int(first_s[p]), int(from_s[p]),
-                              int(end_s[p] - from_s[p]), 0, {}};
+        const uint32_t i = k - units_s[p], rows = rows_s[p], tiles = tiles_of(rows), chunks = group_chunks(p);
+        const uint32_t runs = runs_of(chunks, each), full = tiles / 4, rest = tiles % 4;
+        uint32_t run = 0, tile = tiles;  // (past the last: a unit of no tile)
+        if (i < 4 * full * runs) {
+            const uint32_t q = i / (4 * runs);
+            run = (i - q * 4 * runs) / 4;
+            tile = 4 * q + i % 4;
+        } else if (i < tiles * runs) {
+            run = (i - 4 * full * runs) / rest;
+            tile = 4 * full + (i - 4 * full * runs) % rest;
+        }
+        plan.unit()[k] = Unit{int(p), int(tile), int(rows), int(first_s[p]), int(run * each),
+                              int(min(chunks, (run + 1) * each)), int(from_s[p]), int(end_s[p] - from_s[p]), 0, {}};
     }
 }
 
@@ -434,22 +389,19 @@ template <int QK, bool QQ>
 __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at)
 {
     constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
-    constexpr int LD = VD + 4, NW = 4;
-    __shared__ __align__(16) float sc_s[NW][64];
-    __shared__ __align__(16) float mo[NW][kCols][LD];
-    __shared__ floatx4_t ms[NW][kCols];  // maximum, more, weight
+    __shared__ __align__(16) float sc_s[4][64];
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
-    // (both asked for at once: the list has as many places as the grid blocks)
+    // (both asked for at once: the list has as many places as the grid waves)
+    const uint32_t unit = 4 * blockIdx.x + uint32_t(w);
     const Head hd = *at.plan.head();
-    const Unit un = at.plan.unit()[blockIdx.x];
-    if (!made_for(hd, at.z) || int(blockIdx.x) >= hd.units) return;
+    const Unit un = at.plan.unit()[unit];
+    if (!made_for(hd, at.z) || int(unit) >= hd.units) return;
     const uint32_t kvh = blockIdx.y, R = uint32_t(gown.H / gown.KVH);
     const bool own = un.source < 0;
-    const int wide = un.wide, mine = w & (wide - 1), stream = w / wide, step = NW / wide;
-    const uint32_t ncols = uint32_t(un.rows) * R, tile = 4 * uint32_t(un.quad) + uint32_t(mine);
-    if (tile * kCols >= ncols) return;  // (of a quad of three tiles, whose waves do not meet)
+    const uint32_t ncols = uint32_t(un.rows) * R, tile = uint32_t(un.tile);
+    if (tile * kCols >= ncols) return;
 
     // ---- the wave's columns: what they see, and the query operand.  A column past
     // the end is a copy of the last ----
@@ -500,7 +452,8 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     const uint32_t span = uint32_t(un.span), begin = uint32_t(un.from), slo = begin % cap;
     const uint32_t n0 = min(span, cap - slo), n1 = span - n0;
     const int e0 = int((n0 + 31) / 32), nch = un.end;
-    int ch = un.begin + stream;
+    constexpr int step = 1;
+    int ch = un.begin;
     uint32_t s0 = 0;   // the chunk's first slot,
     uint32_t p0 = 0;   // its position,
     int left = 0;      // positions from there to the part's end; 0 behind the last chunk
@@ -820,59 +773,29 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
         load_v();  // lands during the next scores
     }
 
-    // ---- the sums: a wave's own, or, where waves have shared a tile's chunks, put
-    // together by sixteen threads a column ----
+    // ---- the sums ----
     l_run += ndl::wave_xor<16>(l_run);
     l_run += ndl::wave_xor<32>(l_run);
     l_run = ((__float_as_int(cf0) < 0) & (l_run != 0.0f)) ? NAN : l_run;
-    // the sums are left as 2^more of what has a weight of 1/2 to 1: of values near
-    // fp32's end the sum may be beyond it, the mean is not
+    // left as 2^more of what has a weight of 1/2 to 1: of values near fp32's end the
+    // sum may be beyond it, the mean is not
     const int more = __builtin_amdgcn_frexp_expf(l_run);
-    // (from here on the maximum is in bits; -inf: sums are 0, or NaN where a score was)
-    const float mb = m_run == -INFINITY ? -INFINITY : mu, lb = __builtin_amdgcn_ldexpf(l_run, -more);
-    const size_t slot = (size_t(un.slot) + mine) * gown.KVH + kvh;
-    if (step == 1) {
-        // (m + more may be rounded, M with it; m - M is not)
-        const float M = mb + float(more), by = mb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mb - M + float(more));
-        float *po = at.part_o + (slot * kCols + n) * VD + 16 * qd;
-        // lane (n, qd) holds V columns 16 qd + 4 i + c
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            floatx4_t o;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more) * by;
-            *reinterpret_cast<floatx4_t *>(po + 4 * i) = o;
-        }
-        if (qd == 0) *reinterpret_cast<floatx2_t *>(at.part_ml + (slot * kCols + n) * 2) = floatx2_t{M, lb * by};
-        return;
-    }
-    if (qd == 0) ms[w][n] = floatx4_t{mb, float(more), lb, 0.0f};
+    // (from here on the maximum is in bits; -inf: sums are 0, or NaN where a score was.
+    // m + more may be rounded, M with it; m - M is not)
+    const float mb = m_run == -INFINITY ? -INFINITY : mu, M = mb + float(more);
+    const float by = mb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mb - M + float(more));
+    const size_t to = (size_t(unit) * gown.KVH + kvh) * kCols + n;
+    float *po = at.part_o + to * VD + 16 * qd;
+    // lane (n, qd) holds V columns 16 qd + 4 i + c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         floatx4_t o;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more);
-        *reinterpret_cast<floatx4_t *>(&mo[w][n][16 * qd + 4 * i]) = o;
+        for (int c = 0; c < 4; ++c) o[c] = __builtin_amdgcn_ldexpf(acc[c][i], vexp - 1 - more) * by;
+        *reinterpret_cast<floatx4_t *>(po + 4 * i) = o;
     }
-    __syncthreads();
-    const int col = t >> 4;
-    for (int j = 0; j < wide; ++j) {
-        // against a maximum 2^3 above the largest, so that no sum of eight leaves the
-        // values' range
-        float M = -INFINITY, L = 0.0f;
-        floatx4_t O{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = j; i < NW; i += wide) M = fmaxf(M, ms[i][col][0] + ms[i][col][1]);
-        M += 3.0f;
-        for (int i = j; i < NW; i += wide) {
-            const floatx4_t z = ms[i][col];
-            const float by = z[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(z[0] - M + z[1]);
-            L += z[2] * by;
-            O += *reinterpret_cast<const floatx4_t *>(&mo[i][col][4 * (t & 15)]) * by;
-        }
-        const size_t to = ((size_t(un.slot) + j) * gown.KVH + kvh) * kCols + col;
-        *reinterpret_cast<floatx4_t *>(at.part_o + to * VD + 4 * (t & 15)) = O;
-        if ((t & 15) == 0) *reinterpret_cast<floatx2_t *>(at.part_ml + to * 2) = floatx2_t{M, L};
-    }
+    if (qd == 0)
+        *reinterpret_cast<floatx2_t *>(at.part_ml + to * 2) = floatx2_t{M, __builtin_amdgcn_ldexpf(l_run, -more) * by};
 }
 
 // The sums of a (row, head) meet: a wave each, a lane a run of chunks, then a lane a
@@ -887,26 +810,22 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t fi
     float *out = at.out + (size_t(row) * H + head) * VD;
     const Head hd = *at.plan.head();
     const Seats seats = at.plan.seat()[row];
-    if (!made_for(hd, at.z) || seats.own.column > 0) {
+    if (!made_for(hd, at.z) || seats.is > 0) {
         out[lane] = NAN;
         return;
     }
-    if (seats.own.column < 0) return;
+    if (seats.is < 0) return;
     // the first run's sums, their number and how far apart they are (slots)
-    auto find = [&](const Seat &s, uint32_t f, uint32_t &to, int &runs, uint32_t &apart) {
-        const bool next = f / (4 * kCols) != uint32_t(s.column) / (4 * kCols);
-        const uint32_t n0 = uint32_t(s.runs) & 0xffff, w0 = uint32_t(s.wides) & 15;
-        runs = int(next ? uint32_t(s.runs) >> 16 : n0);
-        apart = (next ? uint32_t(s.wides) >> 4 : w0) * uint32_t(at.z.KVH) * kCols;
-        to = ((uint32_t(s.slot) + (next ? n0 * w0 : 0) + f / kCols % 4) * uint32_t(at.z.KVH) + kvh) * kCols + f % kCols;
-    };
-    const uint32_t n = row % at.z.rows;
-    Seat own = seats.own;
-    own.column = int(n * R);
     uint32_t to[2], apart[2];
     int runs[2];
-    find(seats.prefix, uint32_t(seats.prefix.column) + r, to[0], runs[0], apart[0]);
-    find(own, n * R + r, to[1], runs[1], apart[1]);
+    auto find = [&](const Seat &s, int i) {
+        const uint32_t f = uint32_t(s.column) + r, tile = f / kCols, q4 = tile & ~3u;
+        runs[i] = s.runs;
+        apart[i] = min(uint32_t(s.tiles) - q4, 4u) * uint32_t(at.z.KVH) * kCols;
+        to[i] = ((uint32_t(s.unit) + q4 * uint32_t(s.runs) + (tile - q4)) * uint32_t(at.z.KVH) + kvh) * kCols + f % kCols;
+    };
+    find(seats.prefix, 0);
+    find(seats.own, 1);
     const int all = runs[0] + runs[1];
     float M = -INFINITY, L = 0.0f, O = 0.0f;
     for (int j0 = 0; j0 < all; j0 += 64) {
@@ -971,7 +890,7 @@ Sizes sizes_of(const nd_kv_geom *g, size_t prefix_cap, size_t count, size_t rows
                  prefixes ? int(prefix_cap) : 1};
 }
 
-size_t partial_floats(const Sizes &z) { return size_t(layout_of(z).slots) * z.KVH * kCols * (VD + 2); }
+size_t partial_floats(const Sizes &z) { return size_t(layout_of(z).units) * z.KVH * kCols * (VD + 2); }
 
 }  // namespace
 
@@ -1052,12 +971,12 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     void *ws = nullptr;
     if (int rc = nd::call_workspace(ctx, partial_floats(a.z) * sizeof(float), work, work_bytes, &ws)) return rc;
     a.part_o = static_cast<float *>(ws);
-    a.part_ml = a.part_o + size_t(a.plan.l.slots) * a.z.KVH * kCols * VD;
+    a.part_ml = a.part_o + size_t(a.plan.l.units) * a.z.KVH * kCols * VD;
     nd_kv_geom pg = *g;
     pg.cap = a.z.pcap;
     auto *fn = g->qk_head_dim == 48 ? (quant_query ? prefix_kernel<48, true> : prefix_kernel<48, false>)
                                     : (quant_query ? prefix_kernel<64, true> : prefix_kernel<64, false>);
-    hipLaunchKernelGGL(fn, dim3(a.plan.l.units, unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
+    hipLaunchKernelGGL(fn, dim3(a.plan.l.units / 4, unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
                        make_geom(&pg), a);
     if (int rc = nd::check_launch("attend_prefix_i8")) return rc;
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
