@@ -28,6 +28,8 @@ constexpr size_t kMaxSessions = 65535, kMaxRows = 256, kMaxAll = size_t(1) << 20
 constexpr int kPlanMagic = 0x6e645031;
 constexpr uint32_t kWaves = 4096;  // four a SIMD
 constexpr uint32_t kLeast = 4;     // chunks a wave, at least
+constexpr uint32_t kExtra = 3;     // what a unit costs beside its chunks, in chunks
+constexpr uint64_t kTile = uint64_t(1) << 40;
 
 struct Head {
     int magic, count, rows, prefixes, heads, kv_heads, cap, prefix_cap;
@@ -51,8 +53,8 @@ struct Seats {
 
 struct Unit {
     int source, tile, rows, first;  // prefix, or ~session; its rows, the first one's place
-    int begin, end, from, span;     // chunks of the positions from .. from + span - 1
-    int used, pad[7];               // own: positions before the step
+    int run, runs, from, span;      // chunks run, run + runs, .. of the positions from .. from + span - 1
+    int used, chunks, pad[6];       // own: positions before the step; chunks of the span
 };
 
 struct Layout {
@@ -209,6 +211,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     auto tiles_of = [&](uint32_t rows) { return (rows * R + kCols - 1) / kCols; };
     auto own_chunks = [&](const Want &w) { return chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)); };
     auto group_chunks = [&](uint32_t p) { return chunks_of(from_s[p], end_s[p] - from_s[p], uint32_t(z.pcap)); };
+    // (chunks of all tiles below 2^40, tiles below 2^24)
     auto add_weight = [&](uint64_t v) {
         v = ndl::last_lane(ndl::wave_scan(v));
         if (lane == 0 && v) atomicAdd(reinterpret_cast<unsigned long long *>(&weight_s), v);
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     sessions(S, [&](uint32_t i, const Want &w) {
         const uint32_t m = uint32_t(w.rows());
         if (!m) return;
-        weight += uint64_t(tiles_of(m)) * own_chunks(w);
+        weight += uint64_t(tiles_of(m)) * (own_chunks(w) | kTile);
         if (w.prefix < 0) return;
         atomicAdd(&rows_s[w.prefix], m);
         atomicMin(&from_s[w.prefix], uint32_t(w.from));
@@ -229,11 +232,14 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     __syncthreads();
     weight = 0;
     for (uint32_t p = t; p < P; p += NT)
-        if (rows_s[p]) weight += uint64_t(tiles_of(rows_s[p])) * group_chunks(p);
+        if (rows_s[p]) weight += uint64_t(tiles_of(rows_s[p])) * (group_chunks(p) | kTile);
     add_weight(weight);
     __syncthreads();
-    // (a chunk more than the share: no more units than that many and the tiles)
-    const double share = double(weight_s) / double(max(1u, kWaves / uint32_t(z.KVH)));
+    // ---- the length of a run: each wave's share of all chunks, a unit counted as kExtra
+    // more for its beginning and end (a run more: no more units than places and tiles).
+    // The prefixes' units, the longest, come first, and short ones fill the gaps ----
+    const double places = double(max(1u, kWaves / uint32_t(z.KVH)));
+    const double share = (double(weight_s & (kTile - 1)) + double(kExtra) * double(weight_s >> 40)) / places;
     const uint32_t each = uint32_t(fmin(fmax(share + 1.0, double(kLeast)), 1048576.0));
 
     // ---- where each group's rows and units begin ----
@@ -299,8 +305,8 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
         for (uint32_t q = 0; 4 * q < tiles; ++q)
             for (uint32_t k = 0; k < runs; ++k)
                 for (uint32_t j = 4 * q; j < min(tiles, 4 * q + 4); ++j)
-                    plan.unit()[unit++] = Unit{~int(i0), int(j), int(m), 0, int(k * each), int(min(chunks, (k + 1) * each)),
-                                               mine.lo, mine.span, mine.used, {}};
+                    plan.unit()[unit++] = Unit{~int(i0), int(j), int(m), 0, int(k), int(runs),
+                                               mine.lo, mine.span, mine.used, int(chunks), {}};
         there_s[t] = mine.bad ? ~mine.there : mine.there;
         at_s[t] = int(rank);
         used_s[t] = mine.used;
@@ -360,8 +366,8 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
             run = (i - 4 * full * runs) / rest;
             tile = 4 * full + (i - 4 * full * runs) % rest;
         }
-        plan.unit()[k] = Unit{int(p), int(tile), int(rows), int(first_s[p]), int(run * each),
-                              int(min(chunks, (run + 1) * each)), int(from_s[p]), int(end_s[p] - from_s[p]), 0, {}};
+        plan.unit()[k] = Unit{int(p), int(tile), int(rows), int(first_s[p]), int(run), int(runs),
+                              int(from_s[p]), int(end_s[p] - from_s[p]), 0, int(chunks), {}};
     }
 }
 
@@ -374,7 +380,7 @@ struct Attend {
     size_t kv_stride, pkv_stride;
     const float *q;
     float *out, *part_o, *part_ml;  // sums of (slot, kv head, column), and their maximum and weight
-    Divisor by_rep;
+    Divisor by_rep, by_kvh;
     float scale2;  // |scale| log2(e); below 0 where scale is no number
     int negative;  // scale < 0
 };
@@ -394,37 +400,19 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
     // (both asked for at once: the list has as many places as the grid waves)
-    const uint32_t unit = 4 * blockIdx.x + uint32_t(w);
+    const uint32_t block = at.by_kvh.quotient(blockIdx.x), kvh = blockIdx.x - block * uint32_t(gown.KVH);
+    const uint32_t unit = 4 * block + uint32_t(w);
     const Head hd = *at.plan.head();
     const Unit un = at.plan.unit()[unit];
     if (!made_for(hd, at.z) || int(unit) >= hd.units) return;
-    const uint32_t kvh = blockIdx.y, R = uint32_t(gown.H / gown.KVH);
+    const uint32_t R = uint32_t(gown.H / gown.KVH);
     const bool own = un.source < 0;
     const uint32_t ncols = uint32_t(un.rows) * R, tile = uint32_t(un.tile);
     if (tile * kCols >= ncols) return;
 
-    // ---- the wave's columns: what they see, and the query operand.  A column past
-    // the end is a copy of the last ----
     const uint32_t f = min(tile * kCols + uint32_t(n), ncols - 1), r = at.by_rep.quotient(f);
-    uint32_t row, lo, hi;
-    if (own) {
-        const uint32_t end = uint32_t(un.used) + r;  // the row's own position, below 2^31
-        row = uint32_t(~un.source) * at.z.rows + r;
-        lo = hd.window && end + 1 > uint32_t(hd.window) ? end + 1 - uint32_t(hd.window) : 0;
-        hi = end;
-    } else {
-        const Place pl = at.plan.place()[uint32_t(un.first) + r];
-        row = uint32_t(pl.row);
-        lo = uint32_t(pl.from);
-        hi = 0x7fffffff;
-    }
-    const uint32_t head = kvh * R + f - r * R;
-    float v[SL];
-    {
-        const float *qh = at.q + (size_t(row) * gown.H + head) * QK + qd * SL;
-#pragma unroll
-        for (int e = 0; e < SL; ++e) v[e] = qh[e];
-    }
+    Place pl{};
+    if (!own) pl = at.plan.place()[uint32_t(un.first) + r];
     const uint32_t cap = uint32_t(own ? gown.cap : gp.cap);
     const uint8_t *blk = own ? at.kv + size_t(~un.source) * at.kv_stride : at.pkv + size_t(un.source) * at.pkv_stride;
     const size_t v_off = own ? gown.v_off : gp.v_off, ks_off = own ? gown.ks_off : gp.ks_off;
@@ -433,27 +421,12 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     // K scales, and vs_off - ks_off bytes on (KVH cap 4, below 2^32) the V scales
     const uint32_t to_vs = uint32_t((own ? gown.vs_off : gp.vs_off) - ks_off);
     const rows_t sb = rows_at(blk + ks_off + size_t(kvh) * cap * 4, to_vs + cap * 4);
-    // the first position that all columns see, and the last
-    uint32_t tlo = lo, thi = hi;
-    auto both = [&](auto distance) {
-        constexpr int D = decltype(distance)::value;
-        tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
-        thi = min(thi, uint32_t(ndl::wave_xor_int<D>(int(thi))));
-    };
-    both(std::integral_constant<int, 1>{});
-    both(std::integral_constant<int, 2>{});
-    both(std::integral_constant<int, 4>{});
-    both(std::integral_constant<int, 8>{});
-    tlo = __builtin_amdgcn_readfirstlane(tlo);
-    thi = __builtin_amdgcn_readfirstlane(thi);
-
     // ---- the walk: up to the ring's end, then from its start, in chunks of 32 (the
     // last of a part shorter).  It is no longer than the ring, so it wraps once ----
     const uint32_t span = uint32_t(un.span), begin = uint32_t(un.from), slo = begin % cap;
     const uint32_t n0 = min(span, cap - slo), n1 = span - n0;
-    const int e0 = int((n0 + 31) / 32), nch = un.end;
-    constexpr int step = 1;
-    int ch = un.begin;
+    const int e0 = int((n0 + 31) / 32), nch = un.chunks, step = un.runs;
+    int ch = un.run;
     uint32_t s0 = 0;   // the chunk's first slot,
     uint32_t p0 = 0;   // its position,
     int left = 0;      // positions from there to the part's end; 0 behind the last chunk
@@ -496,6 +469,40 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     place(ch);
     load_k();
     load_v();
+
+    // ---- the wave's columns: what they see, and the query operand, asked for while
+    // the first chunk is on its way.  A column past the end is a copy of the last ----
+    uint32_t row, lo, hi;
+    if (own) {
+        const uint32_t end = uint32_t(un.used) + r;  // the row's own position, below 2^31
+        row = uint32_t(~un.source) * at.z.rows + r;
+        lo = hd.window && end + 1 > uint32_t(hd.window) ? end + 1 - uint32_t(hd.window) : 0;
+        hi = end;
+    } else {
+        row = uint32_t(pl.row);
+        lo = uint32_t(pl.from);
+        hi = 0x7fffffff;
+    }
+    const uint32_t head = kvh * R + f - r * R;
+    float v[SL];
+    {
+        const float *qh = at.q + (size_t(row) * gown.H + head) * QK + qd * SL;
+#pragma unroll
+        for (int e = 0; e < SL; ++e) v[e] = qh[e];
+    }
+    // the first position that all columns see, and the last
+    uint32_t tlo = lo, thi = hi;
+    auto both = [&](auto distance) {
+        constexpr int D = decltype(distance)::value;
+        tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
+        thi = min(thi, uint32_t(ndl::wave_xor_int<D>(int(thi))));
+    };
+    both(std::integral_constant<int, 1>{});
+    both(std::integral_constant<int, 2>{});
+    both(std::integral_constant<int, 4>{});
+    both(std::integral_constant<int, 8>{});
+    tlo = __builtin_amdgcn_readfirstlane(tlo);
+    thi = __builtin_amdgcn_readfirstlane(thi);
 
     // ---- the query operand, while the first chunk is on its way ----
     float cf0;                        // factor of a score, in bits, is |cf0| 2^(kexp - sh)
@@ -966,6 +973,7 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     a.q = q;
     a.out = out;
     a.by_rep = Divisor::of(uint32_t(g->num_heads / g->num_kv_heads));
+    a.by_kvh = Divisor::of(uint32_t(g->num_kv_heads));
     a.scale2 = scale == scale ? float(double(scale < 0 ? -scale : scale) * 1.4426950408889634) : -1.0f;
     a.negative = scale < 0;
     void *ws = nullptr;
@@ -976,7 +984,7 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     pg.cap = a.z.pcap;
     auto *fn = g->qk_head_dim == 48 ? (quant_query ? prefix_kernel<48, true> : prefix_kernel<48, false>)
                                     : (quant_query ? prefix_kernel<64, true> : prefix_kernel<64, false>);
-    hipLaunchKernelGGL(fn, dim3(a.plan.l.units / 4, unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
+    hipLaunchKernelGGL(fn, dim3(a.plan.l.units / 4 * unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
                        make_geom(&pg), a);
     if (int rc = nd::check_launch("attend_prefix_i8")) return rc;
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
