@@ -391,24 +391,25 @@ __device__ inline bool made_for(const Head &h, const Sizes &z)
            h.heads == z.H && h.kv_heads == z.KVH && h.cap == z.cap && h.prefix_cap == z.pcap;
 }
 
-template <int QK, bool QQ>
-__global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at)
+// Operands of a chunk that a block's waves share, twice: one is read while the next
+// one is laid down.  K as it goes into the products (codes, or f16), 16 positions
+// after 16; V as f16, column 4 n + c of eight positions a lane.
+struct Shared {
+    uint32_t sc[4][64];
+    uint32_t k[2][4][64][4], v[2][4][64][4];
+};
+
+template <int QK, bool QQ, bool TOGETHER>
+__device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Attend &at, const Head &hd, const Unit &un,
+                                     uint32_t unit, uint32_t kvh, Shared &sh_s)
 {
     constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
-    __shared__ __align__(16) float sc_s[4][64];
-
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
-    // (both asked for at once: the list has as many places as the grid waves)
-    const uint32_t block = at.by_kvh.quotient(blockIdx.x), kvh = blockIdx.x - block * uint32_t(gown.KVH);
-    const uint32_t unit = 4 * block + uint32_t(w);
-    const Head hd = *at.plan.head();
-    const Unit un = at.plan.unit()[unit];
-    if (!made_for(hd, at.z) || int(unit) >= hd.units) return;
     const uint32_t R = uint32_t(gown.H / gown.KVH);
-    const bool own = un.source < 0;
+    const bool own = !TOGETHER && un.source < 0;
     const uint32_t ncols = uint32_t(un.rows) * R, tile = uint32_t(un.tile);
-    if (tile * kCols >= ncols) return;
+    float *sc_s = reinterpret_cast<float *>(sh_s.sc[w]);
 
     const uint32_t f = min(tile * kCols + uint32_t(n), ncols - 1), r = at.by_rep.quotient(f);
     Place pl{};
@@ -426,49 +427,104 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     const uint32_t span = uint32_t(un.span), begin = uint32_t(un.from), slo = begin % cap;
     const uint32_t n0 = min(span, cap - slo), n1 = span - n0;
     const int e0 = int((n0 + 31) / 32), nch = un.chunks, step = un.runs;
-    int ch = un.run;
-    uint32_t s0 = 0;   // the chunk's first slot,
-    uint32_t p0 = 0;   // its position,
-    int left = 0;      // positions from there to the part's end; 0 behind the last chunk
-    int stop = 0;      // the part's last chunk, and one
-    auto place = [=, &s0, &p0, &left, &stop](int i) {
+    struct Chunk {
+        int ch, left, stop;  // its number; positions from p0 to the part's end, 0 behind the last; the part's last and one
+        uint32_t s0, p0;     // its first slot and position
+    } now, ahead;            // that whose scores come next, and together the one whose K and V do
+    auto put = [=](Chunk &c, int i) {
         const bool second = i >= e0;
         const uint32_t off = 32u * uint32_t(second ? i - e0 : i);
-        s0 = i >= nch ? 0u : (second ? 0u : slo) + off;
-        p0 = begin + (second ? n0 : 0u) + off;
-        left = i >= nch ? 0 : int((second ? n1 : n0) - off);
-        stop = second ? nch : min(e0, nch);
+        c.ch = i;
+        c.s0 = i >= nch ? 0u : (second ? 0u : slo) + off;
+        c.p0 = begin + (second ? n0 : 0u) + off;
+        c.left = i >= nch ? 0 : int((second ? n1 : n0) - off);
+        c.stop = second ? nch : min(e0, nch);
     };
-    uint32_t kr[2][KD], vr[8];
+    auto next = [=](Chunk &c) {
+        if (c.ch + step < c.stop) [[likely]] {
+            c.ch += step;
+            c.s0 += 32u * uint32_t(step);
+            c.p0 += 32u * uint32_t(step);
+            c.left -= 32 * step;
+        } else {
+            asm volatile("");  // (a branch, not thirty selects in every chunk)
+            put(c, c.ch + step);
+        }
+    };
+    // alone: a wave's K rows and V; together: the part that it lays down for all, K
+    // dwords of half `w & 1` of 16 positions `w >> 1`, V of positions 2 w, 2 w + 1 of
+    // every eight
+    uint32_t kr[2][KD], vr[TOGETHER ? 2 : 8];
     float scr = 0.0f;
-    const uint32_t kl = uint32_t(n * QK + qd * SL), vl = uint32_t(4 * qd * VD + 4 * n);
+    const uint32_t kl = TOGETHER ? uint32_t((16 * (w >> 1) + n) * QK + qd * SL + 8 * (w & 1)) : uint32_t(n * QK + qd * SL);
+    const uint32_t vl = uint32_t((4 * qd + (TOGETHER ? 16 * (w >> 1) + 2 * (w & 1) : 0)) * VD + 4 * n);
     const uint32_t scl = (lane & 31) * 4 + (lane < 32 ? 0u : to_vs);
     // loads of K and V are never conditional: past the last chunk they read some slot
-    auto load_k = [&]() {
+    auto load_k = [&](uint32_t s0) {
         const uint32_t o = here(kl + s0 * QK);
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            if constexpr (KD == 3) {
-                const auto r = __builtin_amdgcn_raw_buffer_load_b96(kb, o + 16 * a * QK, 0, 0);
-#pragma unroll
-                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+        if constexpr (TOGETHER) {
+            if (KD == 3 && (w & 1)) {
+                kr[0][0] = __builtin_amdgcn_raw_buffer_load_b32(kb, o, 0, 0);
             } else {
-                const auto r = __builtin_amdgcn_raw_buffer_load_b128(kb, o + 16 * a * QK, 0, 0);
+                const auto r = __builtin_amdgcn_raw_buffer_load_b64(kb, o, 0, 0);
+                kr[0][0] = r[0], kr[0][1] = r[1];
+            }
+        } else {
 #pragma unroll
-                for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+            for (int a = 0; a < 2; ++a) {
+                if constexpr (KD == 3) {
+                    const auto r = __builtin_amdgcn_raw_buffer_load_b96(kb, o + 16 * a * QK, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+                } else {
+                    const auto r = __builtin_amdgcn_raw_buffer_load_b128(kb, o + 16 * a * QK, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < KD; ++d) kr[a][d] = r[d];
+                }
             }
         }
+    };
+    auto load_scales = [&](uint32_t s0) {
         scr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sb, scl + s0 * 4, 0, 0));
     };
-    auto load_v = [&]() {
+    auto load_v = [&](uint32_t s0) {
         const uint32_t o = here(vl + s0 * VD);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < (TOGETHER ? 2 : 8); ++j)
             vr[j] = __builtin_amdgcn_raw_buffer_load_b32(vb, o + (16 * (j >> 2) + (j & 3)) * VD, 0, 0);
     };
-    place(ch);
-    load_k();
-    load_v();
+    // the wave's part into buffer `to`
+    auto lay_down = [&](int to) {
+        uint32_t *kk = &sh_s.k[to][QQ ? w >> 1 : w][lane][QQ ? 2 * (w & 1) : 0];
+        if (KD == 3 && (w & 1)) {
+            const uint32_t u = kr[0][0] ^ 0x80808080u;
+            if constexpr (QQ)
+                kk[0] = kr[0][0];
+            else
+                kk[0] = f16_pair<0>(u), kk[1] = f16_pair<1>(u);
+        } else {
+            const uint32_t u0 = kr[0][0] ^ 0x80808080u, u1 = kr[0][1] ^ 0x80808080u;
+            if constexpr (QQ)
+                kk[0] = kr[0][0], kk[1] = kr[0][1];
+            else
+                kk[0] = f16_pair<0>(u0), kk[1] = f16_pair<1>(u0), kk[2] = f16_pair<0>(u1), kk[3] = f16_pair<1>(u1);
+        }
+        const uint32_t v0 = vr[0] ^ 0x80808080u, v1 = vr[1] ^ 0x80808080u;
+        sh_s.v[to][0][lane][w] = f16_codes<0>(v0, v1);
+        sh_s.v[to][1][lane][w] = f16_codes<1>(v0, v1);
+        sh_s.v[to][2][lane][w] = f16_codes<2>(v0, v1);
+        sh_s.v[to][3][lane][w] = f16_codes<3>(v0, v1);
+    };
+    // all waves' parts are there, and read
+    auto meet = [&]() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    put(now, un.run);
+    load_k(now.s0);
+    load_scales(now.s0);
+    load_v(now.s0);
 
     // ---- the wave's columns: what they see, and the query operand, asked for while
     // the first chunk is on its way.  A column past the end is a copy of the last ----
@@ -588,7 +644,18 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     uint32_t watch = 0;
     int vmet = 0x10000;                 // vexp then, and 3
 
-    for (; ch < nch; ch += step) {
+    int buf = 0;
+    if constexpr (TOGETHER) {
+        lay_down(0);
+        ahead = now;
+        next(ahead);
+        load_k(ahead.s0);
+        load_v(ahead.s0);
+        meet();
+    }
+    while (now.ch < nch) {
+        const uint32_t p0 = now.p0;
+        const int left = now.left;
         // ---- the positions each column sees ----
         const bool full = p0 >= tlo && p0 + 31 <= thi && left >= 32;
         uint32_t vis = 0xffffffffu;
@@ -646,14 +713,14 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
         sc = __builtin_amdgcn_ldexpf(sc, shift);
         const uint32_t few = uint32_t(__builtin_amdgcn_ballot_w64(sc < 2.0f) >> 32);
         uint32_t small = left < 32 ? few & ((1u << left) - 1u) : few;
-        sc_s[w][lane] = sc;
+        sc_s[lane] = sc;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         floatx4_t ks[2], vs[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-            ks[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][16 * a + 4 * qd]);
-            vs[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[w][32 + 16 * a + 4 * qd]);
+            ks[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[16 * a + 4 * qd]);
+            vs[a] = *reinterpret_cast<const floatx4_t *>(&sc_s[32 + 16 * a + 4 * qd]);
         }
         __builtin_amdgcn_wave_barrier();
         // ---- scores ----
@@ -661,7 +728,13 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
         if constexpr (QQ) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const intx4_t kf{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
+                intx4_t kf;
+                if constexpr (TOGETHER) {
+                    kf = *reinterpret_cast<const intx4_t *>(sh_s.k[buf][a][lane]);
+                    if constexpr (KD == 3) kf[3] = 0;
+                } else {
+                    kf = intx4_t{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
+                }
                 const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi, intx4_t{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * a + i] = float(d[i]) * ks[a][i];
@@ -670,11 +743,23 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 uint32_t kp[2 * KD];
+                if constexpr (TOGETHER) {
+                    const u32x4_t lo4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a][lane]);
+                    kp[0] = lo4[0], kp[1] = lo4[1], kp[2] = lo4[2], kp[3] = lo4[3];
+                    if constexpr (KD == 3) {
+                        const uint2 hi2 = *reinterpret_cast<const uint2 *>(sh_s.k[buf][2 * a + 1][lane]);
+                        kp[4] = hi2.x, kp[5] = hi2.y;
+                    } else {
+                        const u32x4_t hi4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a + 1][lane]);
+                        kp[4] = hi4[0], kp[5] = hi4[1], kp[2 * KD - 2] = hi4[2], kp[2 * KD - 1] = hi4[3];
+                    }
+                } else {
 #pragma unroll
-                for (int d = 0; d < KD; ++d) {
-                    const uint32_t u = kr[a][d] ^ 0x80808080u;
-                    kp[2 * d] = f16_pair<0>(u);
-                    kp[2 * d + 1] = f16_pair<1>(u);
+                    for (int d = 0; d < KD; ++d) {
+                        const uint32_t u = kr[a][d] ^ 0x80808080u;
+                        kp[2 * d] = f16_pair<0>(u);
+                        kp[2 * d + 1] = f16_pair<1>(u);
+                    }
                 }
                 floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -694,16 +779,18 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
                 for (int i = 0; i < 4; ++i) s[4 * a + i] = d[i] * ks[a][i];
             }
         }
-        // the next chunk: its K lands during the softmax and the values
-        if (ch + step < stop) [[likely]] {
-            s0 += 32u * uint32_t(step);
-            p0 += 32u * uint32_t(step);
-            left -= 32 * step;
+        // the next chunk: its K lands during the softmax and the values; together, it has
+        // landed, and the one after it does
+        next(now);
+        load_scales(now.s0);
+        if constexpr (TOGETHER) {
+            lay_down(buf ^ 1);
+            next(ahead);
+            load_k(ahead.s0);
+            load_v(ahead.s0);
         } else {
-            asm volatile("");  // (a branch, not thirty selects in every chunk)
-            place(ch + step);
+            load_k(now.s0);
         }
-        load_k();
         // ---- softmax: each lane its column's eight positions ----
         if (!full) {
 #pragma unroll
@@ -752,21 +839,33 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(i8_at(vr[j], c) * 0x1p-9f, wt[j], acc[c], 0, 0, 0);
+                for (int c = 0; c < 4; ++c) {
+                    float code;
+                    if constexpr (TOGETHER)
+                        code = float(reinterpret_cast<const _Float16 *>(sh_s.v[buf][c][lane])[j]);
+                    else
+                        code = i8_at(vr[j], c) * 0x1p-9f;
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(code, wt[j], acc[c], 0, 0, 0);
+                }
 #pragma unroll
             for (int j = 0; j < 8; ++j) wt[j] = 0.0f;
         }
         {
-            uint32_t ph[4], pl[4], u[8];
+            uint32_t ph[4], pl[4], u[TOGETHER ? 2 : 8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) split2(wt[2 * j], wt[2 * j + 1], ph[j], pl[j]);
+            if constexpr (!TOGETHER) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
+                for (int j = 0; j < 8; ++j) u[j] = vr[j] ^ 0x80808080u;
+            }
             auto column = [&](auto cc) {
                 constexpr int c = decltype(cc)::value;
-                const f16x8_t vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]),
-                                                 f16_codes<c>(u[4], u[5]), f16_codes<c>(u[6], u[7]));
+                f16x8_t vf;
+                if constexpr (TOGETHER)
+                    vf = *reinterpret_cast<const f16x8_t *>(sh_s.v[buf][c][lane]);
+                else
+                    vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]), f16_codes<c>(u[4], u[5]),
+                                       f16_codes<c>(u[6], u[7]));
                 acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(pl[0], pl[1], pl[2], pl[3]), acc[c],
                                                                 0, 0, 0);
                 acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, vec4<f16x8_t>(ph[0], ph[1], ph[2], ph[3]), acc[c],
@@ -777,7 +876,12 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
             column(std::integral_constant<int, 2>{});
             column(std::integral_constant<int, 3>{});
         }
-        load_v();  // lands during the next scores
+        if constexpr (TOGETHER) {
+            meet();
+            buf ^= 1;
+        } else {
+            load_v(now.s0);  // lands during the next scores
+        }
     }
 
     // ---- the sums ----
@@ -803,6 +907,28 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     }
     if (qd == 0)
         *reinterpret_cast<floatx2_t *>(at.part_ml + to * 2) = floatx2_t{M, __builtin_amdgcn_ldexpf(l_run, -more) * by};
+}
+
+// A block's four units: of four tiles of a prefix over the same chunks, together, or
+// each for itself.
+template <int QK, bool QQ>
+__global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at)
+{
+    __shared__ __align__(16) Shared sh_s;
+    const uint32_t w = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+    const uint32_t block = at.by_kvh.quotient(blockIdx.x), kvh = blockIdx.x - block * uint32_t(gown.KVH);
+    const uint32_t unit = 4 * block + w;
+    // (both asked for at once: the list has as many places as the grid waves)
+    const Head hd = *at.plan.head();
+    const Unit un = at.plan.unit()[unit];
+    if (!made_for(hd, at.z) || int(unit) >= hd.units) return;
+    const uint32_t ncols = uint32_t(un.rows) * uint32_t(gown.H / gown.KVH), tile = uint32_t(un.tile);
+    if (tile * kCols >= ncols) return;
+    // (a prefix's first unit is a multiple of four, and its full quads come first)
+    if (un.source >= 0 && (tile | 3) * kCols < ncols)
+        walk<QK, QQ, true>(gown, gp, at, hd, un, unit, kvh, sh_s);
+    else
+        walk<QK, QQ, false>(gown, gp, at, hd, un, unit, kvh, sh_s);
 }
 
 // The sums of a (row, head) meet: a wave each, a lane a run of chunks, then a lane a
