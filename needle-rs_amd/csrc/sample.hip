@@ -6,10 +6,10 @@
 // weights, added up, reach a target.  So no row is sorted:
 //   a short top-k: the row's tokens are counted in bins that follow the order, those
 //     up to the bin of the k-th are listed, and the list is put in order;
-//   else: weights are added up in the bins, the bin of a target is found, and its
-//     tokens alone are listed;
-//   anything unusual (more tokens in a bin than a list holds, infinite logits): the
-//     row is searched in finer and finer bins, by the digits of the order.
+//   else: weights are added up in the bins, the bin of a target is found, its tokens'
+//     in finer ones, and the few of that are looked at one by one;
+//   anything unusual (too many equal logits, infinite ones): the row is searched in
+//     finer and finer bins, by the digits of the order.
 // Weights are whole numbers, exp((l - M) / T) in units of 2^-s, worked out in fp64: a
 // pick next to a border is the border's and not the rounding's, and sums of whole
 // numbers are the same in any order.  s is 49, or less where a bound on a long row's
@@ -26,13 +26,14 @@
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kPer = 8, kSlice = kPer * kThreads;
-constexpr int kBins = kThreads;  // one a thread
+constexpr int kSlice = 8192;
+constexpr int kBins = 1024;
 constexpr int kList = 512;       // tokens that are put in order, a thread each
-constexpr int kShort = 448;      // the longest top-k that is listed
+constexpr int kShort = 448;      // the longest top-k that is listed whole
+constexpr int kFew = 64;         // tokens of a bin that are looked at one by one
 constexpr int kMostScale = 49;
 constexpr uint32_t kNoBin = 0xffff;
+constexpr int kMarked = -2;      // a row that is left to the search
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start anywhere
 
@@ -178,8 +179,8 @@ __device__ inline int bin_of(const Row &r, float l)
 
 struct Shared {
     uint64_t weight[kBins], list[kList], sums[kList];
-    uint64_t room[kWaves], range[kWaves], best[3];
-    uint32_t count[kBins], listed, bin, in[3];
+    uint64_t room[3][16], best[3];
+    uint32_t count[kBins], listed, bin;
 };
 
 // Where a target lies: the token, the weights up to it and its own.
@@ -187,22 +188,23 @@ struct Cut {
     uint64_t place, upto, weight;
 };
 
-// The whole numbers of the threads before this one added up, and of all.
+// The whole numbers of the threads before this one added up, and of all (a barrier;
+// `room` is not used again before another).
+template <int NT>
 __device__ inline uint64_t block_scan(uint64_t v, uint64_t &before, uint64_t *room)
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint64_t up = ndl::wave_scan(v);
     if (lane == 63) room[w] = up;
     __syncthreads();
-    uint64_t all = 0, mine = up - v;
+    uint64_t all = 0;
+    before = up - v;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < NT / 64; ++i) {
         const uint64_t x = room[i];
-        mine += i < w ? x : 0;
+        before += i < w ? x : 0;
         all += x;
     }
-    __syncthreads();
-    before = mine;
     return all;
 }
 
@@ -223,16 +225,46 @@ __device__ inline void done(const Sample &s, size_t row, int next, double chance
     }
 }
 
+// top and low over the block; every thread gets both (a barrier, as block_scan).
+template <int NT>
+__device__ inline void meet(float &top, float &low, uint64_t *room)
+{
+    top = ndl::wave_max64(top);
+    low = -ndl::wave_max64(-low);
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = uint64_t(__float_as_uint(low)) << 32 | __float_as_uint(top);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        const uint64_t x = room[i];
+        top = fmaxf(top, __uint_as_float(uint32_t(x)));
+        low = fminf(low, __uint_as_float(uint32_t(x >> 32)));
+    }
+}
+
+template <int NT>
+__device__ inline float sum_over(float v, uint64_t *room)
+{
+    v = ndl::wave_sum64(v);
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = __float_as_uint(v);
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) v += __uint_as_float(uint32_t(room[i]));
+    return v;
+}
+
 // ---- a row by finer and finer bins --------------------------------------------
 
 // Any row, whatever its logits and rules, from memory: a block.
+template <int NT>
 __device__ __forceinline__ void search(const Sample &s, size_t row, Row r, Shared &h)
 {
-    const int t = threadIdx.x, lane = t & 63;
+    const int t = threadIdx.x;
     const float *x = s.x + row * s.x_stride;
+    constexpr int B = kBins / NT;
     auto clear = [&]() {
         __syncthreads();
-        h.count[t] = 0, h.weight[t] = 0;
+        for (int b = t; b < kBins; b += NT) h.count[b] = 0, h.weight[b] = 0;
         __syncthreads();
     };
     auto add = [&](int b, uint64_t w) {
@@ -242,16 +274,21 @@ __device__ __forceinline__ void search(const Sample &s, size_t row, Row r, Share
     uint64_t tokens = 0, all = 0;
     auto scan = [&]() {  // to sums up to each bin
         __syncthreads();
-        uint64_t c = h.count[t], w = h.weight[t], before;
-        tokens = block_scan(c, before, h.room);
-        h.count[t] = uint32_t(before + c);
-        all = block_scan(w, before, h.room);
-        h.weight[t] = before + w;
+        uint64_t c[B], w[B], cs = 0, ws = 0, cb, wb;
+#pragma unroll
+        for (int e = 0; e < B; ++e) cs += c[e] = h.count[B * t + e], ws += w[e] = h.weight[B * t + e];
+        tokens = block_scan<NT>(cs, cb, h.room[0]);
+        all = block_scan<NT>(ws, wb, h.room[1]);
+#pragma unroll
+        for (int e = 0; e < B; ++e) {
+            h.count[B * t + e] = uint32_t(cb += c[e]);
+            h.weight[B * t + e] = wb += w[e];
+        }
         __syncthreads();
     };
     auto each = [&](auto f) {
 #pragma unroll 1
-        for (int i = t; i < s.n; i += kThreads) {
+        for (int i = t; i < s.n; i += NT) {
             const float l = x[i];
             const uint64_t w = weight_of(r, l);
             if (w) f(l, i, w);
@@ -260,13 +297,8 @@ __device__ __forceinline__ void search(const Sample &s, size_t row, Row r, Share
     // the unit
     float bound = 0.0f;
 #pragma unroll 1
-    for (int i = t; i < s.n; i += kThreads) bound += bound_of(r, x[i]);
-    bound = ndl::wave_sum64(bound);
-    __syncthreads();
-    if (lane == 0) h.room[t >> 6] = __float_as_uint(bound);
-    __syncthreads();
-    bound = 0.0f;
-    for (int i = 0; i < kWaves; ++i) bound += __uint_as_float(uint32_t(h.room[i]));
+    for (int i = t; i < s.n; i += NT) bound += bound_of(r, x[i]);
+    bound = sum_over<NT>(bound, h.room[2]);
     r.scale = scale_of(bound);
     // The cuts one after another: behind the k-th token, where the weights come to
     // top_p, and the draw: each the first token at which the tokens or the weights reach
@@ -299,10 +331,10 @@ __device__ __forceinline__ void search(const Sample &s, size_t row, Row r, Share
         // the first digit has six)
         for (int shift = 60;; shift -= 10) {
             // the bin in which the target lies
-            {
-                const uint64_t now = before + (by_count ? h.count[t] : h.weight[t]);
-                const uint64_t was = before + (t == 0 ? 0 : by_count ? h.count[t - 1] : h.weight[t - 1]);
-                if (was < target && now >= target) h.bin = uint32_t(t);
+            for (int b = t; b < kBins; b += NT) {
+                const uint64_t now = before + (by_count ? h.count[b] : h.weight[b]);
+                const uint64_t was = before + (b == 0 ? 0 : by_count ? h.count[b - 1] : h.weight[b - 1]);
+                if (was < target && now >= target) h.bin = uint32_t(b);
             }
             if (t == 0) h.listed = 0;
             __syncthreads();
@@ -361,40 +393,15 @@ __device__ __forceinline__ void search(const Sample &s, size_t row, Row r, Share
 
 // ---- the common ways ------------------------------------------------------------
 
-// top and low over the block; every thread gets both (a barrier).
-__device__ inline void meet(float &top, float &low, Shared &h)
-{
-    top = ndl::wave_max64(top);
-    low = -ndl::wave_max64(-low);
-    if ((threadIdx.x & 63) == 0) h.range[threadIdx.x >> 6] = uint64_t(__float_as_uint(low)) << 32 | __float_as_uint(top);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const uint64_t x = h.range[i];
-        top = fmaxf(top, __uint_as_float(uint32_t(x)));
-        low = fminf(low, __uint_as_float(uint32_t(x >> 32)));
-    }
-}
-
-__device__ inline float sum_over(float v, uint64_t *room)
-{
-    v = ndl::wave_sum64(v);
-    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = __float_as_uint(v);
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) v += __uint_as_float(uint32_t(room[i]));
-    __syncthreads();
-    return v;
-}
-
 // A slice's logits in registers (what is no token, NaN too, is -inf), and their bins,
 // two a word.
+template <int NT>
 struct Held {
+    static constexpr int kPer = kSlice / NT;
     float v[kPer];
     uint32_t b[kPer / 2];
     int t0;
-    __device__ inline int at(int j) const { return t0 + (j >> 2) * 4 * kThreads + 4 * int(threadIdx.x) + (j & 3); }
+    __device__ inline int at(int j) const { return t0 + (j >> 2) * 4 * NT + 4 * int(threadIdx.x) + (j & 3); }
     __device__ inline void load(const float *x, int from, int n)
     {
         t0 = from;
@@ -422,30 +429,37 @@ struct Held {
             low = fminf(low, v[j] > -INFINITY ? v[j] : INFINITY);
         }
     }
-    // the tokens' bins, and, in h.weight, their number or weights
-    template <bool WEIGHTS>
+    // the tokens' bins, and in those their weights (of a finite top)
+    template <bool WEIGHTS, bool COUNT>
     __device__ inline void lay(const Row &r, Shared &h)
     {
         const double top = double(r.top);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const double d = double(v[j]) - top;  // (a finite top)
+            const double d = double(v[j]) - top;
             uint32_t bin = kNoBin;
             if (d >= r.low) {
                 bin = uint32_t(bin_of(r, v[j]));
+                if constexpr (COUNT) atomicAdd(&h.count[bin], 1u);
                 if constexpr (WEIGHTS)
                     atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[bin]), units_of(d * r.by, r.scale));
-                else
-                    atomicAdd(reinterpret_cast<uint32_t *>(&h.weight[bin]), 1u);
             }
             b[j / 2] = j & 1 ? b[j / 2] | bin << 16 : bin;
         }
     }
+    // f of the tokens of bins from .. to and of one more
     template <typename F>
-    __device__ inline void each(F f) const
+    __device__ inline void each(const Row &, uint32_t from, uint32_t to, F f) const
     {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) f(v[j], at(j), j & 1 ? b[j / 2] >> 16 : b[j / 2] & 0xffff);
+        for (int j = 0; j < kPer; ++j) {
+            const uint32_t bin = j & 1 ? b[j / 2] >> 16 : b[j / 2] & 0xffff;
+            if (bin - from <= to - from) {
+                float l = v[j];
+                asm volatile("" : "+v"(l));  // (the order of all of them is not worked out ahead, and kept)
+                f(l, order_of(l, at(j)));
+            }
+        }
     }
     // the number of the first logit that is `top`, over the block
     __device__ inline int first(float top, uint64_t *room) const
@@ -457,82 +471,110 @@ struct Held {
         for (int d = 32; d; d /= 2) i = min(i, __shfl_xor(i, d));
         if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = uint64_t(i);
         __syncthreads();
-        for (int k = 0; k < kWaves; ++k) i = min(i, int(room[k]));
+        for (int k = 0; k < NT / 64; ++k) i = min(i, int(room[k]));
         return i;
     }
 };
 
 // What the slices have listed, a wave a slice.
+template <int NT>
 struct Lists {
     const uint64_t *list;
     const Part *part;
     int slices;
     template <typename F>
-    __device__ inline void all(F f) const
+    __device__ inline void all(const Row &r, F f) const
     {
-        for (int i = int(threadIdx.x >> 6); i < slices; i += kWaves)
-            for (int j = int(threadIdx.x & 63); j < part[i].listed; j += 64) f(list[size_t(i) * kList + j]);
+        for (int i = int(threadIdx.x >> 6); i < slices; i += NT / 64) {
+            const int many = part[i].listed;
+            for (int j = int(threadIdx.x & 63); j < many; j += 64) {
+                const uint64_t o = list[size_t(i) * kList + j];
+                const float l = logit_of(o);
+                if (token(r, l)) f(l, o);
+            }
+        }
     }
-    // (their bins are worked out twice)
-    template <bool WEIGHTS>
+    template <bool WEIGHTS, bool COUNT>
     __device__ inline void lay(const Row &r, Shared &h) const
     {
-        all([&](uint64_t o) {
-            const float l = logit_of(o);
-            if (token(r, l)) atomicAdd(reinterpret_cast<uint32_t *>(&h.weight[bin_of(r, l)]), 1u);
+        all(r, [&](float l, uint64_t) { atomicAdd(&h.count[bin_of(r, l)], 1u); });
+    }
+    template <typename F>
+    __device__ inline void each(const Row &r, uint32_t from, uint32_t to, F f) const
+    {
+        all(r, [&](float l, uint64_t o) {
+            if (uint32_t(bin_of(r, l)) - from <= to - from) f(l, o);
         });
     }
 };
 
-// The tokens of bins from .. to of `src`, added to the list; what is beyond its room is
-// counted alone.
-__device__ inline void collect(const Held &src, const Row &, uint32_t from, uint32_t to, Shared &h)
+__device__ inline void enlist(Shared &h, uint64_t o)
 {
-    src.each([&](float l, int i, uint32_t bin) {
-        if (bin - from <= to - from) {
-            const uint32_t at = atomicAdd(&h.listed, 1u);
-            if (at < uint32_t(kList)) h.list[at] = order_of(l, i);
-        }
-    });
+    const uint32_t at = atomicAdd(&h.listed, 1u);  // (what is beyond the list's room is counted alone)
+    if (at < uint32_t(kList)) h.list[at] = o;
 }
 
-__device__ inline void collect(const Lists &src, const Row &r, uint32_t from, uint32_t to, Shared &h)
-{
-    src.all([&](uint64_t o) {
-        const float l = logit_of(o);
-        if (token(r, l) && uint32_t(bin_of(r, l)) - from <= to - from) {
-            const uint32_t at = atomicAdd(&h.listed, 1u);
-            if (at < uint32_t(kList)) h.list[at] = o;
+// A thread's bins' tokens (or weights) and those before them.
+template <int NT, typename T>
+struct Bins {
+    static constexpr int B = kBins / NT;
+    uint64_t v[B], before, all;
+    __device__ inline void read(const T *from, uint64_t *room)
+    {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < B; ++e) sum += v[e] = from[B * int(threadIdx.x) + e];
+        all = block_scan<NT>(sum, before, room);
+    }
+    // f of the bin in which they reach `target`, and of what comes before it
+    template <typename F>
+    __device__ inline void with(uint64_t target, F f) const
+    {
+        uint64_t was = before;
+#pragma unroll
+        for (int e = 0; e < B; ++e) {
+            if (was < target && was + v[e] >= target) f(uint32_t(B * int(threadIdx.x) + e), was, v[e]);
+            was += v[e];
         }
-    });
-}
+    }
+    // f of what comes before bin b
+    template <typename F>
+    __device__ inline void at(uint32_t b, F f) const
+    {
+        uint64_t was = before;
+#pragma unroll
+        for (int e = 0; e < B; ++e) {
+            if (uint32_t(B * int(threadIdx.x) + e) == b) f(was);
+            was += v[e];
+        }
+    }
+};
 
 // Lists the tokens up to the bin of the `want`-th and says how many, -1: more than a
-// list holds; `want` becomes the tokens' number, if that is less.  h.weight and
+// list holds; `want` becomes the tokens' number, if that is less.  h.count and
 // h.listed are 0.
-template <typename Src>
+template <int NT, typename Src>
 __device__ inline int list_first(const Row &r, int &want, Shared &h, Src &src)
 {
-    const int t = threadIdx.x;
-    src.template lay<false>(r, h);
+    src.template lay<false, true>(r, h);
     __syncthreads();
-    const uint64_t mine = uint32_t(h.weight[t]);
-    uint64_t before;
-    const int all = int(block_scan(mine, before, h.room));
-    want = min(want, all);
-    if (int(before) < want && int(before + mine) >= want) {
-        h.bin = uint32_t(t);
-        h.best[0] = before + mine;
-    }
+    Bins<NT, uint32_t> c;
+    c.read(h.count, h.room[1]);
+    want = min(want, int(c.all));
+    c.with(uint64_t(want), [&](uint32_t bin, uint64_t was, uint64_t v) {
+        h.bin = bin;
+        h.best[0] = was + v;
+    });
     __syncthreads();
-    const int last = int(h.bin), many = int(h.best[0]);
+    const int many = int(h.best[0]);
     if (many > kList) return -1;
-    collect(src, r, 0, uint32_t(last), h);
+    src.each(r, 0, h.bin, [&](float, uint64_t o) { enlist(h, o); });
     __syncthreads();
     return many;
 }
 
 // Draws from the first `want` of the `many` tokens listed.
+template <int NT>
 __device__ inline void draw_listed(const Sample &s, size_t row, Row r, int want, int many, Shared &h)
 {
     const int t = threadIdx.x;
@@ -546,7 +588,7 @@ __device__ inline void draw_listed(const Sample &s, size_t row, Row r, int want,
     __syncthreads();
     const uint64_t mine = t < want ? h.sums[t] : 0, w = t < want ? weight_of(r, logit_of(mine)) : 0;
     uint64_t before;
-    uint64_t sum = block_scan(w, before, h.room);
+    uint64_t sum = block_scan<NT>(w, before, h.room[2]);
     if (r.p < 1.0f) {
         uint64_t need = part_of(sum, fmaxf(r.p, 0.0f), true);
         need = need ? need : 1;
@@ -562,72 +604,130 @@ __device__ inline void draw_listed(const Sample &s, size_t row, Row r, int want,
     }
 }
 
-// The bin in which the weights up to it reach `target` and those before it, from the
-// weight of each thread's bin (a barrier).
-__device__ inline uint32_t bin_with(uint64_t target, uint64_t before, uint64_t mine, uint64_t &skip, Shared &h, int place)
+// A token's place in its bin, 0 .. kBins - 1 in the order.
+__device__ inline int part_of_bin(const Row &r, float l, uint32_t bin)
 {
-    if (before < target && before + mine >= target) {
-        h.best[place] = before;
-        h.in[place] = threadIdx.x;
-    }
-    __syncthreads();
-    skip = h.best[place];
-    return h.in[place];
+    const float x = l == r.top ? 0.0f : (r.top - l) * r.bins;
+    return int(fminf((x - float(bin)) * float(kBins), float(kBins - 1)));
 }
 
-// Of the tokens listed (`many`, of bins one after another, `skip` being the weights of
-// the bins before them) the one at which the weights reach `target` (barriers).
-__device__ inline Cut cut_at(uint64_t target, uint64_t skip, int many, const Row &r, Shared &h)
+// The token of bins from .. to of `src` at which the tokens (COUNT) or the weights reach
+// `target`; `skip` of them, and weights `skipw`, lie before the bins.  The bins' tokens
+// are listed, a thread each, and, where a bin has more than a few, sorted into finer
+// ones.  false: more than a list holds.
+template <int NT, bool COUNT, typename Src>
+__device__ inline bool cut_in(uint64_t target, uint32_t from, uint32_t to, uint64_t skip, uint64_t skipw, const Row &r,
+                              Shared &h, const Src &src, Cut &cut)
 {
     const int t = threadIdx.x;
+    constexpr int B = kBins / NT;
+    if (t == 0) h.listed = 0;
+    __syncthreads();
+    src.each(r, from, to, [&](float, uint64_t o) { enlist(h, o); });
+#pragma unroll
+    for (int e = 0; e < B; ++e) h.weight[B * t + e] = 0, h.count[B * t + e] = 0;
+    __syncthreads();
+    int many = int(h.listed);
+    if (many > kList) return false;
     uint64_t mine = 0, w = 0;
-    if (t < many) {
+    bool in = t < many;
+    if (in) {
         mine = h.list[t];
         w = weight_of(r, logit_of(mine));
-        h.sums[t] = w;
     }
-    __syncthreads();
-    if (t < many) {
-        uint64_t upto = skip;
-        for (int j = 0; j < many; ++j) upto += h.list[j] <= mine ? h.sums[j] : 0;
-        if (upto >= target && upto - w < target) {
+    if (many > kFew && from == to) {
+        const int part = in ? part_of_bin(r, logit_of(mine), from) : -1;
+        if (in) {
+            atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[part]), w);
+            if constexpr (COUNT) atomicAdd(&h.count[part], 1u);
+        }
+        if (t == 0) h.listed = 0;
+        __syncthreads();
+        Bins<NT, uint64_t> bw;
+        bw.read(h.weight, h.room[1]);
+        if constexpr (COUNT) {
+            Bins<NT, uint32_t> bc;
+            bc.read(h.count, h.room[2]);
+            bc.with(target - skip, [&](uint32_t b, uint64_t was, uint64_t) {
+                h.bin = b;
+                h.best[0] = skip + was;
+            });
+            __syncthreads();
+            bw.at(h.bin, [&](uint64_t was) { h.best[1] = skipw + was; });
+        } else {
+            bw.with(target - skip, [&](uint32_t b, uint64_t was, uint64_t) {
+                h.bin = b;
+                h.best[0] = h.best[1] = skip + was;
+            });
+        }
+        __syncthreads();
+        skip = h.best[0], skipw = h.best[1];
+        in = part == int(h.bin);
+        if (in) {
+            const uint32_t to_ = atomicAdd(&h.listed, 1u);
+            h.list[to_] = mine;
+            h.sums[to_] = w;
+        }
+        __syncthreads();
+        many = int(h.listed);
+    } else {
+        if (in) h.sums[t] = w;
+        __syncthreads();
+    }
+    if (in) {
+        uint64_t upto = 0, rank = 0;
+        for (int j = 0; j < many; ++j)
+            if (h.list[j] <= mine) upto += h.sums[j], ++rank;
+        const uint64_t now = skip + (COUNT ? rank : upto);
+        if (now >= target && now - (COUNT ? 1 : w) < target) {
             h.best[0] = mine;
-            h.best[1] = upto;
+            h.best[1] = skipw + upto;
             h.best[2] = w;
         }
     }
     __syncthreads();
-    const Cut cut{h.best[0], h.best[1], h.best[2]};
+    cut = Cut{h.best[0], h.best[1], h.best[2]};
     __syncthreads();
-    return cut;
+    return true;
 }
 
-// Draws from all tokens by their bins' weights in h.weight; false: a bin that matters
-// has more tokens than a list holds.
-__device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Shared &h, const Held &src)
+// Draws from all tokens by their bins' weights in h.weight (and, with a top-k, their
+// number in h.count); false: too many in a bin.
+template <int NT, typename Src>
+__device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Shared &h, const Src &src)
 {
-    const int t = threadIdx.x;
-    const uint64_t mine = h.weight[t];
-    uint64_t before, skip;
-    uint64_t sum = block_scan(mine, before, h.room);
-    uint32_t listed = kNoBin;
-    int many = 0;
+    Bins<NT, uint64_t> w;
+    w.read(h.weight, h.room[1]);
+    uint64_t sum = w.all;
     Cut cut{};
     auto find = [&](uint64_t target) {
-        const uint32_t bin = bin_with(target, before, mine, skip, h, 0);
-        if (bin != listed) {
-            __syncthreads();
-            if (t == 0) h.listed = 0;
-            __syncthreads();
-            collect(src, r, bin, bin, h);
-            __syncthreads();
-            listed = bin;
-            many = int(h.listed);
-        }
-        if (many > kList) return false;
-        cut = cut_at(target, skip, many, r, h);
-        return true;
+        w.with(target, [&](uint32_t b, uint64_t was, uint64_t) {
+            h.bin = b;
+            h.best[0] = was;
+        });
+        __syncthreads();
+        const uint32_t bin = h.bin;
+        const uint64_t skip = h.best[0];
+        return cut_in<NT, false>(target, bin, bin, skip, skip, r, h, src, cut);
     };
+    if (r.k > 0) {
+        Bins<NT, uint32_t> c;
+        c.read(h.count, h.room[2]);
+        if (uint64_t(r.k) < c.all) {
+            c.with(uint64_t(r.k), [&](uint32_t b, uint64_t was, uint64_t) {
+                h.bin = b;
+                h.best[0] = was;
+            });
+            __syncthreads();
+            const uint32_t bin = h.bin;
+            const uint64_t skip = h.best[0];
+            w.at(bin, [&](uint64_t was) { h.best[1] = was; });
+            __syncthreads();
+            const uint64_t skipw = h.best[1];
+            if (!cut_in<NT, true>(uint64_t(r.k), bin, bin, skip, skipw, r, h, src, cut)) return false;
+            sum = cut.upto;
+        }
+    }
     if (r.p < 1.0f) {
         const uint64_t need = part_of(sum, fmaxf(r.p, 0.0f), true);
         if (!find(need ? need : 1)) return false;
@@ -639,37 +739,71 @@ __device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Sh
     return true;
 }
 
-// Rows of one slice: a block a row.
-__global__ __launch_bounds__(kThreads) void sample_kernel(Sample s, size_t first)
+// Rows of one slice: a block a row.  SEARCH: what is unusual is searched here, at the
+// price of registers; else the row is marked for a launch after this one.
+template <int NT, bool SEARCH>
+__global__ __launch_bounds__(NT) void sample_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
     const size_t row = first + blockIdx.x;
     const int t = threadIdx.x;
-    Held v;
+    Held<NT> v;
     v.load(s.x + row * s.x_stride, 0, s.n);
     Row r = rules_of(s, row);
-    h.weight[t] = 0;
+    for (int b = t; b < kBins; b += NT) h.weight[b] = 0, h.count[b] = 0;
     if (t == 0) h.listed = 0;
     float top, low;
     v.range(top, low);
-    meet(top, low, h);
+    meet<NT>(top, low, h.room[0]);
     if (top == -INFINITY) return done(s, row, -1, 0.0);
     range_of(r, top, low);
-    if (r.greedy) return done(s, row, v.first(top, h.room), 1.0);
-    if (r.k > 0 && r.k <= kShort && top < INFINITY) {
-        int want = r.k;
-        const int many = list_first(r, want, h, v);
-        if (many >= 0) return draw_listed(s, row, r, want, many, h);
-    } else if (r.k <= 0 && top < INFINITY) {
-        r.scale = kMostScale;
-        v.lay<true>(r, h);
-        __syncthreads();
-        if (draw_binned(s, row, r, h, v)) return;
+    if (r.greedy) return done(s, row, v.first(top, h.room[1]), 1.0);
+    if (top < INFINITY) {
+        if (r.k > 0 && r.k <= kShort) {
+            int want = r.k;
+            const int many = list_first<NT>(r, want, h, v);
+            if (many >= 0) return draw_listed<NT>(s, row, r, want, many, h);
+        } else {
+            r.scale = kMostScale;
+            if (r.k > 0)
+                v.template lay<true, true>(r, h);
+            else
+                v.template lay<true, false>(r, h);
+            __syncthreads();
+            if (draw_binned<NT>(s, row, r, h, v)) return;
+        }
     }
-    search(s, row, r, h);
+    if constexpr (SEARCH) {
+        __syncthreads();
+        search<NT>(s, row, r, h);
+    } else if (t == 0) {
+        s.next[row] = kMarked;
+    }
+}
+
+// The rows marked.
+__global__ __launch_bounds__(512) void search_kernel(Sample s, size_t first)
+{
+    __shared__ Shared h;
+    const size_t row = first + blockIdx.x;
+    if (s.next[row] != kMarked) return;
+    const float *x = s.x + row * s.x_stride;
+    Row r = rules_of(s, row);
+    float top = -INFINITY, low = INFINITY;
+    for (int i = threadIdx.x; i < s.n; i += 512) {
+        const float l = x[i];
+        top = l > top ? l : top;
+        low = l > -INFINITY ? fminf(low, l) : low;
+    }
+    meet<512>(top, low, h.room[0]);
+    range_of(r, top, low);
+    search<512>(s, row, r, h);
 }
 
 // ---- rows of several slices -------------------------------------------------------
+
+constexpr int kThreads = 512;  // of a slice's block
+constexpr int kDraw = 1024;    // of a row's
 
 enum Way { kSearch, kListed, kBinned };
 __device__ inline Way way_of(const Row &r)
@@ -677,22 +811,29 @@ __device__ inline Way way_of(const Row &r)
     return r.top == INFINITY ? kSearch : r.k <= 0 ? kBinned : r.k <= kShort ? kListed : kSearch;
 }
 
-// A row's largest and lowest logit and the bound on its weights, from its parts.
-__device__ inline float join_parts(const Sample &s, size_t row, Row &r, Shared &h)
+// A row's largest and lowest logit from its parts (a barrier).
+template <int NT>
+__device__ inline void join_parts(const Sample &s, size_t row, Row &r, uint64_t *room)
 {
     const Part *part = s.part + row * s.slices;
     float top = -INFINITY, low = INFINITY;
-    for (int i = threadIdx.x; i < s.slices; i += kThreads) {
+    for (int i = threadIdx.x; i < s.slices; i += NT) {
         top = fmaxf(top, part[i].top);
         low = fminf(low, part[i].low);
     }
-    meet(top, low, h);
+    meet<NT>(top, low, room);
     range_of(r, top, low);
-    if (top == -INFINITY || top == INFINITY) return 1.0f;
+}
+
+// And the unit, by the bound on its weights (a barrier).
+template <int NT>
+__device__ inline void join_scale(const Sample &s, size_t row, Row &r, uint64_t *room)
+{
+    const Part *part = s.part + row * s.slices;
     float b = 0.0f;
-    for (int i = threadIdx.x; i < s.slices; i += kThreads)
+    for (int i = threadIdx.x; i < s.slices; i += NT)
         if (part[i].top > -INFINITY) b += part[i].sum * bound_of(r, part[i].top);
-    return sum_over(b, h.room);
+    r.scale = scale_of(sum_over<NT>(b, room));
 }
 
 // A slice's part and its own short top-k.
@@ -701,29 +842,31 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Sample s, size_t first)
     __shared__ Shared h;
     const size_t row = first + blockIdx.x / unsigned(s.slices);
     const int slice = int(blockIdx.x % unsigned(s.slices)), t = threadIdx.x;
-    Held v;
+    Held<kThreads> v;
     v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
     Row r = rules_of(s, row);
-    h.weight[t] = 0;
+    for (int b = t; b < kBins; b += kThreads) {
+        h.count[b] = 0;
+        if (slice == 0) s.bins[row * kBins + b] = 0;
+    }
     if (t == 0) h.listed = 0;
     float top, low;
     v.range(top, low);
-    meet(top, low, h);
+    meet<kThreads>(top, low, h.room[0]);
     range_of(r, top, low);
-    if (slice == 0) s.bins[row * kBins + t] = 0;
     Part p{top, low, 0.0f, 0};
     if (top > -INFINITY) {
         if (r.greedy) {
-            p.listed = v.first(top, h.room);
+            p.listed = v.first(top, h.room[1]);
         } else if (way_of(r) == kListed) {
             int want = r.k;
-            p.listed = list_first(r, want, h, v);
+            p.listed = list_first<kThreads>(r, want, h, v);
             if (t < p.listed) s.list[(row * s.slices + slice) * kList + t] = h.list[t];
         } else if (way_of(r) == kBinned) {
             float b = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) b += bound_of(r, v.v[j]);
-            p.sum = sum_over(b, h.room);
+            for (int j = 0; j < v.kPer; ++j) b += bound_of(r, v.v[j]);
+            p.sum = sum_over<kThreads>(b, h.room[1]);
         }
     }
     if (t == 0) s.part[row * s.slices + slice] = p;
@@ -737,48 +880,61 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Sample s, size_t first)
     const int slice = int(blockIdx.x % unsigned(s.slices)), t = threadIdx.x;
     Row r = rules_of(s, row);
     if (r.greedy || r.k > 0) return;
-    Held v;
+    Held<kThreads> v;
     v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
-    h.weight[t] = 0;
+    for (int b = t; b < kBins; b += kThreads) h.weight[b] = 0;
     float top, low;
     v.range(top, low);
-    const float bound = join_parts(s, row, r, h);
+    join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
-    r.scale = scale_of(bound);
-    v.lay<true>(r, h);
+    join_scale<kThreads>(s, row, r, h.room[1]);
+    v.template lay<true, false>(r, h);
     __syncthreads();
-    if (const uint64_t w = h.weight[t])
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[row * kBins + t]), w);
+    for (int b = t; b < kBins; b += kThreads)
+        if (const uint64_t w = h.weight[b])
+            atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[row * kBins + b]), w);
 }
 
 // Which bins of a row matter: the one where the weights come to top_p (`last`), and
 // those where the draw may be, whatever token of `last` the run ends at (from .. to).
-struct Bins {
+struct Matter {
     uint32_t from, to, last;
     uint64_t skip, skip_last, sum;  // weights before `from`, before `last`, of all
 };
 
-__device__ inline Bins bins_of(const Sample &s, size_t row, const Row &r, Shared &h)
+template <int NT>
+__device__ inline Matter matter_of(const Sample &s, size_t row, const Row &r, Shared &h)
 {
-    const uint64_t mine = s.bins[row * kBins + threadIdx.x];
-    Bins b{};
-    uint64_t before, most, least, no;
-    b.sum = block_scan(mine, before, h.room);
-    most = least = b.sum;
-    b.last = kBins;
+    Bins<NT, uint64_t> w;
+    w.read(s.bins + row * kBins, h.room[2]);
+    Matter m{};
+    m.sum = w.all;
+    m.last = kNoBin - 1;
+    uint64_t least = w.all, most = w.all;
     if (r.p < 1.0f) {
-        const uint64_t need = part_of(b.sum, fmaxf(r.p, 0.0f), true);
-        b.last = bin_with(need ? need : 1, before, mine, b.skip_last, h, 0);
-        if (threadIdx.x == b.last) h.sums[0] = before + mine;
+        const uint64_t need = part_of(w.all, fmaxf(r.p, 0.0f), true);
+        w.with(need ? need : 1, [&](uint32_t b, uint64_t was, uint64_t v) {
+            h.bin = b;
+            h.best[0] = was;
+            h.best[1] = was + v;
+        });
         __syncthreads();
-        least = b.skip_last + 1;
-        most = h.sums[0];
+        m.last = h.bin;
+        m.skip_last = h.best[0];
+        least = m.skip_last + 1;
+        most = h.best[1];
     }
     const uint64_t a = part_of(least, r.u, false) + 1, z = part_of(most, r.u, false) + 1;
-    b.from = bin_with(a < least ? a : least, before, mine, b.skip, h, 1);
-    b.to = bin_with(z < most ? z : most, before, mine, no, h, 2);
+    w.with(a < least ? a : least, [&](uint32_t b, uint64_t was, uint64_t) {
+        h.sums[0] = b;
+        h.sums[1] = was;
+    });
+    w.with(z < most ? z : most, [&](uint32_t b, uint64_t, uint64_t) { h.sums[2] = b; });
     __syncthreads();
-    return b;
+    m.from = uint32_t(h.sums[0]);
+    m.skip = h.sums[1];
+    m.to = uint32_t(h.sums[2]);
+    return m;
 }
 
 // The tokens of those bins.
@@ -789,21 +945,18 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
     const int slice = int(blockIdx.x % unsigned(s.slices)), t = threadIdx.x;
     Row r = rules_of(s, row);
     if (r.greedy || r.k > 0) return;
-    Held v;
+    Held<kThreads> v;
     v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
     if (t == 0) h.listed = 0;
     float top, low;
     v.range(top, low);
-    join_parts(s, row, r, h);
+    join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
-    const Bins b = bins_of(s, row, r, h);
+    const Matter m = matter_of<kThreads>(s, row, r, h);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < v.kPer; ++j) {
         const uint32_t bin = token(r, v.v[j]) ? uint32_t(bin_of(r, v.v[j])) : kNoBin;
-        if (bin == b.last || bin - b.from <= b.to - b.from) {
-            const uint32_t at = atomicAdd(&h.listed, 1u);
-            if (at < uint32_t(kList)) h.list[at] = order_of(v.v[j], v.at(j));
-        }
+        if (bin == m.last || bin - m.from <= m.to - m.from) enlist(h, order_of(v.v[j], v.at(j)));
     }
     __syncthreads();
     const int many = int(h.listed);
@@ -811,15 +964,15 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
     if (t == 0) s.part[row * s.slices + slice].listed = many <= kList ? many : -1;
 }
 
-__global__ __launch_bounds__(kThreads) void draw_kernel(Sample s, size_t first)
+__global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
     const size_t row = first + blockIdx.x;
     const int t = threadIdx.x;
     Row r = rules_of(s, row);
-    h.weight[t] = 0;
+    h.count[t] = 0;
     if (t == 0) h.listed = 0;
-    const float bound = join_parts(s, row, r, h);
+    join_parts<kDraw>(s, row, r, h.room[0]);
     if (r.top == -INFINITY) return done(s, row, -1, 0.0);
     const Part *part = s.part + row * s.slices;
     if (r.greedy) {
@@ -830,42 +983,32 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Sample s, size_t first)
         }
         return;
     }
-    Lists lists{s.list + row * s.slices * kList, part, s.slices};
+    const Lists<kDraw> lists{s.list + row * s.slices * kList, part, s.slices};
     int few = 1;
-    for (int i = t; i < s.slices; i += kThreads) few &= part[i].listed >= 0;
+    for (int i = t; i < s.slices; i += kDraw) few &= part[i].listed >= 0;
     if (__syncthreads_and(few)) {
         if (way_of(r) == kListed) {
             int want = r.k;
-            const int many = list_first(r, want, h, lists);
-            if (many >= 0) return draw_listed(s, row, r, want, many, h);
+            const int many = list_first<kDraw>(r, want, h, lists);
+            if (many >= 0) return draw_listed<kDraw>(s, row, r, want, many, h);
         } else if (way_of(r) == kBinned) {
-            r.scale = scale_of(bound);
-            const Bins b = bins_of(s, row, r, h);
-            // the tokens of one run of bins, then of the other
-            auto find = [&](uint64_t target, uint32_t from, uint32_t to, uint64_t skip, Cut &cut) {
-                if (t == 0) h.listed = 0;
-                __syncthreads();
-                collect(lists, r, from, to, h);
-                __syncthreads();
-                const int many = int(h.listed);
-                if (many > kList) return false;
-                cut = cut_at(target, skip, many, r, h);
-                return true;
-            };
+            join_scale<kDraw>(s, row, r, h.room[1]);
+            const Matter m = matter_of<kDraw>(s, row, r, h);
             Cut cut{};
-            uint64_t sum = b.sum;
+            uint64_t sum = m.sum;
             bool good = true;
             if (r.p < 1.0f) {
                 const uint64_t need = part_of(sum, fmaxf(r.p, 0.0f), true);
-                good = find(need ? need : 1, b.last, b.last, b.skip_last, cut);
+                good = cut_in<kDraw, false>(need ? need : 1, m.last, m.last, m.skip_last, m.skip_last, r, h, lists, cut);
                 sum = cut.upto;
             }
             const uint64_t target = part_of(sum, r.u, false) + 1;
-            if (good && find(target < sum ? target : sum, b.from, b.to, b.skip, cut))
+            if (good && cut_in<kDraw, false>(target < sum ? target : sum, m.from, m.to, m.skip, m.skip, r, h, lists, cut))
                 return done(s, row, int(cut.place & 0xffffff), double(cut.weight) / double(sum));
         }
     }
-    search(s, row, r, h);
+    __syncthreads();
+    search<kDraw>(s, row, r, h);
 }
 
 size_t slices_of(size_t n) { return (n + kSlice - 1) / kSlice; }
@@ -899,12 +1042,22 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         s.part = reinterpret_cast<Part *>(s.list + count * slices * kList);
     }
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
-    const size_t most = 0xffffffff / kThreads / slices;
+    const size_t most = 0xffffffff / kDraw / slices;
+    // few rows: as many threads a row as there are, and no launch more; many: rows in
+    // flight (1024 rows of 8192 in 512 and 1024 threads %%)
+    const bool few = count <= size_t(ctx->num_cus > 0 ? ctx->num_cus : 256);
     for (size_t first = 0; first < count; first += most) {
         const unsigned rows = unsigned(std::min(most, count - first)), blocks = rows * unsigned(slices);
         if (slices == 1) {
-            hipLaunchKernelGGL(sample_kernel, dim3(rows), dim3(kThreads), 0, ctx->stream, s, first);
-            if (int rc = nd::check_launch("sample_rows")) return rc;
+            if (few) {
+                hipLaunchKernelGGL((sample_kernel<1024, true>), dim3(rows), dim3(1024), 0, ctx->stream, s, first);
+                if (int rc = nd::check_launch("sample_rows")) return rc;
+            } else {
+                hipLaunchKernelGGL((sample_kernel<512, false>), dim3(rows), dim3(512), 0, ctx->stream, s, first);
+                if (int rc = nd::check_launch("sample_rows")) return rc;
+                hipLaunchKernelGGL(search_kernel, dim3(rows), dim3(512), 0, ctx->stream, s, first);
+                if (int rc = nd::check_launch("sample_search")) return rc;
+            }
             continue;
         }
         hipLaunchKernelGGL(slice_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
@@ -914,7 +1067,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         if (int rc = nd::check_launch("sample_bins")) return rc;
         hipLaunchKernelGGL(gather_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_gather")) return rc;
-        hipLaunchKernelGGL(draw_kernel, dim3(rows), dim3(kThreads), 0, ctx->stream, s, first);
+        hipLaunchKernelGGL(draw_kernel, dim3(rows), dim3(kDraw), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_draw")) return rc;
     }
     return ND_OK;
