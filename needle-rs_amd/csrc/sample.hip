@@ -52,6 +52,7 @@ struct Sample {
     int32_t *next;
     float *prob;
     int slices;       // of a row; more than one:
+    int blocks;       // a row's, that share the slices in the second and third launch
     Part *part;       // [rows][slices]
     uint64_t *bins;   // [rows][kBins]
     uint64_t *list;   // [rows][slices][kList]
@@ -418,13 +419,18 @@ struct Held {
             }
         }
     }
-    // the largest and the lowest token's
+    __device__ inline void clean()
+    {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] = v[j] > -INFINITY ? v[j] : -INFINITY;
+    }
+    // (cleaned) the largest and the lowest token's
     __device__ inline void range(float &top, float &low)
     {
+        clean();
         top = -INFINITY, low = INFINITY;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            v[j] = v[j] > -INFINITY ? v[j] : -INFINITY;
             top = fmaxf(top, v[j]);
             low = fminf(low, v[j] > -INFINITY ? v[j] : INFINITY);
         }
@@ -611,36 +617,39 @@ __device__ inline int part_of_bin(const Row &r, float l, uint32_t bin)
     return int(fminf((x - float(bin)) * float(kBins), float(kBins - 1)));
 }
 
-// The token of bins from .. to of `src` at which the tokens (COUNT) or the weights reach
-// `target`; `skip` of them, and weights `skipw`, lie before the bins.  The bins' tokens
-// are listed, a thread each, and, where a bin has more than a few, sorted into finer
-// ones.  false: more than a list holds.
+// The token of a bin of `src` at which the tokens (COUNT) or the weights reach `target`;
+// `skip` of them, and weights `skipw`, lie before the bin.  The bin's tokens are
+// listed, a thread each, and, where they are more than a few, sorted into finer
+// ones (gone through once more for that, if they are more than a list holds).  false:
+// too many all the same.
 template <int NT, bool COUNT, typename Src>
-__device__ inline bool cut_in(uint64_t target, uint32_t from, uint32_t to, uint64_t skip, uint64_t skipw, const Row &r,
+__device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint64_t skipw, const Row &r,
                               Shared &h, const Src &src, Cut &cut)
 {
     const int t = threadIdx.x;
     constexpr int B = kBins / NT;
     if (t == 0) h.listed = 0;
     __syncthreads();
-    src.each(r, from, to, [&](float, uint64_t o) { enlist(h, o); });
+    src.each(r, bin, bin, [&](float, uint64_t o) { enlist(h, o); });
 #pragma unroll
     for (int e = 0; e < B; ++e) h.weight[B * t + e] = 0, h.count[B * t + e] = 0;
     __syncthreads();
     int many = int(h.listed);
-    if (many > kList) return false;
+    const bool all = many <= kList;  // are listed
     uint64_t mine = 0, w = 0;
-    bool in = t < many;
+    bool in = all && t < many;
     if (in) {
         mine = h.list[t];
         w = weight_of(r, logit_of(mine));
     }
-    if (many > kFew && from == to) {
-        const int part = in ? part_of_bin(r, logit_of(mine), from) : -1;
-        if (in) {
-            atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[part]), w);
-            if constexpr (COUNT) atomicAdd(&h.count[part], 1u);
-        }
+    if (many > kFew) {
+        auto lay = [&](int b, uint64_t v) {
+            atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[b]), v);
+            if constexpr (COUNT) atomicAdd(&h.count[b], 1u);
+        };
+        const int part = in ? part_of_bin(r, logit_of(mine), bin) : -1;
+        if (in) lay(part, w);
+        if (!all) src.each(r, bin, bin, [&](float l, uint64_t) { lay(part_of_bin(r, l, bin), weight_of(r, l)); });
         if (t == 0) h.listed = 0;
         __syncthreads();
         Bins<NT, uint64_t> bw;
@@ -662,18 +671,23 @@ __device__ inline bool cut_in(uint64_t target, uint32_t from, uint32_t to, uint6
         }
         __syncthreads();
         skip = h.best[0], skipw = h.best[1];
-        in = part == int(h.bin);
-        if (in) {
-            const uint32_t to_ = atomicAdd(&h.listed, 1u);
-            h.list[to_] = mine;
-            h.sums[to_] = w;
-        }
+        const int fine = int(h.bin);
+        if (in && part == fine) enlist(h, mine);
+        if (!all)
+            src.each(r, bin, bin, [&](float l, uint64_t o) {
+                if (part_of_bin(r, l, bin) == fine) enlist(h, o);
+            });
         __syncthreads();
         many = int(h.listed);
-    } else {
-        if (in) h.sums[t] = w;
-        __syncthreads();
+        in = t < many;
+        if (in && many <= kList) {
+            mine = h.list[t];
+            w = weight_of(r, logit_of(mine));
+        }
     }
+    if (many > kList) return false;
+    if (in) h.sums[t] = w;
+    __syncthreads();
     if (in) {
         uint64_t upto = 0, rank = 0;
         for (int j = 0; j < many; ++j)
@@ -708,7 +722,7 @@ __device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Sh
         __syncthreads();
         const uint32_t bin = h.bin;
         const uint64_t skip = h.best[0];
-        return cut_in<NT, false>(target, bin, bin, skip, skip, r, h, src, cut);
+        return cut_in<NT, false>(target, bin, skip, skip, r, h, src, cut);
     };
     if (r.k > 0) {
         Bins<NT, uint32_t> c;
@@ -724,7 +738,7 @@ __device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Sh
             w.at(bin, [&](uint64_t was) { h.best[1] = was; });
             __syncthreads();
             const uint64_t skipw = h.best[1];
-            if (!cut_in<NT, true>(uint64_t(r.k), bin, bin, skip, skipw, r, h, src, cut)) return false;
+            if (!cut_in<NT, true>(uint64_t(r.k), bin, skip, skipw, r, h, src, cut)) return false;
             sum = cut.upto;
         }
     }
@@ -872,23 +886,27 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Sample s, size_t first)
     if (t == 0) s.part[row * s.slices + slice] = p;
 }
 
-// The weights of the slices of rows without a top-k in their rows' bins.
+// The weights of rows without a top-k in their rows' bins.
 __global__ __launch_bounds__(kThreads) void bins_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
-    const size_t row = first + blockIdx.x / unsigned(s.slices);
-    const int slice = int(blockIdx.x % unsigned(s.slices)), t = threadIdx.x;
+    const size_t row = first + blockIdx.x / unsigned(s.blocks);
+    const int block = int(blockIdx.x % unsigned(s.blocks)), t = threadIdx.x;
     Row r = rules_of(s, row);
     if (r.greedy || r.k > 0) return;
     Held<kThreads> v;
-    v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
+    v.load(s.x + row * s.x_stride, block * kSlice, s.n);
     for (int b = t; b < kBins; b += kThreads) h.weight[b] = 0;
-    float top, low;
-    v.range(top, low);
     join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
     join_scale<kThreads>(s, row, r, h.room[1]);
-    v.template lay<true, false>(r, h);
+    for (int slice = block;;) {
+        v.clean();
+        v.template lay<true, false>(r, h);
+        slice += s.blocks;
+        if (slice >= s.slices) break;
+        v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
+    }
     __syncthreads();
     for (int b = t; b < kBins; b += kThreads)
         if (const uint64_t w = h.weight[b])
@@ -899,7 +917,6 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Sample s, size_t first)
 // those where the draw may be, whatever token of `last` the run ends at (from .. to).
 struct Matter {
     uint32_t from, to, last;
-    uint64_t skip, skip_last, sum;  // weights before `from`, before `last`, of all
 };
 
 template <int NT>
@@ -907,61 +924,60 @@ __device__ inline Matter matter_of(const Sample &s, size_t row, const Row &r, Sh
 {
     Bins<NT, uint64_t> w;
     w.read(s.bins + row * kBins, h.room[2]);
-    Matter m{};
-    m.sum = w.all;
-    m.last = kNoBin - 1;
+    Matter m{0, 0, kNoBin - 1};
     uint64_t least = w.all, most = w.all;
     if (r.p < 1.0f) {
         const uint64_t need = part_of(w.all, fmaxf(r.p, 0.0f), true);
         w.with(need ? need : 1, [&](uint32_t b, uint64_t was, uint64_t v) {
             h.bin = b;
-            h.best[0] = was;
+            h.best[0] = was + 1;
             h.best[1] = was + v;
         });
         __syncthreads();
         m.last = h.bin;
-        m.skip_last = h.best[0];
-        least = m.skip_last + 1;
+        least = h.best[0];
         most = h.best[1];
     }
     const uint64_t a = part_of(least, r.u, false) + 1, z = part_of(most, r.u, false) + 1;
-    w.with(a < least ? a : least, [&](uint32_t b, uint64_t was, uint64_t) {
-        h.sums[0] = b;
-        h.sums[1] = was;
-    });
-    w.with(z < most ? z : most, [&](uint32_t b, uint64_t, uint64_t) { h.sums[2] = b; });
+    w.with(a < least ? a : least, [&](uint32_t b, uint64_t, uint64_t) { h.sums[0] = b; });
+    w.with(z < most ? z : most, [&](uint32_t b, uint64_t, uint64_t) { h.sums[1] = b; });
     __syncthreads();
     m.from = uint32_t(h.sums[0]);
-    m.skip = h.sums[1];
-    m.to = uint32_t(h.sums[2]);
+    m.to = uint32_t(h.sums[1]);
     return m;
 }
 
-// The tokens of those bins.
+// The tokens of those bins, slice by slice.
 __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
-    const size_t row = first + blockIdx.x / unsigned(s.slices);
-    const int slice = int(blockIdx.x % unsigned(s.slices)), t = threadIdx.x;
+    const size_t row = first + blockIdx.x / unsigned(s.blocks);
+    const int block = int(blockIdx.x % unsigned(s.blocks)), t = threadIdx.x;
     Row r = rules_of(s, row);
     if (r.greedy || r.k > 0) return;
     Held<kThreads> v;
-    v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
-    if (t == 0) h.listed = 0;
-    float top, low;
-    v.range(top, low);
+    v.load(s.x + row * s.x_stride, block * kSlice, s.n);
     join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
     const Matter m = matter_of<kThreads>(s, row, r, h);
+    for (int slice = block;;) {
+        if (t == 0) h.listed = 0;
+        __syncthreads();
+        v.clean();
 #pragma unroll
-    for (int j = 0; j < v.kPer; ++j) {
-        const uint32_t bin = token(r, v.v[j]) ? uint32_t(bin_of(r, v.v[j])) : kNoBin;
-        if (bin == m.last || bin - m.from <= m.to - m.from) enlist(h, order_of(v.v[j], v.at(j)));
+        for (int j = 0; j < v.kPer; ++j) {
+            const uint32_t bin = uint32_t(bin_of(r, v.v[j]));
+            if ((bin == m.last || bin - m.from <= m.to - m.from) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)));
+        }
+        __syncthreads();
+        const int many = int(h.listed);
+        if (t < many && many <= kList) s.list[(row * s.slices + slice) * kList + t] = h.list[t];
+        if (t == 0) s.part[row * s.slices + slice].listed = many <= kList ? many : -1;
+        slice += s.blocks;
+        if (slice >= s.slices) break;
+        v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
+        __syncthreads();
     }
-    __syncthreads();
-    const int many = int(h.listed);
-    if (t < many && many <= kList) s.list[(row * s.slices + slice) * kList + t] = h.list[t];
-    if (t == 0) s.part[row * s.slices + slice].listed = many <= kList ? many : -1;
 }
 
 __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
@@ -992,19 +1008,10 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
             const int many = list_first<kDraw>(r, want, h, lists);
             if (many >= 0) return draw_listed<kDraw>(s, row, r, want, many, h);
         } else if (way_of(r) == kBinned) {
-            join_scale<kDraw>(s, row, r, h.room[1]);
-            const Matter m = matter_of<kDraw>(s, row, r, h);
-            Cut cut{};
-            uint64_t sum = m.sum;
-            bool good = true;
-            if (r.p < 1.0f) {
-                const uint64_t need = part_of(sum, fmaxf(r.p, 0.0f), true);
-                good = cut_in<kDraw, false>(need ? need : 1, m.last, m.last, m.skip_last, m.skip_last, r, h, lists, cut);
-                sum = cut.upto;
-            }
-            const uint64_t target = part_of(sum, r.u, false) + 1;
-            if (good && cut_in<kDraw, false>(target < sum ? target : sum, m.from, m.to, m.skip, m.skip, r, h, lists, cut))
-                return done(s, row, int(cut.place & 0xffffff), double(cut.weight) / double(sum));
+            join_scale<kDraw>(s, row, r, h.room[2]);
+            h.weight[t] = s.bins[row * kBins + t];
+            __syncthreads();
+            if (draw_binned<kDraw>(s, row, r, h, lists)) return;
         }
     }
     __syncthreads();
@@ -1033,7 +1040,9 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
     ND_REQUIRE(count == 1 || x_stride >= n, "row stride %zu below n %zu", x_stride, n);
     const nd_sampling none{}, &r = sampling ? *sampling : none;
     const size_t slices = slices_of(n);
-    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices)};
+    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices), 0};
+    // (a row's blocks, of about four a CU; each finds out what matters for itself)
+    s.blocks = int(std::min(slices, std::max<size_t>(1, 1024 / count)));
     if (slices > 1) {
         void *ws = nullptr;
         if (int rc = nd::call_workspace(ctx, count * row_bytes(slices), work, work_bytes, &ws)) return rc;
@@ -1044,7 +1053,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
     const size_t most = 0xffffffff / kDraw / slices;
     // few rows: as many threads a row as there are, and no launch more; many: rows in
-    // flight (1024 rows of 8192 in 512 and 1024 threads %%)
+    // flight
     const bool few = count <= size_t(ctx->num_cus > 0 ? ctx->num_cus : 256);
     for (size_t first = 0; first < count; first += most) {
         const unsigned rows = unsigned(std::min(most, count - first)), blocks = rows * unsigned(slices);
@@ -1063,9 +1072,9 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         hipLaunchKernelGGL(slice_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_slices")) return rc;
         // (only rows without a top-k have anything to do here, which the host does not see)
-        hipLaunchKernelGGL(bins_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
+        hipLaunchKernelGGL(bins_kernel, dim3(rows * unsigned(s.blocks)), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_bins")) return rc;
-        hipLaunchKernelGGL(gather_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
+        hipLaunchKernelGGL(gather_kernel, dim3(rows * unsigned(s.blocks)), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_gather")) return rc;
         hipLaunchKernelGGL(draw_kernel, dim3(rows), dim3(kDraw), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_draw")) return rc;
