@@ -513,9 +513,10 @@ typedef struct nd_sampling {
  * sum; so u = 0 draws the first maximum.  -1 where a row has no token.
  * prob[i] (may be NULL) = the chance that token had, 1 for a greedy row, 0 for
  * none.  u is taken as 0 below 0 or as a NaN, as the last token's at 1 and
- * above.  Weights are fp64 exponentials as whole numbers of a unit of which
- * the row's sum has 2^60 or more, so sums are exact and a pick is the border's;
- * tokens of less than half a unit are never drawn.  sampling may be NULL.  n <= 2^24, count < 2^31.  `work` as for nd_attend_tree_i8, of
+ * above.  Weights are fp64 exponentials as whole numbers of 2^-49 of the
+ * largest (or of 2^-61 of the row's sum, where that is more), so sums are
+ * exact and a pick is the border's; tokens of less than half of that are never
+ * drawn.  sampling may be NULL.  n <= 2^24, count < 2^31.  `work` as for nd_attend_tree_i8, of
  * nd_sample_rows_work(..) bytes.  The reference's generate takes a
  * temperature alone (needle-c/src/v3.rs:219-250). */
 size_t nd_sample_rows_work(nd_ctx *ctx, size_t count, size_t n);
@@ -692,6 +693,16 @@ int nd_v3_prefill(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32
  * with stop tokens truncates each row at its first one. */
 int nd_v3_generate(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32_t *first,
                    size_t steps, int32_t *tokens);
+
+/* nd_v3_generate with each step's token drawn instead of picked: session i's
+ * in step k by u[k * sessions + i] (device, [steps][sessions]) from the step's
+ * logits under `sampling` (its device arrays have a number a session; NULL:
+ * none), as nd_sample_rows draws it.  The reference's loop with a temperature
+ * (needle-infer/src/v3_engine.rs:254-312), whose random numbers are its own:
+ * a temperature of 0 for every session gives nd_v3_generate's tokens. */
+int nd_v3_generate_sampled(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32_t *first,
+                           size_t steps, const nd_sampling *sampling, const float *u,
+                           int32_t *tokens);
 
 /* nd_v3_generate for n (1..8) batches of one model at once, from one host
  * thread: batch i on context ctxs[i] (its own stream), from first[i], into

@@ -2727,6 +2727,9 @@ struct StepRun {
     // tokens == nullptr: this step's tokens are b->next on the device (the
     // previous step's choices); the greedy choices are also written here
     int32_t *argmax_also = nullptr;
+    // the step's choice is drawn by these rules and numbers (nd_v3_generate_sampled)
+    const nd_sampling *sampling = nullptr;
+    const float *draws = nullptr;
 
     int begin(const int32_t *tokens);
     int enqueue(int phase, bool argmax);
@@ -3171,7 +3174,11 @@ int StepRun::enqueue(int phase, bool argmax)
                        m->final_norm, b->xh, nl, d, m->pre_x, C);
     LCHK("k_final");
     CK(project(ctx, m->embedding, b->xh, S, 0, rows, b->logits));
-    if (argmax) {
+    if (argmax && draws) {
+        CK(nd_sample_rows(ctx, b->logits, rows, size_t(S), rows, sampling, draws, b->next, nullptr,
+                          nullptr, 0));
+        ND_HIP(hipMemcpyAsync(argmax_also, b->next, size_t(S) * 4, hipMemcpyDeviceToDevice, st));
+    } else if (argmax) {
         hipLaunchKernelGGL(k_argmax, dim3(S), dim3(kT), 0, st, b->logits, int(rows), b->next,
                            argmax_also);
         LCHK("k_argmax");
@@ -3327,11 +3334,14 @@ int gen_begin(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32_t *
 
 // Step k of the loop: enqueued, nothing waited for (the host runs ahead of
 // the device up to the staging ring's depth).
-int gen_step(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, size_t k)
+int gen_step(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, size_t k,
+             const nd_sampling *sampling = nullptr, const float *u = nullptr)
 {
     const int S = b->B;
     StepRun r{ctx, m, b, 1};
     r.argmax_also = b->gen_out + k * S;
+    r.sampling = sampling;
+    r.draws = u ? u + k * S : nullptr;
     int rc = r.begin(nullptr);
     for (int ph = -1; ph <= r.L && rc == ND_OK; ++ph) rc = r.enqueue(ph, true);
     if (rc == ND_OK)
@@ -3378,6 +3388,21 @@ int nd_v3_generate(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int3
     if (int rc = gen_begin(ctx, m, b, first, steps)) return rc;
     for (size_t k = 0; k < steps; ++k)
         if (int rc = gen_step(ctx, m, b, k)) return rc;
+    return gen_end(ctx, m, b, first, steps, tokens);
+}
+
+int nd_v3_generate_sampled(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32_t *first,
+                           size_t steps, const nd_sampling *sampling, const float *u,
+                           int32_t *tokens)
+{
+    ND_ENTER(ctx);
+    ND_REQUIRE(m && b && first && tokens && (u || steps == 0), "null argument");
+    nd::Hold hold(b->owner, "the batch");
+    if (hold.rc) return hold.rc;
+    if (steps == 0) return ND_OK;
+    if (int rc = gen_begin(ctx, m, b, first, steps)) return rc;
+    for (size_t k = 0; k < steps; ++k)
+        if (int rc = gen_step(ctx, m, b, k, sampling, u)) return rc;
     return gen_end(ctx, m, b, first, steps, tokens);
 }
 

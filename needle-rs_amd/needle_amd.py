@@ -11,6 +11,7 @@ GPU raises.  torch supplies device memory and the stream only.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import os
 import re
@@ -115,6 +116,7 @@ _SIGS = [
     ("nd_v3_batch_create_chunked", C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, C.POINTER(_vp)]),
     ("nd_v3_prefill", C.c_int, [_vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     ("nd_v3_generate", C.c_int, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    ("nd_v3_generate_sampled", C.c_int, [_vp, _vp, _vp, _vp, _sz, C.POINTER(Sampling), _vp, _vp]),
     ("nd_v3_generate_many", C.c_int, [_vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     ("nd_v3_cact_config", C.c_int, [_vp, _sz, _vp, C.POINTER(_sz)]),
     ("nd_v3_model_from_cact", C.c_int, [_vp, _vp, _sz, C.POINTER(_vp)]),
@@ -893,6 +895,11 @@ def prefix_plan_bytes(g, sessions, rows, prefixes):
     return lib().nd_prefix_plan_bytes(C.byref(g), sessions, rows, prefixes)
 
 
+@functools.lru_cache(maxsize=256)
+def _plan_bytes(heads, kv_heads, sessions, rows, prefixes):
+    return lib().nd_prefix_plan_bytes(C.byref(KvGeom(heads, kv_heads, 16, 16, 1)), sessions, rows, prefixes)
+
+
 def prefix_plan(ctx, g, prefix_cap, prefix_len, used, prefix_of=None, length=None, rows=1, window=0, plan=None,
                 maps=None):
     """A step of `rows` rows a session laid out (nd_prefix_plan): prefix_len [P]
@@ -907,16 +914,20 @@ def prefix_plan(ctx, g, prefix_cap, prefix_len, used, prefix_of=None, length=Non
     torch = _torch()
     i32 = torch.int32
     s, p = used.numel(), prefix_len.numel() if prefix_len is not None else 0
-    nb = prefix_plan_bytes(g, s, rows, p)
     data = plan.data if isinstance(plan, PrefixPlan) else plan
     if data is None:
-        data = _empty(ctx, (max(nb, 1),), torch.uint8)
-    if maps is None:
-        maps = tuple(_empty(ctx, (s, rows), i32) for _ in range(4)) + (_empty(ctx, (s * rows,), i32),
-                                                                       _empty(ctx, (p + 1,), i32))
-    need = (s * rows,) * 5 + (p + 1,)
-    names = ("pos", "rot", "from", "lo", "order", "first")
-    m = PrefixMaps(*(_dev_arg(ctx, t, i32, f"maps: {n}", k) for t, n, k in zip(maps or (None,) * 6, names, need)))
+        data = _empty(ctx, (max(_plan_bytes(g.num_heads, g.num_kv_heads, s, rows, p), 1),), torch.uint8)
+    n = s * rows
+    if maps is None:  # parts of one tensor
+        ints = _empty(ctx, (5 * n + p + 1,), i32)
+        at = ints.data_ptr()
+        m = PrefixMaps(at, at + 4 * n, at + 8 * n, at + 12 * n, at + 16 * n, at + 20 * n)
+        maps = ints.as_strided((4, s, rows), (n, rows, 1)).unbind(0) + (ints.as_strided((n,), (1,), 4 * n),
+                                                                        ints.as_strided((p + 1,), (1,), 5 * n))
+    else:
+        names = ("pos", "rot", "from", "lo", "order", "first")
+        need = (n,) * 5 + (p + 1,)
+        m = PrefixMaps(*(_dev_arg(ctx, t, i32, f"maps: {w}", k) for t, w, k in zip(maps or (None,) * 6, names, need)))
     _check(lib().nd_prefix_plan(
         ctx.h, C.byref(g), prefix_cap, s, rows, p, _dev_arg(ctx, prefix_of, i32, "prefix_of", s),
         _dev_arg(ctx, prefix_len, i32, "prefix_len", p), _dev_arg(ctx, used, i32, "used"),
@@ -1224,6 +1235,26 @@ class V3Batch:
         _check(lib().nd_v3_generate(self.ctx.h, self.model.h, self.h,
                                     tok.ctypes.data_as(C.c_void_p), steps,
                                     out.ctypes.data_as(C.c_void_p)))
+        return out
+
+    def sampled(self, first, u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """A step for each row of u ([steps][sessions] fp32 on the device), from
+        first[i], each session's token drawn by its number under its own rules
+        ([sessions] device tensors, as for sample_rows): returns [sessions][steps]
+        (nd_v3_generate_sampled)."""
+        torch = _torch()
+        f32, n = torch.float32, self.sessions
+        tok = np.ascontiguousarray(first, np.int32).reshape(n)
+        if u.dim() != 2 or u.shape[1] != n:
+            raise ValueError(f"u: shape {tuple(u.shape)}, expected [steps][{n}]")
+        steps = u.shape[0]
+        out = np.zeros((n, steps), np.int32)
+        c = self.ctx
+        rules = Sampling(_dev_arg(c, temperature, f32, "temperature", n), _dev_arg(c, min_p, f32, "min_p", n),
+                         _dev_arg(c, top_k, torch.int32, "top_k", n), _dev_arg(c, top_p, f32, "top_p", n))
+        _check(lib().nd_v3_generate_sampled(c.h, self.model.h, self.h, tok.ctypes.data_as(C.c_void_p), steps,
+                                            C.byref(rules), _dev_arg(c, u, f32, "u", steps * n),
+                                            out.ctypes.data_as(C.c_void_p)))
         return out
 
     @staticmethod
