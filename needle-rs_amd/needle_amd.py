@@ -882,6 +882,16 @@ def logits_adjust_work(ctx, count, n):
 
 # ---- a batch that shares its prompts -------------------------------------------
 
+@functools.lru_cache(maxsize=256)
+def _head_scale(qk):
+    return float(np.float32(1.0) / np.sqrt(np.float32(qk)))
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes_of(heads, kv_heads, qk, vd, cap):
+    return kv_block_bytes(KvGeom(heads, kv_heads, qk, vd, cap))
+
+
 class PrefixPlan:
     """What prefix_plan leaves for attend_prefix_i8: the work list of a step's
     rows (`data`, a uint8 device tensor) and the sizes it was made for."""
@@ -949,31 +959,30 @@ def attend_prefix_i8(ctx, g, kv, kv_stride, prefix_kv, prefix_stride, plan, q, s
     tensor of attend_prefix_i8_work() bytes, needed while a graph is captured."""
     torch = _torch()
     f32, u8 = torch.float32, torch.uint8
-    s, n, p, cap = plan.sizes[:4]
+    s, n, p, cap, heads, kv_heads, own = plan.sizes
     if q.dim() != 3 or q.shape[:2] != (s, n):
         raise ValueError(f"q: shape {tuple(q.shape)}, expected [{s}][{n}][heads * qk]")
-    if plan.sizes[4:] != (g.num_heads, g.num_kv_heads, g.cap):
+    if (heads, kv_heads, own) != (g.num_heads, g.num_kv_heads, g.cap):
         raise ValueError("plan: made for another geometry")
-    wo = g.num_heads * g.v_head_dim
+    qk, vd = g.qk_head_dim, g.v_head_dim
     if scale is None:
-        scale = float(np.float32(1.0) / np.sqrt(np.float32(g.qk_head_dim)))
+        scale = _head_scale(qk)
     if out is None:
-        out = _empty(ctx, (s, n, wo), f32)
+        out = _empty(ctx, (s, n, heads * vd), f32)
         with torch.cuda.stream(ctx.stream):
             out.zero_()
-    blocks = kv_block_bytes(g) + (s - 1) * kv_stride if s else 0
+    blocks = _bytes_of(heads, kv_heads, qk, vd, own) + (s - 1) * kv_stride if s else 0
     many = 0
     if p:
-        many = kv_block_bytes(KvGeom(g.num_heads, g.num_kv_heads, g.qk_head_dim, g.v_head_dim, cap)) + \
-            (p - 1) * prefix_stride
+        many = _bytes_of(heads, kv_heads, qk, vd, cap) + (p - 1) * prefix_stride
         if prefix_kv is None:
             raise ValueError("prefix_kv: the plan has prefixes")
     wp, wb = _work_arg(ctx, work)
     _check(lib().nd_attend_prefix_i8(
         ctx.h, C.byref(g), _dev_arg(ctx, kv, u8, "kv", blocks), kv_stride, s, n,
         _dev_arg(ctx, prefix_kv, u8, "prefix_kv", many), prefix_stride, cap, p, _dev_arg(ctx, plan.data, u8, "plan"),
-        _dev_arg(ctx, q, f32, "q", s * n * g.num_heads * g.qk_head_dim), scale, int(bool(quant_query)),
-        _dev_arg(ctx, out, f32, "out", s * n * wo), wp, wb))
+        _dev_arg(ctx, q, f32, "q", s * n * heads * qk), scale, int(bool(quant_query)),
+        _dev_arg(ctx, out, f32, "out", s * n * heads * vd), wp, wb))
     return out
 
 
