@@ -380,7 +380,7 @@ struct Attend {
     size_t kv_stride, pkv_stride;
     const float *q;
     float *out, *part_o, *part_ml;  // sums of (slot, kv head, column), and their maximum and weight
-    Divisor by_rep, by_kvh;
+    Divisor by_rep;
     float scale2;  // |scale| log2(e); below 0 where scale is no number
     int negative;  // scale < 0
 };
@@ -912,12 +912,11 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
 // A block's four units: of four tiles of a prefix over the same chunks, together, or
 // each for itself.
 template <int QK, bool QQ>
-__global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at)
+__global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at, uint32_t first)
 {
     __shared__ __align__(16) Shared sh_s;
     const uint32_t w = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
-    const uint32_t block = at.by_kvh.quotient(blockIdx.x), kvh = blockIdx.x - block * uint32_t(gown.KVH);
-    const uint32_t unit = 4 * block + w;
+    const uint32_t unit = 4 * (first + blockIdx.y) + w, kvh = blockIdx.x;
     // (both asked for at once: the list has as many places as the grid waves)
     const Head hd = *at.plan.head();
     const Unit un = at.plan.unit()[unit];
@@ -1099,7 +1098,6 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     a.q = q;
     a.out = out;
     a.by_rep = Divisor::of(uint32_t(g->num_heads / g->num_kv_heads));
-    a.by_kvh = Divisor::of(uint32_t(g->num_kv_heads));
     a.scale2 = scale == scale ? float(double(scale < 0 ? -scale : scale) * 1.4426950408889634) : -1.0f;
     a.negative = scale < 0;
     void *ws = nullptr;
@@ -1110,10 +1108,14 @@ int nd_attend_prefix_i8(nd_ctx *ctx, const nd_kv_geom *g, const void *kv, size_t
     pg.cap = a.z.pcap;
     auto *fn = g->qk_head_dim == 48 ? (quant_query ? prefix_kernel<48, true> : prefix_kernel<48, false>)
                                     : (quant_query ? prefix_kernel<64, true> : prefix_kernel<64, false>);
-    hipLaunchKernelGGL(fn, dim3(a.plan.l.units / 4 * unsigned(g->num_kv_heads)), dim3(256), 0, ctx->stream, make_geom(g),
-                       make_geom(&pg), a);
-    if (int rc = nd::check_launch("attend_prefix_i8")) return rc;
-    // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
+    // HIP counts a launch's threads in 32 bits (and its second axis' blocks in 16): units
+    // and rows beyond that go in further launches
+    const uint32_t quads = a.plan.l.units / 4, each = std::min(65535u, ((1u << 24) - 1) / uint32_t(g->num_kv_heads));
+    for (uint32_t first = 0; first < quads; first += each) {
+        hipLaunchKernelGGL(fn, dim3(unsigned(g->num_kv_heads), std::min(each, quads - first)), dim3(256), 0, ctx->stream,
+                           make_geom(g), make_geom(&pg), a, first);
+        if (int rc = nd::check_launch("attend_prefix_i8")) return rc;
+    }
     const size_t step = (size_t(1) << 25) / size_t(g->num_heads);
     for (size_t first = 0; first < count * rows; first += step) {
         const uint32_t total = uint32_t(std::min(step, count * rows - first) * g->num_heads);

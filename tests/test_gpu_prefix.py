@@ -372,6 +372,16 @@ def test_offsets_beyond_32_bits(ctx):
     assert torch.equal(got, b.attend()) and rng is not None
 
 
+@pytest.mark.parametrize("H,KVH,S,rows", [(4096, 4096, 1100, 1), (1500, 1500, 3000, 1), (16, 2, 65535, 9)])
+def test_many_heads_and_more_units_than_a_launch_holds(ctx, H, KVH, S, rows):
+    """Sessions over one block give the bits of one session."""
+    b = Batch(ctx, 19, (H, KVH, 48), [], [5], rows=rows)
+    b.check()
+    plan, _ = nd.prefix_plan(ctx, b.g, 1, None, _i32([5] * S), rows=rows)
+    got = nd.attend_prefix_i8(ctx, b.g, b.kv, 0, None, 0, plan, dev(b.q).expand(S, -1, -1).contiguous())
+    assert (got == b.attend()).all()
+
+
 # ---- refusals -----------------------------------------------------------------------
 
 def test_refusals(ctx):
