@@ -455,8 +455,8 @@ int nd_logits_adjust(nd_ctx *ctx, const float *x, size_t x_stride, size_t count,
  * that receives the attention's work list, for any number of
  * nd_attend_prefix_i8 calls with the same geometry, prefix_cap, count, rows
  * and prefixes: a step's layers of one window share it.  At most 65535
- * sessions, 2^20 rows in all and 2048 prefixes.  No reference counterpart: a
- * V3Engine owns its whole cache.
+ * sessions, 2^20 rows in all, 4096 heads and 2048 prefixes.  No reference
+ * counterpart: a V3Engine owns its whole cache.
  */
 typedef struct nd_prefix_maps {
     int32_t *pos, *rot, *from, *lo, *order, *first;
@@ -699,7 +699,9 @@ int nd_v3_generate(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int3
  * logits under `sampling` (its device arrays have a number a session; NULL:
  * none), as nd_sample_rows draws it.  The reference's loop with a temperature
  * (needle-infer/src/v3_engine.rs:254-312), whose random numbers are its own:
- * a temperature of 0 for every session gives nd_v3_generate's tokens. */
+ * a temperature of 0 for every session gives nd_v3_generate's tokens.  Logits
+ * without a number give -1, which the next step takes as any id that is not
+ * one: as the last. */
 int nd_v3_generate_sampled(nd_ctx *ctx, const nd_v3_model *m, nd_v3_batch *b, const int32_t *first,
                            size_t steps, const nd_sampling *sampling, const float *u,
                            int32_t *tokens);

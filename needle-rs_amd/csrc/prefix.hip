@@ -29,7 +29,6 @@ constexpr int kPlanMagic = 0x6e645031;
 constexpr uint32_t kWaves = 4096;  // four a SIMD
 constexpr uint32_t kLeast = 4;     // chunks a wave, at least
 constexpr uint32_t kExtra = 3;     // what a unit costs beside its chunks, in chunks
-constexpr uint64_t kTile = uint64_t(1) << 40;
 
 struct Head {
     int magic, count, rows, prefixes, heads, kv_heads, cap, prefix_cap;
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     auto tiles_of = [&](uint32_t rows) { return (rows * R + kCols - 1) / kCols; };
     auto own_chunks = [&](const Want &w) { return chunks_of(uint32_t(w.lo), uint32_t(w.span), uint32_t(z.cap)); };
     auto group_chunks = [&](uint32_t p) { return chunks_of(from_s[p], end_s[p] - from_s[p], uint32_t(z.pcap)); };
-    // (chunks of all tiles below 2^40, tiles below 2^24)
+    // (at most 8 heads a kv head, so 2^21 tiles or less, of 2^19 + 1 chunks)
     auto add_weight = [&](uint64_t v) {
         v = ndl::last_lane(ndl::wave_scan(v));
         if (lane == 0 && v) atomicAdd(reinterpret_cast<unsigned long long *>(&weight_s), v);
@@ -222,7 +221,7 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     sessions(S, [&](uint32_t i, const Want &w) {
         const uint32_t m = uint32_t(w.rows());
         if (!m) return;
-        weight += uint64_t(tiles_of(m)) * (own_chunks(w) | kTile);
+        weight += uint64_t(tiles_of(m)) * (own_chunks(w) + kExtra);
         if (w.prefix < 0) return;
         atomicAdd(&rows_s[w.prefix], m);
         atomicMin(&from_s[w.prefix], uint32_t(w.from));
@@ -232,14 +231,14 @@ __global__ __launch_bounds__(NT) void plan_kernel(Sizes z, Requests r, PlanOf pl
     __syncthreads();
     weight = 0;
     for (uint32_t p = t; p < P; p += NT)
-        if (rows_s[p]) weight += uint64_t(tiles_of(rows_s[p])) * (group_chunks(p) | kTile);
+        if (rows_s[p]) weight += uint64_t(tiles_of(rows_s[p])) * (group_chunks(p) + kExtra);
     add_weight(weight);
     __syncthreads();
     // ---- the length of a run: each wave's share of all chunks, a unit counted as kExtra
     // more for its beginning and end (a run more: no more units than places and tiles).
     // The prefixes' units, the longest, come first, and short ones fill the gaps ----
     const double places = double(max(1u, kWaves / uint32_t(z.KVH)));
-    const double share = (double(weight_s & (kTile - 1)) + double(kExtra) * double(weight_s >> 40)) / places;
+    const double share = double(weight_s) / places;
     const uint32_t each = uint32_t(fmin(fmax(share + 1.0, double(kLeast)), 1048576.0));
 
     // ---- where each group's rows and units begin ----

@@ -129,12 +129,14 @@ __device__ inline void range_of(Row &r, float top, float low)
 __device__ inline double behind(const Row &r, float l) { return l == r.top ? 0.0 : double(l) - double(r.top); }
 __device__ inline bool token(const Row &r, float l) { return behind(r, l) >= r.low; }
 
-// 2^z in units of 2^-scale (scale <= 50), to the nearest, for a z <= 0.  2^f, |f| <=
-// 1/2, by the polynomial of degree 11 through its values at Chebyshev's nodes (2e-17
-// of it off).  What 2^52 is added to keeps its whole part in the low 52 bits.
-__device__ inline uint64_t units_of(double z, int scale)
+// 2^(d by) in units of 2^-scale (scale <= 50), to the nearest, for a d <= 0.  2^f, |f|
+// <= 1/2, by the polynomial of degree 11 through its values at Chebyshev's nodes (2e-17
+// of it off).  What 2^52 is added to keeps its whole part in the low 52 bits.  (f is
+// written as the one operation that it is, lest one caller's is and another's is not:
+// a token's weight is the same number wherever it is worked out.)
+__device__ inline uint64_t units_of(double d, double by, int scale)
 {
-    const double n = __builtin_rint(z), f = z - n;
+    const double n = __builtin_rint(d * by), f = __builtin_fma(d, by, -n);
     constexpr double c[] = {1.0,
                             0.6931471805599453,
                             0.24022650695910158,
@@ -158,7 +160,7 @@ __device__ inline uint64_t units_of(double z, int scale)
 __device__ inline uint64_t weight_of(const Row &r, float l)
 {
     const double d = behind(r, l);
-    return d >= r.low ? units_of(d * r.by, r.scale) : 0;
+    return d >= r.low ? units_of(d, r.by, r.scale) : 0;
 }
 
 // A little more than the weight (and 1 for some that are no tokens).
@@ -448,7 +450,7 @@ struct Held {
                 bin = uint32_t(bin_of(r, v[j]));
                 if constexpr (COUNT) atomicAdd(&h.count[bin], 1u);
                 if constexpr (WEIGHTS)
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[bin]), units_of(d * r.by, r.scale));
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[bin]), units_of(d, r.by, r.scale));
             }
             b[j / 2] = j & 1 ? b[j / 2] | bin << 16 : bin;
         }
@@ -613,8 +615,8 @@ __device__ inline void draw_listed(const Sample &s, size_t row, Row r, int want,
 // A token's place in its bin, 0 .. kBins - 1 in the order.
 __device__ inline int part_of_bin(const Row &r, float l, uint32_t bin)
 {
-    const float x = l == r.top ? 0.0f : (r.top - l) * r.bins;
-    return int(fminf((x - float(bin)) * float(kBins), float(kBins - 1)));
+    const float x = l == r.top ? 0.0f : __builtin_fmaf(r.top - l, r.bins, -float(bin));
+    return int(fminf(fmaxf(x * float(kBins), 0.0f), float(kBins - 1)));
 }
 
 // The token of a bin of `src` at which the tokens (COUNT) or the weights reach `target`;

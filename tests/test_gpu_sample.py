@@ -219,6 +219,25 @@ def test_a_row_alone_is_the_row_in_a_batch(ctx):
             assert one[0][0] == want[0][i] and one[1][0] == want[1][i]
 
 
+@pytest.mark.parametrize("rules", [dict(temperature=1.3), dict(top_k=300, top_p=0.97), dict(top_k=2000, top_p=0.9), dict(min_p=0.2)])
+@pytest.mark.parametrize("n", [700, 8192])
+def test_few_rows_are_the_rows_of_many(ctx, n, rules):
+    """Ordinary rows, equal and neighbouring logits, infinite ones and none, in 600 rows and in threes."""
+    rng = np.random.default_rng(n)
+    x, u = _logits(rng, 600, n), rng.random(600).astype(np.float32)
+    x[1::8] = 2.5
+    x[2::8] = np.float32(3) + rng.integers(0, 3, (75, n)).astype(np.float32) * np.float32(2.0 ** -22)
+    x[3::8, ::3] = np.inf
+    x[4::8] = np.nan
+    x[5::8, 1:] = -np.inf
+    x[6::8] = -3.4028235e38
+    want = _run(ctx, x, u, rules)
+    for i in range(0, 48, 3):
+        got = _run(ctx, x[i:i + 3], u[i:i + 3], rules)
+        assert np.array_equal(got[0], want[0][i:i + 3]) and np.array_equal(got[1], want[1][i:i + 3]), i
+    assert (want[0][4::8] == -1).all() and (want[0][5::8] == 0).all() and (want[0][3::8] % 3 == 0).all()
+
+
 def test_the_largest_row(ctx):
     n = 1 << 24
     x = torch.full((2, n), -5.0, device="cuda")
