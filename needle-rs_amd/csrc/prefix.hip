@@ -761,19 +761,20 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
                     }
                 }
                 floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int pc = 1; pc >= 0; --pc) {  // the small pieces first
-                    const uint32_t *qq = qp[pc];
-                    // qk 48: a lane's last four codes, doubled to the 32-wide
-                    // product's eight against four zeros of the query
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        vec4<f16x8_t>(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1]),
-                        KD == 3 ? vec4<f16x8_t>(qq[4], qq[5], 0u, 0u)
-                                : vec4<f16x8_t>(qq[4], qq[5], qq[2 * KD - 2], qq[2 * KD - 1]),
-                        d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(kp[0], kp[1], kp[2], kp[3]),
-                                                               vec4<f16x8_t>(qq[0], qq[1], qq[2], qq[3]), d, 0, 0, 0);
+auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, uint32_t q1, uint32_t q2, uint32_t q3) {
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(k0, k1, k2, k3), vec4<f16x8_t>(q0, q1, q2, q3), d, 0, 0, 0);
+                };
+                const uint32_t *qh = qp[0], *ql = qp[1];
+                if constexpr (KD == 3) {
+                    // a lane's last four codes meet both pieces in one product
+                    add(kp[0], kp[1], kp[2], kp[3], ql[0], ql[1], ql[2], ql[3]);
+                    add(kp[4], kp[5], kp[4], kp[5], ql[4], ql[5], qh[4], qh[5]);
+                } else {  // the small pieces first
+                    add(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1], ql[4], ql[5], ql[2 * KD - 2], ql[2 * KD - 1]);
+                    add(kp[0], kp[1], kp[2], kp[3], ql[0], ql[1], ql[2], ql[3]);
+                    add(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1], qh[4], qh[5], qh[2 * KD - 2], qh[2 * KD - 1]);
                 }
+                add(kp[0], kp[1], kp[2], kp[3], qh[0], qh[1], qh[2], qh[3]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * a + i] = d[i] * ks[a][i];
             }
