@@ -930,6 +930,8 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
         walk<QK, QQ, false>(gown, gp, at, hd, un, unit, kvh, sh_s);
 }
 
+constexpr int kAtOnce = 8;
+
 // The sums of a (row, head) meet: a wave each, a lane a run of chunks, then a lane a
 // column.
 __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t first, uint32_t total)
@@ -960,8 +962,24 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t fi
     find(seats.own, 1);
     const int all = runs[0] + runs[1];
     float M = -INFINITY, L = 0.0f, O = 0.0f;
+    const float *own = at.part_o + size_t(to[1]) * VD, *po = runs[0] ? at.part_o + size_t(to[0]) * VD : own;
+    size_t step = size_t(apart[runs[0] ? 0 : 1]) * VD;
+    int left = runs[0];  // of the prefix
     for (int j0 = 0; j0 < all; j0 += 64) {
-        const int j = j0 + lane, many = min(64, all - j0), olds = min(max(runs[0] - j0, 0), many);
+        const int j = j0 + lane, many = min(64, all - j0);
+        // the sums of run e of these (the prefix's, then the own ones), four a time; the
+        // first are asked for ahead of what they are multiplied by
+        float o[kAtOnce] = {};
+        auto load = [&](int e0) {
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (j0 + e0 + k >= min(all, j0 + 64)) break;
+                o[k] = po[lane];
+                po += step;
+                if (--left == 0) po = own, step = size_t(apart[1]) * VD;
+            }
+        };
+        load(0);
         float m = -INFINITY, l = 0.0f;
         if (j < all) {
             const size_t p = j < runs[0] ? to[0] + size_t(j) * apart[0] : to[1] + size_t(j - runs[0]) * apart[1];
@@ -977,20 +995,14 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t fi
         const float now = L * was, sum = now + wave_sum(l * by);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, share = by * inv;
         O *= now * inv;
-        // lane by lane of this round: the prefix's runs, then the own ones
-        auto add = [&](const float *po, size_t step, int e0, int e1) {
-            int e = e0;
-            for (; e + 4 <= e1; e += 4, po += 4 * step) {
-                const float o[4] = {po[lane], po[step + lane], po[2 * step + lane], po[3 * step + lane]};
+        for (int e = 0;;) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    O += o[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), e + k));
-            }
-            for (; e < e1; ++e, po += step)
-                O += po[lane] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), e));
-        };
-        add(at.part_o + (to[0] + size_t(j0) * apart[0]) * VD, size_t(apart[0]) * VD, 0, olds);
-        add(at.part_o + (to[1] + size_t(max(j0 - runs[0], 0)) * apart[1]) * VD, size_t(apart[1]) * VD, olds, many);
+            for (int k = 0; k < kAtOnce; ++k)
+                if (e + k < many) O += o[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), e + k));
+            e += kAtOnce;
+            if (e >= many) break;
+            load(e);
+        }
         L = sum;
     }
     out[lane] = L != L ? NAN : O;
