@@ -114,25 +114,35 @@ __device__ inline uint64_t dpp_or_zero(uint64_t x)
     return uint64_t(dpp_or_zero<C, ROWS>(uint32_t(x >> 32))) << 32 | dpp_or_zero<C, ROWS>(uint32_t(x));
 }
 
-// The whole numbers of lanes 0 .. this one added up (T: uint32_t or uint64_t): within
-// rows of 16 by row_shr 1, 2, 4, 8, then each odd row takes the last lane of the row
-// before it (row_bcast:15) and the upper half lane 31 (row_bcast:31).
+// The whole numbers of the lanes up to this one added up (T: uint32_t or uint64_t), in
+// its row of 16 by row_shr 1, 2, 4, 8; in the wave: then each odd row takes the last
+// lane of the row before it (row_bcast:15) and the upper half lane 31 (row_bcast:31).
 template <typename T>
-__device__ inline T wave_scan(T v)
+__device__ inline T row_scan(T v)
 {
     v += dpp_or_zero<0x111, 0xf>(v);
     v += dpp_or_zero<0x112, 0xf>(v);
     v += dpp_or_zero<0x114, 0xf>(v);
-    v += dpp_or_zero<0x118, 0xf>(v);
+    return v + dpp_or_zero<0x118, 0xf>(v);
+}
+
+template <typename T>
+__device__ inline T wave_scan(T v)
+{
+    v = row_scan(v);
     v += dpp_or_zero<0x142, 0xa>(v);
     return v + dpp_or_zero<0x143, 0xc>(v);
 }
 
-__device__ inline uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
-__device__ inline uint64_t last_lane(uint64_t x)
+// A lane's number, in scalar registers.
+__device__ inline uint64_t of_lane(uint64_t x, int lane)
 {
-    return uint64_t(last_lane(uint32_t(x >> 32))) << 32 | last_lane(uint32_t(x));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(x >> 32), lane));
+    return uint64_t(hi) << 32 | uint32_t(__builtin_amdgcn_readlane(int(uint32_t(x)), lane));
 }
+
+__device__ inline uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
+__device__ inline uint64_t last_lane(uint64_t x) { return of_lane(x, 63); }
 
 // v summed with its partners at lane distances D, 2 D, .., 32, in that
 // order (lanes sharing l mod D end with their group's total).

@@ -153,17 +153,14 @@ constexpr int kPlanSessions = 64;
 template <int NT>
 __device__ inline void block_scan(uint64_t v, uint64_t &before, uint64_t &all, uint64_t *room)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const uint64_t up = ndl::wave_scan(v);
     if (lane == 63) room[w] = up;
     __syncthreads();
-    before = up - v, all = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-        const uint64_t x = room[i];
-        before += i < w ? x : 0;
-        all += x;
-    }
+    // the waves' (16 at most) in the first lanes
+    const uint64_t x = ndl::row_scan(room[lane & (NT / 64 - 1)]);
+    before = up - v + (w ? ndl::of_lane(x, w - 1) : 0);
+    all = ndl::of_lane(x, NT / 64 - 1);
 }
 
 // A block lays out kPlanSessions sessions, and its share of the prefixes' units.  What

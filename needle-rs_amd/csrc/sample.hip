@@ -136,7 +136,8 @@ __device__ inline bool token(const Row &r, float l) { return behind(r, l) >= r.l
 // a token's weight is the same number wherever it is worked out.)
 __device__ inline uint64_t units_of(double d, double by, int scale)
 {
-    const double n = __builtin_rint(d * by), f = __builtin_fma(d, by, -n);
+    // d by + scale as a whole number in the low bits of `at`, and the rest of it
+    const double whole = 0x1.8p52 + double(scale), at = __builtin_fma(d, by, whole), f = __builtin_fma(d, by, whole - at);
     constexpr double c[] = {1.0,
                             0.6931471805599453,
                             0.24022650695910158,
@@ -152,8 +153,9 @@ __device__ inline uint64_t units_of(double d, double by, int scale)
     double p = c[11];
 #pragma unroll
     for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, c[i]);
-    const double q = __builtin_ldexp(p, int(n) + scale) + 0x1p52;
-    return uint64_t(__double_as_longlong(q)) & 0xfffffffffffffull;
+    // (the exponent moves by at - 2^52 3/2: -64 .. 50)
+    const int64_t q = __double_as_longlong(p) + int64_t(uint64_t(uint32_t(__double_as_longlong(at))) << 52);
+    return uint64_t(__double_as_longlong(__longlong_as_double(q) + 0x1p52)) & 0xfffffffffffffull;
 }
 
 // The weight of a logit in units; 0: no token.
@@ -196,19 +198,14 @@ struct Cut {
 template <int NT>
 __device__ inline uint64_t block_scan(uint64_t v, uint64_t &before, uint64_t *room)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const uint64_t up = ndl::wave_scan(v);
     if (lane == 63) room[w] = up;
     __syncthreads();
-    uint64_t all = 0;
-    before = up - v;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-        const uint64_t x = room[i];
-        before += i < w ? x : 0;
-        all += x;
-    }
-    return all;
+    // the waves' (16 at most) in the first lanes
+    const uint64_t x = ndl::row_scan(room[lane & (NT / 64 - 1)]);
+    before = up - v + (w ? ndl::of_lane(x, w - 1) : 0);
+    return ndl::of_lane(x, NT / 64 - 1);
 }
 
 __device__ inline uint64_t order_of(float l, int i) { return uint64_t(place_of(l)) << 24 | uint32_t(i); }
@@ -429,12 +426,13 @@ struct Held {
     // (cleaned) the largest and the lowest token's
     __device__ inline void range(float &top, float &low)
     {
-        clean();
         top = -INFINITY, low = INFINITY;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
+            const bool is = v[j] > -INFINITY;
+            low = fminf(low, is ? v[j] : INFINITY);
+            v[j] = is ? v[j] : -INFINITY;
             top = fmaxf(top, v[j]);
-            low = fminf(low, v[j] > -INFINITY ? v[j] : INFINITY);
         }
     }
     // the tokens' bins, and in those their weights (of a finite top)
@@ -447,7 +445,7 @@ struct Held {
             const double d = double(v[j]) - top;
             uint32_t bin = kNoBin;
             if (d >= r.low) {
-                bin = uint32_t(bin_of(r, v[j]));
+                bin = uint32_t(fminf((r.top - v[j]) * r.bins, float(kBins - 1)));  // bin_of
                 if constexpr (COUNT) atomicAdd(&h.count[bin], 1u);
                 if constexpr (WEIGHTS)
                     atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[bin]), units_of(d, r.by, r.scale));
