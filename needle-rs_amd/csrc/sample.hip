@@ -6,8 +6,8 @@
 // weights, added up, reach a target.  So no row is sorted:
 //   a short top-k: the row's tokens are counted in bins that follow the order, those
 //     up to the bin of the k-th are listed, and the list is put in order;
-//   else: weights are added up in the bins, the bin of a target is found, its tokens'
-//     in finer ones, and the few of that are looked at one by one;
+//   else: weights (with a top-k tokens too) are added up in the bins, the bin of a target
+//     is found, its tokens' in finer ones, and the few of that are looked at one by one;
 //   anything unusual (too many equal logits, infinite ones): the row is searched in
 //     finer and finer bins, by the digits of the order.
 // Weights are whole numbers, exp((l - M) / T) in units of 2^-s, worked out in fp64: a
@@ -56,6 +56,7 @@ struct Sample {
     Part *part;       // [rows][slices]
     uint64_t *bins;   // [rows][kBins]
     uint64_t *list;   // [rows][slices][kList]
+    uint32_t *count;  // [rows][kBins]
 };
 
 // The order of the floats as that of whole numbers, the largest first (-0 as 0).
@@ -543,14 +544,14 @@ struct Bins {
             was += v[e];
         }
     }
-    // f of what comes before bin b
+    // f of what comes before bin b, and of the bin
     template <typename F>
     __device__ inline void at(uint32_t b, F f) const
     {
         uint64_t was = before;
 #pragma unroll
         for (int e = 0; e < B; ++e) {
-            if (uint32_t(B * int(threadIdx.x) + e) == b) f(was);
+            if (uint32_t(B * int(threadIdx.x) + e) == b) f(was, v[e]);
             was += v[e];
         }
     }
@@ -662,7 +663,7 @@ __device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint
                 h.best[0] = skip + was;
             });
             __syncthreads();
-            bw.at(h.bin, [&](uint64_t was) { h.best[1] = skipw + was; });
+            bw.at(h.bin, [&](uint64_t was, uint64_t) { h.best[1] = skipw + was; });
         } else {
             bw.with(target - skip, [&](uint32_t b, uint64_t was, uint64_t) {
                 h.bin = b;
@@ -735,7 +736,7 @@ __device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Sh
             __syncthreads();
             const uint32_t bin = h.bin;
             const uint64_t skip = h.best[0];
-            w.at(bin, [&](uint64_t was) { h.best[1] = was; });
+            w.at(bin, [&](uint64_t was, uint64_t) { h.best[1] = was; });
             __syncthreads();
             const uint64_t skipw = h.best[1];
             if (!cut_in<NT, true>(uint64_t(r.k), bin, skip, skipw, r, h, src, cut)) return false;
@@ -822,7 +823,7 @@ constexpr int kDraw = 1024;    // of a row's
 enum Way { kSearch, kListed, kBinned };
 __device__ inline Way way_of(const Row &r)
 {
-    return r.top == INFINITY ? kSearch : r.k <= 0 ? kBinned : r.k <= kShort ? kListed : kSearch;
+    return r.top == INFINITY ? kSearch : r.k > 0 && r.k <= kShort ? kListed : kBinned;
 }
 
 // A row's largest and lowest logit from its parts (a barrier).
@@ -861,7 +862,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Sample s, size_t first)
     Row r = rules_of(s, row);
     for (int b = t; b < kBins; b += kThreads) {
         h.count[b] = 0;
-        if (slice == 0) s.bins[row * kBins + b] = 0;
+        if (slice == 0) s.bins[row * kBins + b] = 0, s.count[row * kBins + b] = 0;
     }
     if (t == 0) h.listed = 0;
     float top, low;
@@ -886,64 +887,101 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Sample s, size_t first)
     if (t == 0) s.part[row * s.slices + slice] = p;
 }
 
-// The weights of rows without a top-k in their rows' bins.
+// Of rows without a short top-k: the weights, and with a long one the tokens' number, in
+// their rows' bins.
 __global__ __launch_bounds__(kThreads) void bins_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
     const size_t row = first + blockIdx.x / unsigned(s.blocks);
     const int block = int(blockIdx.x % unsigned(s.blocks)), t = threadIdx.x;
     Row r = rules_of(s, row);
-    if (r.greedy || r.k > 0) return;
+    if (r.greedy || (r.k > 0 && r.k <= kShort)) return;
     Held<kThreads> v;
     v.load(s.x + row * s.x_stride, block * kSlice, s.n);
-    for (int b = t; b < kBins; b += kThreads) h.weight[b] = 0;
+    for (int b = t; b < kBins; b += kThreads) {
+        h.weight[b] = 0;
+        if (r.k > 0) h.count[b] = 0;
+    }
     join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
     join_scale<kThreads>(s, row, r, h.room[1]);
     for (int slice = block;;) {
         v.clean();
-        v.template lay<true, false>(r, h);
+        if (r.k > 0)
+            v.template lay<true, true>(r, h);
+        else
+            v.template lay<true, false>(r, h);
         slice += s.blocks;
         if (slice >= s.slices) break;
         v.load(s.x + row * s.x_stride, slice * kSlice, s.n);
     }
     __syncthreads();
-    for (int b = t; b < kBins; b += kThreads)
+    for (int b = t; b < kBins; b += kThreads) {
         if (const uint64_t w = h.weight[b])
             atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[row * kBins + b]), w);
+        if (r.k > 0)
+            if (const uint32_t c = h.count[b]) atomicAdd(&s.count[row * kBins + b], c);
+    }
 }
 
-// Which bins of a row matter: the one where the weights come to top_p (`last`), and
-// those where the draw may be, whatever token of `last` the run ends at (from .. to).
-struct Matter {
-    uint32_t from, to, last;
+// Which bins of a row matter: that of the k-th token (`cut`), those where the weights may
+// come to top_p, whatever token the first k end at, and those where the draw may be.
+struct Range {
+    uint32_t from, to;
+    __device__ inline bool has(uint32_t bin) const { return bin - from <= to - from; }
 };
+
+struct Matter {
+    uint32_t cut;
+    Range nucleus, draw;
+    __device__ inline bool has(uint32_t bin) const { return bin == cut || nucleus.has(bin) || draw.has(bin); }
+};
+
+__device__ inline uint32_t scalar(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 
 template <int NT>
 __device__ inline Matter matter_of(const Sample &s, size_t row, const Row &r, Shared &h)
 {
     Bins<NT, uint64_t> w;
     w.read(s.bins + row * kBins, h.room[2]);
-    Matter m{0, 0, kNoBin - 1};
-    uint64_t least = w.all, most = w.all;
-    if (r.p < 1.0f) {
-        const uint64_t need = part_of(w.all, fmaxf(r.p, 0.0f), true);
-        w.with(need ? need : 1, [&](uint32_t b, uint64_t was, uint64_t v) {
-            h.bin = b;
-            h.best[0] = was + 1;
-            h.best[1] = was + v;
+    Matter m{kNoBin, Range{kNoBin, kNoBin}, Range{}};
+    uint64_t least = w.all, most = w.all;  // that stay
+    if (r.k > 0) {
+        Bins<NT, uint32_t> c;
+        c.read(s.count + row * kBins, h.room[1]);
+        if (uint64_t(r.k) < c.all) {
+            c.with(uint64_t(r.k), [&](uint32_t b, uint64_t, uint64_t) { h.bin = b; });
+            __syncthreads();
+            m.cut = scalar(h.bin);
+            w.at(m.cut, [&](uint64_t was, uint64_t v) {
+                h.best[0] = was;
+                h.best[1] = was + v;
+            });
+            __syncthreads();
+            // (its last token may weigh less than half a unit)
+            least = h.best[0] ? h.best[0] : 1;
+            most = h.best[1];
+        }
+    }
+    // the bins of the tokens at which the weights reach a .. z, and what those come to
+    auto reach = [&](uint64_t a, uint64_t z) {
+        w.with(a, [&](uint32_t b, uint64_t, uint64_t) { h.sums[0] = b; });
+        w.with(z, [&](uint32_t b, uint64_t was, uint64_t v) {
+            h.sums[1] = b;
+            h.sums[2] = was + v;
         });
         __syncthreads();
-        m.last = h.bin;
-        least = h.best[0];
-        most = h.best[1];
+        return Range{scalar(uint32_t(h.sums[0])), scalar(uint32_t(h.sums[1]))};
+    };
+    if (r.p < 1.0f) {
+        const uint64_t a = part_of(least, fmaxf(r.p, 0.0f), true), z = part_of(most, fmaxf(r.p, 0.0f), true);
+        least = a ? a : 1;
+        m.nucleus = reach(least, z ? z : 1);
+        most = h.sums[2] < most ? h.sums[2] : most;
+        __syncthreads();
     }
     const uint64_t a = part_of(least, r.u, false) + 1, z = part_of(most, r.u, false) + 1;
-    w.with(a < least ? a : least, [&](uint32_t b, uint64_t, uint64_t) { h.sums[0] = b; });
-    w.with(z < most ? z : most, [&](uint32_t b, uint64_t, uint64_t) { h.sums[1] = b; });
-    __syncthreads();
-    m.from = uint32_t(h.sums[0]);
-    m.to = uint32_t(h.sums[1]);
+    m.draw = reach(a < least ? a : least, z < most ? z : most);
     return m;
 }
 
@@ -954,7 +992,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
     const size_t row = first + blockIdx.x / unsigned(s.blocks);
     const int block = int(blockIdx.x % unsigned(s.blocks)), t = threadIdx.x;
     Row r = rules_of(s, row);
-    if (r.greedy || r.k > 0) return;
+    if (r.greedy || (r.k > 0 && r.k <= kShort)) return;
     Held<kThreads> v;
     v.load(s.x + row * s.x_stride, block * kSlice, s.n);
     join_parts<kThreads>(s, row, r, h.room[0]);
@@ -967,7 +1005,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
 #pragma unroll
         for (int j = 0; j < v.kPer; ++j) {
             const uint32_t bin = uint32_t(bin_of(r, v.v[j]));
-            if ((bin == m.last || bin - m.from <= m.to - m.from) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)));
+            if (m.has(bin) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)));
         }
         __syncthreads();
         const int many = int(h.listed);
@@ -1010,6 +1048,7 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
         } else if (way_of(r) == kBinned) {
             join_scale<kDraw>(s, row, r, h.room[2]);
             h.weight[t] = s.bins[row * kBins + t];
+            h.count[t] = s.count[row * kBins + t];
             __syncthreads();
             if (draw_binned<kDraw>(s, row, r, h, lists)) return;
         }
@@ -1020,7 +1059,7 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
 
 size_t slices_of(size_t n) { return (n + kSlice - 1) / kSlice; }
 
-size_t row_bytes(size_t slices) { return slices > 1 ? kBins * 8 + slices * (kList * 8 + sizeof(Part)) : 0; }
+size_t row_bytes(size_t slices) { return slices > 1 ? kBins * 12 + slices * (kList * 8 + sizeof(Part)) : 0; }
 
 }  // namespace
 
@@ -1040,7 +1079,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
     ND_REQUIRE(count == 1 || x_stride >= n, "row stride %zu below n %zu", x_stride, n);
     const nd_sampling none{}, &r = sampling ? *sampling : none;
     const size_t slices = slices_of(n);
-    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices), 0};
+    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices), 0, nullptr, nullptr, nullptr, nullptr};
     // (a row's blocks, of about four a CU; each finds out what matters for itself)
     s.blocks = int(std::min(slices, std::max<size_t>(1, 1024 / count)));
     if (slices > 1) {
@@ -1048,7 +1087,8 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         if (int rc = nd::call_workspace(ctx, count * row_bytes(slices), work, work_bytes, &ws)) return rc;
         s.bins = static_cast<uint64_t *>(ws);
         s.list = s.bins + count * kBins;
-        s.part = reinterpret_cast<Part *>(s.list + count * slices * kList);
+        s.count = reinterpret_cast<uint32_t *>(s.list + count * slices * kList);
+        s.part = reinterpret_cast<Part *>(s.count + count * kBins);
     }
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
     const size_t most = 0xffffffff / kDraw / slices;
@@ -1071,7 +1111,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         }
         hipLaunchKernelGGL(slice_kernel, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_slices")) return rc;
-        // (only rows without a top-k have anything to do here, which the host does not see)
+        // (only rows without a short top-k have anything to do here, which the host does not see)
         hipLaunchKernelGGL(bins_kernel, dim3(rows * unsigned(s.blocks)), dim3(kThreads), 0, ctx->stream, s, first);
         if (int rc = nd::check_launch("sample_bins")) return rc;
         hipLaunchKernelGGL(gather_kernel, dim3(rows * unsigned(s.blocks)), dim3(kThreads), 0, ctx->stream, s, first);
