@@ -496,8 +496,8 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
             const uint32_t u = kr[0][0] ^ 0x80808080u;
             if constexpr (QQ)
                 kk[0] = kr[0][0];
-            else
-                kk[0] = f16_pair<0>(u), kk[1] = f16_pair<1>(u);
+            else  // (twice: the product that takes both pieces of the query)
+                *reinterpret_cast<u32x4_t *>(kk) = vec4<u32x4_t>(f16_pair<0>(u), f16_pair<1>(u), f16_pair<0>(u), f16_pair<1>(u));
         } else {
             const uint32_t u0 = kr[0][0] ^ 0x80808080u, u1 = kr[0][1] ^ 0x80808080u;
             if constexpr (QQ)
@@ -560,7 +560,7 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
     float cf0;                        // factor of a score, in bits, is |cf0| 2^(kexp - sh)
     int sh;
     intx4_t qi;                       // QQ: codes
-    uint32_t qp[2][KD == 3 ? 6 : 8];  // else: f16 pieces
+    uint32_t qp[2][8];                // else: f16 pieces
     {
         if (at.negative) {
             asm volatile("");  // (a branch)
@@ -653,7 +653,7 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
         const uint32_t p0 = now.p0;
         const int left = now.left;
         // ---- the positions each column sees ----
-        const bool full = p0 >= tlo && p0 + 31 <= thi && left >= 32;
+        const bool full = p0 >= tlo && left >= 32 && (TOGETHER || p0 + 31 <= thi);  // (thi of a prefix: all)
         uint32_t vis = 0xffffffffu;
         if (!full) {
             vis = left < 32 ? (1u << left) - 1u : 0xffffffffu;
@@ -738,17 +738,12 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
         } else {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                uint32_t kp[2 * KD];
+                uint32_t kp[8];  // qk 48: the last two twice
                 if constexpr (TOGETHER) {
                     const u32x4_t lo4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a][lane]);
                     kp[0] = lo4[0], kp[1] = lo4[1], kp[2] = lo4[2], kp[3] = lo4[3];
-                    if constexpr (KD == 3) {
-                        const uint2 hi2 = *reinterpret_cast<const uint2 *>(sh_s.k[buf][2 * a + 1][lane]);
-                        kp[4] = hi2.x, kp[5] = hi2.y;
-                    } else {
-                        const u32x4_t hi4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a + 1][lane]);
-                        kp[4] = hi4[0], kp[5] = hi4[1], kp[2 * KD - 2] = hi4[2], kp[2 * KD - 1] = hi4[3];
-                    }
+                    const u32x4_t hi4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a + 1][lane]);
+                    kp[4] = hi4[0], kp[5] = hi4[1], kp[6] = hi4[2], kp[7] = hi4[3];
                 } else {
 #pragma unroll
                     for (int d = 0; d < KD; ++d) {
@@ -756,21 +751,21 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
                         kp[2 * d] = f16_pair<0>(u);
                         kp[2 * d + 1] = f16_pair<1>(u);
                     }
+                    if constexpr (KD == 3) kp[6] = kp[4], kp[7] = kp[5];
                 }
                 floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
 auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, uint32_t q1, uint32_t q2, uint32_t q3) {
                     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(k0, k1, k2, k3), vec4<f16x8_t>(q0, q1, q2, q3), d, 0, 0, 0);
                 };
                 const uint32_t *qh = qp[0], *ql = qp[1];
-                if constexpr (KD == 3) {
-                    // a lane's last four codes meet both pieces in one product
-                    add(kp[0], kp[1], kp[2], kp[3], ql[0], ql[1], ql[2], ql[3]);
-                    add(kp[4], kp[5], kp[4], kp[5], ql[4], ql[5], qh[4], qh[5]);
-                } else {  // the small pieces first
-                    add(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1], ql[4], ql[5], ql[2 * KD - 2], ql[2 * KD - 1]);
-                    add(kp[0], kp[1], kp[2], kp[3], ql[0], ql[1], ql[2], ql[3]);
-                    add(kp[4], kp[5], kp[2 * KD - 2], kp[2 * KD - 1], qh[4], qh[5], qh[2 * KD - 2], qh[2 * KD - 1]);
-                }
+                // the small pieces first; of qk 48 a lane's last four codes meet both
+                // pieces in one product
+                if constexpr (KD == 4) add(kp[4], kp[5], kp[6], kp[7], ql[4], ql[5], ql[6], ql[7]);
+                add(kp[0], kp[1], kp[2], kp[3], ql[0], ql[1], ql[2], ql[3]);
+                if constexpr (KD == 3)
+                    add(kp[4], kp[5], kp[6], kp[7], ql[4], ql[5], qh[4], qh[5]);
+                else
+                    add(kp[4], kp[5], kp[6], kp[7], qh[4], qh[5], qh[6], qh[7]);
                 add(kp[0], kp[1], kp[2], kp[3], qh[0], qh[1], qh[2], qh[3]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * a + i] = d[i] * ks[a][i];
