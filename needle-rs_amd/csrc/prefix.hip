@@ -547,7 +547,7 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
     auto both = [&](auto distance) {
         constexpr int D = decltype(distance)::value;
         tlo = max(tlo, uint32_t(ndl::wave_xor_int<D>(int(tlo))));
-        thi = min(thi, uint32_t(ndl::wave_xor_int<D>(int(thi))));
+        if constexpr (!TOGETHER) thi = min(thi, uint32_t(ndl::wave_xor_int<D>(int(thi))));
     };
     both(std::integral_constant<int, 1>{});
     both(std::integral_constant<int, 2>{});
@@ -572,7 +572,9 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
         for (int e = 0; e < SL; e += 2) a = max3(a, __builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1]));
         a = fmaxf(a, ndl::wave_xor<16>(a));
         a = fmaxf(a, ndl::wave_xor<32>(a));
-        float nan = 0.0f;
+        float nan = 0.0f;  // or NaN: of a NaN or an infinity
+#pragma unroll
+        for (int e = 0; e < SL; ++e) nan = __builtin_fmaf(v[e], 0.0f, nan);
         if constexpr (QQ) {
             // quant_rows (model.rs:289-293): the codes and the head's scale
             const float qs = a > 0.0f ? a / 127.0f : 1.0f;
@@ -584,7 +586,6 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
                 // the float below a half, for every |y| < 2^22
                 const float y = v[e] * inv;
                 const float r = __builtin_amdgcn_fmed3f(y + copysignf(0.49999997f, y), -128.0f, 127.5f);
-                nan = y != y ? y : nan;
                 dw[e >> 2] |= (uint32_t(int32_t(r)) & 0xffu) << (8 * (e & 3));
             }
             qi = intx4_t{int(dw[0]), int(dw[1]), int(dw[2]), int(dw[3])};
@@ -595,7 +596,6 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
             sh = a > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(a) : 0;
 #pragma unroll
             for (int e = 0; e < SL; ++e) {
-                nan = v[e] - v[e] != 0.0f ? NAN : nan;
                 v[e] = __builtin_amdgcn_ldexpf(v[e], sh);
             }
 #pragma unroll
