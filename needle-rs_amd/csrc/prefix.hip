@@ -1,6 +1,24 @@
 // A batch that shares its prompts: the rows of a step laid out from the requests'
 // lengths, and attention over prefixes that are held once and over the sessions'
 // own blocks.
+//
+// A (row, head)'s positions lie in two sources, its prefix's block and its session's:
+//   out = sum_s 2^(x_s - M) V_s / sum_s 2^(x_s - M),  x_s = scale log2(e) q . K_s
+// A sum over any part of them is three numbers' worth: its own M, the weights' sum and
+// the 64 weighted sums of V, and parts meet by M = max M_i, each times 2^(M_i - M).  So
+// the rows of all sessions behind a prefix are columns of one matrix product over it:
+// its codes are read for 16 columns at a time (a tile), or for 64 (four tiles together),
+// and only the sessions' own blocks are read row by row.
+//
+// What bounds it (MI355X; a call, both kernels):
+//   512 rows of 12 heads over 2 behind 8000 positions, fp32 queries: 49 us.  Vector
+//     instructions: about 100 for a chunk of 512 scores (8 exponentials, 16 to split the
+//     weights, 20 to turn the wave's share of K and V, 24 for scores and weights), of
+//     which 20 more cost 3 us; 14 matrix products of 16 cycles lie beside them.
+//   200 sessions of 12 x 64 heads, 500 own positions each, seven prompts: 50 us, 170 MB
+//     at 3.4 TB/s; a large copy would take 35.
+//   64 sessions behind 2000 positions, query codes: 12.5 us, of which 8.7 are the first
+//     kernel, one pass through memory and four chunks a wave, and 4 the join's.
 #include "nd_attn_pieces.h"
 #include "nd_internal.h"
 #include "nd_kv_internal.h"
@@ -26,6 +44,9 @@ constexpr size_t kMaxSessions = 65535, kMaxRows = 256, kMaxAll = size_t(1) << 20
 // the same chunks: unit base + 4 q runs + k w + j is run k of tile 4 q + j, w the
 // tiles of quad q.
 constexpr int kPlanMagic = 0x6e645031;
+// Kernel times: with half as many waves 512 rows behind 8000 positions 46 -> 54 us, with
+// twice as many 24 x 33 rows 26 -> 28 and their join 7.5 -> 9.3; with runs of 2 chunks 64
+// rows 10.4 -> 11.4 and their join 4.3 -> 5.8, of 8 128 rows in windows 15 -> 17.
 constexpr uint32_t kWaves = 4096;  // four a SIMD
 constexpr uint32_t kLeast = 4;     // chunks a wave, at least
 constexpr uint32_t kExtra = 3;     // what a unit costs beside its chunks, in chunks
@@ -163,6 +184,11 @@ __device__ inline void block_scan(uint64_t v, uint64_t &before, uint64_t &all, u
     all = ndl::of_lane(x, NT / 64 - 1);
 }
 
+// 4001 sessions of up to 5 rows behind 90 prompts: 12.3 us, 0.9 MB written; 5 sessions:
+// 5.7.  Latency: the requests, three scans, and the units one after another.  Blocks of
+// 256 threads where they hold every session and prefix (of 1024 there: 6.4 us), of 1024
+// for the rest.
+//
 // A block lays out kPlanSessions sessions, and its share of the prefixes' units.  What
 // it has to know of the rest -- the groups, and what the sessions before its own come
 // to -- it works out from the requests itself (65535 of them are 64 a thread), so that
@@ -387,25 +413,24 @@ __device__ inline bool made_for(const Head &h, const Sizes &z)
            h.heads == z.H && h.kv_heads == z.KVH && h.cap == z.cap && h.prefix_cap == z.pcap;
 }
 
-// Operands of a chunk that a block's waves share, twice: one is read while the next
-// one is laid down.  K as it goes into the products (codes, or f16), 16 positions
-// after 16; V as f16, column 4 n + c of eight positions a lane.
+// Operands of a chunk that a block's waves share (of an fp32 query), twice: one is read
+// while the next one is laid down.  K as f16, 16 positions after 16; V as f16, column
+// 4 n + c of eight positions a lane.
 struct Shared {
-    uint32_t sc[4][64];
     uint32_t k[2][4][64][4], v[2][4][64][4];
 };
 
 template <int QK, bool QQ, bool TOGETHER>
 __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Attend &at, const Head &hd, const Unit &un,
-                                     uint32_t unit, uint32_t kvh, Shared &sh_s)
+                                     uint32_t unit, uint32_t kvh, float *sc_s, Shared *sh_s)
 {
+    static_assert(!(QQ && TOGETHER), "of query codes each wave reads K for itself");
     constexpr int SL = QK / 4, KD = SL / 4;  // a lane's slice of a K row; its dwords (3 or 4)
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, qd = lane >> 4;
     const uint32_t R = uint32_t(gown.H / gown.KVH);
     const bool own = !TOGETHER && un.source < 0;
     const uint32_t ncols = uint32_t(un.rows) * R, tile = uint32_t(un.tile);
-    float *sc_s = reinterpret_cast<float *>(sh_s.sc[w]);
 
     const uint32_t f = min(tile * kCols + uint32_t(n), ncols - 1), r = at.by_rep.quotient(f);
     Place pl{};
@@ -491,25 +516,19 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
     };
     // the wave's part into buffer `to`
     auto lay_down = [&](int to) {
-        uint32_t *kk = &sh_s.k[to][QQ ? w >> 1 : w][lane][QQ ? 2 * (w & 1) : 0];
-        if (KD == 3 && (w & 1)) {
-            const uint32_t u = kr[0][0] ^ 0x80808080u;
-            if constexpr (QQ)
-                kk[0] = kr[0][0];
-            else  // (twice: the product that takes both pieces of the query)
-                *reinterpret_cast<u32x4_t *>(kk) = vec4<u32x4_t>(f16_pair<0>(u), f16_pair<1>(u), f16_pair<0>(u), f16_pair<1>(u));
+        u32x4_t *kk = reinterpret_cast<u32x4_t *>(sh_s->k[to][w][lane]);
+        const uint32_t u0 = kr[0][0] ^ 0x80808080u;
+        if (KD == 3 && (w & 1)) {  // (twice: the product that takes both pieces of the query)
+            *kk = vec4<u32x4_t>(f16_pair<0>(u0), f16_pair<1>(u0), f16_pair<0>(u0), f16_pair<1>(u0));
         } else {
-            const uint32_t u0 = kr[0][0] ^ 0x80808080u, u1 = kr[0][1] ^ 0x80808080u;
-            if constexpr (QQ)
-                kk[0] = kr[0][0], kk[1] = kr[0][1];
-            else
-                kk[0] = f16_pair<0>(u0), kk[1] = f16_pair<1>(u0), kk[2] = f16_pair<0>(u1), kk[3] = f16_pair<1>(u1);
+            const uint32_t u1 = kr[0][1] ^ 0x80808080u;
+            *kk = vec4<u32x4_t>(f16_pair<0>(u0), f16_pair<1>(u0), f16_pair<0>(u1), f16_pair<1>(u1));
         }
         const uint32_t v0 = vr[0] ^ 0x80808080u, v1 = vr[1] ^ 0x80808080u;
-        sh_s.v[to][0][lane][w] = f16_codes<0>(v0, v1);
-        sh_s.v[to][1][lane][w] = f16_codes<1>(v0, v1);
-        sh_s.v[to][2][lane][w] = f16_codes<2>(v0, v1);
-        sh_s.v[to][3][lane][w] = f16_codes<3>(v0, v1);
+        sh_s->v[to][0][lane][w] = f16_codes<0>(v0, v1);
+        sh_s->v[to][1][lane][w] = f16_codes<1>(v0, v1);
+        sh_s->v[to][2][lane][w] = f16_codes<2>(v0, v1);
+        sh_s->v[to][3][lane][w] = f16_codes<3>(v0, v1);
     };
     // all waves' parts are there, and read
     auto meet = [&]() {
@@ -724,13 +743,7 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
         if constexpr (QQ) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                intx4_t kf;
-                if constexpr (TOGETHER) {
-                    kf = *reinterpret_cast<const intx4_t *>(sh_s.k[buf][a][lane]);
-                    if constexpr (KD == 3) kf[3] = 0;
-                } else {
-                    kf = intx4_t{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
-                }
+                const intx4_t kf{int(kr[a][0]), int(kr[a][1]), int(kr[a][2]), KD == 3 ? 0 : int(kr[a][KD - 1])};
                 const intx4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qi, intx4_t{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * a + i] = float(d[i]) * ks[a][i];
@@ -740,9 +753,9 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
             for (int a = 0; a < 2; ++a) {
                 uint32_t kp[8];  // qk 48: the last two twice
                 if constexpr (TOGETHER) {
-                    const u32x4_t lo4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a][lane]);
+                    const u32x4_t lo4 = *reinterpret_cast<const u32x4_t *>(sh_s->k[buf][2 * a][lane]);
                     kp[0] = lo4[0], kp[1] = lo4[1], kp[2] = lo4[2], kp[3] = lo4[3];
-                    const u32x4_t hi4 = *reinterpret_cast<const u32x4_t *>(sh_s.k[buf][2 * a + 1][lane]);
+                    const u32x4_t hi4 = *reinterpret_cast<const u32x4_t *>(sh_s->k[buf][2 * a + 1][lane]);
                     kp[4] = hi4[0], kp[5] = hi4[1], kp[6] = hi4[2], kp[7] = hi4[3];
                 } else {
 #pragma unroll
@@ -834,7 +847,7 @@ auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, 
                 for (int c = 0; c < 4; ++c) {
                     float code;
                     if constexpr (TOGETHER)
-                        code = float(reinterpret_cast<const _Float16 *>(sh_s.v[buf][c][lane])[j]);
+                        code = float(reinterpret_cast<const _Float16 *>(sh_s->v[buf][c][lane])[j]);
                     else
                         code = i8_at(vr[j], c) * 0x1p-9f;
                     acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(code, wt[j], acc[c], 0, 0, 0);
@@ -854,7 +867,7 @@ auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, 
                 constexpr int c = decltype(cc)::value;
                 f16x8_t vf;
                 if constexpr (TOGETHER)
-                    vf = *reinterpret_cast<const f16x8_t *>(sh_s.v[buf][c][lane]);
+                    vf = *reinterpret_cast<const f16x8_t *>(sh_s->v[buf][c][lane]);
                 else
                     vf = vec4<f16x8_t>(f16_codes<c>(u[0], u[1]), f16_codes<c>(u[2], u[3]), f16_codes<c>(u[4], u[5]),
                                        f16_codes<c>(u[6], u[7]));
@@ -901,12 +914,19 @@ auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, 
         *reinterpret_cast<floatx2_t *>(at.part_ml + to * 2) = floatx2_t{M, __builtin_amdgcn_ldexpf(l_run, -more) * by};
 }
 
-// A block's four units: of four tiles of a prefix over the same chunks, together, or
-// each for itself.
+// A block's four units, each for itself: a wave turns its chunk's K and V into operands
+// in its registers.  Or, of four tiles of a prefix over the same chunks, together: a wave
+// turns a quarter of them, in LDS, and reads all back, two buffers in turn (four, and a
+// meeting every other chunk: the same time).  512 rows over 2 kv heads, fp32 queries, together
+// and alone (us): runs of 7 chunks 20.6, 19.3; 12 26.4, 27.0; 16 31.6, 33.1; 26 46.2, 50.3.
+// Of query codes K needs no turning, and V's alone is not worth the meetings: 7 20.1, 18.3;
+// 16 30.1, 29.8; 26 43.7, 43.8.
+constexpr int kTogether = 10;  // chunks of a run
+
 template <int QK, bool QQ>
 __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Attend at, uint32_t first)
 {
-    __shared__ __align__(16) Shared sh_s;
+    __shared__ __align__(16) float sc_s[4][64];
     const uint32_t w = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
     const uint32_t unit = 4 * (first + blockIdx.y) + w, kvh = blockIdx.x;
     // (both asked for at once: the list has as many places as the grid waves)
@@ -915,17 +935,24 @@ __global__ __launch_bounds__(256, 4) void prefix_kernel(Geom gown, Geom gp, Atte
     if (!made_for(hd, at.z) || int(unit) >= hd.units) return;
     const uint32_t ncols = uint32_t(un.rows) * uint32_t(gown.H / gown.KVH), tile = uint32_t(un.tile);
     if (tile * kCols >= ncols) return;
-    // (a prefix's first unit is a multiple of four, and its full quads come first)
-    if (un.source >= 0 && (tile | 3) * kCols < ncols)
-        walk<QK, QQ, true>(gown, gp, at, hd, un, unit, kvh, sh_s);
-    else
-        walk<QK, QQ, false>(gown, gp, at, hd, un, unit, kvh, sh_s);
+    if constexpr (!QQ) {
+        __shared__ __align__(16) Shared sh_s;
+        // (a prefix's first unit is a multiple of four, and its full quads come first.  One
+        // condition: as three branches the 46 us of the largest step are 48)
+        if (int(un.source >= 0) & int((tile | 3) * kCols < ncols) & int(un.chunks >= kTogether * un.runs))
+            walk<QK, QQ, true>(gown, gp, at, hd, un, unit, kvh, sc_s[w], &sh_s);
+        else
+            walk<QK, QQ, false>(gown, gp, at, hd, un, unit, kvh, sc_s[w], nullptr);
+    } else {
+        walk<QK, QQ, false>(gown, gp, at, hd, un, unit, kvh, sc_s[w], nullptr);
+    }
 }
 
 constexpr int kAtOnce = 8;
 
 // The sums of a (row, head) meet: a wave each, a lane a run of chunks, then a lane a
-// column.
+// column.  Four dependent reads, 3 to 7.5 us a call; the first sums are asked for ahead of
+// their weights (one row of 8 runs: 3.9 -> 3.0 us).
 __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t first, uint32_t total)
 {
     const uint32_t oh = blockIdx.x * 4 + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
