@@ -312,6 +312,90 @@ def test_sums_of_large_values(ctx, quant):
     b.check(quant, tol=TOL * 3.3e38)
 
 
+# ---- long runs of many rows, whose tiles lay K and V down for each other ------------
+
+LONG = [(128, 128, 48), (256, 128, 64)]
+
+
+def _long(seed, shape, ctx, S=70, plen=701, **kw):
+    """70 sessions behind one prefix on 128 kv heads: runs of 10 chunks and more (a
+    wave's share of the chunks of all tiles, three more a tile, and one)."""
+    H, KVH, _ = shape
+    b = Batch(ctx, seed, shape, [plen], [i * 7 % 40 for i in range(S)], **kw)
+    tiles, chunks = -(-S * (H // KVH) // 16), -(-min(plen, kw.get("window") or plen) // 32)
+    each = (tiles * (chunks + 3) + S * 4) // (4096 // KVH) + 1
+    assert tiles >= 4 and chunks // -(-chunks // each) >= 10
+    return b
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("shape", LONG)
+@pytest.mark.parametrize("S,plen,window", [(64, 700, 0), (70, 673, 0), (79, 1409, 0), (70, 701, 690), (64, 1500, 740)])
+def test_long_runs(ctx, shape, S, plen, window, quant):
+    kw = dict(window=window, pcap=window + 1, cap=41) if window else {}
+    _long(21, shape, ctx, S, plen, **kw).check(quant, sessions={0, 5, 17, S // 2, S - 1})
+
+
+@pytest.mark.parametrize("shape", LONG)
+@pytest.mark.parametrize("k_size,v_size", [(1e-6, 1e6), (30.0, 1e-12), (1e-30, 1e-30), (3.0, 1e30), (1e34, 1.0), (1e-38, 1e36)])
+def test_long_runs_of_values_of_any_size(ctx, shape, k_size, v_size):
+    _long(22, shape, ctx, k_size=k_size, v_size=v_size, q_size=min(1 / k_size, 1e30)).check(tol=TOL * v_size, sessions={0, 33, 69})
+
+
+@pytest.mark.parametrize("shape", LONG)
+@pytest.mark.parametrize("garbage", [np.nan, np.inf, 3e38, -1e-40])
+def test_long_runs_and_what_is_no_number(ctx, shape, garbage):
+    """Garbage where no row looks; then queries and a V scale that are no numbers."""
+    H, KVH, QK = shape
+    b = _long(23, shape, ctx, window=690, pcap=720)
+    want = host(b.attend())
+    off, first = nd.kv_offsets(b.pg), 701 + 1 - 690  # the earliest window begins there
+    for part in ("ks", "vs"):
+        f = b.pkv[off[part]:off[part] + 4 * KVH * 720].view(torch.float32).view(KVH, 720)
+        f[:, :first] = garbage
+        f[:, 701:] = garbage
+    assert np.array_equal(host(b.attend()), want)
+    b.q.reshape(70, H, QK)[3, 5, 1] = np.nan
+    b.q.reshape(70, H, QK)[40, 64, 2] = garbage if not np.isfinite(garbage) else np.nan
+    vs = b.pkv[off["vs"]:off["vs"] + 4 * KVH * 720].view(torch.float32).view(KVH, 720)
+    vs[9, 300] = np.nan
+    got, want = host(b.attend()).reshape(70, H, 64), want.reshape(70, H, 64)
+    hit, R = np.zeros((70, H), bool), H // KVH
+    hit[3, 5] = hit[40, 64] = True
+    hit[:, 9 * R:10 * R] = True
+    assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("sink", [1e-9, 1e-20, 0.0])
+@pytest.mark.parametrize("ahead", [5, 25, 60])
+def test_long_runs_behind_a_row_of_next_to_no_values(ctx, ahead, sink):
+    """As above (701 + 1 .. 40 other positions)."""
+    shape = H, KVH, QK = LONG[0]
+    b = _long(24, shape, ctx, cap=41)
+    rng = np.random.default_rng(25)
+    k = np.zeros((701, KVH, QK))
+    k[337, :, 0] = 1.0
+    v = rng.uniform(1, 2, (701, KVH * 64))
+    v[337] = sink * rng.uniform(1, 2, KVH * 64)
+    _positive(b, b.pg, b.pkv, b.pnb, 0, np.arange(701), k.reshape(701, -1), v)
+    for i in range(70):
+        _positive(b, b.g, b.kv, b.nb, i, np.arange(41), np.zeros((41, KVH * QK)), rng.uniform(1, 2, (41, KVH * 64)))
+    b.q[:] = 0
+    b.q.reshape(70, 1, H, QK)[..., 0] = ahead * np.log(2) * np.sqrt(QK)
+    size = 1.5 * (741 + sink * 2.0 ** ahead) / (701 + 2.0 ** ahead)
+    b.check(tol=TOL * max(size, 2.0 ** -40) * 1.5, sessions={0, 35, 69})
+
+
+def test_long_runs_of_large_values(ctx):
+    b = _long(26, LONG[0], ctx)
+    rng = np.random.default_rng(27)
+    _positive(b, b.pg, b.pkv, b.pnb, 0, np.arange(701), rng.normal(size=(701, 128 * 48)), rng.uniform(2.5e38, 3.3e38, (701, 128 * 64)))
+    for i in range(70):
+        n = b.used[i] + 1
+        _positive(b, b.g, b.kv, b.nb, i, np.arange(n), rng.normal(size=(n, 128 * 48)), rng.uniform(2.5e38, 3.3e38, (n, 128 * 64)))
+    b.check(tol=TOL * 3.3e38, sessions={0, 35, 69})
+
+
 def test_sessions_over_one_block_and_strides(ctx):
     """kv_stride 0, and blocks further apart than they are large."""
     b = Batch(ctx, 15, (8, 4, 64), [60, 30], [9, 9], [0, 1])
