@@ -21,12 +21,12 @@
 // the bins that matter listed in a third; a block a row ends.
 //
 // What bounds it (MI355X; kernels):
-//   one row of 8192, every rule: 6.2 us, one block's phases one after another.
+//   one row of 8192, every rule: 5.5 us, one block's phases one after another.
 //   1024 rows of 8192, top-p 0.9: 22.6 us (34 MB, 7 at a large copy's rate).  Vector
 //     instructions, 70 a token: 30 for its weight and bin, the rest for the row's range,
 //     the two searches and the scans.  (Registers leave two blocks a CU; with bounds for
 //     four, which spill, the time is the same.)
-//   320 rows of 8191, the whole distribution: 15 us, two blocks on some of the CUs.
+//   320 rows of 8191, the whole distribution: 14 us, two blocks on some of the CUs.
 //   200 rows of 100003 (80 MB): top-k 50 in all 42 us (25 of them the slices), no top-k
 //     90 (18, bins 36, gather 22, draw 14), top-k 1000 96.
 #include "nd_internal.h"
@@ -764,13 +764,17 @@ __device__ inline bool draw_binned(const Sample &s, size_t row, const Row &r, Sh
     return true;
 }
 
+constexpr int kThreads = 512;  // of a row's block, or a slice's
+
 // Rows of one slice: a block a row.  SEARCH: what is unusual is searched here, at the
-// price of registers; else the row is marked for a launch after this one.  1024 threads
-// where a CU has a row at most (one row of 8192: 6.2 us), 512 where it has more, and
-// rows wait for each other's phases (of 1024 threads 1024 rows took 31 us, of 512 25).
-template <int NT, bool SEARCH>
-__global__ __launch_bounds__(NT) void sample_kernel(Sample s, size_t first)
+// price of registers; else the row is marked for a launch after this one.  Rows of 8192,
+// top-p 0.9, with and without (us, a launch more of half a microsecond not counted): 320
+// 12.8, 13.5; 512 14.6, 14.9; 1024 23.8, 22.4; 3000 59, 51.  (Of 1024 threads, with: 1 row
+// 8.1 against 7.8, 320 17.2, 1024 34.)
+template <bool SEARCH>
+__global__ __launch_bounds__(kThreads) void sample_kernel(Sample s, size_t first)
 {
+    constexpr int NT = kThreads;
     __shared__ Shared h;
     const size_t row = first + blockIdx.x;
     const int t = threadIdx.x;
@@ -809,7 +813,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(Sample s, size_t first)
 }
 
 // The rows marked.
-__global__ __launch_bounds__(512) void search_kernel(Sample s, size_t first)
+__global__ __launch_bounds__(kThreads) void search_kernel(Sample s, size_t first)
 {
     __shared__ Shared h;
     const size_t row = first + blockIdx.x;
@@ -817,19 +821,18 @@ __global__ __launch_bounds__(512) void search_kernel(Sample s, size_t first)
     const float *x = s.x + row * s.x_stride;
     Row r = rules_of(s, row);
     float top = -INFINITY, low = INFINITY;
-    for (int i = threadIdx.x; i < s.n; i += 512) {
+    for (int i = threadIdx.x; i < s.n; i += kThreads) {
         const float l = x[i];
         top = l > top ? l : top;
         low = l > -INFINITY ? fminf(low, l) : low;
     }
-    meet<512>(top, low, h.room[0]);
+    meet<kThreads>(top, low, h.room[0]);
     range_of(r, top, low);
-    search<512>(s, row, r, h);
+    search<kThreads>(s, row, r, h);
 }
 
 // ---- rows of several slices -------------------------------------------------------
 
-constexpr int kThreads = 512;  // of a slice's block
 constexpr int kDraw = 1024;    // of a row's
 
 enum Way { kSearch, kListed, kBinned };
@@ -1104,19 +1107,18 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
     }
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
     const size_t most = 0xffffffff / kDraw / slices;
-    // few rows: as many threads a row as there are, and no launch more; many: rows in
-    // flight
-    const bool few = count <= size_t(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    // two blocks a CU are what its registers hold
+    const bool few = count <= 2 * size_t(ctx->num_cus > 0 ? ctx->num_cus : 256);
     for (size_t first = 0; first < count; first += most) {
         const unsigned rows = unsigned(std::min(most, count - first)), blocks = rows * unsigned(slices);
         if (slices == 1) {
             if (few) {
-                hipLaunchKernelGGL((sample_kernel<1024, true>), dim3(rows), dim3(1024), 0, ctx->stream, s, first);
+                hipLaunchKernelGGL(sample_kernel<true>, dim3(rows), dim3(kThreads), 0, ctx->stream, s, first);
                 if (int rc = nd::check_launch("sample_rows")) return rc;
             } else {
-                hipLaunchKernelGGL((sample_kernel<512, false>), dim3(rows), dim3(512), 0, ctx->stream, s, first);
+                hipLaunchKernelGGL(sample_kernel<false>, dim3(rows), dim3(kThreads), 0, ctx->stream, s, first);
                 if (int rc = nd::check_launch("sample_rows")) return rc;
-                hipLaunchKernelGGL(search_kernel, dim3(rows), dim3(512), 0, ctx->stream, s, first);
+                hipLaunchKernelGGL(search_kernel, dim3(rows), dim3(kThreads), 0, ctx->stream, s, first);
                 if (int rc = nd::check_launch("sample_search")) return rc;
             }
             continue;
