@@ -24,8 +24,8 @@
 //   one row of 8192, every rule: 5.5 us, one block's phases one after another.
 //   1024 rows of 8192, top-p 0.9: 22.6 us (34 MB, 7 at a large copy's rate).  Vector
 //     instructions, 70 a token: 30 for its weight and bin, the rest for the row's range,
-//     the two searches and the scans.  (Registers leave two blocks a CU; with bounds for
-//     four, which spill, the time is the same.)
+//     the two searches and the scans.  (80 registers leave three blocks a CU; held to 64,
+//     which spills, four blocks took no less.)
 //   320 rows of 8191, the whole distribution: 14 us, two blocks on some of the CUs.
 //   200 rows of 100003 (80 MB): top-k 50 in all 42 us (25 of them the slices), no top-k
 //     90 (18, bins 36, gather 22, draw 14), top-k 1000 96.
