@@ -474,8 +474,8 @@ int nd_prefix_plan(nd_ctx *ctx, const nd_kv_geom *g, size_t prefix_cap, size_t c
  * prefix_cap slots) and of its own (kv + i * kv_stride bytes, the step's keys
  * and values already written), position p at slot p % the block's slots.
  * Heads and quant_query as in nd_attend_step_i8.  Rows that are not there are
- * not written, bad rows are NaN, and so is every row if `plan` was made for
- * other sizes; a head whose query holds a NaN or an infinity gives NaN.  A
+ * not written, bad rows are NaN, and so is every row if what `plan` holds was
+ * made for other sizes (its memory is that of these all the same); a head whose query holds a NaN or an infinity gives NaN.  A
  * prefix is read for all of its rows at once.  Precision as
  * nd_attend_tree_i8.  qk 48 or 64, v 64, at most 2^29 positions x kv heads a
  * block and 4096 heads; out must not overlap q.  `work` as for

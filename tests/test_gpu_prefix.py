@@ -466,6 +466,16 @@ def test_many_heads_and_more_units_than_a_launch_holds(ctx, H, KVH, S, rows):
     assert (got == b.attend()).all()
 
 
+def test_a_plan_without_the_room_of_its_sizes(ctx):
+    b = Batch(ctx, 28, (12, 2, 48), [40], [5, 7, 9])
+    plan, _ = b.plan()
+    with pytest.raises(ValueError, match="plan"):
+        b.attend(plan=nd.PrefixPlan(plan.data[:-64], plan.sizes))
+    many = nd.PrefixPlan(plan.data, (300, *plan.sizes[1:]))
+    with pytest.raises(ValueError, match="plan"):
+        nd.attend_prefix_i8(ctx, b.g, b.kv, 0, b.pkv, 0, many, torch.zeros(300, 1, 576, device="cuda"))
+
+
 # ---- refusals -----------------------------------------------------------------------
 
 def test_refusals(ctx):
