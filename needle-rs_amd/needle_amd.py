@@ -236,6 +236,7 @@ class Ctx:
     def __init__(self, device=0, stream=None):
         torch = _torch()
         self.device = device
+        self.like = {}  # a tensor of no elements of each type that was asked for
         if stream is None:
             stream = torch.cuda.current_stream(device)
         self.stream = stream
@@ -690,7 +691,10 @@ def _empty(ctx, shape, dtype):
     torch's current stream is done with it too where that is another one."""
     torch = _torch()
     if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:  # (1 us less than current_stream)
-        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
+        like = ctx.like.get(dtype)
+        if like is None:
+            like = ctx.like[dtype] = torch.empty(0, dtype=dtype, device=ctx.stream.device)
+        return like.new_empty(shape)  # (0.6 us less than empty)
     with torch.cuda.stream(ctx.stream):
         t = torch.empty(shape, dtype=dtype, device=ctx.stream.device)
     t.record_stream(torch.cuda.current_stream(ctx.device))

@@ -267,6 +267,31 @@ def test_a_drawn_loop_is_its_steps_drawn(ctx):
     a.close(), b.close(), dm.close()
 
 
+def test_a_drawn_loop_over_a_long_vocabulary(ctx):
+    """Logits of several slices, whose workspace is the context's."""
+    g = V.small_geometry(4)
+    g.update(vocab_size=20000, out_vocab=20000)
+    g, recs = V.build_records(g, seed=6)
+    dm = nd.V3Model(ctx, g, recs, V.CODEBOOK)
+    assert dm.rows == 20000
+    sessions, steps = 2, 8
+    a, b = (nd.V3Batch(dm, sessions, max_len=40, max_chunk=20) for _ in range(2))
+    prompts = np.stack([V.prompt_tokens(20, 50 + i) for i in range(sessions)])
+    first = a.prefill(prompts)
+    assert np.array_equal(first, b.prefill(prompts))
+    u = torch.rand(steps, sessions, device="cuda")
+    rules = dict(temperature=torch.tensor([0.9, 1.5], device="cuda"), top_k=torch.tensor([900, 0], dtype=torch.int32, device="cuda"),
+                 top_p=torch.tensor([0.9, 0.95], device="cuda"))
+    got = b.sampled(first, u, **rules)
+    logits, tok = torch.empty(sessions, dm.rows, device="cuda"), first
+    for k in range(steps):
+        a.step(tok, logits=logits, want_next=False)
+        tok = host(nd.sample_rows(ctx, logits, u[k], **rules)[0])
+        assert np.array_equal(tok, got[:, k]), k
+    assert len(np.unique(got)) > 3
+    a.close(), b.close(), dm.close()
+
+
 def test_a_cold_loop_is_the_greedy_one(ctx):
     dm, ((a, first), (b, _)) = _model(ctx, 2, 12)
     want = a.greedy(first, 12)
