@@ -466,6 +466,29 @@ def test_many_heads_and_more_units_than_a_launch_holds(ctx, H, KVH, S, rows):
     assert (got == b.attend()).all()
 
 
+@pytest.mark.parametrize("quant", [False, True])
+def test_positions_at_the_end_of_32_bits(ctx, quant):
+    """Rings whose last position is 2^31 - 1: a session's, and a prefix's with a session behind it."""
+    top = 2 ** 31 - 1
+    b = Batch(ctx, 29, (12, 2, 48), [top - 70, 0], [67, top - 2, 2 ** 30], [0, 1, -1], rows=3, window=75, cap=80, pcap=77)
+    rng = np.random.default_rng(30)
+    for g, blk, nb, i, end in ((b.pg, b.pkv, b.pnb, 0, top - 70), (b.g, b.kv, b.nb, 1, top + 1), (b.g, b.kv, b.nb, 2, 2 ** 30 + 3)):
+        pos = np.arange(end - 77, end)  # three windows of 75
+        _positive(b, g, blk, nb, i, pos, rng.normal(size=(77, 96)), rng.normal(size=(77, 128)))
+    assert not b.bad.any() and b.maps["rot"].max() == top
+    b.check(quant)
+
+
+def test_no_sessions(ctx):
+    g = nd.kv_geom(12, 2, 48, 64, 8)
+    kv, nb = nd.kv_alloc(g, 1)
+    for plen in (None, [5, 0]):
+        plan, maps = nd.prefix_plan(ctx, g, 8, _i32(plen), _i32([]))
+        assert [t.numel() for t in maps] == [0, 0, 0, 0, 0, len(plen or []) + 1] and not host(maps[5]).any()
+        out = nd.attend_prefix_i8(ctx, g, kv, nb, kv if plen else None, 0, plan, torch.zeros(0, 1, 576, device="cuda"))
+        assert out.shape == (0, 1, 768)
+
+
 def test_a_plan_without_the_room_of_its_sizes(ctx):
     b = Batch(ctx, 28, (12, 2, 48), [40], [5, 7, 9])
     plan, _ = b.plan()

@@ -266,6 +266,12 @@ def test_rows_beyond_32_bits_of_offset(ctx):
     assert got[-1].item() == n - 2 and (got[:-1] == 12345).all()
 
 
+def test_no_rows(ctx):
+    for n in (5, 20000):
+        token, chance = nd.sample_rows(ctx, torch.zeros(0, n, device="cuda"), torch.zeros(0, device="cuda"))
+        assert token.shape == chance.shape == (0,)
+
+
 def test_refusals(ctx):
     x, u = torch.zeros(3, 100, device="cuda"), torch.zeros(3, device="cuda")
     for bad in (lambda: nd.sample_rows(ctx, x.double(), u), lambda: nd.sample_rows(ctx, x.cpu(), u),
