@@ -493,22 +493,36 @@ struct Held {
     }
 };
 
-// What the slices have listed, a wave a slice.
+// What the slices have listed, a wave a slice.  The first of a wave are asked for ahead of
+// the row's rules.
 template <int NT>
 struct Lists {
     const uint64_t *list;
     const Part *part;
-    int slices;
+    int slices, many0;
+    uint64_t o0;
+    __device__ inline Lists(const Sample &s, size_t row)
+        : list(s.list + row * s.slices * kList), part(s.part + row * s.slices), slices(s.slices), many0(0), o0(0)
+    {
+        const int i = int(threadIdx.x >> 6);
+        if (i < slices) {
+            many0 = part[i].listed;
+            o0 = list[size_t(i) * kList + (threadIdx.x & 63)];
+        }
+    }
     template <typename F>
     __device__ inline void all(const Row &r, F f) const
     {
-        for (int i = int(threadIdx.x >> 6); i < slices; i += NT / 64) {
+        const int lane = int(threadIdx.x & 63), first = int(threadIdx.x >> 6);
+        auto take = [&](uint64_t o) {
+            const float l = logit_of(o);
+            if (token(r, l)) f(l, o);
+        };
+        if (lane < many0) take(o0);
+        for (int j = lane + 64; j < many0; j += 64) take(list[size_t(first) * kList + j]);
+        for (int i = first + NT / 64; i < slices; i += NT / 64) {
             const int many = part[i].listed;
-            for (int j = int(threadIdx.x & 63); j < many; j += 64) {
-                const uint64_t o = list[size_t(i) * kList + j];
-                const float l = logit_of(o);
-                if (token(r, l)) f(l, o);
-            }
+            for (int j = lane; j < many; j += 64) take(list[size_t(i) * kList + j]);
         }
     }
     template <bool WEIGHTS, bool COUNT>
@@ -590,18 +604,31 @@ __device__ inline int list_first(const Row &r, int &want, Shared &h, Src &src)
     return many;
 }
 
+// f of the places of the list's first `many` and their number in it, four at a time: what
+// is behind them counts as the last of all (a barrier).
+template <typename F>
+__device__ inline void listed_all(Shared &h, int many, F f)
+{
+    const int t = threadIdx.x, all = (many + 3) & ~3;
+    if (t >= many && t < all) h.list[t] = ~uint64_t(0);
+    __syncthreads();
+    if ((t & ~63) >= many) return;  // (a wave without a place in it)
+    for (int j = 0; j < all; j += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(h.list[j + e], j + e);
+    }
+}
+
 // Draws from the first `want` of the `many` tokens listed.
 template <int NT>
 __device__ inline void draw_listed(const Sample &s, size_t row, Row r, int want, int many, Shared &h)
 {
     const int t = threadIdx.x;
     r.scale = kMostScale;
-    if (t < many) {
-        const uint64_t mine = h.list[t];
-        int rank = 0;
-        for (int j = 0; j < many; ++j) rank += h.list[j] < mine;
-        h.sums[rank] = mine;
-    }
+    const uint64_t own = t < many ? h.list[t] : 0;
+    int rank = 0;
+    listed_all(h, many, [&](uint64_t o, int) { rank += o < own; });
+    if (t < many) h.sums[rank] = own;
     __syncthreads();
     const uint64_t mine = t < want ? h.sums[t] : 0, w = t < want ? weight_of(r, logit_of(mine)) : 0;
     uint64_t before;
@@ -698,11 +725,14 @@ __device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint
     }
     if (many > kList) return false;
     if (in) h.sums[t] = w;
-    __syncthreads();
+    uint64_t upto = 0;
+    uint32_t rank = 0;
+    listed_all(h, many, [&](uint64_t o, int j) {
+        const bool is = o <= mine;
+        upto += is ? h.sums[j] : 0;
+        rank += is;
+    });
     if (in) {
-        uint64_t upto = 0, rank = 0;
-        for (int j = 0; j < many; ++j)
-            if (h.list[j] <= mine) upto += h.sums[j], ++rank;
         const uint64_t now = skip + (COUNT ? rank : upto);
         if (now >= target && now - (COUNT ? 1 : w) < target) {
             h.best[0] = mine;
@@ -1038,6 +1068,7 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
     __shared__ Shared h;
     const size_t row = first + blockIdx.x;
     const int t = threadIdx.x;
+    const Lists<kDraw> lists(s, row);
     Row r = rules_of(s, row);
     h.count[t] = 0;
     if (t == 0) h.listed = 0;
@@ -1052,7 +1083,6 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
         }
         return;
     }
-    const Lists<kDraw> lists{s.list + row * s.slices * kList, part, s.slices};
     int few = 1;
     for (int i = t; i < s.slices; i += kDraw) few &= part[i].listed >= 0;
     if (__syncthreads_and(few)) {
