@@ -27,8 +27,8 @@
 //     the two searches and the scans.  (80 registers leave three blocks a CU; held to 64,
 //     which spills, four blocks took no less.)
 //   320 rows of 8191, the whole distribution: 14 us, two blocks on some of the CUs.
-//   200 rows of 100003 (80 MB): top-k 50 in all 42 us (25 of them the slices), no top-k
-//     90 (18, bins 36, gather 22, draw 14), top-k 1000 96.
+//   200 rows of 100003 (80 MB): top-k 50 in all 41 us (25 of them the slices), no top-k
+//     88 (17, bins 36, gather 22, draw 12), top-k 1000 92.
 #include "nd_internal.h"
 #include "nd_lanes.h"
 
@@ -192,6 +192,9 @@ __device__ inline int bin_of(const Row &r, float l)
 {
     return l == r.top ? 0 : int(fminf((r.top - l) * r.bins, float(kBins - 1)));
 }
+
+// The same where the largest logit is finite.
+__device__ inline uint32_t bin_below(const Row &r, float l) { return uint32_t(fminf((r.top - l) * r.bins, float(kBins - 1))); }
 
 struct Shared {
     uint64_t weight[kBins], list[kList], sums[kList];
@@ -456,7 +459,7 @@ struct Held {
             const double d = double(v[j]) - top;
             uint32_t bin = kNoBin;
             if (d >= r.low) {
-                bin = uint32_t(fminf((r.top - v[j]) * r.bins, float(kBins - 1)));  // bin_of
+                bin = bin_below(r, v[j]);
                 if constexpr (COUNT) atomicAdd(&h.count[bin], 1u);
                 if constexpr (WEIGHTS)
                     atomicAdd(reinterpret_cast<unsigned long long *>(&h.weight[bin]), units_of(d, r.by, r.scale));
@@ -1049,7 +1052,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
         v.clean();
 #pragma unroll
         for (int j = 0; j < v.kPer; ++j) {
-            const uint32_t bin = uint32_t(bin_of(r, v.v[j]));
+            const uint32_t bin = bin_below(r, v.v[j]);
             if (m.has(bin) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)));
         }
         __syncthreads();
