@@ -45,7 +45,9 @@ constexpr size_t kMaxSessions = 65535, kMaxRows = 256, kMaxAll = size_t(1) << 20
 // tiles of quad q.
 constexpr int kPlanMagic = 0x6e645031;
 // Kernel times: with half as many waves 512 rows behind 8000 positions 46 -> 54 us, with
-// twice as many 24 x 33 rows 26 -> 28 and their join 7.5 -> 9.3; with runs of 2 chunks 64
+// twice as many 24 x 33 rows 26 -> 28 and their join 7.5 -> 9.3; with 3600, a card not quite
+// full, 200 rows of 12 x 64 45 -> 42 (the last 14 blocks of a full one begin when others end),
+// but 512 rows 46 -> 49 and 24 x 33 rows 25 -> 26.5.  With runs of 2 chunks 64
 // rows 10.4 -> 11.4 and their join 4.3 -> 5.8, of 8 128 rows in windows 15 -> 17.
 constexpr uint32_t kWaves = 4096;  // four a SIMD
 constexpr uint32_t kLeast = 4;     // chunks a wave, at least
