@@ -199,7 +199,7 @@ __device__ inline uint32_t bin_below(const Row &r, float l) { return uint32_t(fm
 struct Shared {
     uint64_t weight[kBins], list[kList], sums[kList];
     uint64_t room[3][16], best[3];
-    uint32_t count[kBins], listed, bin;
+    uint32_t count[kBins], listed, finer, bin;  // finer: what cut_in lists the second time
 };
 
 // Where a target lies: the token, the weights up to it and its own.
@@ -542,9 +542,9 @@ struct Lists {
     }
 };
 
-__device__ inline void enlist(Shared &h, uint64_t o)
+__device__ inline void enlist(Shared &h, uint64_t o, uint32_t &listed)
 {
-    const uint32_t at = atomicAdd(&h.listed, 1u);  // (what is beyond the list's room is counted alone)
+    const uint32_t at = atomicAdd(&listed, 1u);  // (what is beyond the list's room is counted alone)
     if (at < uint32_t(kList)) h.list[at] = o;
 }
 
@@ -602,7 +602,7 @@ __device__ inline int list_first(const Row &r, int &want, Shared &h, Src &src)
     __syncthreads();
     const int many = int(h.best[0]);
     if (many > kList) return -1;
-    src.each(r, 0, h.bin, [&](float, uint64_t o) { enlist(h, o); });
+    src.each(r, 0, h.bin, [&](float, uint64_t o) { enlist(h, o, h.listed); });
     __syncthreads();
     return many;
 }
@@ -669,9 +669,11 @@ __device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint
 {
     const int t = threadIdx.x;
     constexpr int B = kBins / NT;
-    if (t == 0) h.listed = 0;
+    // (the two lists' lengths are cleared here, both: between the barrier that ends the first
+    // list and a wave's reading of its length nothing may write that)
+    if (t == 0) h.listed = h.finer = 0;
     __syncthreads();
-    src.each(r, bin, bin, [&](float, uint64_t o) { enlist(h, o); });
+    src.each(r, bin, bin, [&](float, uint64_t o) { enlist(h, o, h.listed); });
 #pragma unroll
     for (int e = 0; e < B; ++e) h.weight[B * t + e] = 0, h.count[B * t + e] = 0;
     __syncthreads();
@@ -691,7 +693,6 @@ __device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint
         const int part = in ? part_of_bin(r, logit_of(mine), bin) : -1;
         if (in) lay(part, w);
         if (!all) src.each(r, bin, bin, [&](float l, uint64_t) { lay(part_of_bin(r, l, bin), weight_of(r, l)); });
-        if (t == 0) h.listed = 0;
         __syncthreads();
         Bins<NT, uint64_t> bw;
         bw.read(h.weight, h.room[1]);
@@ -713,13 +714,13 @@ __device__ inline bool cut_in(uint64_t target, uint32_t bin, uint64_t skip, uint
         __syncthreads();
         skip = h.best[0], skipw = h.best[1];
         const int fine = int(h.bin);
-        if (in && part == fine) enlist(h, mine);
+        if (in && part == fine) enlist(h, mine, h.finer);
         if (!all)
             src.each(r, bin, bin, [&](float l, uint64_t o) {
-                if (part_of_bin(r, l, bin) == fine) enlist(h, o);
+                if (part_of_bin(r, l, bin) == fine) enlist(h, o, h.finer);
             });
         __syncthreads();
-        many = int(h.listed);
+        many = int(h.finer);
         in = t < many;
         if (in && many <= kList) {
             mine = h.list[t];
@@ -1053,7 +1054,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Sample s, size_t first
 #pragma unroll
         for (int j = 0; j < v.kPer; ++j) {
             const uint32_t bin = bin_below(r, v.v[j]);
-            if (m.has(bin) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)));
+            if (m.has(bin) && token(r, v.v[j])) enlist(h, order_of(v.v[j], v.at(j)), h.listed);
         }
         __syncthreads();
         const int many = int(h.listed);

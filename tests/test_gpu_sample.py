@@ -291,3 +291,16 @@ def test_refusals(ctx):
     assert L.nd_sample_rows(ctx.h, None, 0, 0, 5, None, None, None, None, None, 0) == nd.ND_OK
     assert L.nd_sample_rows(ctx.h, p, 0, 1, 100, None, q, q, None, None, 0) == nd.ND_OK  # one row: any stride
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(top_p=0.5), dict(top_k=600), dict(top_k=900, top_p=0.8)])
+@pytest.mark.parametrize("rows,n,width", [(40, 2000, 0.3), (40, 8192, 0.1), (600, 2000, 0.3), (600, 5000, 0.02), (40, 30000, 0.3),
+                                          (40, 30000, 0.02)])
+def test_bins_of_many_tokens(ctx, rows, n, width, rules):
+    """Targets in bins (of 2^(1/16)) of 65 to 512 tokens, and of thousands, which are listed twice: every row's
+    weights but the largest lie within `width` of another."""
+    rng = np.random.default_rng(rows + n)
+    x = (-4 - width * rng.random((rows, n))).astype(np.float32)
+    x[:, n // 3] = 0.0
+    x[:, n // 2] = -60.0
+    _check(ctx, x, (0.2 + 0.79 * rng.random(rows)).astype(np.float32), rules)
