@@ -121,8 +121,9 @@ __device__ inline Row rules_of(const Sample &s, size_t row)
     r.by = r.greedy ? 1.0 : 1.4426950408889634 / double(r.T);
     // (weights below 2^-64 are no whole unit)
     r.low = fmax(-64.0 / r.by, -1e300);
-    if (mp > 0.0f) r.low = fmax(r.low, double(r.T) * log(double(mp)));
-    if (r.greedy || mp >= 1.0f) r.low = 0.0;
+    // (of an infinite temperature every weight is 1, which a min_p up to 1 lets stay)
+    if (mp > 0.0f && r.T < INFINITY) r.low = fmax(r.low, mp < 1.0f ? double(r.T) * log(double(mp)) : 0.0);
+    if (r.greedy) r.low = 0.0;
     return r;
 }
 

@@ -304,3 +304,22 @@ def test_bins_of_many_tokens(ctx, rows, n, width, rules):
     x[:, n // 3] = 0.0
     x[:, n // 2] = -60.0
     _check(ctx, x, (0.2 + 0.79 * rng.random(rows)).astype(np.float32), rules)
+
+
+@pytest.mark.parametrize("n", [5, 900, 9000, 30000])
+def test_an_infinite_temperature_with_min_p(ctx, n):
+    """exp(d / inf) is 1 for every finite d, which a min_p of 1 or less lets stay; above 1 the first maximum alone."""
+    rng = np.random.default_rng(n)
+    x, u = _logits(rng, 8, n), rng.random(8).astype(np.float32)
+    x[1::2, 1::3] = -np.inf
+    x[2] = np.where(rng.random(n) < 0.5, 3e38, -3e38)
+    for kw in (dict(), dict(top_p=0.5), dict(top_k=600)):
+        for min_p in (1.0, 1 - 2.0 ** -24, 1e-44):
+            got, prob = _run(ctx, x, u, dict(temperature=np.inf, min_p=min_p, **kw))
+            for i in range(8):
+                by = np.argsort(-x[i], kind="stable")[:np.isfinite(x[i]).sum()]
+                by = by[:kw.get("top_k")]
+                kept = int(np.ceil(kw["top_p"] * len(by))) if "top_p" in kw else len(by)
+                assert got[i] == by[P.draw_in_whole_numbers([1] * kept, u[i])] and prob[i] == np.float32(1 / kept), (i, min_p)
+        got, prob = _run(ctx, x, u, dict(temperature=np.inf, min_p=1 + 2.0 ** -23, **kw))
+        assert (got == np.argmax(x, 1)).all() and (prob == 1).all()
