@@ -181,9 +181,9 @@ __device__ inline uint64_t weight_of(const Row &r, float l)
 __device__ inline float bound_of(const Row &r, float l)
 {
     // (the argument is off by 2^-22 of its size, of 64 at most where it counts; a factor
-    // of 0 would make no number of -inf)
-    const float d = l == r.top ? 0.0f : l - r.top;
-    return l > -INFINITY ? __builtin_amdgcn_exp2f(d * fmaxf(float(r.by), 0x1p-149f)) * 1.0001f : 0.0f;
+    // of 0 would make no number of -inf, and an infinite one none of 0)
+    const float d = l == r.top ? 0.0f : l - r.top, by = fminf(fmaxf(float(r.by), 0x1p-149f), 0x1.fffffep127f);
+    return l > -INFINITY ? __builtin_amdgcn_exp2f(d * by) * 1.0001f : 0.0f;
 }
 
 // The scale for weights that come to `sum` or less: below 2^62 units.

@@ -323,3 +323,18 @@ def test_an_infinite_temperature_with_min_p(ctx, n):
                 assert got[i] == by[P.draw_in_whole_numbers([1] * kept, u[i])] and prob[i] == np.float32(1 / kept), (i, min_p)
         got, prob = _run(ctx, x, u, dict(temperature=np.inf, min_p=1 + 2.0 ** -23, **kw))
         assert (got == np.argmax(x, 1)).all() and (prob == 1).all()
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(top_p=0.4), dict(top_k=20000)])
+@pytest.mark.parametrize("n", [8192, 33000, 70001, 300000])
+def test_the_lowest_temperature_over_equal_and_neighbouring_logits(ctx, n, rules):
+    """1 / T beyond fp32: more ties than 64 bits hold in units of 2^-49, and logits as far apart as T, which weigh 1 / e."""
+    t = float(np.float32(1e-45))
+    rng = np.random.default_rng(n)
+    u = rng.random(6).astype(np.float32)
+    got, prob = _run(ctx, np.full((6, n), 2.0), u, dict(temperature=t, **rules))
+    kept = min(n, rules.get("top_k", n))
+    kept = int(np.ceil(float(np.float32(rules["top_p"])) * kept)) if "top_p" in rules else kept
+    for i in range(6):
+        assert got[i] == P.draw_in_whole_numbers([1] * kept, u[i]) and prob[i] == np.float32(1 / kept)
+    _check(ctx, (-rng.integers(0, 5, (6, n)) * t).astype(np.float32), u, dict(temperature=t, **rules), least=0.8)
