@@ -177,13 +177,13 @@ __device__ inline uint64_t weight_of(const Row &r, float l)
     return d >= r.low ? units_of(d, r.by, r.scale) : 0;
 }
 
-// A little more than the weight (and 1 for some that are no tokens).
+// A little more than the weight; 0: no token.  (The argument is worked out in fp64, whose
+// range holds any two logits' distance and any 1 / T, and rounded by 2^-24 of its size, of
+// 64 at most.)
 __device__ inline float bound_of(const Row &r, float l)
 {
-    // (the argument is off by 2^-22 of its size, of 64 at most where it counts; a factor
-    // of 0 would make no number of -inf, and an infinite one none of 0)
-    const float d = l == r.top ? 0.0f : l - r.top, by = fminf(fmaxf(float(r.by), 0x1p-149f), 0x1.fffffep127f);
-    return l > -INFINITY ? __builtin_amdgcn_exp2f(d * by) * 1.0001f : 0.0f;
+    const double d = behind(r, l);
+    return d >= r.low ? __builtin_amdgcn_exp2f(float(d * r.by)) * 1.0001f : 0.0f;
 }
 
 // The scale for weights that come to `sum` or less: below 2^62 units.

@@ -338,3 +338,15 @@ def test_the_lowest_temperature_over_equal_and_neighbouring_logits(ctx, n, rules
     for i in range(6):
         assert got[i] == P.draw_in_whole_numbers([1] * kept, u[i]) and prob[i] == np.float32(1 / kept)
     _check(ctx, (-rng.integers(0, 5, (6, n)) * t).astype(np.float32), u, dict(temperature=t, **rules), least=0.8)
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(top_p=0.7), dict(top_k=200000, top_p=0.9), dict(min_p=0.01)])
+@pytest.mark.parametrize("temperature", [3e38, 1.5e38, 3.4028235e38])
+def test_logits_further_apart_than_the_largest_number(ctx, temperature, rules):
+    """The largest logit and the rest at both ends of fp32, at a temperature under which the rest weighs as much."""
+    n, rng = 300000, np.random.default_rng(31)
+    x = np.full((4, n), -3e38, np.float32)
+    x[1:] = -(1.5e38 + 1.9e38 * rng.random((3, n)))
+    x[np.arange(4), [7, n // 2, n - 1, 8192]] = 3e38
+    x[3] = (6.8e38 * (rng.random(n) - 0.5)).astype(np.float32)
+    _check(ctx, x, (0.02 + 0.97 * rng.random(4)).astype(np.float32), dict(temperature=temperature, **rules), least=0.7)
