@@ -67,6 +67,7 @@ struct Sample {
     uint64_t *bins;   // [rows][kBins]
     uint64_t *list;   // [rows][slices][kList]
     uint32_t *count;  // [rows][kBins]
+    int *scale;       // [rows], of rows by their bins
 };
 
 // The order of the floats as that of whole numbers, the largest first (-0 as 0).
@@ -890,15 +891,15 @@ __device__ inline void join_parts(const Sample &s, size_t row, Row &r, uint64_t 
     range_of(r, top, low);
 }
 
-// And the unit, by the bound on its weights (a barrier).
-template <int NT>
+// And the unit, by the bound on its weights (a barrier).  Only the bins' launch works it
+// out, and leaves it for the draw: in another order of the sum it may be another.
 __device__ inline void join_scale(const Sample &s, size_t row, Row &r, uint64_t *room)
 {
     const Part *part = s.part + row * s.slices;
     float b = 0.0f;
-    for (int i = threadIdx.x; i < s.slices; i += NT)
+    for (int i = threadIdx.x; i < s.slices; i += kThreads)
         if (part[i].top > -INFINITY) b += part[i].sum * bound_of(r, part[i].top);
-    r.scale = scale_of(sum_over<NT>(b, room));
+    r.scale = scale_of(sum_over<kThreads>(b, room));
 }
 
 // A slice's part and its own short top-k.
@@ -954,7 +955,8 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(Sample s, size_t first)
     }
     join_parts<kThreads>(s, row, r, h.room[0]);
     if (r.top == -INFINITY || way_of(r) != kBinned) return;
-    join_scale<kThreads>(s, row, r, h.room[1]);
+    join_scale(s, row, r, h.room[1]);
+    if (block == 0 && t == 0) s.scale[row] = r.scale;
     for (int slice = block;;) {
         v.clean();
         if (r.k > 0)
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
             const int many = list_first<kDraw>(r, want, h, lists);
             if (many >= 0) return draw_listed<kDraw>(s, row, r, want, many, h);
         } else if (way_of(r) == kBinned) {
-            join_scale<kDraw>(s, row, r, h.room[2]);
+            r.scale = s.scale[row];
             h.weight[t] = s.bins[row * kBins + t];
             h.count[t] = s.count[row * kBins + t];
             __syncthreads();
@@ -1109,7 +1111,7 @@ __global__ __launch_bounds__(kDraw) void draw_kernel(Sample s, size_t first)
 
 size_t slices_of(size_t n) { return (n + kSlice - 1) / kSlice; }
 
-size_t row_bytes(size_t slices) { return slices > 1 ? kBins * 12 + slices * (kList * 8 + sizeof(Part)) : 0; }
+size_t row_bytes(size_t slices) { return slices > 1 ? kBins * 12 + slices * (kList * 8 + sizeof(Part)) + 4 : 0; }
 
 }  // namespace
 
@@ -1129,7 +1131,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
     ND_REQUIRE(count == 1 || x_stride >= n, "row stride %zu below n %zu", x_stride, n);
     const nd_sampling none{}, &r = sampling ? *sampling : none;
     const size_t slices = slices_of(n);
-    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices), 0, nullptr, nullptr, nullptr, nullptr};
+    Sample s{x, r.temperature, r.min_p, r.top_p, u, r.top_k, x_stride, int(n), next, prob, int(slices), 0, nullptr, nullptr, nullptr, nullptr, nullptr};
     // (a row's blocks, of about four a CU; each finds out what matters for itself)
     s.blocks = int(std::min(slices, std::max<size_t>(1, 1024 / count)));
     if (slices > 1) {
@@ -1139,6 +1141,7 @@ int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, s
         s.list = s.bins + count * kBins;
         s.count = reinterpret_cast<uint32_t *>(s.list + count * slices * kList);
         s.part = reinterpret_cast<Part *>(s.count + count * kBins);
+        s.scale = reinterpret_cast<int *>(s.part + count * slices);
     }
     // HIP counts a launch's threads in 32 bits: rows beyond that go in further launches
     const size_t most = 0xffffffff / kDraw / slices;

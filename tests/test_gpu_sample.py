@@ -350,3 +350,24 @@ def test_logits_further_apart_than_the_largest_number(ctx, temperature, rules):
     x[np.arange(4), [7, n // 2, n - 1, 8192]] = 3e38
     x[3] = (6.8e38 * (rng.random(n) - 0.5)).astype(np.float32)
     _check(ctx, x, (0.02 + 0.97 * rng.random(4)).astype(np.float32), dict(temperature=temperature, **rules), least=0.7)
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(top_p=0.9), dict(top_k=6000000, top_p=0.5)])
+def test_a_long_rows_unit_is_one(ctx, rules):
+    """Rows of 1500 slices of 8192 whose bound on the sum lies at a power of two: added up in another order
+    (of these seeds, of 1024 threads instead of 512) it rounds to the other side, and the unit is twice or half of it."""
+    n, infinite = 1500 * 8192, torch.tensor([float("inf")], device="cuda")
+    there = int(2 ** 23 / (1.001 * float(np.float32(1.0001)) ** 2))
+    for seed in (1, 2, 4, 12, 13):
+        rng = np.random.default_rng(seed)
+        x = np.full(n, -np.inf, np.float32)
+        ids = rng.permutation(n)[:there]
+        x[ids] = 20 * rng.random(there) - 10
+        x = dev(x)[None]
+        by = torch.sort(x[0], descending=True, stable=True)[1]
+        kept = min(there, rules.get("top_k", there))
+        kept = int(np.ceil(float(np.float32(rules["top_p"])) * kept)) if "top_p" in rules else kept
+        full = {k: torch.tensor([v], dtype=torch.int32 if k in I32 else torch.float32, device="cuda") for k, v in rules.items()}
+        for u in (0.125, 0.515625, 0.875):  # (u kept is exact in fp64)
+            got, prob = nd.sample_rows(ctx, x, torch.tensor([u], device="cuda"), temperature=infinite, **full)
+            assert got.item() == by[int(u * kept)].item() and host(prob)[0] == np.float32(1 / kept), (seed, u)
