@@ -499,6 +499,77 @@ def test_a_plan_without_the_room_of_its_sizes(ctx):
         nd.attend_prefix_i8(ctx, b.g, b.kv, 0, b.pkv, 0, many, torch.zeros(300, 1, 576, device="cuda"))
 
 
+# ---- the shipped geometry's long runs, thousands of sessions, far rows ---------------
+
+@pytest.mark.parametrize("shape,S,N,plen,window", [((12, 2, 48), 300, 1, 6400, 0), ((12, 2, 48), 24, 33, 2500, 0), ((12, 2, 48), 40, 20, 2600, 2400),
+                                                   ((16, 2, 64), 240, 1, 6001, 0), ((5, 1, 48), 1000, 1, 4500, 0), ((8, 4, 64), 120, 10, 3300, 3000)])
+def test_long_runs_of_few_kv_heads(ctx, shape, S, N, plen, window):
+    """fp32 queries whose tiles lay K and V down for each other, two to eight heads a kv head: a group of `S`
+    sessions in runs of 10 chunks and more, a short prefix and sessions without one beside it."""
+    rng = np.random.default_rng(S)
+    H, KVH, _ = shape
+    which = [0] * S + [1, -1, 1]
+    used = list(rng.integers(0, 40, S + 3))
+    length = [N] * (S - 1) + list(rng.integers(1, N + 1, 4))
+    b = Batch(ctx, S, shape, [plen, 90], used, which, length, N, window, pcap=window + 50 if window else None)
+    tiles, chunks = sum(length[:S]) * (H // KVH) // 16, (min(plen, window) if window else plen) // 32
+    each = tiles * (chunks + 3) // (4096 // KVH) + 1
+    assert tiles >= 8 and chunks // -(-chunks // each) >= 10
+    b.check(sessions={0, 1, S // 2, S - 1, S, S + 1, S + 2})
+
+
+@pytest.mark.parametrize("S,N,count,window", [(4097, 1, 1, 0), (4200, 3, 7, 50), (9000, 2, 300, 0), (65535, 1, 2048, 33), (65535, 16, 5, 0)])
+def test_maps_of_thousands_of_sessions(ctx, S, N, count, window):
+    """More sessions than a block's threads hold at once."""
+    rng = np.random.default_rng(S + N)
+    plen, used, which, length = _requests(rng, S, N, count, 200, 90)
+    _, maps = nd.prefix_plan(ctx, nd.kv_geom(12, 2, 48, 64, 90 + N), 201, _i32(plen), _i32(used), prefix_of=_i32(which),
+                             length=_i32(length), rows=N, window=window)
+    want = P.layout(201, 90 + N, plen, used, which, length, N, window)[2]
+    for t, k in zip(maps, ("pos", "rot", "from", "lo", "order", "first")):
+        assert np.array_equal(host(t), want[k]), k
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_of_thousands_of_sessions(ctx, quant):
+    S = 4500
+    rng = np.random.default_rng(40)
+    b = Batch(ctx, 41, (5, 1, 48), [130, 70, 0, 33], list(rng.integers(0, 12, S)), list(rng.integers(-1, 4, S)),
+              list(rng.integers(0, 3, S)), 2)
+    b.check(quant, sessions={0, 63, 64, 1023, 1024, 4095, 4096, 4097, 4200, S - 1})
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_a_session_whatever_else_the_step_holds(ctx, quant):
+    """The same session alone, behind others of its prefix and beside other prefixes: each time within the
+    tolerance of the same 64-bit sums."""
+    b = Batch(ctx, 42, (12, 2, 48), [700, 90], [33, 5, 20, 0, 12, 33, 7], [0, 0, 1, -1, 0, 1, 0], rows=2)
+    whole = host(b.attend(quant))
+    b.check(quant)
+    for keep in ([0], [1, 0], [2, 3, 0, 5], [6, 5, 4, 0]):
+        kv = torch.cat([b.kv[i * b.nb:(i + 1) * b.nb] for i in keep])
+        plan, _ = nd.prefix_plan(ctx, b.g, b.pcap, _i32(b.plen), _i32([b.used[i] for i in keep]),
+                                 prefix_of=_i32([b.which[i] for i in keep]), rows=2)
+        got = host(nd.attend_prefix_i8(ctx, b.g, kv, b.nb, b.pkv, b.pnb, plan, dev(b.q[keep]), quant_query=quant))
+        assert np.abs(got - whole[keep]).max() <= 2 * TOL
+
+
+def test_queries_and_outputs_beyond_32_bits(ctx):
+    """2^20 rows of 65 heads: 4.3e9 numbers of each.  Sessions over one block give the bits of seven."""
+    S, N, H = 65535, 16, 65
+    b = Batch(ctx, 43, (H, H, 64), [], [5], rows=N)
+    base = torch.randn(7, H * 64, device="cuda")
+    i, n = torch.arange(S, device="cuda")[:, None], torch.arange(N, device="cuda")
+    q = base[(i * N + n).view(-1) % 7].view(S, N, H * 64)
+    want = nd.attend_prefix_i8(ctx, b.g, b.kv, 0, None, 0, nd.prefix_plan(ctx, b.g, 1, None, _i32([5] * 7), rows=N)[0], q[:7].clone())
+    plan, _ = nd.prefix_plan(ctx, b.g, 1, None, _i32([5] * S), rows=N)
+    got = nd.attend_prefix_i8(ctx, b.g, b.kv, 0, None, 0, plan, q)
+    assert torch.isfinite(want).all()
+    for first in range(0, S, 7 * 1024):
+        part = got[first:first + 7 * 1024]
+        assert torch.equal(part, want.repeat(1025, 1, 1)[:len(part)])
+
+
 # ---- refusals -----------------------------------------------------------------------
 
 def test_refusals(ctx):

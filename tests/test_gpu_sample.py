@@ -371,3 +371,16 @@ def test_a_long_rows_unit_is_one(ctx, rules):
         for u in (0.125, 0.515625, 0.875):  # (u kept is exact in fp64)
             got, prob = nd.sample_rows(ctx, x, torch.tensor([u], device="cuda"), temperature=infinite, **full)
             assert got.item() == by[int(u * kept)].item() and host(prob)[0] == np.float32(1 / kept), (seed, u)
+
+
+@pytest.mark.parametrize("temperature", [1e30, 1e38, 3.4028235e38])
+@pytest.mark.parametrize("n", [40, 3000, 20000])
+def test_tokens_alike_at_a_very_high_temperature(ctx, n, temperature):
+    """Logits less than 100 apart weigh 1 - 1e-28 or more of each other: as many units."""
+    rng = np.random.default_rng(n)
+    x, u = _logits(rng, 12, n), rng.random(12).astype(np.float32)
+    by = np.argsort(-x, 1, kind="stable")
+    for kw, kept in ((dict(), n), (dict(top_k=17), 17), (dict(top_k=2000), min(n, 2000)), (dict(top_p=0.25), n // 4)):
+        got, prob = _run(ctx, x, u, dict(temperature=temperature, **kw))
+        assert got.tolist() == [by[i, P.draw_in_whole_numbers([1] * kept, u[i])] for i in range(12)], kw
+        assert (prob == np.float32(1 / kept)).all(), kw
