@@ -475,9 +475,9 @@ int nd_prefix_plan(nd_ctx *ctx, const nd_kv_geom *g, size_t prefix_cap, size_t c
  * and values already written), position p at slot p % the block's slots.
  * Heads and quant_query as in nd_attend_step_i8.  Rows that are not there are
  * not written, bad rows are NaN, and so is every row if what `plan` holds was
- * made for other sizes (its memory is that of these all the same); a head whose query holds a NaN or an infinity gives NaN.  A
- * prefix is read for all of its rows at once.  Precision as
- * nd_attend_tree_i8.  qk 48 or 64, v 64, at most 2^29 positions x kv heads a
+ * made for other sizes (its memory is that of these all the same); a head
+ * whose query holds a NaN or an infinity gives NaN.  A prefix is read for all
+ * of its rows at once.  Precision as nd_attend_tree_i8.  qk 48 or 64, v 64, at most 2^29 positions x kv heads a
  * block and 4096 heads; out must not overlap q.  `work` as for
  * nd_attend_tree_i8, of nd_attend_prefix_i8_work(..) bytes. */
 size_t nd_attend_prefix_i8_work(nd_ctx *ctx, const nd_kv_geom *g, size_t count, size_t rows,
@@ -514,11 +514,13 @@ typedef struct nd_sampling {
  * prob[i] (may be NULL) = the chance that token had, 1 for a greedy row, 0 for
  * none.  u is taken as 0 below 0 or as a NaN, as the last token's at 1 and
  * above.  Weights are fp64 exponentials as whole numbers of 2^-49 of the
- * largest (or of 2^-61 of the row's sum, where that is more), so sums are
- * exact and a pick is the border's; tokens of less than half of that are never
- * drawn.  sampling may be NULL.  n <= 2^24, count < 2^31.  `work` as for nd_attend_tree_i8, of
- * nd_sample_rows_work(..) bytes.  The reference's generate takes a
- * temperature alone (needle-c/src/v3.rs:219-250). */
+ * largest, so sums are exact and a pick is the border's; tokens of less than
+ * half of that are never drawn.  In a row above 8192 logits with a top_k above
+ * 448 or none, or with very many equal logits, the unit may be larger: up to
+ * 2^-61 of the sum of the row's weights before the rules, and so 2^-37 of the
+ * largest at most.  sampling may be NULL.  n <= 2^24, count < 2^31.
+ * `work` as for nd_attend_tree_i8, of nd_sample_rows_work(..) bytes.  The
+ * reference's generate takes a temperature alone (needle-c/src/v3.rs:219-250). */
 size_t nd_sample_rows_work(nd_ctx *ctx, size_t count, size_t n);
 int nd_sample_rows(nd_ctx *ctx, const float *x, size_t x_stride, size_t count, size_t n,
                    const nd_sampling *sampling, const float *u, int32_t *next, float *prob,

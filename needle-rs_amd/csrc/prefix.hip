@@ -11,12 +11,12 @@
 // and only the sessions' own blocks are read row by row.
 //
 // What bounds it (MI355X; a call, both kernels):
-//   512 rows of 12 heads over 2 behind 8000 positions, fp32 queries: 49 us.  Vector
+//   512 rows of 12 heads over 2 behind 8000 positions, fp32 queries: 48 us.  Vector
 //     instructions: about 100 for a chunk of 512 scores (8 exponentials, 16 to split the
 //     weights, 20 to turn the wave's share of K and V, 24 for scores and weights), of
 //     which 20 more cost 3 us; 14 matrix products of 16 cycles lie beside them.
-//   200 sessions of 12 x 64 heads, 500 own positions each, seven prompts: 50 us, 170 MB
-//     at 3.4 TB/s; a large copy would take 35.
+//   200 sessions of 12 x 64 heads, 500 own positions each, seven prompts: 50 us, 168 MB
+//     at 3.4 TB/s (at 3.7 in the first kernel's 45); a large copy would take 35.
 //   64 sessions behind 2000 positions, query codes: 12.5 us, of which 8.7 are the first
 //     kernel, one pass through memory and four chunks a wave, and 4 the join's.
 #include "nd_attn_pieces.h"
@@ -769,8 +769,10 @@ __device__ __forceinline__ void walk(const Geom &gown, const Geom &gp, const Att
                     if constexpr (KD == 3) kp[6] = kp[4], kp[7] = kp[5];
                 }
                 floatx4_t d{0.0f, 0.0f, 0.0f, 0.0f};
-auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, uint32_t q1, uint32_t q2, uint32_t q3) {
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(k0, k1, k2, k3), vec4<f16x8_t>(q0, q1, q2, q3), d, 0, 0, 0);
+                auto add = [&](uint32_t k0, uint32_t k1, uint32_t k2, uint32_t k3, uint32_t q0, uint32_t q1,
+                               uint32_t q2, uint32_t q3) {
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vec4<f16x8_t>(k0, k1, k2, k3),
+                                                               vec4<f16x8_t>(q0, q1, q2, q3), d, 0, 0, 0);
                 };
                 const uint32_t *qh = qp[0], *ql = qp[1];
                 // the small pieces first; of qk 48 a lane's last four codes meet both
@@ -988,7 +990,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Attend at, uint32_t fi
     int left = runs[0];  // of the prefix
     for (int j0 = 0; j0 < all; j0 += 64) {
         const int j = j0 + lane, many = min(64, all - j0);
-        // the sums of run e of these (the prefix's, then the own ones), four a time; the
+        // the sums of run e of these (the prefix's, then the own ones), eight a time; the
         // first are asked for ahead of what they are multiplied by
         float o[kAtOnce] = {};
         auto load = [&](int e0) {

@@ -12,8 +12,9 @@
 //     finer and finer bins, by the digits of the order.
 // Weights are whole numbers, exp((l - M) / T) in units of 2^-s, worked out in fp64: a
 // pick next to a border is the border's and not the rounding's, and sums of whole
-// numbers are the same in any order.  s is 49, or less where a bound on a long row's
-// sum asks for it: the sum stays below 2^62 and has 2^49 units at least.
+// numbers are the same in any order.  s is 49, or less (37 or more) where a bound on the
+// weights of all of a long row's tokens, before top-k and top-p, asks for it: their sum
+// stays below 2^62.
 //
 // A block a row of up to kSlice logits, which stay in its registers.  Longer rows: a
 // block a slice looks for its largest logit and lists its own short top-k; where
@@ -21,14 +22,15 @@
 // the bins that matter listed in a third; a block a row ends.
 //
 // What bounds it (MI355X; kernels):
-//   one row of 8192, every rule: 5.5 us, one block's phases one after another.
-//   1024 rows of 8192, top-p 0.9: 22.6 us (34 MB, 7 at a large copy's rate).  Vector
+//   one row of 8192, every rule: 5.6 us, one block's phases one after another.
+//   1024 rows of 8192, top-p 0.9: 22.8 us (34 MB, 7 at a large copy's rate).  Vector
 //     instructions, 70 a token: 30 for its weight and bin, the rest for the row's range,
 //     the two searches and the scans.  (80 registers leave three blocks a CU; held to 64,
 //     which spills, four blocks took no less.)
 //   320 rows of 8191, the whole distribution: 14 us, two blocks on some of the CUs.
-//   200 rows of 100003 (80 MB): top-k 50 in all 41 us (25 of them the slices), no top-k
-//     88 (17, bins 36, gather 22, draw 12), top-k 1000 92.
+//   200 rows of 100003 (80 MB, 17 at a large copy's rate; a call): top-k 50 in all 34 us,
+//     no top-k 85 (slices 20, bins 36, gather 22, draw 12), top-k 1000 87.  The bins: fp64
+//     weights, five blocks a row with up to three slices one after another.
 #include "nd_internal.h"
 #include "nd_lanes.h"
 

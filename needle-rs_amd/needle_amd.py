@@ -984,7 +984,8 @@ def attend_prefix_i8(ctx, g, kv, kv_stride, prefix_kv, prefix_stride, plan, q, s
     wp, wb = _work_arg(ctx, work)
     _check(lib().nd_attend_prefix_i8(
         ctx.h, C.byref(g), _dev_arg(ctx, kv, u8, "kv", blocks), kv_stride, s, n,
-        _dev_arg(ctx, prefix_kv, u8, "prefix_kv", many), prefix_stride, cap, p, _dev_arg(ctx, plan.data, u8, "plan", _plan_bytes(heads, kv_heads, s, n, p)),
+        _dev_arg(ctx, prefix_kv, u8, "prefix_kv", many), prefix_stride, cap, p,
+        _dev_arg(ctx, plan.data, u8, "plan", _plan_bytes(heads, kv_heads, s, n, p)),
         _dev_arg(ctx, q, f32, "q", s * n * heads * qk), scale, int(bool(quant_query)),
         _dev_arg(ctx, out, f32, "out", s * n * heads * vd), wp, wb))
     return out
